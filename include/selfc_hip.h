@@ -430,6 +430,53 @@ int selfc_globalagg_bwd_x(const float* x, const float* dy, float* dx, const floa
                         float* dfcb_clip, float* dwmap_clip, void* scratch, size_t scratch_bytes,
                         int N, int T, int H, int W, const float* dy_amax, float* dx_amax_out, void* stream);
 
+/* ---- a residual feed-forward layer over pixels or tokens: norm, product, optimizer step (no counterpart in the reference) ----
+ * Number types of these entry points are the caller's, not the library's operand type: 0 = fp32, 1 = bf16, 2 = f16, 3 = e4m3 (OCP,
+ * no infinities).  Pitches (ld*) count elements.  Row counts may be 0: nothing is launched (dw / db: zeros). */
+
+/* csrc/rmsnorm.hip.  h = x + r rounded to `dtype` (r and h together, or both NULL: h is x), y = h / sqrt(mean(h^2) + eps) * w over the
+ * last axis of C <= 16384 values.  q8_scale NULL: y of `dtype`; else y is e4m3 and q8_scale[row] its step (largest |y| = 448 steps; 1 for
+ * a row of zeros).  w: fp32 (w_f32) or `dtype`.  h and y are written without gaps. */
+int selfc_rmsnorm(const void* x, size_t ldx, const void* r, size_t ldr, const void* w, int w_f32, void* h, void* y, float* q8_scale,
+                  size_t rows, int C, int dtype, float eps, void* stream);
+/* Gradient with respect to x (= r's) and w: dx = the norm's part + dh (dh NULL: none), dw of w's type.  dy, dh, dx without gaps; dx or dw
+ * may be NULL; partial: selfc_rmsnorm_bwd_floats floats (only with dw). */
+size_t selfc_rmsnorm_bwd_floats(size_t rows, int C);
+int selfc_rmsnorm_bwd(const void* h, size_t ldh, const void* w, int w_f32, const void* dy, const void* dh, void* dx, void* dw,
+                      float* partial, size_t rows, int C, int dtype, float eps, void* stream);
+
+/* csrc/linear.hip.  y[rows][n] = act(x w^T + bias) + res; x [rows][k], w [n][k] of in_dtype bf16 / f16 (out_dtype the same) or e4m3 (then
+ * x_scale[rows] and w_scale[n] multiply the sums; out_dtype 0..2).  act: 0 none, 1 ReLU, 2 LeakyReLU(0.2), 3 GELU (erf), 4 SiLU.
+ * bias, res: out_dtype or NULL.  x and w: 16-byte aligned, pitch and k whole 16-byte pieces (selfc_pack_rows makes such rows of any
+ * others).  slope (or NULL): u16 [rows][roundup(n, 8)], receives act' for selfc_linear_dz.  ws: selfc_linear_ws_floats(rows, n, k,
+ * bytes of in_dtype) floats. */
+size_t selfc_linear_ws_floats(size_t rows, int cols, int sum, int elem_bytes);
+int selfc_pack_rows(const void* src, size_t ld, void* dst, size_t rows, int cols, int ldd, int elem_bytes, void* stream);
+int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const float* x_scale, const float* w_scale, const void* bias, int act,
+                 const void* res, size_t ldr, void* y, void* slope, float* ws, size_t rows, int n, int k, int in_dtype, int out_dtype, void* stream);
+/* dz = dy * slope (slope NULL: dy) into rows of pitch lddz = roundup(n, 8) with zeros behind them, and / or db = its column sums;
+ * partial: selfc_linear_dz_floats floats (only with db). */
+size_t selfc_linear_dz_floats(size_t rows, int n);
+int selfc_linear_dz(const void* dy, size_t lddy, const void* slope, void* dz, size_t lddz, void* db, float* partial, size_t rows, int n, int dtype, void* stream);
+/* dx[rows][k] = dz w and dw[n][k] = dz^T x; dz, w, x 16-byte aligned with pitches of whole 16-byte pieces, zeros in dz behind column n.
+ * ws: selfc_linear_ws_floats(rows, k, n, 2) and (n, k, rows, 2) floats.  rows >= 1 for dw. */
+int selfc_linear_dx(const void* dz, size_t lddz, const void* w, size_t ldw, void* dx, float* ws, size_t rows, int n, int k, int dtype, void* stream);
+int selfc_linear_dw(const void* dz, size_t lddz, const void* x, size_t ldx, void* dw, float* ws, size_t rows, int n, int k, int dtype, void* stream);
+
+/* csrc/adamw.hip.  One AdamW step of `count` tensors (a HOST array; it is read before the call returns) of one `dtype`.  A tensor
+ * without a gradient is left as it is.  State: m and v hold all tensors, tensor i from the sum of roundup(n_j, selfc_adamw_block())
+ * over j < i on; state_bits 32: fp32; 8: e4m3 (m) and e5m2 (v) with one power-of-two step per block in m_scale / v_scale.
+ * step: this step's number, from 1 on, or a device fp32 scalar per tensor; lr likewise.  norm (device, selfc_grad_norm) with max_norm:
+ * gradients are scaled by min(1, max_norm / (norm + 1e-6)); the gradients themselves are not written.  seed: of the 8-bit dither. */
+typedef struct { void* param; const void* grad; const float* step; size_t n; } selfc_adamw_tensor;
+int selfc_adamw_block(void);
+int selfc_adamw_step(const selfc_adamw_tensor* tensors, int count, int dtype, int state_bits, void* m, void* v, float* m_scale,
+                     float* v_scale, float lr, const float* lr_dev, double beta1, double beta2, float eps, float weight_decay,
+                     double step, unsigned seed, const float* norm, float max_norm, void* stream);
+/* out = 2-norm over the gradients of all tensors that have one; partial: selfc_grad_norm_partials(count) doubles */
+size_t selfc_grad_norm_partials(int count);
+int selfc_grad_norm(const selfc_adamw_tensor* tensors, int count, int dtype, double* partial, float* out, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,387 @@
+// AdamW over a list of tensors in as few launches as the kernel-argument segment allows, with the moments in 32 or in 8 bits,
+// and the global norm of a list of gradients.
+//
+//   g' = g min(1, max_norm / (|g| + 1e-6))            (only with max_norm)
+//   m' = b1 m + (1 - b1) g',   v' = b2 v + (1 - b2) g'^2
+//   p' = p (1 - lr wd) - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+//
+// Arithmetic in fp32, every operation of the moments rounded by itself (no contraction): in 8 bits the outcome of a comparison
+// hangs on their last bit, and this way it is the same for every implementation of the formulas above.
+//
+// The moments of all tensors live in one buffer each; a tensor starts at a multiple of 256 values, so a block of 256 belongs to
+// one tensor.  In 8 bits each block has two power-of-two scales.  m is held as e4m3 (largest value of the block in [128, 256)
+// steps of its scale), v as e5m2 (in [2^14, 2^15)): v spans twice the octaves that m does, because it is m's square.
+// Rounding: v moves by 0.1 % of itself per step at b2 = 0.999 while a step of its code is 12 to 25 % - rounded to nearest it would
+// never move.  So a value is rounded down after adding u steps, u in [0, 1) from an integer hash of (seed, step, tensor, place):
+// right on average.  With scales that are powers of two a value that is on the grid stays on it when the scale changes, so the
+// noise enters only with the few values that move (a fixed grid moves with probability 0.001 |g^2/v - 1| / 0.18 per step: about
+// 30 % standard deviation of v, 15 % of the step's size, against 160 % if every step re-rounded every value).  A nonzero v never
+// rounds to zero: m / sqrt(v) stays bounded.  Values that are not finite are held as NaN and do not enter their block's scale.
+//
+// Bound: memory (28 bytes a value in 32 bits; 16 in 8 bits with fp32 tensors, 10 with 16-bit ones) - about 60 vector
+// instructions a value for the 8-bit form, which is near the rate at which the memory delivers.
+#include "pointwise.hpp"
+#include <math.h>
+
+namespace selfc {
+namespace {
+
+constexpr int AW_BLOCK = 256;              // values per scale; also what one wave handles at a time, four consecutive ones per lane
+constexpr int AW_U = 4;                    // blocks per wave: their loads are in flight together
+constexpr int AW_CHUNK = 4 * AW_U * AW_BLOCK;
+constexpr int AW_MAX = 96;                 // tensors per launch: 96 entries of 40 bytes stay below 4 KiB of kernel arguments
+
+struct AwEntry { void* p; const void* g; const float* step; unsigned long long n; unsigned block0, wg0; };
+struct AwTable {
+  AwEntry e[AW_MAX];
+  int count, place0;
+};
+struct AwHyper {
+  const float *lr_dev, *norm;
+  double beta1_d, beta2_d;
+  float lr, bc1, bc2s, b1, omb1, b2, omb2, eps, wd, max_norm;
+  unsigned seed, key;
+};
+
+__host__ __device__ inline unsigned aw_mix(unsigned x) {        // multipliers: digits of pi
+  x ^= x >> 16; x *= 0x85A308D3u;
+  x ^= x >> 15; x *= 0x13198A2Fu;
+  return x ^ (x >> 16);
+}
+__host__ __device__ inline double aw_pow(double b, unsigned long long e) {
+  double r = 1.0;
+  for (; e; e >>= 1, b *= b)
+    if (e & 1) r *= b;
+  return r;
+}
+
+// which tensor of the table holds workgroup `wg`: entries start at ascending workgroups, two entries per lane
+__device__ __forceinline__ int aw_find(const AwTable& t, const unsigned wg) {
+  const int lane = threadIdx.x & 63;
+  const bool a = lane < t.count && t.e[lane].wg0 <= wg;
+  const int j = lane + 64;
+  const bool b = j < t.count && t.e[j < AW_MAX ? j : 0].wg0 <= wg;
+  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(a)) + __popcll(__ballot(b)) - 1);
+}
+
+__device__ __forceinline__ unsigned wave_umax(unsigned v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned w = __shfl_xor(v, o);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+
+// the block's scale 2^(floor(log2 most) - top), not below 2^-126; 1 for an empty block.  `inv` = 1 / scale, exact.
+__device__ __forceinline__ float aw_scale(const unsigned most, const int top, float& inv) {
+  int e = (int)(most >> 23) - top;           // biased exponent of the scale
+  e = e < 1 ? 1 : e;
+  if (most == 0) e = 127;
+  inv = __builtin_bit_cast(float, (unsigned)(254 - e) << 23);
+  return __builtin_bit_cast(float, (unsigned)e << 23);
+}
+
+// |y| rounded down after adding u steps of the 8-bit format's grid (least: exponent of its smallest normal number, digits: of its
+// mantissa); not a number if y is not finite
+template <int LEAST, int DIGITS, bool FLOOR>
+__device__ __forceinline__ float aw_round(const float y, const float u) {
+  const unsigned ay = __builtin_bit_cast(unsigned, y) & 0x7fffffffu;
+  int e = (int)(ay >> 23);
+  e = e < 127 + LEAST ? 127 + LEAST : e;
+  const float q = __builtin_bit_cast(float, (unsigned)(e - DIGITS) << 23);
+  const float iq = __builtin_bit_cast(float, (unsigned)(254 - e + DIGITS) << 23);
+  float k = floorf(__builtin_bit_cast(float, ay) * iq + u);
+  if (FLOOR) k = ay ? fmaxf(k, 1.f) : k;
+  const float r = __builtin_copysignf(k * q, y);
+  return ay < 0x7f800000u ? r : __builtin_nanf("");
+}
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(256) void adamw_kernel(const AwTable tab, const AwHyper hy, void* const m_, void* const v_,
+                                                    float* const ms, float* const vs) {
+#pragma clang fp contract(off)
+  const unsigned wg = blockIdx.x;
+  const int ti = aw_find(tab, wg);
+  const AwEntry& en = tab.e[ti];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  T* const p = (T*)en.p;
+  const T* const g = (const T*)en.g;
+  const unsigned long long n = en.n;
+  const unsigned long long base = (unsigned long long)(wg - en.wg0) * AW_CHUNK + (unsigned)wave * (AW_U * AW_BLOCK);
+  if (base >= n) return;
+  const size_t blk0 = (size_t)en.block0 + (size_t)(base / AW_BLOCK);       // first of this wave's blocks in the state
+  const size_t s0 = blk0 * AW_BLOCK;
+
+  constexpr bool NARROW = sizeof(T) == 2;
+  const bool vec = (((size_t)p | (size_t)g) & (NARROW ? 7 : 15)) == 0;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  float pv[AW_U][4], gv[AW_U][4], mv[AW_U][4], vv[AW_U][4];
+  unsigned m8[AW_U], v8[AW_U];
+#pragma unroll
+  for (int u = 0; u < AW_U; ++u) {
+    const unsigned long long at = base + u * AW_BLOCK + lane * 4;
+    if (base + u * AW_BLOCK < n) {
+      if (vec && at + 4 <= n) {
+        const T4 a = *reinterpret_cast<const T4*>(p + at), b = *reinterpret_cast<const T4*>(g + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { pv[u][i] = (float)a[i]; gv[u][i] = (float)b[i]; }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          pv[u][i] = at + i < n ? (float)p[at + i] : 0.f;
+          gv[u][i] = at + i < n ? (float)g[at + i] : 0.f;
+        }
+      }
+      const size_t st = s0 + u * AW_BLOCK + lane * 4;
+      if constexpr (BITS == 32) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)m_ + st), b = *reinterpret_cast<const f32x4*>((const float*)v_ + st);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { mv[u][i] = a[i]; vv[u][i] = b[i]; }
+      } else {
+        m8[u] = *reinterpret_cast<const unsigned*>((const unsigned char*)m_ + st);
+        v8[u] = *reinterpret_cast<const unsigned*>((const unsigned char*)v_ + st);
+        const float sm = ms[blk0 + u], sv = vs[blk0 + u];
+        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(m8[u], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(m8[u], true);
+        const f32x2 c = __builtin_amdgcn_cvt_pk_f32_bf8(v8[u], false), d = __builtin_amdgcn_cvt_pk_f32_bf8(v8[u], true);
+        mv[u][0] = a[0] * sm; mv[u][1] = a[1] * sm; mv[u][2] = b[0] * sm; mv[u][3] = b[1] * sm;
+        vv[u][0] = c[0] * sv; vv[u][1] = c[1] * sv; vv[u][2] = d[0] * sv; vv[u][3] = d[1] * sv;
+      }
+    }
+  }
+
+  // what the step's number and the rate make of the formulas: from the host, or (captured steps) from device memory
+  float bc1 = hy.bc1, bc2s = hy.bc2s;
+  unsigned key = hy.key;
+  if (en.step) {
+    const unsigned long long t = (unsigned long long)*en.step;
+    bc1 = (float)(1.0 - aw_pow(hy.beta1_d, t));
+    bc2s = (float)sqrt(1.0 - aw_pow(hy.beta2_d, t));
+    key = aw_mix(hy.seed ^ aw_mix((unsigned)t));
+  }
+  const float lr = hy.lr_dev ? *hy.lr_dev : hy.lr;
+  const float keep = 1.f - lr * hy.wd, rate = lr / bc1, ibc2 = 1.f / bc2s;
+  float coef = 1.f;
+  if (hy.norm) coef = fminf(hy.max_norm / (*hy.norm + 1e-6f), 1.f);
+  const bool clip = hy.norm != nullptr;
+  const unsigned tkey = aw_mix(key ^ aw_mix((unsigned)(tab.place0 + ti)));
+
+#pragma unroll
+  for (int u = 0; u < AW_U; ++u) {
+    if (base + u * AW_BLOCK >= n) break;
+    const unsigned long long at = base + u * AW_BLOCK + lane * 4;
+    unsigned mmost = 0, vmost = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float gi = gv[u][i];
+      if (clip) gi = gi * coef;
+      const float mi = hy.b1 * mv[u][i] + hy.omb1 * gi;
+      const float vi = hy.b2 * vv[u][i] + hy.omb2 * (gi * gi);
+      mv[u][i] = mi;
+      vv[u][i] = vi;
+      // one-ulp square root and reciprocal: the step is a small part of p, its last bits are below p's
+      const float den = __builtin_amdgcn_sqrtf(vi) * ibc2 + hy.eps;
+      pv[u][i] = pv[u][i] * keep - rate * (mi * __builtin_amdgcn_rcpf(den));
+      if constexpr (BITS == 8) {
+        const unsigned am = __builtin_bit_cast(unsigned, mi) & 0x7fffffffu, av = __builtin_bit_cast(unsigned, vi) & 0x7fffffffu;
+        const bool in = at + i < n;
+        mmost = in && am < 0x7f800000u && am > mmost ? am : mmost;
+        vmost = in && av < 0x7f800000u && av > vmost ? av : vmost;
+      }
+    }
+    if (vec && at + 4 <= n) {
+      T4 a;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = (T)pv[u][i];
+      *reinterpret_cast<T4*>(p + at) = a;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (at + i < n) p[at + i] = (T)pv[u][i];
+    }
+    const size_t st = s0 + u * AW_BLOCK + lane * 4;
+    if constexpr (BITS == 32) {
+      float* const mp = (float*)m_ + st;
+      float* const vp = (float*)v_ + st;
+      if (at + 4 <= n) {
+        *reinterpret_cast<f32x4*>(mp) = f32x4{mv[u][0], mv[u][1], mv[u][2], mv[u][3]};
+        *reinterpret_cast<f32x4*>(vp) = f32x4{vv[u][0], vv[u][1], vv[u][2], vv[u][3]};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (at + i < n) { mp[i] = mv[u][i]; vp[i] = vv[u][i]; }
+      }
+    } else {
+      float im, iv;
+      const float sm = aw_scale(wave_umax(mmost), 7, im), sv = aw_scale(wave_umax(vmost), 14, iv);
+      float mq[4], vq[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned x = aw_mix((unsigned)(at + i) ^ tkey);
+        mq[i] = at + i < n ? aw_round<-6, 3, false>(mv[u][i] * im, (float)(x & 0xffffu) * 0x1p-16f) : 0.f;
+        vq[i] = at + i < n ? aw_round<-14, 2, true>(vv[u][i] * iv, (float)(x >> 16) * 0x1p-16f) : 0.f;
+      }
+      int a = __builtin_amdgcn_cvt_pk_fp8_f32(mq[0], mq[1], 0, false);
+      a = __builtin_amdgcn_cvt_pk_fp8_f32(mq[2], mq[3], a, true);
+      int b = __builtin_amdgcn_cvt_pk_bf8_f32(vq[0], vq[1], 0, false);
+      b = __builtin_amdgcn_cvt_pk_bf8_f32(vq[2], vq[3], b, true);
+      *reinterpret_cast<int*>((unsigned char*)m_ + st) = a;
+      *reinterpret_cast<int*>((unsigned char*)v_ + st) = b;
+      if (lane == 0) { ms[blk0 + u] = sm; vs[blk0 + u] = sv; }
+    }
+  }
+}
+
+// ---- |g| over a list: per-workgroup sums of squares in fp64 (an fp32 square overflows from 2^64 on), then one workgroup adds them
+// in a fixed order
+constexpr int GN_WG = 1024;
+template <typename T>
+__global__ __launch_bounds__(256) void grad_norm_kernel(const AwTable tab, const unsigned chunks, double* const partial) {
+  double acc = 0.0;
+  for (unsigned c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const AwEntry& en = tab.e[aw_find(tab, c)];
+    const T* const g = (const T*)en.g;
+    const unsigned long long base = (unsigned long long)(c - en.wg0) * AW_CHUNK;
+    const unsigned long long left = en.n - base;
+    const T* const q = g + base;
+    const bool vec = aligned16((const void*)q);
+#pragma unroll
+    for (int j = 0; j < AW_CHUNK / 2048; ++j) {
+      const long at = j * 2048 + threadIdx.x * 8;
+      if ((unsigned long long)at < left) {
+        float v[8];
+        const unsigned long long l = left - at;
+        load8(q + at, l > 8 ? 8 : (long)l, vec, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc += (double)v[i] * (double)v[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) acc += __shfl_xor(acc, o);
+  __shared__ double red[4];
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) partial[blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
+}
+__global__ __launch_bounds__(1024) void grad_norm_final_kernel(const double* const partial, const int n, float* const out) {
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < n; i += 1024) acc += partial[i];
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) acc += __shfl_xor(acc, o);
+  __shared__ double red[16];
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = acc;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0.0;
+    for (int i = 0; i < 16; ++i) s += red[i];
+    *out = (float)sqrt(s);
+  }
+}
+
+// the tensors [i, i + AW_MAX) that have values and a gradient, as a table; returns how many workgroups they take
+struct AwFill {
+  size_t block = 0;         // state blocks in front of tensor i (tensors without a gradient keep theirs)
+  int i = 0;
+  unsigned long long next(const selfc_adamw_tensor* const ts, const int count, AwTable& tab, bool& ok) {
+    unsigned long long wgs = 0;
+    tab.count = 0;
+    tab.place0 = i;
+    int left = AW_MAX;
+    for (; i < count && left > 0; ++i, --left) {
+      // an entry per tensor, so that its number in the table gives its place in the list; an empty one takes no workgroup
+      const selfc_adamw_tensor& t = ts[i];
+      const size_t blocks = (t.n + AW_BLOCK - 1) / AW_BLOCK;
+      const unsigned long long need = t.grad && t.n ? (t.n + AW_CHUNK - 1) / AW_CHUNK : 0;
+      if (block > 0xffffffffull || wgs + need > 0x7fffffffull) { ok = false; return 0; }
+      tab.e[tab.count++] = AwEntry{t.param, t.grad, t.step, t.n, (unsigned)block, (unsigned)wgs};
+      wgs += need;
+      block += blocks;
+    }
+    return wgs;
+  }
+};
+
+}  // namespace
+}  // namespace selfc
+
+using namespace selfc;
+
+extern "C" {
+
+int selfc_adamw_block(void) { return AW_BLOCK; }
+
+int selfc_adamw_step(const selfc_adamw_tensor* tensors, int count, int dtype, int state_bits, void* m, void* v, float* m_scale,
+                     float* v_scale, float lr, const float* lr_dev, double beta1, double beta2, float eps, float weight_decay,
+                     double step, unsigned seed, const float* norm, float max_norm, void* stream) {
+  if (!tensors || count < 0 || (state_bits != 32 && state_bits != 8) || dtype < 0 || dtype > 2) return SELFC_EINVAL;
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return SELFC_EINVAL;
+  bool any = false, host_step = false;
+  for (int i = 0; i < count; ++i) {
+    if (!tensors[i].grad || !tensors[i].n) continue;
+    any = true;
+    if (!tensors[i].param || !aligned_to(tensors[i].param, dtype ? 2 : 4) || !aligned_to(tensors[i].grad, dtype ? 2 : 4)) return SELFC_EINVAL;
+    host_step |= tensors[i].step == nullptr;
+  }
+  if (!any) return SELFC_OK;
+  if (host_step && !(step >= 1.0)) return SELFC_EINVAL;
+  if (!m || !v || !aligned_to(m, 16) || !aligned_to(v, 16) || (state_bits == 8 && (!m_scale || !v_scale))) return SELFC_EINVAL;
+  AwHyper hy{};
+  hy.lr_dev = lr_dev; hy.norm = norm; hy.beta1_d = beta1; hy.beta2_d = beta2; hy.lr = lr;
+  hy.bc1 = (float)(1.0 - pow(beta1, step)); hy.bc2s = (float)sqrt(1.0 - pow(beta2, step));
+  hy.b1 = (float)beta1; hy.omb1 = (float)(1.0 - beta1); hy.b2 = (float)beta2; hy.omb2 = (float)(1.0 - beta2);
+  hy.eps = eps; hy.wd = weight_decay; hy.max_norm = max_norm; hy.seed = seed;
+  hy.key = aw_mix(seed ^ aw_mix((unsigned)(unsigned long long)(step > 0.0 ? step : 0.0)));
+  AwFill fill;
+  AwTable tab;
+  hipStream_t s = (hipStream_t)stream;
+  bool ok = true;
+  { AwFill dry; while (dry.i < count && ok) dry.next(tensors, count, tab, ok); }      // refuse before anything is launched
+  if (!ok) return SELFC_EINVAL;
+  while (fill.i < count) {
+    const unsigned long long wgs = fill.next(tensors, count, tab, ok);
+    if (!wgs) continue;
+    const dim3 grid((unsigned)wgs), blk(256);
+    if (state_bits == 32) {
+      if (dtype == 0) hipLaunchKernelGGL((adamw_kernel<float, 32>), grid, blk, 0, s, tab, hy, m, v, m_scale, v_scale);
+      else if (dtype == 1) hipLaunchKernelGGL((adamw_kernel<b16, 32>), grid, blk, 0, s, tab, hy, m, v, m_scale, v_scale);
+      else hipLaunchKernelGGL((adamw_kernel<h16, 32>), grid, blk, 0, s, tab, hy, m, v, m_scale, v_scale);
+    } else {
+      if (dtype == 0) hipLaunchKernelGGL((adamw_kernel<float, 8>), grid, blk, 0, s, tab, hy, m, v, m_scale, v_scale);
+      else if (dtype == 1) hipLaunchKernelGGL((adamw_kernel<b16, 8>), grid, blk, 0, s, tab, hy, m, v, m_scale, v_scale);
+      else hipLaunchKernelGGL((adamw_kernel<h16, 8>), grid, blk, 0, s, tab, hy, m, v, m_scale, v_scale);
+    }
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return pw_rc(e);
+  }
+  return SELFC_OK;
+}
+
+size_t selfc_grad_norm_partials(int count) { return count < 1 ? 1 : (size_t)((count + AW_MAX - 1) / AW_MAX) * GN_WG; }
+
+int selfc_grad_norm(const selfc_adamw_tensor* tensors, int count, int dtype, double* partial, float* out, void* stream) {
+  if (!tensors || count < 0 || !partial || !out || dtype < 0 || dtype > 2) return SELFC_EINVAL;
+  for (int i = 0; i < count; ++i)
+    if (tensors[i].grad && !aligned_to(tensors[i].grad, dtype ? 2 : 4)) return SELFC_EINVAL;
+  AwTable tab;
+  bool ok = true;
+  { AwFill dry; while (dry.i < count && ok) dry.next(tensors, count, tab, ok); }
+  if (!ok) return SELFC_EINVAL;
+  AwFill fill;
+  hipStream_t s = (hipStream_t)stream;
+  int used = 0;
+  while (fill.i < count) {
+    const unsigned long long chunks = fill.next(tensors, count, tab, ok);
+    if (!chunks) continue;
+    const int wgs = chunks < GN_WG ? (int)chunks : GN_WG;
+    const dim3 grid((unsigned)wgs), blk(256);
+    if (dtype == 0) hipLaunchKernelGGL((grad_norm_kernel<float>), grid, blk, 0, s, tab, (unsigned)chunks, partial + used);
+    else if (dtype == 1) hipLaunchKernelGGL((grad_norm_kernel<b16>), grid, blk, 0, s, tab, (unsigned)chunks, partial + used);
+    else hipLaunchKernelGGL((grad_norm_kernel<h16>), grid, blk, 0, s, tab, (unsigned)chunks, partial + used);
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return pw_rc(e);
+    used += wgs;
+  }
+  hipLaunchKernelGGL(grad_norm_final_kernel, dim3(1), dim3(1024), 0, s, partial, used, out);
+  return pw_rc(hipGetLastError());
+}
+
+}  // extern "C"

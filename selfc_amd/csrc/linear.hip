@@ -1,0 +1,650 @@
+// Matrix products of rows with a weight, with everything that follows the product in the same launch:
+//   y[m][n] = act( sx[m] sw[n] sum_k x[m][k] W[n][k] + b[n] ) + r[m][n]                       (sx, sw: 8-bit operands only)
+// for 16-bit operands with the gradients
+//   dz = dy act'(z),   dx = dz W,   dW = dz^T x,   db = sum over rows of dz
+// and for e4m3 operands (one scale per row of x and of W) without.  Sums in fp32 on the matrix units.
+//
+// One kernel computes out[q][p] = sum over r of Q(q, r) P(p, r); an operand is either stored with r contiguous ("straight": x and W
+// of the forward product) or with r as its row index ("crossed": W in dx, both in dW), and the latter is transposed on the way
+// from shared memory to registers (ds_read_b64_tr_b16), never in memory.
+//
+// The derivative act'(z) is kept for the backward pass as a 16-bit fixed-point number (steps of 2^-15 from -0.5; 65535: not a
+// number): every activation here has its derivative in [-0.13, 1.13], 0 and 1 are exact, and the error 2^-16 is 1/128 of
+// what keeping z in bf16 would cost - after it the backward pass needs neither z nor the activation's formula.
+#include "pointwise.hpp"
+#include "prof.hpp"
+#include <math.h>
+
+namespace selfc {
+
+int pw_colsum(const float* partial, int rows, int C, int dtype, void* out, hipStream_t s);      // rmsnorm.hip
+
+namespace {
+
+enum { ACT_NONE, ACT_RELU, ACT_LRELU, ACT_GELU, ACT_SILU };
+
+typedef h16 h16x8 __attribute__((ext_vector_type(8)));
+typedef b16 b16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+
+// ---- what follows the product ---------------------------------------------------------------------------------------------
+struct Epilogue {
+  void* out;                      // [M][ldo] of `dtype`
+  const void *bias, *res;         // [N]; [M][ldr]
+  const float *qs, *ps;           // scales of the rows and of the columns
+  unsigned short* d;              // [M][ldd] derivative
+  size_t ldo, ldr, ldd;
+  int dtype, act, vec;            // vec: 8 values at a time are aligned and inside a row
+};
+
+__device__ __forceinline__ void act_apply(const int act, const float z, float& y, float& d) {
+  if (act == ACT_NONE) { y = z; d = 1.f; }
+  else if (act == ACT_RELU) { d = z > 0.f ? 1.f : 0.f; y = z > 0.f || z != z ? z : 0.f; }
+  else if (act == ACT_LRELU) { d = z > 0.f ? 1.f : 0.2f; y = z * d; }
+  else if (act == ACT_GELU) {
+    const float phi = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+    const float zc = fminf(fmaxf(z, -20.f), 20.f);                                        // infinities: 0 times the density
+    y = phi == 0.f ? 0.f : z * phi;
+    d = phi + zc * (__expf(-0.5f * zc * zc) * 0.39894228040143268f);
+  } else {
+    const float s = 1.f / (1.f + __expf(-z));
+    const float zc = fminf(fmaxf(z, -80.f), 80.f);
+    y = s == 0.f ? 0.f : z * s;
+    d = s * (1.f + zc * (1.f - s));
+  }
+}
+__device__ __forceinline__ unsigned short act_code(const float d) {
+  const float c = rintf(d * 32768.f) + 16384.f;
+  return d != d ? (unsigned short)65535 : (unsigned short)fminf(fmaxf(c, 0.f), 65534.f);
+}
+__device__ __forceinline__ float act_slope(const unsigned c) {
+  return c == 65535u ? __builtin_nanf("") : (float)((int)c - 16384) * 0x1p-15f;
+}
+
+__device__ __forceinline__ void load8_as(const int dtype, const void* const p, const size_t at, const long left, const bool vec, float* const v) {
+  if (dtype == 0) load8((const float*)p + at, left, vec, v);
+  else if (dtype == 1) load8((const b16*)p + at, left, vec, v);
+  else load8((const h16*)p + at, left, vec, v);
+}
+
+// eight neighbouring columns of one row: acc is the product's sum, b and ps the columns' bias and scale
+__device__ __forceinline__ void epilogue8(const Epilogue& e, const float* const acc, const int row, const int col, const int left,
+                                          const float* const b, const float* const ps) {
+  float y[8], d[8], r[8];
+  const float qs = e.qs ? e.qs[row] : 1.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float z = acc[i];
+    if (e.qs) z *= qs * ps[i];
+    act_apply(e.act, z + b[i], y[i], d[i]);
+  }
+  if (e.d) {
+    unsigned short* const dp = e.d + (size_t)row * e.ldd + col;              // ldd is a multiple of 8: always 16 bytes at a time
+    u16x8 c;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = act_code(d[i]);
+    *reinterpret_cast<u16x8*>(dp) = c;
+  }
+  if (e.res) {
+    load8_as(e.dtype, e.res, (size_t)row * e.ldr + col, left, e.vec, r);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] += r[i];
+  }
+  const size_t at = (size_t)row * e.ldo + col;
+  if (e.dtype == 0) store8((float*)e.out + at, left, e.vec, y);
+  else if (e.dtype == 1) store8((b16*)e.out + at, left, e.vec, y);
+  else store8((h16*)e.out + at, left, e.vec, y);
+}
+__device__ __forceinline__ void epilogue_columns(const Epilogue& e, const int col, const int left, float* const b, float* const ps) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) { b[i] = 0.f; ps[i] = 1.f; }
+  if (e.bias) load8_as(e.dtype, e.bias, col, left, false, b);
+  if (e.ps) load8(e.ps + col, left, false, ps);
+}
+
+// ---- the product ----------------------------------------------------------------------------------------------------------
+struct GemmArgs {
+  const void *q, *p;
+  size_t ldq, ldp;                // pitches in elements
+  int M, N, R;                    // rows and columns of the output, length of the sum (R: a multiple of 16 bytes where an operand is straight)
+  int qx, px;                     // crossed operands: readable columns (a multiple of 8)
+  int splits, per;                // parts of the sum, and stages of each
+  float* ws;                      // [splits][M][ldw] partial sums when splits > 1
+  size_t ldw;
+  Epilogue e;
+};
+
+// global -> shared memory without registers: lane i's 16 bytes land at lds + 16 i; an offset beyond the resource reads zeros
+__device__ __forceinline__ void dma16(const i32x4 rsrc, const unsigned voff, const unsigned lds) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds) : "memory");
+}
+template <int VM>
+__device__ __forceinline__ void wait_barrier() {            // loads but the last VM done, own LDS reads done; then everybody's
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(VM) : "memory");
+}
+
+template <typename T> struct Mma;
+template <> struct Mma<h16> {
+  static __device__ __forceinline__ f32x4 run(const i32x4 a, const i32x4 b, const f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h16x8, a), __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Mma<b16> {
+  static __device__ __forceinline__ f32x4 run(const i32x4 a, const i32x4 b, const f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b16x8, a), __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+  }
+};
+// e4m3 x e4m3: 32 values per lane; both operands hand over the same two 16-byte pieces, so whichever k they belong to, it is the same
+__device__ __forceinline__ f32x4 mma8(const i32x4 a0, const i32x4 a1, const i32x4 b0, const i32x4 b1, const f32x4 c) {
+  const i32x8 a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7), b = __builtin_shufflevector(b0, b1, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+}
+
+// One operand's side of a stage: B rows (straight: [B][128 bytes]) or B columns (crossed: [64][B] 16-bit values) in shared memory.
+// 16-byte pieces are stored at a permuted place of their row so that the reads below never meet in a bank: the loads write shared
+// memory in lane order, so the permutation is applied to the global address.
+template <int B, bool X, int ES, int NT>
+struct Side {
+  static constexpr int LOADS = B * 8 / NT;                  // 16-byte pieces per thread and stage
+  static constexpr int RB = X ? B * 2 : 128;                // bytes of a row in shared memory
+  unsigned voff[LOADS];                                     // byte offset of each piece from the stage's base, or out of range
+  int kk[LOADS];                                            // its place along the sum
+  const char* base;                                         // the stage's base
+  const char* end;
+  size_t step;                                              // bytes from one stage to the next
+
+  static __device__ __forceinline__ int swz(const int r) {  // crossed: which pair of pieces row r moves its columns by
+    return B >= 128 ? (r & 3) | ((r >> 3) & 1) << 2 : ((r >> 1) & 1) | ((r >> 3) & 1) << 1;
+  }
+  __device__ __forceinline__ void init(const void* const src, const size_t ld, const int i0, const int extent, const int R, const int stage0) {
+    constexpr int PIECE = 16 / ES;
+    const char* const s = (const char*)src;
+    if (X) {
+      step = 64 * ld * ES;
+      base = s + (size_t)i0 * ES + (size_t)stage0 * step;
+      end = s + ((size_t)(R - 1) * ld + extent) * ES;
+    } else {
+      step = 128;
+      base = s + (size_t)i0 * ld * ES + (size_t)stage0 * 128;
+      end = s + (size_t)(extent - 1) * ld * ES + (((size_t)R * ES + 15) & ~(size_t)15);
+    }
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int it = 0; it < LOADS; ++it) {
+      const int l = it * NT + tid;
+      if (X) {
+        const int r = l / (B / 8), c = (l % (B / 8)) ^ (swz(r) << 1);
+        kk[it] = r;
+        voff[it] = i0 + c * 8 < extent ? (unsigned)(r * ld * ES + c * 16) : BUF_OOB;
+      } else {
+        const int r = l >> 3, c = (l & 7) ^ ((r >> 1) & 7);
+        kk[it] = c * PIECE;
+        voff[it] = i0 + r < extent ? (unsigned)(r * ld * ES + c * 16) : BUF_OOB;
+      }
+    }
+  }
+  // request a stage of which `left` places of the sum remain, and move on to the next
+  __device__ __forceinline__ void load(const unsigned lds, const int left) {
+    const size_t room = (size_t)(end - base);
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)(size_t)base), hi = __builtin_amdgcn_readfirstlane((unsigned)((size_t)base >> 32));
+    const unsigned bytes = __builtin_amdgcn_readfirstlane(room < 0x7fffffffu ? (unsigned)room : 0x7fffffffu);
+    const i32x4 rsrc = {(int)lo, (int)(hi & 0xffffu), (int)bytes, 0x00020000};
+    const unsigned at = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024;
+#pragma unroll
+    for (int it = 0; it < LOADS; ++it) dma16(rsrc, kk[it] < left ? voff[it] : BUF_OOB, at + it * (NT * 16));
+    base += step;
+  }
+};
+
+// fragments of a 16-wide tile: 16 x 32 16-bit values (straight or crossed) or 16 x 64 bytes of 8-bit ones
+template <int B, bool X>
+struct Frag {
+  int a0, a1;            // this lane's addresses in a stage
+  __device__ __forceinline__ void init(const int i0) {        // i0: the wave's first row / column (a multiple of 16)
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    if (X) {
+      const int q = (lane >> 2) & 3, p = lane & 3;
+      const int r = g * 8 + q;
+      a0 = r * (B * 2) + ((Side<B, X, 2, 256>::swz(r) << 5) ^ (i0 << 1)) + p * 8;
+      a1 = 0;
+    } else {
+      const int row = i0 + (lane & 15), sw = (lane >> 1) & 7;
+      a0 = row * 128 + ((g ^ sw) << 4);
+      a1 = row * 128 + (((g ^ sw) ^ 4) << 4);
+    }
+  }
+  // tile t of the wave, half ks of the stage
+  __device__ __forceinline__ i32x4 read(const unsigned char* const side, const int t, const int ks) const {
+    if constexpr (X) {
+      typedef short s16x4 __attribute__((__vector_size__(8)));
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      const unsigned char* const at = side + (a0 ^ (t << 5)) + ks * 32 * (B * 2);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 4 * (B * 2)));
+      typedef short s16x8 __attribute__((ext_vector_type(8)));
+      const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      return __builtin_bit_cast(i32x4, v);
+    } else {
+      return *reinterpret_cast<const i32x4*>(side + (ks ? a1 : a0) + t * 2048);
+    }
+  }
+};
+
+// BQ x BP outputs per workgroup of NQ x NP waves.  T: h16, b16, or unsigned char for e4m3.
+// The stages of the sum (64 values of 16 bits, 128 of 8) go through two shared-memory buffers: while one is multiplied, the loads of
+// the next are on their way to the other; one barrier per stage.
+template <typename T, bool QX, bool PX, int BQ, int BP, int NQ, int NP>
+__global__ __launch_bounds__(NQ * NP * 64) void gemm_kernel(const GemmArgs a) {
+  constexpr int NT = NQ * NP * 64, ES = sizeof(T), BK = 128 / ES;
+  constexpr int SQ = BQ * 128, STAGE = (BQ + BP) * 128;
+  constexpr int WQ = BQ / NQ, WP = BP / NP, TQ = WQ / 16, TP = WP / 16;
+  extern __shared__ __align__(16) unsigned char lds[];
+  const unsigned lds0 = (unsigned)(size_t)(__attribute__((address_space(3))) unsigned char*)lds;
+
+  // workgroup -> (part of the sum, tile): consecutive tiles on one XCD; tiles in bands of 8 rows, so that neighbours share operands
+  const int nq = (a.M + BQ - 1) / BQ, np = (a.N + BP - 1) / BP, tiles = nq * np;
+  int id = xcd_swizzle(blockIdx.x, gridDim.x);
+  const int part = id / tiles;
+  id -= part * tiles;
+  const int band = id / (8 * np), in = id - band * 8 * np, rows = nq - band * 8 < 8 ? nq - band * 8 : 8;
+  const int q0 = (band * 8 + in % rows) * BQ, p0 = (in / rows) * BP;
+  const int stages = (a.R + BK - 1) / BK;
+  const int s0 = part * a.per, s1 = s0 + a.per < stages ? s0 + a.per : stages;
+
+  Side<BQ, QX, ES, NT> sq;
+  Side<BP, PX, ES, NT> sp;
+  sq.init(a.q, a.ldq, q0, QX ? a.qx : a.M, a.R, s0);
+  sp.init(a.p, a.ldp, p0, PX ? a.px : a.N, a.R, s0);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wq = wave / NP, wp = wave % NP;
+  Frag<BQ, QX> fq;
+  Frag<BP, PX> fp;
+  fq.init(wq * WQ);
+  fp.init(wp * WP);
+
+  f32x4 acc[TP][TQ];
+#pragma unroll
+  for (int i = 0; i < TP; ++i)
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  if (s0 < s1) {
+    sq.load(lds0, a.R - s0 * BK);
+    sp.load(lds0 + SQ, a.R - s0 * BK);
+  }
+  for (int s = s0; s < s1; ++s) {
+    const int cur = (s - s0) & 1;
+    wait_barrier<0>();
+    if (s + 1 < s1) {
+      sq.load(lds0 + (cur ^ 1) * STAGE, a.R - (s + 1) * BK);
+      sp.load(lds0 + (cur ^ 1) * STAGE + SQ, a.R - (s + 1) * BK);
+    }
+    const unsigned char* const lq = lds + cur * STAGE;
+    const unsigned char* const lp = lq + SQ;
+    if constexpr (ES == 1) {
+      i32x4 q[TQ][2];
+#pragma unroll
+      for (int j = 0; j < TQ; ++j) { q[j][0] = fq.read(lq, j, 0); q[j][1] = fq.read(lq, j, 1); }
+#pragma unroll
+      for (int i = 0; i < TP; ++i) {
+        const i32x4 p0_ = fp.read(lp, i, 0), p1_ = fp.read(lp, i, 1);
+#pragma unroll
+        for (int j = 0; j < TQ; ++j) acc[i][j] = mma8(p0_, p1_, q[j][0], q[j][1], acc[i][j]);
+      }
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        i32x4 q[TQ], p[TP];
+#pragma unroll
+        for (int j = 0; j < TQ; ++j) q[j] = fq.read(lq, j, ks);
+#pragma unroll
+        for (int i = 0; i < TP; ++i) p[i] = fp.read(lp, i, ks);
+#pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+          for (int j = 0; j < TQ; ++j) acc[i][j] = Mma<T>::run(p[i], q[j], acc[i][j]);
+      }
+    }
+  }
+  wait_barrier<0>();                      // the buffers are free: each wave turns its tiles into rows of its own piece of them
+
+  constexpr int PITCH = WP + 4, LPR = WP / 8, RPP = 64 / LPR;         // floats per row, lanes per row, rows per pass
+  const int lane = threadIdx.x & 63;
+  float* const turn = reinterpret_cast<float*>(lds) + wave * 16 * PITCH;
+  const int col = p0 + wp * WP + (lane % LPR) * 8, left = a.N - col;
+  float b[8], ps[8];
+  if (a.splits == 1) epilogue_columns(a.e, col, left, b, ps);
+#pragma unroll
+  for (int j = 0; j < TQ; ++j) {
+#pragma unroll
+    for (int i = 0; i < TP; ++i)
+      *reinterpret_cast<f32x4*>(turn + (lane & 15) * PITCH + i * 16 + (lane >> 4) * 4) = acc[i][j];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (int k = 0; k < 16 / RPP; ++k) {
+      const int r = k * RPP + lane / LPR, row = q0 + wq * WQ + j * 16 + r;
+      const f32x4 v0 = *reinterpret_cast<const f32x4*>(turn + r * PITCH + (lane % LPR) * 8);
+      const f32x4 v1 = *reinterpret_cast<const f32x4*>(turn + r * PITCH + (lane % LPR) * 8 + 4);
+      if (row < a.M && left > 0) {
+        const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+        if (a.splits == 1) {
+          epilogue8(a.e, v, row, col, left, b, ps);
+        } else {
+          float* const w = a.ws + ((size_t)part * a.M + row) * a.ldw + col;      // ldw is a multiple of 8
+          *reinterpret_cast<f32x4*>(w) = v0;
+          *reinterpret_cast<f32x4*>(w + 4) = v1;
+        }
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// the parts of a divided sum, added in order, and what follows the product
+__global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a) {
+  const int per_row = (a.N + 7) / 8;
+  const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= (size_t)a.M * per_row) return;
+  const int row = (int)(id / per_row), col = (int)(id % per_row) * 8;
+  const float* w = a.ws + (size_t)row * a.ldw + col;
+  float v[8] = {};
+#pragma unroll 4
+  for (int s = 0; s < a.splits; ++s, w += (size_t)a.M * a.ldw) {
+    const f32x4 x = *reinterpret_cast<const f32x4*>(w), y = *reinterpret_cast<const f32x4*>(w + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] += x[i]; v[4 + i] += y[i]; }
+  }
+  float b[8], ps[8];
+  epilogue_columns(a.e, col, a.N - col, b, ps);
+  epilogue8(a.e, v, row, col, a.N - col, b, ps);
+}
+
+// ---- up to 16 rows: the weight is read once, straight into registers ------------------------------------------------------
+// A workgroup owns 16 columns of the output (16 rows of W); its eight waves take turns along the sum, two 64-byte pieces of each
+// weight row at a time, and meet in shared memory.
+template <typename T>
+__global__ __launch_bounds__(512) void gemv_kernel(const GemmArgs a) {
+  constexpr int ES = sizeof(T), PIECE = 16 / ES, NW = 8, U = 4;
+  __shared__ float red[NW][16][17];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  const int p0 = blockIdx.x * 16;
+  const size_t wbytes = ((size_t)((a.N - p0 < 16 ? a.N - p0 : 16) - 1) * a.ldp + a.R) * ES, xbytes = ((size_t)(a.M - 1) * a.ldq + a.R) * ES;
+  const buf_rsrc rw = make_rsrc((const char*)a.p + (size_t)p0 * a.ldp * ES, (unsigned)wbytes);
+  const buf_rsrc rx = make_rsrc(a.q, (unsigned)xbytes);
+  const unsigned wrow = p0 + i < a.N ? (unsigned)(i * a.ldp * ES) : BUF_OOB, xrow = i < a.M ? (unsigned)(i * a.ldq * ES) : BUF_OOB;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const int stages = (a.R + 8 * PIECE - 1) / (8 * PIECE);          // 128 bytes of a row per stage
+  for (int s = wave; s < stages; s += NW * U) {
+    i32x4 w[U][2], x[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int piece = (s + u * NW) * 8 + h * 4 + g;
+        const bool in = piece * PIECE < a.R;
+        const unsigned off = (unsigned)piece * 16;
+        w[u][h] = __builtin_bit_cast(i32x4, buffer_load_b128(rw, in && wrow != BUF_OOB ? wrow + off : BUF_OOB, 0));
+        x[u][h] = __builtin_bit_cast(i32x4, buffer_load_b128(rx, in && xrow != BUF_OOB ? xrow + off : BUF_OOB, 0));
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if constexpr (ES == 1) {
+        acc = mma8(w[u][0], w[u][1], x[u][0], x[u][1], acc);
+      } else {
+        acc = Mma<T>::run(w[u][0], x[u][0], acc);
+        acc = Mma<T>::run(w[u][1], x[u][1], acc);
+      }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; ++k) red[wave][i][g * 4 + k] = acc[k];          // [row of x][column]
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int row = threadIdx.x >> 1, c = (threadIdx.x & 1) * 8, col = p0 + c;
+    if (row < a.M && col < a.N) {
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        float t = 0.f;
+#pragma unroll
+        for (int wv = 0; wv < NW; ++wv) t += red[wv][row][c + k];
+        v[k] = t;
+      }
+      float b[8], ps[8];
+      epilogue_columns(a.e, col, a.N - col, b, ps);
+      epilogue8(a.e, v, row, col, a.N - col, b, ps);
+    }
+  }
+}
+
+// ---- rows of any width, pitch and offset, laid out again with a pitch of whole 16-byte pieces and zeros behind each row --------
+template <typename T>
+__global__ __launch_bounds__(256) void pack_rows_kernel(const T* const src, const size_t ld, T* const dst, const int cols, const int ldd, const size_t rows) {
+  const int per = ldd * (int)sizeof(T) / 16, PIECE = 16 / (int)sizeof(T);
+  const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (id >= rows * per) return;
+  const size_t row = id / per;
+  const int c = (int)(id - row * per) * PIECE;
+  T v[16 / sizeof(T)];
+#pragma unroll
+  for (int i = 0; i < 16 / (int)sizeof(T); ++i) v[i] = c + i < cols ? src[row * ld + c + i] : T(0);
+  __builtin_memcpy(__builtin_assume_aligned(dst + row * ldd + c, 16), v, 16);
+}
+
+// ---- dz = dy act'(z) with a pitch of whole pieces, and the column sums of each workgroup's rows (db) ----------------------------
+struct DzArgs {
+  const void* dy;
+  const unsigned short* d;        // or NULL: no activation
+  void* dz;                       // or NULL: only the sums
+  float* partial;                 // [gridDim.y][N] or NULL
+  size_t rows, lddy, ldd, lddz;
+  int N, vec;
+};
+template <typename T, int L>
+__global__ __launch_bounds__(256) void dz_kernel(const DzArgs a) {
+  constexpr int G = 256 / L;
+  const int lane = threadIdx.x & (L - 1), grp = threadIdx.x / L;
+  const int col = (blockIdx.x * L + lane) * 8, left = a.N - col;
+  float sum[8] = {};
+  if (left > 0) {
+    for (size_t row = (size_t)blockIdx.y * G + grp; row < a.rows; row += (size_t)gridDim.y * G) {
+      float v[8];
+      load8((const T*)a.dy + row * a.lddy + col, left, a.vec, v);
+      if (a.d) {
+        const u16x8 c = *reinterpret_cast<const u16x8*>(a.d + row * a.ldd + col);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < left ? v[i] * act_slope(c[i]) : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += v[i];
+      if (a.dz) store8((T*)a.dz + row * a.lddz + col, 8, true, v);           // zeros behind the last column
+    }
+  }
+  if (!a.partial) return;
+  __shared__ float red[G][L * 8 + 1];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[grp][lane * 8 + i] = sum[i];
+  __syncthreads();
+  for (int c = threadIdx.x; c < L * 8; c += 256) {
+    const int n = blockIdx.x * L * 8 + c;
+    float t = 0.f;
+    for (int g = 0; g < G; ++g) t += red[g][c];
+    if (n < a.N) a.partial[(size_t)blockIdx.y * a.N + n] = t;
+  }
+}
+
+inline int dz_lanes(const int N) { return N <= 64 ? 8 : N <= 128 ? 16 : N <= 256 ? 32 : 64; }
+inline int dz_groups(const size_t rows, const int N) {
+  const int L = dz_lanes(N), cols = (N + L * 8 - 1) / (L * 8);
+  size_t g = (rows + 256 / L - 1) / (256 / L);
+  const size_t most = 2048 / cols < 64 ? 64 : 2048 / cols;
+  return (int)(g < most ? g : most);
+}
+
+// ---- which tile, and how many parts of the sum ---------------------------------------------------------------------------------
+struct Plan { int tile, splits, per; };
+inline Plan gemm_plan(const int M, const int N, const int R, const int es) {
+  const int stages = (int)(((long)R * es + 127) / 128);
+  const auto tiles = [&](const int b) { return (long)((M + b - 1) / b) * ((N + b - 1) / b); };
+  Plan p{256, 1, stages};
+  if (tiles(256) < 192 || stages < 4) p.tile = 128;
+  if (p.tile == 128 && tiles(128) < 192) p.tile = 64;
+  const long t = tiles(p.tile);
+  if (t < 256 && stages > 8) {                     // too few tiles for 256 compute units: divide the sum, at least 4 stages a part
+    long s = (512 + t - 1) / t;
+    if (s > stages / 4) s = stages / 4;
+    if (s > 256) s = 256;
+    p.splits = s < 1 ? 1 : (int)s;
+  }
+  p.per = (stages + p.splits - 1) / p.splits;
+  if (p.per < 1) p.per = 1;
+  p.splits = (stages + p.per - 1) / p.per;
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+inline size_t up8(const size_t n) { return (n + 7) & ~(size_t)7; }
+
+template <typename T, bool QX, bool PX, int BQ, int BP, int NQ, int NP>
+hipError_t gemm_go(const GemmArgs& a, hipStream_t s) {
+  static std::atomic<unsigned long long> optin{0};
+  constexpr int stage = (BQ + BP) * 128 * 2, turn = NQ * NP * 16 * (BP / NP + 4) * 4, bytes = stage > turn ? stage : turn;
+  const void* const fn = reinterpret_cast<const void*>(&gemm_kernel<T, QX, PX, BQ, BP, NQ, NP>);
+  if (const hipError_t e = lds_optin(fn, bytes, optin); e != hipSuccess) return e;
+  const long wgs = (long)((a.M + BQ - 1) / BQ) * ((a.N + BP - 1) / BP) * a.splits;
+  hipLaunchKernelGGL((gemm_kernel<T, QX, PX, BQ, BP, NQ, NP>), dim3((unsigned)wgs), dim3(NQ * NP * 64), bytes, s, a);
+  return hipGetLastError();
+}
+template <typename T, bool QX, bool PX>
+int gemm_run(GemmArgs a, hipStream_t s) {
+  const Plan p = gemm_plan(a.M, a.N, a.R, sizeof(T));
+  a.splits = p.splits;
+  a.per = p.per;
+  a.ldw = up8(a.N);
+  if (p.splits > 1 && !a.ws) return SELFC_EINVAL;
+  hipError_t e;
+  if (p.tile == 256) e = gemm_go<T, QX, PX, 256, 256, 4, 2>(a, s);
+  else if (p.tile == 128) e = gemm_go<T, QX, PX, 128, 128, 2, 2>(a, s);
+  else e = gemm_go<T, QX, PX, 64, 64, 2, 2>(a, s);
+  if (e != hipSuccess) return pw_rc(e);
+  if (p.splits > 1) {
+    const size_t n = (size_t)a.M * ((a.N + 7) / 8);
+    hipLaunchKernelGGL(gemm_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+    return pw_rc(hipGetLastError());
+  }
+  return SELFC_OK;
+}
+
+constexpr int GEMV_ROWS = 16;
+// shapes whose offsets the kernels hold: 32-bit within a tile, 32-bit numbers of workgroups
+inline bool lin_shape(const size_t M, const int N, const int K) {
+  return M <= 0x3fffffff && N >= 1 && K >= 1 && N <= (1 << 20) && K <= (1 << 20) && (M / 64 + 1) * ((size_t)N / 64 + 1) < (1u << 28);
+}
+inline bool rows_fit(const void* p, const size_t ld, const size_t cols, const size_t es) {     // whole pieces at aligned places
+  return aligned_to(p, 16) && (ld * es) % 16 == 0 && (cols * es) % 16 == 0 && ld < (1u << 21);
+}
+
+Epilogue make_epilogue(void* out, size_t ldo, const void* bias, const void* res, size_t ldr, int dtype, int act, int N) {
+  Epilogue e{};
+  const size_t es = dtype ? 2 : 4;
+  e.out = out; e.bias = bias; e.res = res; e.ldo = ldo; e.ldr = ldr; e.dtype = dtype; e.act = act;
+  e.vec = N % 8 == 0 && aligned_to(out, 16) && (ldo * es) % 16 == 0 && (!res || (aligned_to(res, 16) && (ldr * es) % 16 == 0));
+  return e;
+}
+
+}  // namespace
+}  // namespace selfc
+
+using namespace selfc;
+
+extern "C" {
+
+size_t selfc_linear_ws_floats(size_t rows, int cols, int sum, int elem_bytes) {
+  if (rows < 1 || rows > 0x3fffffff || cols < 1 || sum < 1) return 0;
+  const Plan p = gemm_plan((int)rows, cols, sum, elem_bytes);
+  return p.splits > 1 ? (size_t)p.splits * rows * up8(cols) : 0;
+}
+
+int selfc_pack_rows(const void* src, size_t ld, void* dst, size_t rows, int cols, int ldd, int elem_bytes, void* stream) {
+  if (!src || !dst || cols < 1 || ldd < cols || (elem_bytes != 1 && elem_bytes != 2) || (ldd * elem_bytes) % 16 || !aligned_to(dst, 16)) return SELFC_EINVAL;
+  if (rows == 0) return SELFC_OK;
+  const size_t n = rows * (size_t)(ldd * elem_bytes / 16);
+  if ((n + 255) / 256 > 0x7fffffffull) return SELFC_EINVAL;
+  const dim3 grid((unsigned)((n + 255) / 256)), blk(256);
+  if (elem_bytes == 2) hipLaunchKernelGGL((pack_rows_kernel<unsigned short>), grid, blk, 0, (hipStream_t)stream, (const unsigned short*)src, ld, (unsigned short*)dst, cols, ldd, rows);
+  else hipLaunchKernelGGL((pack_rows_kernel<unsigned char>), grid, blk, 0, (hipStream_t)stream, (const unsigned char*)src, ld, (unsigned char*)dst, cols, ldd, rows);
+  return pw_rc(hipGetLastError());
+}
+
+int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const float* x_scale, const float* w_scale, const void* bias, int act,
+                 const void* res, size_t ldr, void* y, void* slope, float* ws, size_t rows, int n, int k, int in_dtype, int out_dtype, void* stream) {
+  if (rows == 0) return SELFC_OK;
+  if (!x || !w || !y || !lin_shape(rows, n, k) || act < ACT_NONE || act > ACT_SILU || in_dtype < 1 || in_dtype > 3 || out_dtype < 0 || out_dtype > 2) return SELFC_EINVAL;
+  const bool q8 = in_dtype == 3;
+  if (q8 != (x_scale != nullptr) || q8 != (w_scale != nullptr) || (!q8 && in_dtype != out_dtype) || (slope && q8)) return SELFC_EINVAL;
+  const size_t es = q8 ? 1 : 2;
+  if (!rows_fit(x, ldx, k, es) || !rows_fit(w, ldw, k, es)) return SELFC_EINVAL;                 // selfc_pack_rows first
+  if ((rows > 1 && ldx < (size_t)k) || (n > 1 && ldw < (size_t)k) || (res && rows > 1 && ldr < (size_t)n)) return SELFC_EINVAL;
+  GemmArgs a{};
+  a.q = x; a.p = w; a.ldq = ldx; a.ldp = ldw; a.M = (int)rows; a.N = n; a.R = k; a.ws = ws;
+  a.e = make_epilogue(y, n, bias, res, ldr, out_dtype, act, n);
+  a.e.qs = x_scale; a.e.ps = w_scale; a.e.d = (unsigned short*)slope; a.e.ldd = up8(n);
+  hipStream_t s = (hipStream_t)stream;
+  if (rows <= GEMV_ROWS) {
+    a.splits = 1;
+    const dim3 grid((n + 15) / 16), blk(512);
+    if (q8) hipLaunchKernelGGL((gemv_kernel<unsigned char>), grid, blk, 0, s, a);
+    else if (in_dtype == 1) hipLaunchKernelGGL((gemv_kernel<b16>), grid, blk, 0, s, a);
+    else hipLaunchKernelGGL((gemv_kernel<h16>), grid, blk, 0, s, a);
+    return pw_rc(hipGetLastError());
+  }
+  if (q8) return gemm_run<unsigned char, false, false>(a, s);
+  return in_dtype == 1 ? gemm_run<b16, false, false>(a, s) : gemm_run<h16, false, false>(a, s);
+}
+
+size_t selfc_linear_dz_floats(size_t rows, int n) { return n < 1 ? 1 : (size_t)(dz_groups(rows, n) + 1) * n; }
+
+int selfc_linear_dz(const void* dy, size_t lddy, const void* slope, void* dz, size_t lddz, void* db, float* partial, size_t rows, int n, int dtype, void* stream) {
+  if (!dy || n < 1 || (dtype != 1 && dtype != 2) || (db && !partial) || (!dz && !db) || rows > 0x3fffffff) return SELFC_EINVAL;
+  if (dz && (!aligned_to(dz, 16) || lddz % 8 || lddz < up8(n))) return SELFC_EINVAL;
+  if (slope && !aligned_to(slope, 16)) return SELFC_EINVAL;
+  DzArgs a{};
+  a.dy = dy; a.d = (const unsigned short*)slope; a.dz = dz; a.partial = db ? partial : nullptr; a.rows = rows; a.lddy = lddy; a.ldd = up8(n); a.lddz = lddz; a.N = n;
+  a.vec = n % 8 == 0 && aligned_to(dy, 16) && lddy % 8 == 0;
+  hipStream_t s = (hipStream_t)stream;
+  const int L = dz_lanes(n), groups = dz_groups(rows, n);
+  if (groups) {
+    const dim3 grid((n + L * 8 - 1) / (L * 8), groups), blk(256);
+#define DZ(L_)                                                                       \
+  if (dtype == 1) hipLaunchKernelGGL((dz_kernel<b16, L_>), grid, blk, 0, s, a);      \
+  else hipLaunchKernelGGL((dz_kernel<h16, L_>), grid, blk, 0, s, a)
+    if (L == 8) { DZ(8); }
+    else if (L == 16) { DZ(16); }
+    else if (L == 32) { DZ(32); }
+    else { DZ(64); }
+#undef DZ
+    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return pw_rc(e);
+  }
+  return db ? pw_colsum(partial, groups, n, dtype, db, s) : SELFC_OK;
+}
+
+int selfc_linear_dx(const void* dz, size_t lddz, const void* w, size_t ldw, void* dx, float* ws, size_t rows, int n, int k, int dtype, void* stream) {
+  if (rows == 0) return SELFC_OK;
+  if (!dz || !w || !dx || !lin_shape(rows, k, n) || (dtype != 1 && dtype != 2)) return SELFC_EINVAL;
+  if (!rows_fit(dz, lddz, up8(n), 2) || lddz < up8(n) || !rows_fit(w, ldw, up8(k), 2) || ldw < up8(k)) return SELFC_EINVAL;
+  GemmArgs a{};
+  a.q = dz; a.p = w; a.ldq = lddz; a.ldp = ldw; a.M = (int)rows; a.N = k; a.R = n; a.px = (int)up8(k); a.ws = ws;
+  a.e = make_epilogue(dx, k, nullptr, nullptr, 0, dtype, ACT_NONE, k);
+  return dtype == 1 ? gemm_run<b16, false, true>(a, (hipStream_t)stream) : gemm_run<h16, false, true>(a, (hipStream_t)stream);
+}
+
+int selfc_linear_dw(const void* dz, size_t lddz, const void* x, size_t ldx, void* dw, float* ws, size_t rows, int n, int k, int dtype, void* stream) {
+  if (!dz || !x || !dw || !lin_shape(n, k, 1) || rows < 1 || rows > 0x3fffffff || (dtype != 1 && dtype != 2)) return SELFC_EINVAL;
+  if (!rows_fit(dz, lddz, up8(n), 2) || lddz < up8(n) || !rows_fit(x, ldx, up8(k), 2) || ldx < up8(k)) return SELFC_EINVAL;
+  GemmArgs a{};
+  a.q = dz; a.p = x; a.ldq = lddz; a.ldp = ldx; a.M = n; a.N = k; a.R = (int)rows; a.qx = (int)up8(n); a.px = (int)up8(k); a.ws = ws;
+  a.e = make_epilogue(dw, k, nullptr, nullptr, 0, dtype, ACT_NONE, k);
+  return dtype == 1 ? gemm_run<b16, true, true>(a, (hipStream_t)stream) : gemm_run<h16, true, true>(a, (hipStream_t)stream);
+}
+
+}  // extern "C"

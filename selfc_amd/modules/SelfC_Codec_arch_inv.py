@@ -25,7 +25,7 @@ from .Quantization import Quantization
 from .SelfC_GMM_arch_inv import FrequencyAnalyzer as _FrequencyAnalyzer
 from .SelfC_GMM_arch_inv import GlobalAgg as _GlobalAgg
 from .SelfC_GMM_arch_inv import STPNet as _STPNetV2
-from .Subnet_constructor import D2DTInput, subnet
+from .Subnet_constructor import D2DTInput, refuse_ffnet, subnet
 
 TEMP_LEN = 3        # SelfC_Codec_arch_inv.py:77
 
@@ -123,6 +123,7 @@ class SelfCInvNet(nn.Module):
         super().__init__()
         operations = [FrequencyAnalyzer(channel_in, 2)]
         current_channel = channel_in * (2 ** 2 + 1)
+        refuse_ffnet(subnet_type)
         sc = subnet(subnet_type, "xavier")
         for i in range(down_num):
             for _ in range(block_num[i]):

@@ -13,7 +13,7 @@ from .. import _lib, runtime as rt
 from ..global_var import GlobalVar
 from .module_util import HeadOutput, cache_free_state
 from .Inv_arch import InvBlockExp  # noqa: F401  (same class, as in the reference's three copies)
-from .Subnet_constructor import D2DTInput, subnet
+from .Subnet_constructor import D2DTInput, refuse_ffnet, subnet
 
 
 class PixelUnshuffle(nn.Module):
@@ -517,6 +517,7 @@ class SelfCInvNet(nn.Module):
         super().__init__()
         operations = [FrequencyAnalyzer(channel_in)]
         current_channel = channel_in * 17
+        refuse_ffnet(subnet_type)
         sc = subnet(subnet_type, "xavier")
         for i in range(down_num):
             for _ in range(block_num[i]):

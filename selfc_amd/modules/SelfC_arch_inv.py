@@ -18,7 +18,7 @@ from .. import _lib, runtime as rt
 from ..global_var import GlobalVar
 from .module_util import HeadOutput, cache_free_state
 from .Inv_arch import HaarDownsampling, InvBlockExp
-from .Subnet_constructor import D2DTInput, FeatureCalapseBlock, subnet
+from .Subnet_constructor import D2DTInput, FeatureCalapseBlock, refuse_ffnet, subnet
 
 TEMP_LEN = 7
 
@@ -169,6 +169,7 @@ class SelfCInvNet(nn.Module):
         super().__init__()
         operations = []
         current_channel = channel_in
+        refuse_ffnet(subnet_type)
         sc = subnet(subnet_type, "xavier")
         for i in range(down_num):
             operations.append(HaarDownsampling(current_channel))

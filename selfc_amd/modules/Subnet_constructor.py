@@ -229,9 +229,92 @@ class FeatureCalapseBlock(nn.Module):
         return y + res if self.is_res else y
 
 
+class FFNet(nn.Module):
+    __getstate__ = cache_free_state
+    """Per-pixel residual feed-forward subnet (no counterpart in the reference): a product into `width` channels, `depth` layers of
+    [norm, product into 4 x width with GELU, product back] around a residual stream, and a normed product out - on the operators of
+    selfc_amd/pointwise.py, in the library's operand type (f16 or bf16) with fp32 parameters; differentiable.
+
+    The receptive field is one pixel: for splits whose channels hold the neighbourhood already (HaarDownsampling, FrequencyAnalyzer).
+    It takes any channel counts.  `serve_bits = 8` (an attribute; without gradients only): the layers' norms write e4m3 rows and their
+    products run on e4m3 weights, which are made once per version of the parameters."""
+    kind = None                 # not one of the dense-block kernels: InvBlockExp composes it (_forward_composed)
+
+    def __init__(self, channel_in, channel_out, init='xavier', width=64, depth=2, INN_init=True):
+        super().__init__()
+        if width % 8 or width < 8 or depth < 1:
+            raise NotImplementedError("FFNet: width is a positive multiple of 8, depth at least 1")
+        self.channel_in, self.channel_out, self.width = channel_in, channel_out, width
+        self.inp = nn.Linear(channel_in, width)
+        self.norms = nn.ParameterList([nn.Parameter(torch.ones(width)) for _ in range(depth + 1)])
+        self.up = nn.ModuleList([nn.Linear(width, 4 * width) for _ in range(depth)])
+        self.down = nn.ModuleList([nn.Linear(4 * width, width) for _ in range(depth)])
+        self.out = nn.Linear(width, channel_out)
+        (mutil.initialize_weights_xavier if init == 'xavier' else mutil.initialize_weights)([self.inp, *self.up, *self.down], 1)
+        if INN_init:
+            mutil.initialize_weights(self.out, 0)          # identity coupling at the start
+        self.serve_bits = 16
+
+    def forward(self, x):
+        x = rt.as_input(x)
+        n, c, h, w = x.shape
+        if c != self.channel_in:
+            raise RuntimeError(f"expected {self.channel_in} input channels, got {c}")
+        if self.serve_bits not in (8, 16):
+            raise RuntimeError(f"FFNet.serve_bits is {self.serve_bits}, expected 8 or 16")
+        rows = x.permute(0, 2, 3, 1).reshape(n * h * w, c).to(_lib.operand_dtype())
+        y = self._run_rows(rows)
+        return y.view(n, h, w, self.channel_out).permute(0, 3, 1, 2).to(torch.float32, memory_format=torch.contiguous_format)
+
+    def _run_rows(self, rows):
+        from .. import autograd as ag, pointwise as pw
+        dt = rows.dtype
+        train = ag.module_needs_grad(rows, self)
+        if train and self.serve_bits == 8:
+            raise NotImplementedError("FFNet: serve_bits = 8 has no gradients - set it to 16 to train")
+        ps = self._cast(dt) if train else self._laid_out(dt)
+        h = pw.linear(rows, ps["inp.w"], bias=ps["inp.b"])
+        d = None                 # what the last layer adds to the stream
+        for i in range(len(self.up)):
+            if self.serve_bits == 8 and not train:
+                q, s, h = pw.rms_norm_q8(h if d is None else d, ps[f"norm{i}"], residual=None if d is None else h)
+                u = pw.linear_q8(q, s, *ps[f"up{i}.q"], bias=ps[f"up{i}.b"], act="gelu", out_dtype=dt)
+            else:
+                y, h = pw.rms_norm(h if d is None else d, ps[f"norm{i}"], residual=None if d is None else h)
+                u = pw.linear(y, ps[f"up{i}.w"], bias=ps[f"up{i}.b"], act="gelu")
+            d = pw.linear(u, ps[f"down{i}.w"], bias=ps[f"down{i}.b"])
+        y, _ = pw.rms_norm(d, ps[f"norm{len(self.up)}"], residual=h)
+        return pw.linear(y, ps["out.w"], bias=ps["out.b"])
+
+    def _cast(self, dt):
+        """the parameters as the operators take them (differentiable)"""
+        ps = {f"norm{i}": p for i, p in enumerate(self.norms)}
+        for name, m in [("inp", self.inp), ("out", self.out)] + [(f"{k}{i}", m) for k in ("up", "down") for i, m in enumerate(getattr(self, k))]:
+            ps[name + ".w"], ps[name + ".b"] = m.weight.to(dt), m.bias.to(dt)
+        return ps
+
+    def _laid_out(self, dt):
+        key = (dt, self.serve_bits) + rt.params_key(self)
+        if getattr(self, "_ff_key", None) != key:
+            from .. import pointwise as pw
+            with torch.no_grad():
+                self._ff = self._cast(dt)
+                if self.serve_bits == 8:
+                    for i, m in enumerate(self.up):
+                        self._ff[f"up{i}.q"] = pw.quantize_rows(m.weight)
+            self._ff_key = key
+        return self._ff
+
+
+def refuse_ffnet(subnet_type):
+    """For the nets whose blocks run in the dense-block kernels' latent layout."""
+    if subnet_type == 'FFNet':
+        raise NotImplementedError("selfc_amd: this net runs its blocks in the dense-block kernels' layout; FFNet composes with InvBlockExp and InvRescaleNet")
+
+
 def subnet(net_structure, init='xavier'):
     """String-keyed factory, Subnet_constructor.py:719-788.  Live names: 'DBNet', 'D2DTNet' and 'FeatureCalapseBlock'
-    (:731-735); any other name returns None exactly like the reference (it then fails at first use)."""
+    (:731-735) and, beyond the reference's, 'FFNet'; any other name returns None exactly like the reference (it then fails at first use)."""
     def constructor(channel_in, channel_out, gc=32):
         if net_structure == 'DBNet':
             return DenseBlock(channel_in, channel_out, init) if init == 'xavier' else DenseBlock(channel_in, channel_out)
@@ -243,6 +326,8 @@ def subnet(net_structure, init='xavier'):
             if init == 'xavier':
                 return D2DTInput(channel_in, channel_out, init, gc=gc)
             return D2DTInput(channel_in, channel_out)
+        if net_structure == 'FFNet':
+            return FFNet(channel_in, channel_out, init, width=2 * gc)
         return None
 
     return constructor

@@ -1,0 +1,331 @@
+"""Norm and products of per-pixel (or per-token) rows on the kernels of csrc/rmsnorm.hip and csrc/linear.hip.
+
+    y, h = rms_norm(x, weight, residual=r)            h = x + r,  y = h / rms(h) * weight            (differentiable)
+    q, s, h = rms_norm_q8(x, weight, residual=r)      the same with y as e4m3 and a scale per row
+    y = linear(x, w, bias, act="gelu", residual=r)    y = act(x w^T + bias) + r                      (differentiable)
+    y = linear_q8(q, s, wq, ws, ...)                  the same on e4m3 rows and an e4m3 weight (quantize_rows)
+
+The last axis is the row; leading axes may be any.  Rows may have any length, pitch and offset: rows that the kernels cannot read
+in 16-byte pieces are laid out again first (one more launch; widths that are multiples of 8 - of 16 in 8 bits - avoid it).
+Everything runs on the current stream of the tensors' device, allocates from torch's allocator only, and may be captured into a
+graph.  As for every torch module, a backward pass is captured only when no eager graph over the same leaves is alive any more
+(drop the losses of the eager steps first); such a capture is refused here (autograd would end the process).
+Refused with an exception: tensors that are not on one GPU, types other than the ones named, shapes that do not match.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from contextlib import nullcontext
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib, runtime as rt
+
+#: activations of `linear`, by their number in the C ABI
+ACTS = {"none": 0, None: 0, "relu": 1, "lrelu": 2, "gelu": 3, "silu": 4}
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float8_e4m3fn: 3}
+_NAMES = {torch.float32: "float32", torch.bfloat16: "bfloat16", torch.float16: "float16", torch.float8_e4m3fn: "float8_e4m3fn"}
+MAX_NORM_COLS = 16384
+MAX_LINEAR = 1 << 20
+E4M3_MAX = 448.0
+
+
+def on_device(t: torch.Tensor):
+    """The tensor's device as the current one for the duration of a launch."""
+    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _need(cond, what: str):
+    if not cond:
+        raise RuntimeError("selfc_amd: " + what)
+
+
+def _same_device(first: torch.Tensor, **others):
+    _lib.require_gpu(first)
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise RuntimeError(f"selfc_amd: {name} is on {t.device}, the rows are on {first.device}")
+
+
+def _typed(name: str, t: torch.Tensor, *dtypes):
+    if t.dtype not in dtypes:
+        raise RuntimeError(f"selfc_amd: {name} is {t.dtype}, expected {' or '.join(_NAMES[d] for d in dtypes)}")
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """(..., C) as a matrix whose rows are contiguous and do not overlap (a view where one exists)."""
+    t = t.reshape(-1, t.shape[-1])
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t
+
+
+def _pitch(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+
+
+def _pieces(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """(matrix, pitch) that the product's kernels can read: 16-byte aligned rows of whole 16-byte pieces."""
+    es, (rows, cols) = t.element_size(), t.shape
+    per = 16 // es
+    ld = _pitch(t)
+    if t.data_ptr() % 16 == 0 and cols % per == 0 and (rows == 1 or ld % per == 0) and ld < (1 << 21):
+        return t, ld if rows > 1 else cols
+    ldd = -(-cols // per) * per
+    out = torch.empty((rows, ldd), dtype=t.dtype, device=t.device)
+    rt.call("selfc_pack_rows", t.data_ptr(), ld, out.data_ptr(), rows, cols, ldd, es, _lib.stream_ptr())
+    return out, ldd
+
+
+def _ws(rows: int, cols: int, total: int, es: int, device) -> Optional[torch.Tensor]:
+    n = _lib.lib().selfc_linear_ws_floats(rows, cols, total, es)
+    return torch.empty(n, dtype=torch.float32, device=device) if n else None
+
+
+_ptr = rt._ptr
+
+# -- captured backward passes ----------------------------------------------------------------------------------------------------
+_EAGER = "selfc_amd_eager_graph"
+
+
+def _watch_leaves(*tensors):
+    """A leaf's gradient accumulator lives as long as a graph that reaches it and remembers the stream it was made on.  If an eager
+    graph is still alive when a captured backward pass reaches the same leaf, autograd waits for that stream inside the capture and
+    the process ends.  So: accumulators that an eager call reaches are marked, and a call under capture that meets one refuses."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    for t in tensors:
+        if t is not None and t.requires_grad and t.is_leaf:
+            meta = torch.autograd.graph.get_gradient_edge(t).node.metadata
+            if not capturing:
+                meta[_EAGER] = torch.cuda.current_stream(t.device).cuda_stream
+            elif meta.get(_EAGER, None) not in (None, torch.cuda.current_stream(t.device).cuda_stream):
+                raise RuntimeError("selfc_amd: a graph of an earlier eager call over the same parameters is still alive; its gradients cannot "
+                                   "be accumulated inside a capture - drop that call's outputs and losses first")
+
+
+# -- norm ------------------------------------------------------------------------------------------------------------------------
+def _norm_args(x, weight, residual, eps):
+    _same_device(x, weight=weight, residual=residual)
+    _typed("x", x, torch.bfloat16, torch.float16, torch.float32)
+    _typed("weight", weight, *{x.dtype, torch.float32})
+    _need(x.dim() >= 1 and 1 <= x.shape[-1] <= MAX_NORM_COLS, f"rms_norm takes rows of 1 to {MAX_NORM_COLS} values, got {tuple(x.shape)}")
+    _need(weight.shape == (x.shape[-1],), f"weight has shape {tuple(weight.shape)}, the rows have {x.shape[-1]} values")
+    _need(eps >= 0, f"eps is {eps}")
+    if residual is not None:
+        _typed("residual", residual, x.dtype)
+        _need(residual.shape == x.shape, f"residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
+
+
+def _run_norm(x2, r2, weight, eps, q8: bool):
+    rows, cols = x2.shape
+    dev = x2.device
+    y = torch.empty((rows, cols), dtype=torch.float8_e4m3fn if q8 else x2.dtype, device=dev)
+    scale = torch.empty(rows, dtype=torch.float32, device=dev) if q8 else None
+    h = torch.empty((rows, cols), dtype=x2.dtype, device=dev) if r2 is not None else None
+    if rows:
+        rt.call("selfc_rmsnorm", x2.data_ptr(), _pitch(x2), _ptr(r2), 0 if r2 is None else _pitch(r2), weight.data_ptr(),
+                int(weight.dtype == torch.float32), _ptr(h), y.data_ptr(), _ptr(scale), rows, cols, _DTYPE[x2.dtype], eps, _lib.stream_ptr())
+    return y, scale, h
+
+
+class RMSNormFn(torch.autograd.Function):
+    """rms_norm on matrices; the gradient needs h and the weight only (the row's statistic is recomputed)."""
+
+    @staticmethod
+    def forward(ctx, x2, r2, weight, eps):
+        with on_device(x2):
+            y, _, h = _run_norm(x2, r2, weight, eps, False)
+        ctx.eps = eps
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x2 if h is None else h, weight)
+        return (y,) if h is None else (y, h)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight = ctx.saved_tensors
+        want_w = ctx.needs_input_grad[2]
+        want_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        if dy is None:                     # only h was used
+            return (dh if ctx.needs_input_grad[0] else None), (dh if ctx.needs_input_grad[1] else None), None, None
+        rows, cols = h.shape
+        dy = dy.contiguous()
+        dh = dh.contiguous() if dh is not None else None
+        with on_device(h):
+            dx = torch.empty((rows, cols), dtype=h.dtype, device=h.device) if want_x else None
+            dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if want_w else None
+            part = torch.empty(_lib.lib().selfc_rmsnorm_bwd_floats(rows, cols), dtype=torch.float32, device=h.device) if want_w else None
+            if rows:
+                rt.call("selfc_rmsnorm_bwd", h.data_ptr(), _pitch(h), weight.data_ptr(), int(weight.dtype == torch.float32), dy.data_ptr(), _ptr(dh),
+                        _ptr(dx), _ptr(dw), _ptr(part), rows, cols, _DTYPE[h.dtype], ctx.eps, _lib.stream_ptr())
+            elif dw is not None:
+                dw.zero_()
+        return (dx if ctx.needs_input_grad[0] else None), (dx if ctx.needs_input_grad[1] else None), dw, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(y, h): h = x + residual rounded to x's type (x itself without a residual), y = h / sqrt(mean(h^2) + eps) * weight.
+
+    x: bf16, f16 or fp32 rows of up to 16,384 values; weight: x's type or fp32.  Statistics and the weight's gradient are summed in
+    fp32 in a fixed order.  Gradients flow to x, residual and weight, from y and h."""
+    _norm_args(x, weight, residual, eps)
+    weight = weight.contiguous()
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
+        _watch_leaves(x, residual, weight)
+        out = RMSNormFn.apply(_rows(x), None if residual is None else _rows(residual), weight, float(eps))
+        return out[0].view(x.shape), (x if residual is None else out[1].view(x.shape))
+    with on_device(x):
+        y, _, h = _run_norm(_rows(x), None if residual is None else _rows(residual), weight, float(eps), False)
+    return y.view(x.shape), (x if h is None else h.view(x.shape))
+
+
+def _no_grad_only(what: str, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise NotImplementedError(f"selfc_amd: {what} serves only - call it under torch.no_grad() (its 16-bit form has gradients)")
+
+
+def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6):
+    """(q, scale, h): rms_norm with y as float8_e4m3fn, y = q * scale[row] (fp32; the row's largest |y| is 448 steps, a row of zeros has
+    scale 1).  For serving: no gradients."""
+    _norm_args(x, weight, residual, eps)
+    _no_grad_only("rms_norm_q8", x, weight, residual)
+    with on_device(x):
+        q, scale, h = _run_norm(_rows(x), None if residual is None else _rows(residual), weight.contiguous(), float(eps), True)
+    return q.view(x.shape), scale.view(x.shape[:-1]), (x if h is None else h.view(x.shape))
+
+
+# -- product ---------------------------------------------------------------------------------------------------------------------
+def _linear_args(x, weight, bias, act, residual, *dtypes, out_dtype=None):
+    _same_device(x, weight=weight, bias=bias, residual=residual)
+    _typed("x", x, *dtypes)
+    _typed("weight", weight, x.dtype)
+    _need(weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1] and weight.shape[0] >= 1 and weight.shape[1] >= 1,
+          f"x {tuple(x.shape)} does not go with weight {tuple(weight.shape)} (out, in)")
+    _need(max(weight.shape) <= MAX_LINEAR, f"weight {tuple(weight.shape)}: at most {MAX_LINEAR} inputs and outputs")
+    out_dtype = out_dtype or x.dtype
+    if act not in ACTS:
+        raise RuntimeError(f"selfc_amd: act is {act!r}, expected one of {sorted(k for k in ACTS if k)}")
+    if bias is not None:
+        _typed("bias", bias, out_dtype)
+        _need(bias.shape == (weight.shape[0],), f"bias has shape {tuple(bias.shape)}, expected ({weight.shape[0]},)")
+    if residual is not None:
+        _typed("residual", residual, out_dtype)
+        _need(residual.shape == x.shape[:-1] + (weight.shape[0],), f"residual has shape {tuple(residual.shape)}, expected {tuple(x.shape[:-1]) + (weight.shape[0],)}")
+
+
+def _run_linear(xp, ldx, k, wp, ldw, n, xs, ws_, bias, act, r2, out_dtype, want_slope):
+    rows, dev = xp.shape[0], xp.device
+    y = torch.empty((rows, n), dtype=out_dtype, device=dev)
+    slope = torch.empty((rows, -(-n // 8) * 8), dtype=torch.int16, device=dev) if want_slope else None
+    if rows:
+        per = 16 // xp.element_size()
+        work = _ws(rows, n, -(-k // per) * per, xp.element_size(), dev)
+        rt.call("selfc_linear", xp.data_ptr(), ldx, wp.data_ptr(), ldw, _ptr(xs), _ptr(ws_), _ptr(bias), act, _ptr(r2),
+                0 if r2 is None else _pitch(r2), y.data_ptr(), _ptr(slope), _ptr(work), rows, n, -(-k // per) * per, _DTYPE[xp.dtype], _DTYPE[out_dtype],
+                _lib.stream_ptr())
+    return y, slope
+
+
+class LinearFn(torch.autograd.Function):
+    """linear on matrices.  Kept for the backward pass: x and the weight as the kernels read them, and the activation's derivative
+    as 16-bit fixed point."""
+
+    @staticmethod
+    def forward(ctx, x2, weight, bias, r2, act):
+        with on_device(x2):
+            xp, ldx = _pieces(x2)
+            wp, ldw = _pieces(weight)
+            need = ctx.needs_input_grad
+            y, slope = _run_linear(xp, ldx, x2.shape[1], wp, ldw, weight.shape[0], None, None, bias, act, r2, x2.dtype, act != 0 and any(need[:3]))
+        ctx.dims = (x2.shape[0], weight.shape[0], x2.shape[1], ldx, ldw)
+        ctx.save_for_backward(xp if need[1] else None, wp if need[0] else None, slope)
+        ctx.dtype = x2.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        xp, wp, slope = ctx.saved_tensors
+        rows, n, k, ldx, ldw = ctx.dims
+        want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
+        dev, dt, code = dy.device, ctx.dtype, _DTYPE[ctx.dtype]
+        dx = dw = db = None
+        L = _lib.lib()
+        with on_device(dy):
+            g = _rows(dy)
+            if rows == 0:
+                dx = torch.empty((0, k), dtype=dt, device=dev) if want_x else None
+                dw = torch.zeros((n, k), dtype=dt, device=dev) if want_w else None
+                db = torch.zeros(n, dtype=dt, device=dev) if want_b else None
+                return dx, dw, db, (dy if want_r else None), None
+            up = -(-n // 8) * 8
+            products = want_x or want_w
+            as_is = slope is None and n % 8 == 0 and g.data_ptr() % 16 == 0 and (rows == 1 or _pitch(g) % 8 == 0) and _pitch(g) < (1 << 21)
+            dz, lddz = (g, _pitch(g)) if as_is else (torch.empty((rows, up), dtype=dt, device=dev) if products else None, up)
+            if want_b:
+                db = torch.empty(n, dtype=dt, device=dev)
+            if want_b or (products and not as_is):
+                part = torch.empty(L.selfc_linear_dz_floats(rows, n), dtype=torch.float32, device=dev) if want_b else None
+                rt.call("selfc_linear_dz", g.data_ptr(), _pitch(g), _ptr(slope), None if as_is or not products else dz.data_ptr(), up, _ptr(db), _ptr(part),
+                        rows, n, code, _lib.stream_ptr())
+            if want_x:
+                dx = torch.empty((rows, k), dtype=dt, device=dev)
+                work = _ws(rows, k, n, 2, dev)
+                rt.call("selfc_linear_dx", dz.data_ptr(), lddz, wp.data_ptr(), ldw, dx.data_ptr(), _ptr(work), rows, n, k, code, _lib.stream_ptr())
+            if want_w:
+                dw = torch.empty((n, k), dtype=dt, device=dev)
+                work = _ws(n, k, rows, 2, dev)
+                rt.call("selfc_linear_dw", dz.data_ptr(), lddz, xp.data_ptr(), ldx, dw.data_ptr(), _ptr(work), rows, n, k, code, _lib.stream_ptr())
+        return dx, dw, db, (dy if want_r else None), None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: str = "none",
+           residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """act(x weight^T + bias) + residual; x (..., in), weight (out, in), both bf16 or both f16, bias (out,) and residual (..., out) of the
+    same type.  act: "none", "relu", "lrelu" (0.2), "gelu" (erf), "silu".  Sums, bias, activation and residual in fp32, one rounding at the end;
+    in the backward pass dy act'(z) is rounded to x's type once, as the operand of both products.  Up to 16 rows the weight streams
+    through a kernel of its own.  Sums are added in a fixed order."""
+    _linear_args(x, weight, bias, act, residual, torch.bfloat16, torch.float16)
+    x2, w2 = _rows(x), _rows(weight)
+    b = None if bias is None else bias.contiguous()
+    r2 = None if residual is None else _rows(residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        _watch_leaves(x, weight, bias, residual)
+        return LinearFn.apply(x2, w2, b, r2, ACTS[act]).view(x.shape[:-1] + (weight.shape[0],))
+    with on_device(x):
+        xp, ldx = _pieces(x2)
+        wp, ldw = _pieces(w2)
+        y, _ = _run_linear(xp, ldx, x2.shape[1], wp, ldw, weight.shape[0], None, None, b, ACTS[act], r2, x.dtype, False)
+    return y.view(x.shape[:-1] + (weight.shape[0],))
+
+
+def quantize_rows(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, scale) of a weight (out, in): float8_e4m3fn rows with one fp32 scale each, for linear_q8.  Done once per weight."""
+    _need(w.dim() == 2 and w.is_floating_point(), f"quantize_rows expects a float matrix, got {w.dtype} {tuple(w.shape)}")
+    w = w.detach().float()
+    most = w.abs().amax(1) if w.shape[1] else w.new_zeros(w.shape[0])
+    scale = torch.where(most > 0, (most / E4M3_MAX).clamp_(min=2.0 ** -126), torch.ones_like(most))
+    return (w / scale[:, None]).to(torch.float8_e4m3fn), scale
+
+
+def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+              act: str = "none", residual: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """act(x_scale w_scale (x weight^T) + bias) + residual for float8_e4m3fn x (..., in) with a scale per row (rms_norm_q8) and weight
+    (out, in) with a scale per output (quantize_rows); bias and residual of out_dtype (bf16, f16 or fp32).  For serving: no gradients."""
+    if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise RuntimeError(f"selfc_amd: out_dtype is {out_dtype}")
+    _linear_args(x, weight, bias, act, residual, torch.float8_e4m3fn, out_dtype=out_dtype)
+    _no_grad_only("linear_q8", bias, residual, x_scale, w_scale)
+    _same_device(x, x_scale=x_scale, w_scale=w_scale)
+    _typed("x_scale", x_scale, torch.float32)
+    _typed("w_scale", w_scale, torch.float32)
+    _need(x_scale.shape == x.shape[:-1], f"x_scale has shape {tuple(x_scale.shape)}, expected {tuple(x.shape[:-1])}")
+    _need(w_scale.shape == weight.shape[:1], f"w_scale has shape {tuple(w_scale.shape)}, expected ({weight.shape[0]},)")
+    with on_device(x):
+        x2 = _rows(x)
+        xp, ldx = _pieces(x2)
+        wp, ldw = _pieces(_rows(weight))
+        y, _ = _run_linear(xp, ldx, x2.shape[1], wp, ldw, weight.shape[0], x_scale.reshape(-1).contiguous(), w_scale.contiguous(),
+                           None if bias is None else bias.contiguous(), ACTS[act], None if residual is None else _rows(residual), out_dtype, False)
+    return y.view(x.shape[:-1] + (weight.shape[0],))

@@ -31,7 +31,7 @@ import torch
 import torch.nn as nn
 from torch.optim.lr_scheduler import _LRScheduler
 
-from . import _lib, autograd as ag, harness, runtime as rt
+from . import _lib, autograd as ag, harness, optim, runtime as rt
 from .global_var import GlobalVar
 from .modules.Quantization import Quantization
 
@@ -179,7 +179,8 @@ class RescaleTrainer:
 
     train_opt keys are the yml's (train_rescaling_selfc_large.yml:95-121): lr_G, beta1, beta2, weight_decay_G,
     pixel_criterion_forw/back, lambda_fit_forw, lambda_rec_back, lambda_cond_prob, gradient_clipping, lr_scheme,
-    lr_steps, lr_gamma, restarts, restart_weights, clear_state."""
+    lr_steps, lr_gamma, restarts, restart_weights, clear_state.  Two keys beyond the yml's: optimizer ("Adam", the reference's, or "AdamW":
+    decoupled weight decay, optim.AdamW) and state_bits (of AdamW's moments: 32 or 8)."""
 
     def __init__(self, netG: nn.Module, train_opt: dict, capturable: bool = False, flat_grads: bool = None,
                  data_parallel: bool = None, process_group=None, flat_params: bool = None):
@@ -209,7 +210,14 @@ class RescaleTrainer:
         if capturable:
             lr = torch.tensor(float(lr), dtype=torch.float32, device=optim_params[0].device)
         self._adam_kw = dict(lr=lr, weight_decay=wd, betas=(train_opt["beta1"], train_opt["beta2"]), capturable=capturable)
-        self.optimizer_G = torch.optim.Adam(optim_params, **self._adam_kw)
+        kind = train_opt.get("optimizer") or "Adam"
+        if kind not in ("Adam", "AdamW"):
+            raise NotImplementedError(f"optimizer {kind!r}: expected 'Adam' (the reference's) or 'AdamW'")
+        if kind == "AdamW":
+            self.optimizer_G = optim.AdamW(optim_params, state_bits=train_opt.get("state_bits") or 32,
+                                           max_norm=train_opt.get("gradient_clipping") or None, **self._adam_kw)
+        else:
+            self.optimizer_G = torch.optim.Adam(optim_params, **self._adam_kw)
         self.log_dict = OrderedDict()
         self.grad_norm = None
         is_ddp = isinstance(netG, nn.parallel.DistributedDataParallel)
@@ -221,7 +229,7 @@ class RescaleTrainer:
         # the same hyper-parameters; the per-tensor optimizer is rebuilt if a step ever leaves parameters without a gradient
         # (those must be skipped, which a single flat tensor cannot express).
         self.flat_optimizer = False
-        if self.sink is not None and flat_params is not False and optim_params[0].is_cuda and \
+        if kind == "Adam" and self.sink is not None and flat_params is not False and optim_params[0].is_cuda and \
                 len({p_.dtype for p_ in optim_params}) == 1 and len(self.sink.params) == len(optim_params):
             self.optimizer_G = torch.optim.Adam([self.sink.flatten_params()], **self._adam_kw)
             self.flat_optimizer = True
@@ -387,6 +395,14 @@ class RescaleTrainer:
 
     def _load_state_keeping_own_groups(self, sd: dict):
         opt = self.optimizer_G
+        if isinstance(opt, optim.AdamW):
+            if self.graph is not None:
+                for own, saved in zip(opt.param_groups, sd["param_groups"]):
+                    for k_ in ("betas", "eps", "weight_decay"):
+                        if k_ in saved and torch.as_tensor(saved[k_]).tolist() != torch.as_tensor(own[k_]).tolist():
+                            raise RuntimeError(f"optimizer state changes {k_} ({own[k_]!r} -> {saved[k_]!r}), a constant of the captured step: capture again")
+            opt.load_state_dict(sd)                              # in place: a captured step keeps its tensors
+            return
         if len(sd["param_groups"]) != len(opt.param_groups):
             raise ValueError(f"optimizer state has {len(sd['param_groups'])} parameter groups, the trainer's optimizer {len(opt.param_groups)}")
         state = sd.get("state", {})
@@ -482,6 +498,11 @@ class RescaleTrainer:
         """gradient clipping + optimizer step (SelfC_model.py:172-176)."""
         if self.before_clip is not None:
             self.before_clip(self)
+        if isinstance(self.optimizer_G, optim.AdamW):              # clips as it steps; the .grad tensors keep the unclipped gradients
+            self.optimizer_G.step()
+            self.grad_norm = self.optimizer_G.grad_norm
+            rt.invalidate_weights()
+            return
         max_norm = self.train_opt.get("gradient_clipping")
         if _FUSED_ADAM and self.flat_optimizer and self.sink is not None and self._fused_clip_adam(max_norm):
             rt.invalidate_weights()

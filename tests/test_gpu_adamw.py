@@ -1,0 +1,344 @@
+"""selfc_amd/optim.py on the GPU: the step's formulas in 64 bits, the 8-bit format bit for bit, clipping, the optimizer and the trainer."""
+import math
+
+import pytest
+import torch
+
+from test_adamw_cpu import BLOCK, hold, mix_dither, moments
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24
+
+
+def optim():
+    from selfc_amd import optim as o
+    return o
+
+
+SIZES = [1, 5, 256, 257, 4095, 4096, 4097, 77 * 308, 3, 12289]
+
+
+def make(sizes, dt, seed, offset=0):
+    gen = torch.Generator().manual_seed(seed)
+    ps, gs = [], []
+    for i, n in enumerate(sizes):
+        p, g = torch.randn(n + offset, generator=gen) * 0.05, torch.randn(n + offset, generator=gen) * 10.0 ** (-(i % 5) - 1)
+        ps.append(p.to(dt)[offset:])
+        gs.append(g.to(dt)[offset:])
+    return ps, gs
+
+
+def blocks(n):
+    return -(-n // BLOCK)
+
+
+def flat_state(sizes, bits, seed):
+    gen = torch.Generator().manual_seed(seed)
+    size = sum(blocks(n) for n in sizes) * BLOCK
+    inside = torch.cat([torch.arange(blocks(n) * BLOCK) < n for n in sizes])
+    m = torch.randn(size, generator=gen) * 1e-2 * inside
+    v = (torch.randn(size, generator=gen) * 2).exp() * 1e-4 * inside
+    if bits == 32:
+        return m, v, None, None, inside
+    m, ms = hold(m, torch.full((size,), 0.5), 7, -6, 3, False)
+    v, vs = hold(v, torch.full((size,), 0.5), 14, -14, 2, True)
+    return m.to(torch.float8_e4m3fn), v.to(torch.float8_e5m2), ms, vs, inside
+
+
+def wide(ts, sizes, inside):
+    out = torch.zeros(inside.numel())
+    out[inside] = torch.cat([t.float() for t in ts])
+    return out
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("step", [1, 7, 100000])
+def test_step_against_the_formulas(dt, bits, offset, step):
+    """Parameters against 64 bits; the moments, 8-bit codes and scales exactly (they are fp32 operations rounded one by one)."""
+    ps, gs = make(SIZES, dt, 3, offset)
+    m, v, ms, vs, inside = flat_state(SIZES, bits, 4)
+    lr, b1, b2, eps, wd, seed = 3e-3, 0.9, 0.99, 1e-8, 0.1, 1234567
+    if offset:      # views that start one value into their storage
+        dev = [torch.cat([torch.zeros(1, dtype=dt), p]).cuda()[1:] for p in ps], [torch.cat([torch.zeros(1, dtype=dt), g]).cuda()[1:] for g in gs]
+    else:
+        dev = [p.cuda() for p in ps], [g.cuda() for g in gs]
+    st = [None if t is None else t.cuda() for t in (m, v, ms, vs)]
+    version = dev[0][2]._version
+    optim().adamw_step(dev[0], dev[1], *st, step=step, lr=lr, beta1=b1, beta2=b2, eps=eps, weight_decay=wd, seed=seed)
+    assert dev[0][2]._version > version
+    m32, v32 = (m, v) if bits == 32 else (m.float() * ms.repeat_interleave(BLOCK), v.float() * vs.repeat_interleave(BLOCK))
+    mn, vn = moments(m32, v32, wide(gs, SIZES, inside), b1, b2)
+    if bits == 32:
+        assert torch.equal(st[0].cpu()[inside], mn[inside]) and torch.equal(st[1].cpu()[inside], vn[inside])
+        assert not st[0].cpu()[~inside].any() and not st[1].cpu()[~inside].any()
+    else:
+        um, uv = mix_dither(SIZES, seed, step)
+        for got, scale, (want, s) in ((st[0], st[2], hold(mn, um, 7, -6, 3, False)), (st[1], st[3], hold(vn, uv, 14, -14, 2, True))):
+            assert torch.equal(scale.cpu(), s)
+            assert torch.equal(got.cpu().float(), want)
+    mean = mn.double()[inside] / (1 - b1 ** step)
+    den = (vn.double()[inside] / (1 - b2 ** step)).sqrt() + eps
+    p0 = torch.cat(ps).double()
+    want = p0 * (1 - lr * wd) - lr * mean / den
+    got = torch.cat([p.cpu().double() for p in dev[0]])
+    # the step's factors, root, reciprocal and products: 16 roundings; p's own product and difference: 2; the store
+    tol = 16 * U32 * lr * (mean / den).abs() + 3 * U32 * p0.abs() + torch.finfo(dt).eps / 2 * want.abs() * (0 if dt == torch.float32 else 1.001) + 2.0 ** -25
+    assert ((got - want).abs() <= tol).all(), ((got - want).abs() - tol).max()
+
+
+def test_a_tensor_without_gradient_keeps_everything_and_its_place():
+    o = optim()
+    ps, gs = make(SIZES, torch.float32, 5)
+    for bits in (32, 8):
+        m, v, ms, vs, _ = flat_state(SIZES, bits, 6)
+        a = [p.cuda() for p in ps]
+        st = [None if t is None else t.cuda() for t in (m, v, ms, vs)]
+        full = [p.cuda() for p in ps]
+        st2 = [None if t is None else t.clone() for t in st]
+        some = [g.cuda() if i not in (0, 4, 9) else None for i, g in enumerate(gs)]
+        o.adamw_step(a, some, *st, step=3, lr=1e-2)
+        o.adamw_step(full, [g.cuda() for g in gs], *st2, step=3, lr=1e-2)
+        at = 0
+        for i, (p, q, old) in enumerate(zip(a, full, ps)):
+            sl = slice(at, at + blocks(SIZES[i]) * BLOCK)
+            at = sl.stop
+            skipped = i in (0, 4, 9)
+            assert torch.equal(p.cpu(), old) == skipped and (skipped or torch.equal(p, q))
+            if skipped:
+                assert torch.equal(st[0][sl].float().cpu(), m[sl].float()) and torch.equal(st[1][sl].float().cpu(), v[sl].float())
+            else:
+                assert torch.equal(st[0][sl].float(), st2[0][sl].float()) and torch.equal(st[1][sl].float(), st2[1][sl].float())
+
+
+def test_many_tensors_take_several_launches():
+    o = optim()
+    sizes = [((i * 37) % 700) for i in range(250)]          # some are empty
+    ps, gs = make(sizes, torch.float32, 7)
+    m, v, ms, vs, inside = flat_state(sizes, 8, 8)
+    dev = [p.cuda() for p in ps]
+    st = [t.cuda() for t in (m, v, ms, vs)]
+    o.adamw_step(dev, [g.cuda() for g in gs], *st, step=2, lr=1e-2, weight_decay=0.0, seed=5)
+    mn, vn = moments(m.float() * ms.repeat_interleave(BLOCK), v.float() * vs.repeat_interleave(BLOCK), wide(gs, sizes, inside), 0.9, 0.999)
+    um, uv = mix_dither(sizes, 5, 2)
+    want, s = hold(mn, um, 7, -6, 3, False)
+    assert torch.equal(st[0].cpu().float(), want) and torch.equal(st[2].cpu(), s)
+    want, s = hold(vn, uv, 14, -14, 2, True)
+    assert torch.equal(st[1].cpu().float(), want) and torch.equal(st[3].cpu(), s)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16, torch.float16])
+def test_grad_norm(dt):
+    sizes = [0, 1, 7, 4096, 4099, 100001] + [33] * 120
+    _, gs = make(sizes, dt, 9, offset=1)
+    want = math.sqrt(sum(g.double().square().sum().item() for g in gs))
+    dev = [torch.cat([torch.zeros(1, dtype=dt), g]).cuda()[1:] for g in gs]
+    dev[7] = None
+    want7 = math.sqrt(want ** 2 - gs[7].double().square().sum().item())
+    assert abs(optim().grad_norm(dev).item() - want7) <= 2 * U32 * want7
+    big = [torch.full((5000,), 1e25).cuda()] if dt == torch.float32 else []
+    if big:
+        assert abs(optim().grad_norm(big).item() / (1e25 * math.sqrt(5000)) - 1) < 1e-6
+
+
+def test_clipping_is_that_of_scaled_gradients():
+    o = optim()
+    ps, gs = make([300, 41], torch.float32, 10)
+    for max_norm in (0.01, 1e9):
+        a, b = [p.cuda() for p in ps], [p.cuda() for p in ps]
+        z = lambda: torch.zeros(1024, device="cuda")  # noqa: E731
+        g = [t.cuda() for t in gs]
+        n = o.grad_norm(g)
+        sa, sb = (z(), z()), (z(), z())
+        o.adamw_step(a, g, *sa, step=1, lr=1e-2, max_norm=max_norm)
+        coef = torch.clamp(max_norm / (n + 1e-6), max=1.0)
+        o.adamw_step(b, [t * coef for t in g], *sb, step=1, lr=1e-2)
+        assert all(torch.equal(x, y) for x, y in zip(a + list(sa), b + list(sb)))
+        assert torch.equal(g[0].cpu(), gs[0])
+
+
+def test_values_that_are_not_finite_stay_alone_in_8_bits():
+    o = optim()
+    ps, gs = make([600], torch.float32, 11)
+    for bad in (float("nan"), float("inf")):
+        a, b = [ps[0].cuda()], [ps[0].cuda()]
+        mk = lambda: [torch.zeros(768, dtype=torch.uint8, device="cuda").view(t) for t in (torch.float8_e4m3fn, torch.float8_e5m2)] + [torch.ones(3, device="cuda") for _ in range(2)]  # noqa: E731
+        sa, sb = mk(), mk()
+        g = gs[0].clone()
+        g[300] = 0.0
+        o.adamw_step(a, [g.cuda()], *sa, step=1, lr=1e-2)
+        g[300] = bad
+        o.adamw_step(b, [g.cuda()], *sb, step=1, lr=1e-2)
+        keep = torch.arange(600) != 300
+        assert torch.equal(a[0].cpu()[keep], b[0].cpu()[keep]) and torch.isnan(b[0][300])
+        for x, y in zip(sa, sb):
+            x, y = x.float().cpu(), y.float().cpu()
+            assert torch.equal(x[:600][keep[:x.numel()]] if x.numel() > 3 else x, y[:600][keep[:y.numel()]] if y.numel() > 3 else y)
+        assert torch.isnan(sb[0][300].float()) and torch.isnan(sb[1][300].float())
+
+
+def test_tiny_and_huge_gradients_in_8_bits():
+    """Blocks whose moments lie near fp32's ends: finite, and the update is the 32-bit one's."""
+    o = optim()
+    for scale in (1e-22, 1e-12, 1e12, 1e17):
+        g = torch.randn(512, generator=torch.Generator().manual_seed(2)) * scale
+        p = [torch.zeros(512).cuda()]
+        q = [torch.zeros(512).cuda()]
+        s8 = [torch.zeros(512, dtype=torch.uint8, device="cuda").view(t) for t in (torch.float8_e4m3fn, torch.float8_e5m2)] + [torch.ones(2, device="cuda") for _ in range(2)]
+        s32 = [torch.zeros(512, device="cuda") for _ in range(2)]
+        for step in (1, 2):
+            o.adamw_step(p, [g.cuda()], *s8, step=step, lr=1e-3, eps=1e-30)
+            o.adamw_step(q, [g.cuda()], *s32, step=step, lr=1e-3, eps=1e-30)
+            assert torch.isfinite(p[0]).all()
+            if step == 1:
+                assert torch.equal(p[0], q[0])          # the first step's moments were not rounded yet
+        assert all(torch.isfinite(t.float()).all() for t in s8)
+
+
+def test_optimizer_against_torch_and_its_state():
+    """AdamW of this package and torch's over parameter groups, a skipped parameter and channels-last weights; save and resume."""
+    o = optim()
+    gen = torch.Generator().manual_seed(12)
+    shapes = [(33, 7), (40, 8, 3, 3), (5,), (64, 64)]
+    init = [torch.randn(s, generator=gen) * 0.1 for s in shapes]
+    grads = [[torch.randn(s, generator=gen) for s in shapes] for _ in range(5)]
+
+    def build(cls, **kw):
+        ps = [t.clone().cuda() for t in init]
+        ps[1] = ps[1].to(memory_format=torch.channels_last)
+        ps = [torch.nn.Parameter(t) for t in ps]
+        return ps, cls([{"params": ps[:2], "lr": 1e-2}, {"params": ps[2:], "weight_decay": 0.3}], lr=1e-3, weight_decay=0.05, **kw)
+    mine, opt = build(o.AdamW)
+    ref, tref = build(torch.optim.AdamW)
+
+    def run(ps, op, k):
+        for i, p in enumerate(ps):
+            p.grad = None if (k == 2 and i in (1, 3)) else grads[k][i].cuda()
+        op.step()
+    for k in range(5):
+        run(mine, opt, k)
+        run(ref, tref, k)
+        if k == 3:
+            saved = opt.state_dict()
+            saved = {"state": {i: {n: t.clone() for n, t in s.items()} for i, s in saved["state"].items()}, "param_groups": saved["param_groups"]}
+            kept = [p.detach().clone() for p in mine]
+    for p, q in zip(mine, ref):
+        # five steps of at most lr = 1e-2 each way; every factor in fp32
+        assert ((p - q).abs() <= 5 * 32 * U32 * (1e-2 + q.abs())).all()
+    assert opt.state[mine[1]]["step"].item() == 4 and opt.state[mine[0]]["step"].item() == 5
+    again, opt2 = build(o.AdamW)
+    with torch.no_grad():
+        for p, q in zip(again, kept):
+            p.copy_(q)
+    opt2.load_state_dict(saved)
+    run(again, opt2, 4)
+    for p, q in zip(again, mine):
+        assert torch.equal(p, q)
+    opt2.load_state_dict(tref.state_dict())          # torch's state file
+    with pytest.raises(ValueError, match="state_bits"):
+        build(o.AdamW, state_bits=8)[1].load_state_dict(saved)
+
+
+def test_8_bit_state_trains_like_32():
+    """A quadratic: the moments in 8 bits reach the same neighbourhood; and a resumed run repeats the bits."""
+    o = optim()
+    gen = torch.Generator().manual_seed(13)
+    target = torch.randn(2000, generator=gen).cuda()
+
+    def start():
+        p = torch.nn.Parameter(torch.zeros(2000, device="cuda"))
+        return p, o.AdamW([p], lr=1e-2, weight_decay=0.0, state_bits=8, seed=3)
+
+    def run(p, opt, n):
+        for _ in range(n):
+            p.grad = p.detach() - target
+            opt.step()
+    p, opt = start()
+    run(p, opt, 30)
+    sd = opt.state_dict()
+    mid, sd = p.detach().clone(), {"state": {i: {n: t.clone() for n, t in s.items()} for i, s in sd["state"].items()}, "param_groups": sd["param_groups"]}
+    run(p, opt, 30)
+    q, opt2 = start()
+    with torch.no_grad():
+        q.copy_(mid)
+    opt2.load_state_dict(sd)
+    run(q, opt2, 30)
+    assert torch.equal(p, q)
+    assert torch.isfinite(p).all()
+
+
+def test_captured_step_counts_and_follows_the_rate():
+    from selfc_amd import runtime as rt
+    o = optim()
+    for bits in (32, 8):
+        def build():
+            ps = [torch.nn.Parameter(t.cuda()) for t in make([700, 33, 4097], torch.float32, 14)[0]]
+            return ps, torch.tensor(1e-2, device="cuda")
+        gs = [make([700, 33, 4097], torch.float32, 15 + k)[1] for k in range(6)]
+        ps, lr = build()
+        opt = o.AdamW(ps, lr=lr, state_bits=bits, capturable=True, max_norm=0.5)
+        static = [g.cuda() for g in gs[0]]
+        for p, g in zip(ps, static):
+            p.grad = g
+        s = rt.warmup_stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            opt.step()
+        torch.cuda.current_stream().wait_stream(s)
+        graph = rt.new_graph()
+        with rt.graph_capture(graph, ps[0].device):
+            opt.step()
+        eager, lr2 = build()
+        opt2 = o.AdamW(eager, lr=1e-2, state_bits=bits, max_norm=0.5)
+        for k in range(6):
+            for st, g in zip(static, gs[k]):
+                st.copy_(g)
+            for p, g in zip(eager, gs[k]):
+                p.grad = g.cuda()
+            if k == 4:
+                lr.fill_(5e-3)
+                opt2.param_groups[0]["lr"] = 5e-3
+            if k:
+                graph.replay()
+            opt2.step()
+            torch.cuda.synchronize()
+            assert k == 0 or torch.equal(opt.grad_norm, opt2.grad_norm)        # (the graph's own scalar: written by its first replay)
+            for p, q in zip(ps, eager):
+                # 1 - beta^t is formed on the device there and on the host here, both in 64 bits; lr as a float on both sides
+                assert ((p - q).abs() <= (k + 1) * 8 * U32 * (1e-2 + q.abs())).all()
+        with pytest.raises(RuntimeError, match="capturable"):
+            g2 = rt.new_graph()
+            with rt.graph_capture(g2, ps[0].device):
+                opt2.step()
+
+
+def test_trainer_steps_with_adamw():
+    """RescaleTrainer(optimizer: AdamW): eager and captured steps of a small net agree; the state file resumes."""
+    from selfc_amd import GlobalVar
+    from selfc_amd.modules.SelfC_GMM_arch_inv import SelfCInvNet
+    from selfc_amd.train import TRAIN_OPT_LARGE, RescaleTrainer, feed_data
+    GlobalVar.set_Temporal_LEN(7)
+    opt = {"global_module": "nonlocal", "stp_blk_num": 2, "fh_loss": "l2", "scale": 4, "gmm_k": 5}
+    gt = torch.rand(1, 3, 7, 32, 32, generator=torch.Generator().manual_seed(3)).cuda()
+    for bits in (32, 8):
+        logs = []
+        for captured in (False, True):
+            torch.manual_seed(1)
+            net = SelfCInvNet(opt, 3, 3, "D2DTNet", [2, 2], 2).cuda()
+            tr = RescaleTrainer(net, dict(TRAIN_OPT_LARGE, optimizer="AdamW", state_bits=bits, weight_decay_G=0.01), capturable=captured)
+            assert not tr.flat_optimizer
+            real_h, ref_l, _ = feed_data(gt)
+            if captured:
+                tr.capture(real_h, ref_l, warmup=2)
+                log = list(tr.warmup_logs)
+            else:
+                log = [dict(tr.optimize_parameters(real_h, ref_l)) for _ in range(2)]
+            log += [dict(tr.optimize_parameters(real_h, ref_l)) for _ in range(2)]
+            logs.append(log)
+            sd = tr.optimizer_state_dict()
+            tr.load_optimizer_state_dict(sd)
+            assert all(torch.isfinite(p).all() for p in net.parameters())
+        for a, b in zip(*logs):
+            assert abs(a["loss"] / b["loss"] - 1) < 1e-2 and abs(a["grad_norm"] / b["grad_norm"] - 1) < 5e-2

@@ -1,0 +1,361 @@
+"""rms_norm, linear and their 8-bit forms (selfc_amd/pointwise.py) against the formulas in 64 bits on the CPU.
+
+Bounds: a rounding to type t is off by at most eps(t)/2 of the value; a sum of n products in fp32 by at most (n + 8) 2^-24 of the sum of
+their magnitudes; an activation's formula in fp32 by 2^-20 of 1 + |z|; the kept derivative by half a step, 2^-16; values below the
+type's normal range by half its smallest step."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U32 = 2.0 ** -24
+T16 = [torch.bfloat16, torch.float16]
+TINY = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -25, torch.float32: 2.0 ** -149}
+
+
+def pw():
+    from selfc_amd import pointwise
+    return pointwise
+
+
+def within(got, want, tol):
+    got = got.detach().double().cpu()
+    assert got.shape == want.shape
+    assert torch.isfinite(got).all()
+    off = (got - want).abs()
+    worst = (off - tol).max().item() if off.numel() else 0.0
+    assert worst <= 0, f"over the bound by {worst:.3g}; largest difference {off.max().item():.3g}, bound there {tol.expand_as(off).reshape(-1)[off.argmax()].item():.3g}"
+
+
+def u(t):
+    return torch.finfo(t).eps / 2
+
+
+def rnd(gen, *shape, scale=1.0, dtype=torch.float32):
+    return (torch.randn(*shape, generator=gen) * scale).to(dtype)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# norm
+# ---------------------------------------------------------------------------------------------------------------------
+def norm_ref(x, r, w, eps, dt):
+    h = x.double()
+    if r is not None:
+        h = (x.float() + r.float()).to(dt).double()
+    rstd = 1 / (h.pow(2).mean(-1, keepdim=True) + eps).sqrt()
+    return h, rstd, h * rstd * w.double()
+
+
+@pytest.mark.parametrize("dt", T16 + [torch.float32])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (65, 51), (33, 64), (257, 100), (40, 256), (9, 511), (6, 1000), (5, 2048), (4, 2049), (3, 4096), (2, 8191), (2, 16384)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_and_gradient(dt, rows, cols, residual):
+    gen = torch.Generator().manual_seed(rows * 131 + cols)
+    x, w, dy, dh = rnd(gen, rows, cols, dtype=dt), (rnd(gen, cols) * 0.3 + 1).to(dt), rnd(gen, rows, cols, dtype=dt), rnd(gen, rows, cols, dtype=dt)
+    r = rnd(gen, rows, cols, dtype=dt) if residual else None
+    eps = 1e-5
+    h, rstd, y = norm_ref(x, r, w, eps, dt)
+    xd, wd = x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)
+    rd = r.cuda().requires_grad_(True) if residual else None
+    gy, gh = pw().rms_norm(xd, wd, residual=rd, eps=eps)
+    if residual:
+        assert torch.equal(gh.detach().cpu(), h.to(dt))
+        grads = torch.autograd.grad((gy, gh), (xd, wd, rd), (dy.cuda(), dh.cuda()))
+        assert torch.equal(grads[0], grads[2])
+    else:
+        assert gh is xd
+        grads = torch.autograd.grad(gy, (xd, wd), dy.cuda())
+    stat = (cols + 16) * U32
+    within(gy, y, y.abs() * (u(dt) + stat) + TINY[dt])
+    n, g = h * rstd, dy.double() * w.double()
+    dx = rstd * (g - n * (g * n).mean(-1, keepdim=True)) + (dh.double() if residual else 0)
+    size = rstd * (g.abs() + n.abs() * (g * n).abs().mean(-1, keepdim=True))
+    within(grads[0], dx, dx.abs() * u(dt) + 3 * stat * size + (4 * U32 * dh.double().abs() if residual else 0) + TINY[dt])
+    dw, dws = (dy.double() * n).sum(0), (dy.double() * n).abs().sum(0)
+    within(grads[1], dw, dw.abs() * u(dt) + (rows + cols + 24) * U32 * dws + TINY[dt])
+
+
+def test_norm_weight_in_32_bits_strided_rows_and_leading_axes():
+    gen = torch.Generator().manual_seed(5)
+    wide = rnd(gen, 2, 5, 4, 90, dtype=torch.float16)
+    x, r = wide[..., 3:83], rnd(gen, 2, 5, 4, 80, dtype=torch.float16).transpose(0, 2).contiguous().transpose(0, 2)
+    w, dy = rnd(gen, 80) + 1, rnd(gen, 2, 5, 4, 80, dtype=torch.float16)
+    h, rstd, y = norm_ref(x, r, w, 1e-6, torch.float16)
+    big = wide.cuda().requires_grad_(True)
+    wd = w.cuda().requires_grad_(True)
+    gy, gh = pw().rms_norm(big[..., 3:83], wd, residual=r.cuda())
+    within(gy, y, y.abs() * (u(torch.float16) + 96 * U32) + TINY[torch.float16])
+    gx, gw = torch.autograd.grad(gy, (big, wd), dy.cuda())
+    assert gw.dtype == torch.float32 and gx.shape == wide.shape and not gx[..., :3].any() and not gx[..., 83:].any()
+    dw, dws = (dy.double() * h * rstd).sum((0, 1, 2)), (dy.double() * h * rstd).abs().sum((0, 1, 2))
+    within(gw, dw, (40 + 80 + 24) * U32 * dws)
+
+
+@pytest.mark.parametrize("dt", T16 + [torch.float32])
+@pytest.mark.parametrize("rows,cols", [(1, 3), (7, 51), (130, 64), (5, 4096), (2, 16384)])
+def test_norm_q8(dt, rows, cols):
+    gen = torch.Generator().manual_seed(cols)
+    x, w, r = rnd(gen, rows, cols, dtype=dt), (rnd(gen, cols) * 0.3 + 1).to(dt), rnd(gen, rows, cols, dtype=dt)
+    if rows > 2:
+        x[1], r[1] = 0, 0
+    h, _, y = norm_ref(x, r, w, 1e-6, dt)
+    q, scale, gh = pw().rms_norm_q8(x.cuda(), w.cuda(), residual=r.cuda())
+    assert q.dtype == torch.float8_e4m3fn and scale.dtype == torch.float32 and torch.equal(gh.cpu(), h.to(dt))
+    stat = (cols + 20) * U32
+    want = y.abs().amax(-1) / 448
+    want = torch.where(want > 0, want, torch.ones_like(want))
+    within(scale, want, want * stat)
+    # half a step of e4m3: 2^-4 of the value, 2^-10 steps below the normal range
+    within(q.float().cpu() * scale.cpu()[:, None], y, y.abs() * (2.0 ** -4 + 4 * stat) + scale.cpu().double()[:, None] * 2.0 ** -10)
+
+
+def test_norm_rows_that_are_not_finite_stay_alone():
+    x = torch.randn(6, 96, dtype=torch.float32).cuda().half()
+    clean, _ = pw().rms_norm(x, torch.ones(96).cuda())
+    x[2, 5], x[4, 7] = float("nan"), float("inf")
+    y, _ = pw().rms_norm(x, torch.ones(96).cuda())
+    q, s, _ = pw().rms_norm_q8(x, torch.ones(96).cuda())
+    for i in (0, 1, 3, 5):
+        assert torch.equal(y[i], clean[i]) and torch.isfinite(q[i].float()).all()
+    assert torch.isnan(y[2]).all() and torch.isnan(y[4, 7]) and torch.isnan(q[2].float()).all()
+
+
+def test_norm_without_rows():
+    x, w = torch.zeros(0, 64, dtype=torch.bfloat16).cuda().requires_grad_(True), torch.ones(64, dtype=torch.bfloat16).cuda().requires_grad_(True)
+    y, _ = pw().rms_norm(x, w)
+    y.sum().backward()
+    assert y.shape == (0, 64) and not w.grad.any() and x.grad.shape == (0, 64)
+    q, s, _ = pw().rms_norm_q8(x.detach(), w.detach())
+    assert q.shape == (0, 64) and s.shape == (0,)
+
+
+def test_norm_gradient_when_one_output_is_used():
+    gen = torch.Generator().manual_seed(3)
+    x, r, w = (rnd(gen, 4, 32, dtype=torch.float32).cuda().requires_grad_(True) for _ in range(3))
+    w = w[0].detach().clone().requires_grad_(True)
+    y, h = pw().rms_norm(x, w, residual=r)
+    gx, gr, gw = torch.autograd.grad(h.sum(), (x, r, w), allow_unused=True)
+    assert torch.equal(gx, torch.ones_like(gx)) and torch.equal(gr, gx) and gw is None
+    y, h = pw().rms_norm(x, w, residual=r)
+    gx, gw = torch.autograd.grad(y.sum(), (x, w))                      # an expanded gradient
+    assert torch.isfinite(gx).all() and gw.shape == w.shape
+
+
+def test_norm_gradient_against_differences():
+    gen = torch.Generator().manual_seed(11)
+    x, w, dy = rnd(gen, 2, 24).cuda(), (rnd(gen, 24) + 1).cuda(), rnd(gen, 2, 24).cuda()
+    leaf = x.clone().requires_grad_(True)
+    g, = torch.autograd.grad(pw().rms_norm(leaf, w)[0], leaf, dy)
+    for at in ((0, 0), (1, 13), (1, 23)):
+        step = 2.0 ** -6
+        up, down = x.clone(), x.clone()
+        up[at] += step
+        down[at] -= step
+        diff = ((pw().rms_norm(up, w)[0].double() - pw().rms_norm(down, w)[0].double()) * dy.double()).sum().item() / (2 * step)
+        # the difference's third-order term (step^2 / 6 times a third derivative of order 10) and fp32's last bits over the step
+        assert abs(diff - g[at].item()) < 10 * step ** 2 + 24 * 8 * U32 / step
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# product
+# ---------------------------------------------------------------------------------------------------------------------
+def act_ref(z, act):
+    if act == "relu":
+        return z.clamp(min=0), (z > 0).double()
+    if act == "lrelu":
+        return torch.where(z > 0, z, 0.2 * z), torch.where(z > 0, 1.0, 0.2).double()
+    if act == "gelu":
+        cdf = 0.5 * torch.special.erfc(-z / math.sqrt(2))
+        return z * cdf, cdf + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s * (1 + z * (1 - s))
+    return z, torch.ones_like(z)
+
+
+def product_ref(x, w, b, r, act, scale=None):
+    x, w = x.double(), w.double()
+    if scale is not None:
+        x, w = x * scale[0].double()[:, None], w * scale[1].double()[:, None]
+    z = x @ w.t()
+    size = x.abs() @ w.abs().t()
+    if b is not None:
+        z, size = z + b.double(), size + b.double().abs()
+    y, d = act_ref(z, act)
+    if r is not None:
+        y, size = y + r.double(), size + r.double().abs()
+    return z, size, y, d
+
+
+def product_bound(dt, k, z, size, y):
+    # 0.2 in fp32 and the derivative's bound 1.13 are inside the factor 1.2; size holds the residual, whose addition rounds once more
+    return y.abs() * u(dt) * (1 + 2.0 ** -8) + 1.2 * (k + 10) * U32 * size + 2.0 ** -20 * (1 + z.abs()) * 2.0 ** -2 + TINY[dt]
+
+
+SHAPES = [(1, 1, 1), (1, 64, 16), (3, 8, 5), (16, 4096, 40), (16, 51, 204), (17, 64, 64), (33, 51, 3), (65, 200, 130), (128, 128, 128), (130, 520, 72),
+          (300, 64, 129), (257, 130, 257), (700, 96, 8), (70, 2056, 66), (64, 8192, 64)]
+
+
+@pytest.mark.parametrize("dt", T16)
+@pytest.mark.parametrize("m,k,n", SHAPES)
+def test_product(dt, m, k, n):
+    gen = torch.Generator().manual_seed(m * 7 + k * 3 + n)
+    x, w, b, r = rnd(gen, m, k, dtype=dt), rnd(gen, n, k, scale=k ** -0.5, dtype=dt), rnd(gen, n, dtype=dt), rnd(gen, m, n, dtype=dt)
+    for act, bias, res in (("none", None, None), ("relu", b, r), ("lrelu", b, None), ("gelu", b, r), ("silu", None, r)):
+        z, size, y, _ = product_ref(x, w, bias, res, act)
+        got = pw().linear(x.cuda(), w.cuda(), bias=None if bias is None else b.cuda(), act=act, residual=None if res is None else r.cuda())
+        assert got.dtype == dt
+        within(got, y, product_bound(dt, k, z, size, y))
+
+
+@pytest.mark.parametrize("dt", T16)
+@pytest.mark.parametrize("m,k,n", SHAPES + [(2500, 40, 72), (3000, 51, 20)])
+@pytest.mark.parametrize("act", ["none", "lrelu", "gelu"])
+def test_product_gradients(dt, m, k, n, act):
+    gen = torch.Generator().manual_seed(m + k * 5 + n * 11)
+    x, w, b, dy = rnd(gen, m, k, dtype=dt), rnd(gen, n, k, scale=k ** -0.5, dtype=dt), rnd(gen, n, dtype=dt), rnd(gen, m, n, dtype=dt)
+    z, size, y, d = product_ref(x, w, b, None, act)
+    if act == "lrelu":          # next to the kink the sign of z decides: those outputs get no gradient
+        dy = torch.where(z.abs() < 2 * (k + 10) * U32 * size, torch.zeros_like(dy), dy)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    r = torch.zeros(m, n, dtype=dt).cuda().requires_grad_(True)
+    out = pw().linear(leaves[0], leaves[1], bias=leaves[2], act=act, residual=r)
+    gx, gw, gb, gr = torch.autograd.grad(out, leaves + [r], dy.cuda())
+    assert torch.equal(gr.cpu(), dy)
+    X, W, D = x.double(), w.double(), dy.double()
+    dz = D * d
+    # how far dz is off: its rounding, the kept derivative's half step, the derivative's own error from z's (second derivatives below 1)
+    off = dz.abs() * u(dt) + D.abs() * (0 if act in ("none",) else 2.0 ** -16 + 2.0 ** -20 + (0 if act == "lrelu" else (k + 10) * U32 * size)) + TINY[dt]
+    for got, want, mag, err, terms in ((gx, dz @ W, dz.abs() @ W.abs(), off @ W.abs(), n), (gw, dz.t() @ X, dz.abs().t() @ X.abs(), off.t() @ X.abs(), m),
+                                       (gb, dz.sum(0), dz.abs().sum(0), off.sum(0), m)):
+        within(got, want, (want.abs() + err) * u(dt) * 1.01 + err + (terms + 10) * U32 * mag * 1.01 + TINY[dt])
+
+
+@pytest.mark.parametrize("out", T16 + [torch.float32])
+@pytest.mark.parametrize("m,k,n", [(1, 16, 16), (5, 51, 30), (16, 4096, 64), (17, 128, 129), (130, 272, 72), (300, 1000, 260)])
+def test_product_q8(out, m, k, n):
+    gen = torch.Generator().manual_seed(m + k + n)
+    q = rnd(gen, m, k, scale=30.0).clamp(-448, 448).to(torch.float8_e4m3fn)
+    xs = torch.rand(m, generator=gen) * 0.01 + 0.001
+    wq, ws = pw().quantize_rows(rnd(gen, n, k, scale=k ** -0.5))
+    b, r = rnd(gen, n, dtype=out), rnd(gen, m, n, dtype=out)
+    for act in ("none", "silu"):
+        z, size, y, _ = product_ref(q.float(), wq.float(), b, r, act, (xs, ws))
+        got = pw().linear_q8(q.cuda(), xs.cuda(), wq.cuda(), ws.cuda(), bias=b.cuda(), act=act, residual=r.cuda(), out_dtype=out)
+        assert got.dtype == out
+        within(got, y, product_bound(out, k, z, size, y))
+
+
+def test_product_reads_any_pitch_offset_and_order():
+    gen = torch.Generator().manual_seed(9)
+    for dt in T16:
+        xw, ww = rnd(gen, 70, 150, dtype=dt), rnd(gen, 60, 131, dtype=dt)
+        x, w = xw[:, 5:133], ww[:48, 2:130]
+        y = pw().linear(x.cuda(), w.cuda())
+        z, size, ref, _ = product_ref(x, w, None, None, "none")
+        within(y, ref, product_bound(dt, 128, z, size, ref))
+        xt = xw.t()[:64]                                       # (64, 70): columns are contiguous, rows are not
+        wt = ww.t()[:70, :50].t()
+        y = pw().linear(xt.cuda(), wt.cuda())
+        z, size, ref, _ = product_ref(xt, wt, None, None, "none")
+        within(y, ref, product_bound(dt, 70, z, size, ref))
+        x3 = rnd(gen, 3, 4, 5, 24, dtype=dt)
+        r3 = rnd(gen, 3, 5, 4, 48, dtype=dt).transpose(1, 2)
+        y = pw().linear(x3.cuda(), ww[:48, :24].contiguous().cuda(), residual=r3.cuda())
+        z, size, ref, _ = product_ref(x3.reshape(60, 24), ww[:48, :24], None, r3.reshape(60, 48), "none")
+        assert y.shape == (3, 4, 5, 48)
+        within(y.view(60, 48), ref, product_bound(dt, 24, z, size, ref))
+
+
+def test_product_without_rows():
+    x, w, b = (torch.zeros(*s, dtype=torch.float16).cuda().requires_grad_(True) for s in ((0, 40), (24, 40), (24,)))
+    y = pw().linear(x, w, bias=b, act="gelu")
+    y.sum().backward()
+    assert y.shape == (0, 24) and not w.grad.any() and not b.grad.any() and x.grad.shape == (0, 40)
+
+
+def test_product_values_that_are_not_finite_stay_in_their_row():
+    gen = torch.Generator().manual_seed(4)
+    for m in (4, 80):
+        x, w, r = rnd(gen, m, 64, dtype=torch.bfloat16).cuda(), rnd(gen, 48, 64, dtype=torch.bfloat16).cuda(), rnd(gen, m, 48, dtype=torch.bfloat16).cuda()
+        for act in ("none", "relu", "lrelu", "gelu", "silu"):
+            clean = pw().linear(x, w, act=act, residual=r)
+            bad = x.clone()
+            bad[1, 3], bad[3] = float("nan"), 0
+            y = pw().linear(bad, w, act=act, residual=r)
+            assert torch.equal(y[0], clean[0]) and torch.equal(y[2], clean[2]) and torch.isnan(y[1]).all()
+            assert torch.equal(y[3], r[3])
+        one, big = torch.ones(m, 1, dtype=torch.bfloat16).cuda(), torch.full((48, 1), float("inf"), dtype=torch.bfloat16).cuda()
+        big[24:] = float("-inf")
+        for act in ("relu", "gelu", "silu"):
+            leaf = one.clone().requires_grad_(True)
+            bias = torch.zeros(48, dtype=torch.bfloat16).cuda().requires_grad_(True)
+            y = pw().linear(leaf, big, bias=bias, act=act)
+            assert (y[:, :24] == float("inf")).all() and not y[:, 24:].any(), act
+            y.sum().backward()
+            assert (bias.grad[:24] == m).all() and not bias.grad[24:].any(), act
+
+
+def test_two_calls_give_the_same_bits():
+    gen = torch.Generator().manual_seed(8)
+    x, w, b, dy = rnd(gen, 3000, 72, dtype=torch.bfloat16).cuda(), rnd(gen, 40, 72, dtype=torch.bfloat16).cuda(), rnd(gen, 40, dtype=torch.bfloat16).cuda(), rnd(gen, 3000, 40, dtype=torch.bfloat16).cuda()
+    n = (torch.rand(72, generator=gen) + 0.5).cuda()
+
+    def run():
+        leaves = [t.clone().requires_grad_(True) for t in (x, w, b, n)]
+        y = pw().linear(pw().rms_norm(leaves[0], leaves[3])[0], leaves[1], bias=leaves[2], act="gelu")
+        return [y] + list(torch.autograd.grad(y, leaves, dy))
+    for a, c in zip(run(), run()):
+        assert torch.equal(a, c)
+
+
+def test_on_another_stream_and_twice_at_once():
+    gen = torch.Generator().manual_seed(18)
+    x, w, r = rnd(gen, 500, 2056, dtype=torch.float16).cuda(), rnd(gen, 66, 2056, scale=0.02, dtype=torch.float16).cuda(), rnd(gen, 500, 66, dtype=torch.float16).cuda()
+    want = pw().linear(x, w, act="silu", residual=r)
+    torch.cuda.synchronize()
+    from selfc_amd import runtime as rt
+    streams = rt.distinct_streams(2)
+    outs = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            outs.append([pw().linear(x, w, act="silu", residual=r) for _ in range(4)])
+    torch.cuda.synchronize()
+    for o in outs[0] + outs[1]:
+        assert torch.equal(o, want)
+
+
+def test_captured_forward_and_backward_replay():
+    """One captured training pass of a layer, replayed with new inputs between eager calls; and a refused capture."""
+    from selfc_amd import runtime as rt
+    gen = torch.Generator().manual_seed(21)
+    dt = torch.bfloat16
+    w1, w2, nw = rnd(gen, 96, 40, scale=0.2, dtype=dt).cuda(), rnd(gen, 40, 96, scale=0.2, dtype=dt).cuda(), (rnd(gen, 40) + 1).cuda()
+    leaves = [t.requires_grad_(True) for t in (w1, w2, nw)]
+    x, dy = rnd(gen, 300, 40, dtype=dt).cuda(), rnd(gen, 300, 40, dtype=dt).cuda()
+
+    def run(x_):
+        y, h = pw().rms_norm(x_, leaves[2])
+        out = pw().linear(pw().linear(y, leaves[0], act="gelu"), leaves[1], residual=h)
+        return [out.detach()] + list(torch.autograd.grad(out, leaves, dy))
+
+    s = rt.warmup_stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        run(x)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    static = x.clone()
+    g = rt.new_graph()
+    with rt.graph_capture(g, x.device):
+        got = run(static)
+    for k in range(4):
+        fresh = rnd(gen, 300, 40, dtype=dt).cuda()
+        static.copy_(fresh)
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, run(fresh)):
+            assert torch.equal(a, b), k

@@ -1,0 +1,123 @@
+"""What rms_norm, linear and the AdamW step refuse, without a GPU: checks of arguments come before any launch."""
+import ctypes as C
+
+import pytest
+import torch
+
+from selfc_amd import _lib, optim, pointwise as pw
+
+
+def f(*s, dt=torch.float16):
+    return torch.zeros(*s, dtype=dt)
+
+
+@pytest.fixture
+def on_cpu(monkeypatch):
+    """the checks behind the device's: shapes and types of CPU tensors, with every launch turned into an error"""
+    monkeypatch.setattr(_lib, "require_gpu", lambda t: None)
+    monkeypatch.setattr(pw.rt, "call", lambda *a: pytest.fail("launched"))
+
+
+def test_cpu_tensors_are_refused():
+    for call in (lambda: pw.rms_norm(f(2, 4), f(4)), lambda: pw.rms_norm_q8(f(2, 4), f(4)), lambda: pw.linear(f(2, 4), f(3, 4)),
+                 lambda: pw.linear_q8(f(2, 4).to(torch.float8_e4m3fn), f(2, dt=torch.float32), f(3, 4).to(torch.float8_e4m3fn), f(3, dt=torch.float32)),
+                 lambda: optim.grad_norm([f(3)]), lambda: optim.adamw_step([f(3)], [f(3)], f(256, dt=torch.float32), f(256, dt=torch.float32), step=1, lr=1e-3)):
+        with pytest.raises(RuntimeError, match="MI355X"):
+            call()
+
+
+@pytest.mark.parametrize("call,what", [
+    (lambda: pw.rms_norm(f(2, 4, dt=torch.float64), f(4, dt=torch.float64)), "float64"),
+    (lambda: pw.rms_norm(f(2, 4), f(4, dt=torch.bfloat16)), "weight"),
+    (lambda: pw.rms_norm(f(2, 4), f(5)), "weight"),
+    (lambda: pw.rms_norm(f(2, 4), f(4), residual=f(3, 4)), "residual"),
+    (lambda: pw.rms_norm(f(2, 4), f(4), residual=f(2, 4, dt=torch.bfloat16)), "residual"),
+    (lambda: pw.rms_norm(f(1, 16385), f(16385)), "16384"),
+    (lambda: pw.rms_norm(f(2, 0), f(0)), "rows of"),
+    (lambda: pw.rms_norm(f(2, 4), f(4), eps=-1.0), "eps"),
+    (lambda: pw.linear(f(2, 4), f(3, 5)), "weight"),
+    (lambda: pw.linear(f(2, 4), f(3, 4, dt=torch.bfloat16)), "weight"),
+    (lambda: pw.linear(f(2, 4, dt=torch.float32), f(3, 4, dt=torch.float32)), "float32"),
+    (lambda: pw.linear(f(2, 4), f(3, 4), bias=f(4)), "bias"),
+    (lambda: pw.linear(f(2, 4), f(3, 4), residual=f(2, 4)), "residual"),
+    (lambda: pw.linear(f(2, 4), f(3, 4), act="tanh"), "act"),
+    (lambda: pw.linear(f(2, 0), f(3, 0)), "weight"),
+])
+def test_shapes_and_types_are_checked(on_cpu, call, what):
+    with pytest.raises(RuntimeError, match=what):
+        call()
+
+
+def test_q8_forms_have_no_gradient(on_cpu):
+    w = torch.zeros(4, dtype=torch.float16, requires_grad=True)
+    with pytest.raises(NotImplementedError):
+        pw.rms_norm_q8(f(2, 4), w)
+    e = torch.float8_e4m3fn
+    with pytest.raises(NotImplementedError):
+        pw.linear_q8(f(2, 4).to(e), f(2, dt=torch.float32), f(4, 4).to(e), f(4, dt=torch.float32), bias=w, out_dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="x_scale"):
+        pw.linear_q8(f(2, 4).to(e), f(3, dt=torch.float32), f(4, 4).to(e), f(4, dt=torch.float32))
+    with pytest.raises(RuntimeError, match="out_dtype"):
+        pw.linear_q8(f(2, 4).to(e), f(2, dt=torch.float32), f(4, 4).to(e), f(4, dt=torch.float32), out_dtype=torch.float64)
+
+
+def test_quantize_rows():
+    w = torch.randn(5, 40)
+    w[2] = 0
+    q, s = pw.quantize_rows(w)
+    assert q.dtype == torch.float8_e4m3fn and s[2] == 1 and not q[2].float().any()
+    assert ((q.float() * s[:, None] - w).abs() <= w.abs() * 2.0 ** -4 * 1.001 + s[:, None] * 2.0 ** -10).all()
+
+
+def test_adamw_step_checks(monkeypatch):
+    monkeypatch.setattr(_lib, "require_gpu", lambda t: None)
+    monkeypatch.setattr(optim.rt, "call", lambda *a: pytest.fail("launched"))
+    m = lambda n, dt=torch.float32: torch.zeros(n, dtype=dt)  # noqa: E731
+    ok = dict(step=1, lr=1e-3)
+    with pytest.raises(RuntimeError, match="gradient 0"):
+        optim.adamw_step([m(3)], [m(4)], m(256), m(256), **ok)
+    with pytest.raises(RuntimeError, match="tensor 1"):
+        optim.adamw_step([m(3), m(3, torch.float16)], [m(3), m(3, torch.float16)], m(512), m(512), **ok)
+    with pytest.raises(RuntimeError, match="exp_avg"):
+        optim.adamw_step([m(257)], [m(257)], m(256), m(512), **ok)
+    with pytest.raises(RuntimeError, match="scales"):
+        optim.adamw_step([m(3)], [m(3)], m(256, torch.float8_e4m3fn), m(256, torch.float8_e5m2), **ok)
+    with pytest.raises(RuntimeError, match="moments"):
+        optim.adamw_step([m(3)], [m(3)], m(256, torch.float16), m(256), **ok)
+    with pytest.raises(RuntimeError, match="step"):
+        optim.adamw_step([m(3)], [m(3)], m(256), m(256), step=0, lr=1e-3)
+    with pytest.raises(RuntimeError, match="stretch"):
+        t = torch.zeros(4, 6)[:, :3]
+        optim.adamw_step([t], [t], m(256), m(256), **ok)
+    with pytest.raises(RuntimeError, match="betas"):
+        optim.adamw_step([m(3)], [m(3)], m(256), m(256), beta1=1.0, **ok)
+    optim.adamw_step([], [], m(0), m(0), **ok)
+
+
+def test_c_entries_refuse_without_launching():
+    L = _lib.lib()
+    one = C.c_void_p(16)          # never read: every call below is refused by its arguments
+    assert L.selfc_rmsnorm(None, 4, None, 4, one, 1, None, one, None, 2, 4, 2, 1e-6, None) == -1
+    assert L.selfc_rmsnorm(one, 4, one, 4, one, 1, None, one, None, 2, 4, 2, 1e-6, None) == -1           # a residual without its sum
+    assert L.selfc_rmsnorm(one, 4, None, 4, one, 1, None, one, None, 2, 16385, 2, 1e-6, None) == -1
+    assert L.selfc_rmsnorm(one, 4, None, 4, one, 1, None, one, None, 0, 4, 2, 1e-6, None) == 0           # no rows
+    assert L.selfc_linear(C.c_void_p(8), 8, one, 8, None, None, None, 0, None, 0, one, None, None, 2, 8, 8, 2, 2, None) == -1   # not aligned
+    assert L.selfc_linear(one, 9, one, 8, None, None, None, 0, None, 0, one, None, None, 2, 8, 8, 2, 2, None) == -1             # pitch
+    assert L.selfc_linear(one, 8, one, 8, None, None, None, 7, None, 0, one, None, None, 2, 8, 8, 2, 2, None) == -1             # activation
+    assert L.selfc_linear(one, 16, one, 16, None, None, None, 0, None, 0, one, None, None, 2, 8, 16, 3, 2, None) == -1          # scales missing
+    assert L.selfc_linear(one, 8192, one, 8192, None, None, None, 0, None, 0, one, None, None, 64, 64, 8192, 2, 2, None) == -1  # workspace missing
+    assert L.selfc_linear_ws_floats(64, 64, 8192, 2) > 0 and L.selfc_linear_ws_floats(0, 64, 64, 2) == 0
+    assert L.selfc_linear_dw(one, 8, one, 8, one, None, 0, 8, 8, 2, None) == -1
+    assert L.selfc_pack_rows(one, 5, one, 2, 5, 7, 2, None) == -1
+    assert L.selfc_adamw_block() == optim.BLOCK
+
+
+def test_nets_in_the_dense_blocks_layout_refuse_ffnet():
+    from selfc_amd.modules import SelfC_GMM_arch_inv as big
+    from selfc_amd.modules.Subnet_constructor import FFNet, subnet
+    with pytest.raises(NotImplementedError, match="FFNet"):
+        big.SelfCInvNet({"global_module": "nonlocal", "stp_blk_num": 2, "fh_loss": "l2", "scale": 4, "gmm_k": 5}, 3, 3, "FFNet", [1, 1], 2)
+    net = subnet("FFNet", "xavier")(9, 3)
+    assert isinstance(net, FFNet) and net.width == 64 and not net.out.weight.any()
+    with pytest.raises(NotImplementedError):
+        FFNet(3, 3, width=20)
