@@ -4,22 +4,23 @@
 ``train.RescaleTrainer`` uses for ``train_opt["optimizer"] == "AdamW"``."""
 from __future__ import annotations
 
+from operator import attrgetter
 from typing import List, Optional, Sequence
 
 import numpy as np
 import torch
 
 from . import _lib, runtime as rt
-from .pointwise import on_device
+from .pointwise import _stream, on_device
 
 #: values that share a scale of the 8-bit moments; every tensor's moments start at a multiple of it
 BLOCK = 256
 _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def _need(cond, what: str):
+def _need(cond, what):
     if not cond:
-        raise RuntimeError("selfc_amd: " + what)
+        raise RuntimeError("selfc_amd: " + (what if isinstance(what, str) else what()))
 
 
 def state_size(numels: Sequence[int]) -> int:
@@ -37,46 +38,61 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+_T = torch.Tensor
+_dtype_of = attrgetter("dtype")
+
+
+def _one_kind(ts, first, what):
+    """All tensors of the first one's type on its GPU (checked for hundreds of tensors per step: in whole-list passes)."""
+    dt, dev = first.dtype, first.get_device()
+    if set(map(_dtype_of, ts)) != {dt} or set(map(_T.get_device, ts)) != {dev}:
+        i, t = next((i, t) for i, t in enumerate(ts) if t.dtype is not dt or t.get_device() != dev)
+        raise RuntimeError(f"selfc_amd: {what} {i} is {t.dtype} on {t.device}, expected {dt} on {first.device}: one call takes one type on one GPU")
+
+
 def _table(params, grads, steps):
-    """The C table of (parameter, gradient, step, size) per tensor, and the tensors it points to beyond the caller's own."""
+    """The C table of (parameter, gradient, step, size) per tensor, the tensors it points to beyond the caller's own, the first tensor."""
     keep = []
-    tab = np.zeros((len(grads), 4), dtype=np.uint64)
-    first = next((t for t in (params if params is not None else grads) if t is not None), None)
+    n = len(grads)
+    tab = np.zeros((n, 4), dtype=np.uint64)
+    _need(params is None or len(params) == n, lambda: f"{len(params)} tensors and {n} gradients")
+    some = [i for i, g in enumerate(grads) if g is not None]
+    live = grads if len(some) == n else [grads[i] for i in some]
+    first = params[0] if params else live[0] if live else None
     if first is None:
         return tab, keep, None
     _lib.require_gpu(first)
-    dt, dev = first.dtype, first.get_device()
-    if dt not in _DTYPE:
-        raise RuntimeError(f"selfc_amd: {dt} tensors; expected float32, bfloat16 or float16")
+    _need(first.dtype in _DTYPE, lambda: f"{first.dtype} tensors; expected float32, bfloat16 or float16")
     if params is not None:
-        _need(len(params) == len(grads), f"{len(params)} tensors and {len(grads)} gradients")
-        for i, (p, g) in enumerate(zip(params, grads)):
-            if p.dtype is not dt or p.get_device() != dev:
-                raise RuntimeError(f"selfc_amd: tensor {i} is {p.dtype} on {p.device}, the first is {dt} on {first.device}: one call takes one type on one GPU")
-            if g is None:
-                continue
-            if g.dtype is not dt or g.get_device() != dev or g.shape != p.shape:
-                raise RuntimeError(f"selfc_amd: gradient {i} is {g.dtype} {tuple(g.shape)} on {g.device}, its tensor {p.dtype} {tuple(p.shape)} on {p.device}")
-            if not (p.is_contiguous() and g.is_contiguous()):
-                _need(g.layout is torch.strided and _dense(p), f"tensor {i} does not fill one stretch of memory (strides {p.stride()})")
-                if g.stride() != p.stride():
-                    grads[i] = torch.empty_strided(p.shape, p.stride(), dtype=dt, device=p.device).copy_(g)
-                    keep.append(grads[i])
-        tab[:, 0] = [p.data_ptr() for p in params]
-        tab[:, 3] = [p.numel() for p in params]
+        _one_kind(params, first, "tensor")
+    if live:
+        _one_kind(live, first, "gradient")
+    if params is not None:
+        mine = params if len(some) == n else [params[i] for i in some]
+        if list(map(_T.size, mine)) != list(map(_T.size, live)):
+            i = next(k for k, p, g in zip(some, mine, live) if p.shape != g.shape)
+            raise RuntimeError(f"selfc_amd: gradient {i} has shape {tuple(grads[i].shape)}, its tensor {tuple(params[i].shape)}")
+        if not (all(map(_T.is_contiguous, mine)) and all(map(_T.is_contiguous, live))):
+            for i, p, g in zip(some, mine, live):
+                if not (p.is_contiguous() and g.is_contiguous()):
+                    _need(g.layout is torch.strided and _dense(p), lambda: f"tensor {i} does not fill one stretch of memory (strides {p.stride()})")
+                    if g.stride() != p.stride():
+                        grads[i] = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
+                        keep.append(grads[i])
+        tab[:, 0] = list(map(_T.data_ptr, params))
+        tab[:, 3] = list(map(_T.numel, params))
     else:
-        for i, g in enumerate(grads):
-            if g is None:
-                continue
-            if g.dtype is not dt or g.get_device() != dev:
-                raise RuntimeError(f"selfc_amd: gradient {i} is {g.dtype} on {g.device}, the first is {dt} on {first.device}: one call takes one type on one GPU")
-            if not g.is_contiguous() and not _dense(g):
-                grads[i] = g.contiguous()
+        for i in some:
+            if not grads[i].is_contiguous() and not _dense(grads[i]):
+                grads[i] = grads[i].contiguous()
                 keep.append(grads[i])
-        tab[:, 3] = [0 if g is None else g.numel() for g in grads]
-    tab[:, 1] = [0 if g is None else g.data_ptr() for g in grads]
+        tab[some, 3] = [grads[i].numel() for i in some]
+    if len(some) == n:
+        tab[:, 1] = list(map(_T.data_ptr, grads))
+    else:
+        tab[some, 1] = [grads[i].data_ptr() for i in some]
     if steps is not None:
-        tab[:, 2] = [s.data_ptr() for s in steps]
+        tab[:, 2] = list(map(_T.data_ptr, steps))
     return tab, keep, first
 
 
@@ -88,7 +104,7 @@ def grad_norm(grads: Sequence[Optional[torch.Tensor]]) -> torch.Tensor:
     with on_device(first):
         out = torch.empty((), dtype=torch.float32, device=first.device)
         part = torch.empty(_lib.lib().selfc_grad_norm_partials(len(grads)), dtype=torch.float64, device=first.device)
-        rt.call("selfc_grad_norm", tab.ctypes.data, len(grads), _DTYPE[first.dtype], part.data_ptr(), out.data_ptr(), _lib.stream_ptr())
+        rt.call("selfc_grad_norm", tab.ctypes.data, len(grads), _DTYPE[first.dtype], part.data_ptr(), out.data_ptr(), _stream(first))
     return out
 
 
@@ -107,7 +123,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     step: the number of this step (from 1 on), or a list of device scalars, one per tensor, that hold it (captured steps).
     lr: a float or a device scalar.  norm, max_norm: gradients count as scaled by min(1, max_norm / (norm + 1e-6)); norm is a device
     scalar (grad_norm); without it, it is computed here.  The gradients themselves are not changed."""
-    _need(0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0, f"betas are ({beta1}, {beta2})")
+    _need(0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0, lambda: f"betas are ({beta1}, {beta2})")
     grads = list(grads)
     steps = step if isinstance(step, (list, tuple)) else None
     tab, keep, first = _table(params, grads, steps)
@@ -115,21 +131,21 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
         return
     bits8 = exp_avg.dtype is torch.float8_e4m3fn
     if bits8:
-        _need(exp_avg_sq.dtype is torch.float8_e5m2, f"exp_avg is float8_e4m3fn, exp_avg_sq {exp_avg_sq.dtype}: expected float8_e5m2")
+        _need(exp_avg_sq.dtype is torch.float8_e5m2, lambda: f"exp_avg is float8_e4m3fn, exp_avg_sq {exp_avg_sq.dtype}: expected float8_e5m2")
         _need(exp_avg_scale is not None and exp_avg_sq_scale is not None, "8-bit moments need their scales")
     else:
-        _need(exp_avg.dtype is torch.float32 and exp_avg_sq.dtype is torch.float32, f"moments are {exp_avg.dtype} and {exp_avg_sq.dtype}: expected float32, or float8_e4m3fn and float8_e5m2")
+        _need(exp_avg.dtype is torch.float32 and exp_avg_sq.dtype is torch.float32, lambda: f"moments are {exp_avg.dtype} and {exp_avg_sq.dtype}: expected float32, or float8_e4m3fn and float8_e5m2")
     size = int((-(-tab[:, 3].astype(np.int64) // BLOCK)).sum()) * BLOCK
     for name, t, n in (("exp_avg", exp_avg, size), ("exp_avg_sq", exp_avg_sq, size)) + ((("exp_avg_scale", exp_avg_scale, size // BLOCK), ("exp_avg_sq_scale", exp_avg_sq_scale, size // BLOCK)) if bits8 else ()):
-        _need(t.device == first.device and t.is_contiguous() and t.numel() >= n, f"{name}: expected {n} contiguous values on {first.device}, got {tuple(t.shape)} on {t.device}")
-        _need(n == size or t.dtype is torch.float32, f"{name} is {t.dtype}, expected float32")
+        _need(t.device == first.device and t.is_contiguous() and t.numel() >= n, lambda: f"{name}: expected {n} contiguous values on {first.device}, got {tuple(t.shape)} on {t.device}")
+        _need(n == size or t.dtype is torch.float32, lambda: f"{name} is {t.dtype}, expected float32")
     if steps is not None:
         _need(len(steps) == len(grads) and all(s.dtype is torch.float32 and s.get_device() == first.get_device() and s.numel() == 1 for s in steps),
               "step: expected a float32 scalar on the tensors' GPU for each tensor")
         host_step = 1.0
     else:
         host_step = float(step)
-        _need(host_step >= 1 and host_step == int(host_step), f"step is {step}: steps are counted from 1")
+        _need(host_step >= 1 and host_step == int(host_step), lambda: f"step is {step}: steps are counted from 1")
         _need(not torch.cuda.is_current_stream_capturing(), "a captured step needs its number on the device (AdamW(..., capturable=True))")
     lr_dev = lr if torch.is_tensor(lr) and lr.is_cuda else None
     if lr_dev is not None:
@@ -144,7 +160,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
         rt.call("selfc_adamw_step", tab.ctypes.data, len(grads), _DTYPE[first.dtype], 8 if bits8 else 32, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
                 rt._ptr(exp_avg_scale) if bits8 else None, rt._ptr(exp_avg_sq_scale) if bits8 else None, 0.0 if lr_dev is not None else float(lr),
                 rt._ptr(lr_dev), float(beta1), float(beta2), float(eps), float(weight_decay), host_step, int(seed) & 0xFFFFFFFF, rt._ptr(norm),
-                float(max_norm or 0.0), _lib.stream_ptr())
+                float(max_norm or 0.0), _stream(first))
     del keep
     # the kernel wrote through raw pointers: autograd's saved-tensor checks and the packed-weight caches go by version
     torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])

@@ -14,7 +14,6 @@ Refused with an exception: tensors that are not on one GPU, types other than the
 """
 from __future__ import annotations
 
-import ctypes as C
 from contextlib import nullcontext
 from typing import Optional, Tuple
 
@@ -31,50 +30,62 @@ MAX_LINEAR = 1 << 20
 E4M3_MAX = 448.0
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_HERE = nullcontext()
+
+
 def on_device(t: torch.Tensor):
     """The tensor's device as the current one for the duration of a launch."""
-    return nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+    return _HERE if t.get_device() == _current_device() else torch.cuda.device(t.device)
 
 
-def _need(cond, what: str):
-    if not cond:
-        raise RuntimeError("selfc_amd: " + what)
+def _stream(t: torch.Tensor) -> int:
+    """hipStream_t of the current stream of the tensor's device."""
+    return _raw_stream(t.get_device())
 
 
-def _same_device(first: torch.Tensor, **others):
+def _bad(what: str):
+    raise RuntimeError("selfc_amd: " + what)
+
+
+def _elsewhere(first, **others):
     _lib.require_gpu(first)
     for name, t in others.items():
         if t is not None and t.device != first.device:
-            raise RuntimeError(f"selfc_amd: {name} is on {t.device}, the rows are on {first.device}")
+            _bad(f"{name} is on {t.device}, the rows are on {first.device}")
 
 
-def _typed(name: str, t: torch.Tensor, *dtypes):
-    if t.dtype not in dtypes:
-        raise RuntimeError(f"selfc_amd: {name} is {t.dtype}, expected {' or '.join(_NAMES[d] for d in dtypes)}")
+def _bad_type(name: str, t: torch.Tensor, *dtypes):
+    _bad(f"{name} is {t.dtype}, expected {' or '.join(_NAMES[d] for d in dtypes)}")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """(..., C) as a matrix whose rows are contiguous and do not overlap (a view where one exists)."""
-    t = t.reshape(-1, t.shape[-1])
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.is_contiguous():
+        return t
     if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
         t = t.contiguous()
     return t
 
 
 def _pitch(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
+    rows, cols = t.shape
+    return t.stride(0) if rows > 1 else max(cols, 1)
 
 
 def _pieces(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """(matrix, pitch) that the product's kernels can read: 16-byte aligned rows of whole 16-byte pieces."""
     es, (rows, cols) = t.element_size(), t.shape
     per = 16 // es
-    ld = _pitch(t)
-    if t.data_ptr() % 16 == 0 and cols % per == 0 and (rows == 1 or ld % per == 0) and ld < (1 << 21):
-        return t, ld if rows > 1 else cols
+    ld = t.stride(0) if rows > 1 else cols
+    if not t.data_ptr() % 16 and not cols % per and not ld % per and ld < (1 << 21):
+        return t, ld
     ldd = -(-cols // per) * per
     out = torch.empty((rows, ldd), dtype=t.dtype, device=t.device)
-    rt.call("selfc_pack_rows", t.data_ptr(), ld, out.data_ptr(), rows, cols, ldd, es, _lib.stream_ptr())
+    rt.call("selfc_pack_rows", t.data_ptr(), ld, out.data_ptr(), rows, cols, ldd, es, _stream(t))
     return out, ldd
 
 
@@ -89,43 +100,64 @@ _ptr = rt._ptr
 _EAGER = "selfc_amd_eager_graph"
 
 
-def _watch_leaves(*tensors):
+def _watch(out: torch.Tensor):
     """A leaf's gradient accumulator lives as long as a graph that reaches it and remembers the stream it was made on.  If an eager
     graph is still alive when a captured backward pass reaches the same leaf, autograd waits for that stream inside the capture and
-    the process ends.  So: accumulators that an eager call reaches are marked, and a call under capture that meets one refuses."""
+    the process ends.  So: the accumulators that an eager call reaches are marked with its stream, and a call under capture that meets
+    another stream's mark refuses."""
+    here = _raw_stream(out.get_device())
     capturing = torch.cuda.is_current_stream_capturing()
-    for t in tensors:
-        if t is not None and t.requires_grad and t.is_leaf:
-            meta = torch.autograd.graph.get_gradient_edge(t).node.metadata
-            if not capturing:
-                meta[_EAGER] = torch.cuda.current_stream(t.device).cuda_stream
-            elif meta.get(_EAGER, None) not in (None, torch.cuda.current_stream(t.device).cuda_stream):
-                raise RuntimeError("selfc_amd: a graph of an earlier eager call over the same parameters is still alive; its gradients cannot "
-                                   "be accumulated inside a capture - drop that call's outputs and losses first")
+    for node, _ in out.grad_fn.next_functions:
+        if node is None:
+            continue
+        if not hasattr(node, "variable"):                # rows of a leaf with more axes: a view in between
+            node = next((n for n, _ in node.next_functions if n is not None and hasattr(n, "variable")), None)
+            if node is None:
+                continue
+        meta = node.metadata
+        if not capturing:
+            meta[_EAGER] = here
+        elif meta.get(_EAGER, here) != here:
+            _bad("a graph of an earlier eager call over the same parameters is still alive; its gradients cannot be accumulated inside a "
+                 "capture - drop that call's outputs and losses first")
+
+
+def _no_second(ctx):
+    if torch.is_grad_enabled():
+        _bad("no second derivatives (create_graph=True)")
 
 
 # -- norm ------------------------------------------------------------------------------------------------------------------------
 def _norm_args(x, weight, residual, eps):
-    _same_device(x, weight=weight, residual=residual)
-    _typed("x", x, torch.bfloat16, torch.float16, torch.float32)
-    _typed("weight", weight, *{x.dtype, torch.float32})
-    _need(x.dim() >= 1 and 1 <= x.shape[-1] <= MAX_NORM_COLS, f"rms_norm takes rows of 1 to {MAX_NORM_COLS} values, got {tuple(x.shape)}")
-    _need(weight.shape == (x.shape[-1],), f"weight has shape {tuple(weight.shape)}, the rows have {x.shape[-1]} values")
-    _need(eps >= 0, f"eps is {eps}")
+    dt, shape, dev = x.dtype, x.shape, x.device
+    if not x.is_cuda or weight.device != dev or (residual is not None and residual.device != dev):
+        _elsewhere(x, weight=weight, residual=residual)
+    if dt is not torch.bfloat16 and dt is not torch.float16 and dt is not torch.float32:
+        _bad_type("x", x, torch.bfloat16, torch.float16, torch.float32)
+    if weight.dtype is not dt and weight.dtype is not torch.float32:
+        _bad_type("weight", weight, *{dt, torch.float32})
+    if not shape or not 1 <= shape[-1] <= MAX_NORM_COLS:
+        _bad(f"rms_norm takes rows of 1 to {MAX_NORM_COLS} values, got {tuple(shape)}")
+    if weight.dim() != 1 or weight.shape[0] != shape[-1]:
+        _bad(f"weight has shape {tuple(weight.shape)}, the rows have {shape[-1]} values")
+    if not eps >= 0:
+        _bad(f"eps is {eps}")
     if residual is not None:
-        _typed("residual", residual, x.dtype)
-        _need(residual.shape == x.shape, f"residual has shape {tuple(residual.shape)}, x {tuple(x.shape)}")
+        if residual.dtype is not dt:
+            _bad_type("residual", residual, dt)
+        if residual.shape != shape:
+            _bad(f"residual has shape {tuple(residual.shape)}, x {tuple(shape)}")
 
 
 def _run_norm(x2, r2, weight, eps, q8: bool):
     rows, cols = x2.shape
-    dev = x2.device
-    y = torch.empty((rows, cols), dtype=torch.float8_e4m3fn if q8 else x2.dtype, device=dev)
+    dev, dt = x2.device, x2.dtype
+    y = torch.empty((rows, cols), dtype=torch.float8_e4m3fn if q8 else dt, device=dev)
     scale = torch.empty(rows, dtype=torch.float32, device=dev) if q8 else None
-    h = torch.empty((rows, cols), dtype=x2.dtype, device=dev) if r2 is not None else None
+    h = torch.empty((rows, cols), dtype=dt, device=dev) if r2 is not None else None
     if rows:
         rt.call("selfc_rmsnorm", x2.data_ptr(), _pitch(x2), _ptr(r2), 0 if r2 is None else _pitch(r2), weight.data_ptr(),
-                int(weight.dtype == torch.float32), _ptr(h), y.data_ptr(), _ptr(scale), rows, cols, _DTYPE[x2.dtype], eps, _lib.stream_ptr())
+                weight.dtype is torch.float32, _ptr(h), y.data_ptr(), _ptr(scale), rows, cols, _DTYPE[dt], eps, _stream(x2))
     return y, scale, h
 
 
@@ -142,13 +174,13 @@ class RMSNormFn(torch.autograd.Function):
         return (y,) if h is None else (y, h)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dh=None):
+        _no_second(ctx)
         h, weight = ctx.saved_tensors
-        want_w = ctx.needs_input_grad[2]
-        want_x = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        to_x, to_r, want_w, _ = ctx.needs_input_grad
+        want_x = to_x or to_r
         if dy is None:                     # only h was used
-            return (dh if ctx.needs_input_grad[0] else None), (dh if ctx.needs_input_grad[1] else None), None, None
+            return (dh if to_x else None), (dh if to_r else None), None, None
         rows, cols = h.shape
         dy = dy.contiguous()
         dh = dh.contiguous() if dh is not None else None
@@ -157,11 +189,11 @@ class RMSNormFn(torch.autograd.Function):
             dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if want_w else None
             part = torch.empty(_lib.lib().selfc_rmsnorm_bwd_floats(rows, cols), dtype=torch.float32, device=h.device) if want_w else None
             if rows:
-                rt.call("selfc_rmsnorm_bwd", h.data_ptr(), _pitch(h), weight.data_ptr(), int(weight.dtype == torch.float32), dy.data_ptr(), _ptr(dh),
-                        _ptr(dx), _ptr(dw), _ptr(part), rows, cols, _DTYPE[h.dtype], ctx.eps, _lib.stream_ptr())
+                rt.call("selfc_rmsnorm_bwd", h.data_ptr(), _pitch(h), weight.data_ptr(), weight.dtype is torch.float32, dy.data_ptr(), _ptr(dh),
+                        _ptr(dx), _ptr(dw), _ptr(part), rows, cols, _DTYPE[h.dtype], ctx.eps, _stream(h))
             elif dw is not None:
                 dw.zero_()
-        return (dx if ctx.needs_input_grad[0] else None), (dx if ctx.needs_input_grad[1] else None), dw, None
+        return (dx if to_x else None), (dx if to_r else None), dw, None
 
 
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -170,13 +202,16 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     x: bf16, f16 or fp32 rows of up to 16,384 values; weight: x's type or fp32.  Statistics and the weight's gradient are summed in
     fp32 in a fixed order.  Gradients flow to x, residual and weight, from y and h."""
     _norm_args(x, weight, residual, eps)
-    weight = weight.contiguous()
+    x2, r2, weight = _rows(x), None if residual is None else _rows(residual), weight.contiguous()
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
-        _watch_leaves(x, residual, weight)
-        out = RMSNormFn.apply(_rows(x), None if residual is None else _rows(residual), weight, float(eps))
-        return out[0].view(x.shape), (x if residual is None else out[1].view(x.shape))
-    with on_device(x):
-        y, _, h = _run_norm(_rows(x), None if residual is None else _rows(residual), weight, float(eps), False)
+        out = RMSNormFn.apply(x2, r2, weight, float(eps))
+        _watch(out[0])
+        y, h = out if r2 is not None else (out[0], None)
+    else:
+        with on_device(x):
+            y, _, h = _run_norm(x2, r2, weight, float(eps), False)
+    if x.dim() == 2:
+        return y, (x if h is None else h)
     return y.view(x.shape), (x if h is None else h.view(x.shape))
 
 
@@ -196,22 +231,27 @@ def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.
 
 
 # -- product ---------------------------------------------------------------------------------------------------------------------
-def _linear_args(x, weight, bias, act, residual, *dtypes, out_dtype=None):
-    _same_device(x, weight=weight, bias=bias, residual=residual)
-    _typed("x", x, *dtypes)
-    _typed("weight", weight, x.dtype)
-    _need(weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1] and weight.shape[0] >= 1 and weight.shape[1] >= 1,
-          f"x {tuple(x.shape)} does not go with weight {tuple(weight.shape)} (out, in)")
-    _need(max(weight.shape) <= MAX_LINEAR, f"weight {tuple(weight.shape)}: at most {MAX_LINEAR} inputs and outputs")
-    out_dtype = out_dtype or x.dtype
+def _linear_args(x, weight, bias, act, residual, out_dtype):
+    """checks what `linear` and `linear_q8` share; the rows' type is the caller's to check"""
+    dev, shape = x.device, x.shape
+    if not x.is_cuda or weight.device != dev or (bias is not None and bias.device != dev) or (residual is not None and residual.device != dev):
+        _elsewhere(x, weight=weight, bias=bias, residual=residual)
+    if weight.dtype is not x.dtype:
+        _bad_type("weight", weight, x.dtype)
+    if weight.dim() != 2 or not shape or weight.shape[1] != shape[-1] or not 1 <= shape[-1] <= MAX_LINEAR or not 1 <= weight.shape[0] <= MAX_LINEAR:
+        _bad(f"x {tuple(shape)} does not go with weight {tuple(weight.shape)}: (out, in) of 1 to {MAX_LINEAR}")
     if act not in ACTS:
-        raise RuntimeError(f"selfc_amd: act is {act!r}, expected one of {sorted(k for k in ACTS if k)}")
+        _bad(f"act is {act!r}, expected one of {sorted(k for k in ACTS if k)}")
     if bias is not None:
-        _typed("bias", bias, out_dtype)
-        _need(bias.shape == (weight.shape[0],), f"bias has shape {tuple(bias.shape)}, expected ({weight.shape[0]},)")
+        if bias.dtype is not out_dtype:
+            _bad_type("bias", bias, out_dtype)
+        if bias.dim() != 1 or bias.shape[0] != weight.shape[0]:
+            _bad(f"bias has shape {tuple(bias.shape)}, expected ({weight.shape[0]},)")
     if residual is not None:
-        _typed("residual", residual, out_dtype)
-        _need(residual.shape == x.shape[:-1] + (weight.shape[0],), f"residual has shape {tuple(residual.shape)}, expected {tuple(x.shape[:-1]) + (weight.shape[0],)}")
+        if residual.dtype is not out_dtype:
+            _bad_type("residual", residual, out_dtype)
+        if residual.shape != shape[:-1] + weight.shape[:1]:
+            _bad(f"residual has shape {tuple(residual.shape)}, expected {tuple(shape[:-1] + weight.shape[:1])}")
 
 
 def _run_linear(xp, ldx, k, wp, ldw, n, xs, ws_, bias, act, r2, out_dtype, want_slope):
@@ -219,11 +259,11 @@ def _run_linear(xp, ldx, k, wp, ldw, n, xs, ws_, bias, act, r2, out_dtype, want_
     y = torch.empty((rows, n), dtype=out_dtype, device=dev)
     slope = torch.empty((rows, -(-n // 8) * 8), dtype=torch.int16, device=dev) if want_slope else None
     if rows:
-        per = 16 // xp.element_size()
-        work = _ws(rows, n, -(-k // per) * per, xp.element_size(), dev)
+        es = xp.element_size()
+        k = -(-k * es // 16) * 16 // es
+        work = _ws(rows, n, k, es, dev) if rows > 16 else None
         rt.call("selfc_linear", xp.data_ptr(), ldx, wp.data_ptr(), ldw, _ptr(xs), _ptr(ws_), _ptr(bias), act, _ptr(r2),
-                0 if r2 is None else _pitch(r2), y.data_ptr(), _ptr(slope), _ptr(work), rows, n, -(-k // per) * per, _DTYPE[xp.dtype], _DTYPE[out_dtype],
-                _lib.stream_ptr())
+                0 if r2 is None else _pitch(r2), y.data_ptr(), _ptr(slope), _ptr(work), rows, n, k, _DTYPE[xp.dtype], _DTYPE[out_dtype], _stream(xp))
     return y, slope
 
 
@@ -244,12 +284,12 @@ class LinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _no_second(ctx)
         xp, wp, slope = ctx.saved_tensors
         rows, n, k, ldx, ldw = ctx.dims
         want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
-        dev, dt, code = dy.device, ctx.dtype, _DTYPE[ctx.dtype]
+        dev, dt, code, stream = dy.device, ctx.dtype, _DTYPE[ctx.dtype], _stream(dy)
         dx = dw = db = None
         L = _lib.lib()
         with on_device(dy):
@@ -268,15 +308,15 @@ class LinearFn(torch.autograd.Function):
             if want_b or (products and not as_is):
                 part = torch.empty(L.selfc_linear_dz_floats(rows, n), dtype=torch.float32, device=dev) if want_b else None
                 rt.call("selfc_linear_dz", g.data_ptr(), _pitch(g), _ptr(slope), None if as_is or not products else dz.data_ptr(), up, _ptr(db), _ptr(part),
-                        rows, n, code, _lib.stream_ptr())
+                        rows, n, code, stream)
             if want_x:
                 dx = torch.empty((rows, k), dtype=dt, device=dev)
                 work = _ws(rows, k, n, 2, dev)
-                rt.call("selfc_linear_dx", dz.data_ptr(), lddz, wp.data_ptr(), ldw, dx.data_ptr(), _ptr(work), rows, n, k, code, _lib.stream_ptr())
+                rt.call("selfc_linear_dx", dz.data_ptr(), lddz, wp.data_ptr(), ldw, dx.data_ptr(), _ptr(work), rows, n, k, code, stream)
             if want_w:
                 dw = torch.empty((n, k), dtype=dt, device=dev)
                 work = _ws(n, k, rows, 2, dev)
-                rt.call("selfc_linear_dw", dz.data_ptr(), lddz, xp.data_ptr(), ldx, dw.data_ptr(), _ptr(work), rows, n, k, code, _lib.stream_ptr())
+                rt.call("selfc_linear_dw", dz.data_ptr(), lddz, xp.data_ptr(), ldx, dw.data_ptr(), _ptr(work), rows, n, k, code, stream)
         return dx, dw, db, (dy if want_r else None), None
 
 
@@ -286,23 +326,30 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     same type.  act: "none", "relu", "lrelu" (0.2), "gelu" (erf), "silu".  Sums, bias, activation and residual in fp32, one rounding at the end;
     in the backward pass dy act'(z) is rounded to x's type once, as the operand of both products.  Up to 16 rows the weight streams
     through a kernel of its own.  Sums are added in a fixed order."""
-    _linear_args(x, weight, bias, act, residual, torch.bfloat16, torch.float16)
+    dt = x.dtype
+    if dt is not torch.bfloat16 and dt is not torch.float16:
+        _lib.require_gpu(x)
+        _bad_type("x", x, torch.bfloat16, torch.float16)
+    _linear_args(x, weight, bias, act, residual, dt)
     x2, w2 = _rows(x), _rows(weight)
     b = None if bias is None else bias.contiguous()
     r2 = None if residual is None else _rows(residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
-        _watch_leaves(x, weight, bias, residual)
-        return LinearFn.apply(x2, w2, b, r2, ACTS[act]).view(x.shape[:-1] + (weight.shape[0],))
-    with on_device(x):
-        xp, ldx = _pieces(x2)
-        wp, ldw = _pieces(w2)
-        y, _ = _run_linear(xp, ldx, x2.shape[1], wp, ldw, weight.shape[0], None, None, b, ACTS[act], r2, x.dtype, False)
-    return y.view(x.shape[:-1] + (weight.shape[0],))
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        y = LinearFn.apply(x2, w2, b, r2, ACTS[act])
+        _watch(y)
+    else:
+        with on_device(x):
+            xp, ldx = _pieces(x2)
+            wp, ldw = _pieces(w2)
+            y, _ = _run_linear(xp, ldx, x2.shape[1], wp, ldw, weight.shape[0], None, None, b, ACTS[act], r2, dt, False)
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + weight.shape[:1])
 
 
 def quantize_rows(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """(q, scale) of a weight (out, in): float8_e4m3fn rows with one fp32 scale each, for linear_q8.  Done once per weight."""
-    _need(w.dim() == 2 and w.is_floating_point(), f"quantize_rows expects a float matrix, got {w.dtype} {tuple(w.shape)}")
+    if w.dim() != 2 or not w.is_floating_point():
+        _bad(f"quantize_rows expects a float matrix, got {w.dtype} {tuple(w.shape)}")
     w = w.detach().float()
     most = w.abs().amax(1) if w.shape[1] else w.new_zeros(w.shape[0])
     scale = torch.where(most > 0, (most / E4M3_MAX).clamp_(min=2.0 ** -126), torch.ones_like(most))
@@ -314,18 +361,22 @@ def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_sc
     """act(x_scale w_scale (x weight^T) + bias) + residual for float8_e4m3fn x (..., in) with a scale per row (rms_norm_q8) and weight
     (out, in) with a scale per output (quantize_rows); bias and residual of out_dtype (bf16, f16 or fp32).  For serving: no gradients."""
     if out_dtype not in (torch.bfloat16, torch.float16, torch.float32):
-        raise RuntimeError(f"selfc_amd: out_dtype is {out_dtype}")
-    _linear_args(x, weight, bias, act, residual, torch.float8_e4m3fn, out_dtype=out_dtype)
+        _bad(f"out_dtype is {out_dtype}")
+    if x.dtype is not torch.float8_e4m3fn:
+        _bad_type("x", x, torch.float8_e4m3fn)
+    _linear_args(x, weight, bias, act, residual, out_dtype)
     _no_grad_only("linear_q8", bias, residual, x_scale, w_scale)
-    _same_device(x, x_scale=x_scale, w_scale=w_scale)
-    _typed("x_scale", x_scale, torch.float32)
-    _typed("w_scale", w_scale, torch.float32)
-    _need(x_scale.shape == x.shape[:-1], f"x_scale has shape {tuple(x_scale.shape)}, expected {tuple(x.shape[:-1])}")
-    _need(w_scale.shape == weight.shape[:1], f"w_scale has shape {tuple(w_scale.shape)}, expected ({weight.shape[0]},)")
+    if x_scale.device != x.device or w_scale.device != x.device:
+        _elsewhere(x, x_scale=x_scale, w_scale=w_scale)
+    for name, t, shape in (("x_scale", x_scale, x.shape[:-1]), ("w_scale", w_scale, weight.shape[:1])):
+        if t.dtype is not torch.float32:
+            _bad_type(name, t, torch.float32)
+        if t.shape != shape:
+            _bad(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     with on_device(x):
         x2 = _rows(x)
         xp, ldx = _pieces(x2)
         wp, ldw = _pieces(_rows(weight))
         y, _ = _run_linear(xp, ldx, x2.shape[1], wp, ldw, weight.shape[0], x_scale.reshape(-1).contiguous(), w_scale.contiguous(),
                            None if bias is None else bias.contiguous(), ACTS[act], None if residual is None else _rows(residual), out_dtype, False)
-    return y.view(x.shape[:-1] + (weight.shape[0],))
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + weight.shape[:1])
