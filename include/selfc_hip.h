@@ -458,10 +458,21 @@ int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const flo
  * partial: selfc_linear_dz_floats floats (only with db). */
 size_t selfc_linear_dz_floats(size_t rows, int n);
 int selfc_linear_dz(const void* dy, size_t lddy, const void* slope, void* dz, size_t lddz, void* db, float* partial, size_t rows, int n, int dtype, void* stream);
-/* dx[rows][k] = dz w and dw[n][k] = dz^T x; dz, w, x 16-byte aligned with pitches of whole 16-byte pieces, zeros in dz behind column n.
- * ws: selfc_linear_ws_floats(rows, k, n, 2) and (n, k, rows, 2) floats.  rows >= 1 for dw. */
+/* dx[rows][k] = dz w; dw[n][k] = dz^T x and db[n] (or NULL) = dz's column sums.  dz, w, x 16-byte aligned with pitches of whole 16-byte
+ * pieces, zeros in dz behind column n.  ws: selfc_linear_ws_floats(rows, k, n, 2) and selfc_linear_dw_floats floats.  rows >= 1 for dw. */
 int selfc_linear_dx(const void* dz, size_t lddz, const void* w, size_t ldw, void* dx, float* ws, size_t rows, int n, int k, int dtype, void* stream);
-int selfc_linear_dw(const void* dz, size_t lddz, const void* x, size_t ldx, void* dw, float* ws, size_t rows, int n, int k, int dtype, void* stream);
+size_t selfc_linear_dw_floats(size_t rows, int n, int k);
+int selfc_linear_dw(const void* dz, size_t lddz, const void* x, size_t ldx, void* dw, void* db, float* ws, size_t rows, int n, int k, int dtype, void* stream);
+
+/* Narrow layers (selfc_linear_rows_ok(n, k): up to 256 each way, their weight in shared memory): bf16 / f16 rows and weights of any pitch and
+ * offset.  y without gaps, slope as above, xp (or NULL): receives x's rows with pitch roundup(k, 8) and zeros behind them (selfc_linear_dw's
+ * operand).  The backward call makes dx [rows][k] and dz (or NULL; as selfc_linear_dz) from dy and slope (or NULL: no activation).
+ * y, dx, slope, xp, dz 16-byte aligned. */
+int selfc_linear_rows_ok(int n, int k);
+int selfc_linear_rows(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, int act, const void* res, size_t ldr, void* y,
+                      void* slope, void* xp, size_t rows, int n, int k, int dtype, void* stream);
+int selfc_linear_rows_bwd(const void* dy, size_t lddy, const void* slope, const void* w, size_t ldw, void* dx, void* dz,
+                          size_t rows, int n, int k, int dtype, void* stream);
 
 /* csrc/adamw.hip.  One AdamW step of `count` tensors (a HOST array; it is read before the call returns) of one `dtype`.  A tensor
  * without a gradient is left as it is.  State: m and v hold all tensors, tensor i from the sum of roundup(n_j, selfc_adamw_block())

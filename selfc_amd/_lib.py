@@ -45,7 +45,7 @@ SYMBOLS = [
     "selfc_nchw_to_nhwc4_ind", "selfc_nhwc4_to_nchw_ind", "selfc_graph_stats",
     "selfc_fin_job_bytes", "selfc_wgrad_finish_jobs", "selfc_subnet_bwd_phase_d", "selfc_gh_bwd_pair_scratch_bytes", "selfc_gh_bwd_pair", "selfc_recon_loss_blocks", "selfc_recon_loss", "selfc_wg_job_bytes", "selfc_wgrad_run_jobs", "selfc_clip_adam_blocks", "selfc_clip_adam", "selfc_globalagg_bwd_x",
     "selfc_rmsnorm", "selfc_rmsnorm_bwd_floats", "selfc_rmsnorm_bwd", "selfc_linear_ws_floats", "selfc_pack_rows", "selfc_linear", "selfc_linear_dz_floats",
-    "selfc_linear_dz", "selfc_linear_dx", "selfc_linear_dw", "selfc_adamw_block", "selfc_adamw_step", "selfc_grad_norm_partials", "selfc_grad_norm",
+    "selfc_linear_dz", "selfc_linear_rows_ok", "selfc_linear_rows", "selfc_linear_rows_bwd", "selfc_linear_dw_floats", "selfc_linear_dx", "selfc_linear_dw", "selfc_adamw_block", "selfc_adamw_step", "selfc_grad_norm_partials", "selfc_grad_norm",
 ]
 
 
@@ -177,13 +177,16 @@ def lib():
             "selfc_pack_rows": [vp, sz, vp, sz, i, i, i, vp],
             "selfc_linear": [vp, sz, vp, sz, vp, vp, vp, i, vp, sz, vp, vp, vp, sz, i, i, i, i, vp],
             "selfc_linear_dz": [vp, sz, vp, vp, sz, vp, vp, sz, i, i, vp],
+            "selfc_linear_rows_ok": [i, i],
+            "selfc_linear_rows": [vp, sz, vp, sz, vp, i, vp, sz, vp, vp, vp, sz, i, i, i, vp],
+            "selfc_linear_rows_bwd": [vp, sz, vp, vp, sz, vp, vp, sz, i, i, i, vp],
             "selfc_linear_dx": [vp, sz, vp, sz, vp, vp, sz, i, i, i, vp],
-            "selfc_linear_dw": [vp, sz, vp, sz, vp, vp, sz, i, i, i, vp],
+            "selfc_linear_dw": [vp, sz, vp, sz, vp, vp, vp, sz, i, i, i, vp],
             "selfc_adamw_block": [],
             "selfc_adamw_step": [vp, i, i, i, vp, vp, vp, vp, f, vp, d, d, f, f, d, u, vp, f, vp],
             "selfc_grad_norm": [vp, i, i, vp, vp, vp],
         })
-        for name, args in (("selfc_rmsnorm_bwd_floats", [sz, i]), ("selfc_linear_ws_floats", [sz, i, i, i]), ("selfc_linear_dz_floats", [sz, i]),
+        for name, args in (("selfc_rmsnorm_bwd_floats", [sz, i]), ("selfc_linear_ws_floats", [sz, i, i, i]), ("selfc_linear_dz_floats", [sz, i]), ("selfc_linear_dw_floats", [sz, i, i]),
                            ("selfc_grad_norm_partials", [i])):
             getattr(L, name).restype = sz
             getattr(L, name).argtypes = args

@@ -251,7 +251,7 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const AwTable tab, const
       if ((unsigned long long)at < left) {
         float v[8];
         const unsigned long long l = left - at;
-        load8(q + at, l > 8 ? 8 : (long)l, vec, v);
+        load8(q + at, l > 8 ? 8 : (long)l, vec && l >= 8 ? 8 : 1, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc += (double)v[i] * (double)v[i];
       }

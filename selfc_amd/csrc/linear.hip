@@ -36,72 +36,98 @@ struct Epilogue {
   const float *qs, *ps;           // scales of the rows and of the columns
   unsigned short* d;              // [M][ldd] derivative
   size_t ldo, ldr, ldd;
-  int dtype, act, vec;            // vec: 8 values at a time are aligned and inside a row
+  int dtype, act, run;            // run: values per load and store of a row (row_run)
 };
 
-__device__ __forceinline__ void act_apply(const int act, const float z, float& y, float& d) {
-  if (act == ACT_NONE) { y = z; d = 1.f; }
-  else if (act == ACT_RELU) { d = z > 0.f ? 1.f : 0.f; y = z > 0.f || z != z ? z : 0.f; }
-  else if (act == ACT_LRELU) { d = z > 0.f ? 1.f : 0.2f; y = z * d; }
-  else if (act == ACT_GELU) {
-    const float phi = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-    const float zc = fminf(fmaxf(z, -20.f), 20.f);                                        // infinities: 0 times the density
-    y = phi == 0.f ? 0.f : z * phi;
-    d = phi + zc * (__expf(-0.5f * zc * zc) * 0.39894228040143268f);
+// N values z -> activation y and, with D, its derivative d.  GELU: z phi(z) with phi = 1 - erfc(|z| / sqrt 2) / 2 mirrored at 0, erfc by
+// the polynomial of Abramowitz and Stegun 7.1.26 (absolute error 1.5e-7) times the exponential that the derivative needs too.
+template <int N, bool D>
+__device__ __forceinline__ void act_apply(const int act, const float* const z, float* const y, float* const d) {
+  if (act == ACT_NONE) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) { y[i] = z[i]; if (D) d[i] = 1.f; }
+  } else if (act == ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) { y[i] = z[i] <= 0.f ? 0.f : z[i]; if (D) d[i] = z[i] > 0.f ? 1.f : 0.f; }        // a NaN stays one
+  } else if (act == ACT_LRELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) { const float s = z[i] > 0.f ? 1.f : 0.2f; y[i] = z[i] * s; if (D) d[i] = s; }
+  } else if (act == ACT_GELU) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float az = __builtin_amdgcn_fmed3f(fabsf(z[i]), 0.f, 20.f);             // infinities: the exponential is 0 from there on
+      const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, az, 1.f));
+      const float e = __builtin_amdgcn_exp2f(az * az * -0.72134752f);               // exp(-z^2 / 2)
+      float q = fmaf(1.061405429f, t, -1.453152027f);
+      q = fmaf(q, t, 1.421413741f);
+      q = fmaf(q, t, -0.284496736f);
+      q = fmaf(q, t, 0.254829592f);
+      const float tail = 0.5f * q * t * e;                                          // of the normal distribution, beyond |z|
+      const float phi = z[i] > 0.f ? 1.f - tail : tail;
+      y[i] = z[i] < -20.f ? 0.f : z[i] * phi;                                       // (a NaN in z comes through z)
+      if (D) d[i] = fmaf(z[i] < 0.f ? -az : az, e * 0.39894228f, phi);
+    }
   } else {
-    const float s = 1.f / (1.f + __expf(-z));
-    const float zc = fminf(fmaxf(z, -80.f), 80.f);
-    y = s == 0.f ? 0.f : z * s;
-    d = s * (1.f + zc * (1.f - s));
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z[i] * -1.44269504f));
+      y[i] = z[i] < -100.f ? 0.f : z[i] * s;
+      const float zc = __builtin_amdgcn_fmed3f(z[i], -100.f, 100.f);
+      if (D) d[i] = s * fmaf(zc, 1.f - s, 1.f);
+    }
   }
 }
-__device__ __forceinline__ unsigned short act_code(const float d) {
-  const float c = rintf(d * 32768.f) + 16384.f;
-  return d != d ? (unsigned short)65535 : (unsigned short)fminf(fmaxf(c, 0.f), 65534.f);
+// derivative -> 16-bit fixed point, rounded to nearest: (d + 0.5) 2^15 is in [0, 65534] for every activation here
+__device__ __forceinline__ unsigned act_code(const float d, const float z) {
+  const unsigned c = (unsigned)fmaf(d, 32768.f, 16384.5f);
+  return z != z ? 65535u : c;
 }
 __device__ __forceinline__ float act_slope(const unsigned c) {
   return c == 65535u ? __builtin_nanf("") : (float)((int)c - 16384) * 0x1p-15f;
 }
 
-__device__ __forceinline__ void load8_as(const int dtype, const void* const p, const size_t at, const long left, const bool vec, float* const v) {
-  if (dtype == 0) load8((const float*)p + at, left, vec, v);
-  else if (dtype == 1) load8((const b16*)p + at, left, vec, v);
-  else load8((const h16*)p + at, left, vec, v);
+__device__ __forceinline__ void load8_as(const int dtype, const void* const p, const size_t at, const long left, const int run, float* const v) {
+  if (dtype == 0) load8((const float*)p + at, left, run, v);
+  else if (dtype == 1) load8((const b16*)p + at, left, run, v);
+  else load8((const h16*)p + at, left, run, v);
 }
 
 // eight neighbouring columns of one row: acc is the product's sum, b and ps the columns' bias and scale
 __device__ __forceinline__ void epilogue8(const Epilogue& e, const float* const acc, const int row, const int col, const int left,
                                           const float* const b, const float* const ps) {
-  float y[8], d[8], r[8];
+  float z[8], y[8], d[8], r[8];
   const float qs = e.qs ? e.qs[row] : 1.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float z = acc[i];
-    if (e.qs) z *= qs * ps[i];
-    act_apply(e.act, z + b[i], y[i], d[i]);
-  }
+  for (int i = 0; i < 8; ++i) z[i] = (e.qs ? acc[i] * (qs * ps[i]) : acc[i]) + b[i];
   if (e.d) {
-    unsigned short* const dp = e.d + (size_t)row * e.ldd + col;              // ldd is a multiple of 8: always 16 bytes at a time
+    act_apply<8, true>(e.act, z, y, d);
     u16x8 c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = act_code(d[i]);
-    *reinterpret_cast<u16x8*>(dp) = c;
+    for (int i = 0; i < 8; ++i) c[i] = (unsigned short)act_code(d[i], z[i]);
+    *reinterpret_cast<u16x8*>(e.d + (size_t)row * e.ldd + col) = c;          // ldd is a multiple of 8: always 16 bytes at a time
+  } else {
+    act_apply<8, false>(e.act, z, y, d);
   }
   if (e.res) {
-    load8_as(e.dtype, e.res, (size_t)row * e.ldr + col, left, e.vec, r);
+    load8_as(e.dtype, e.res, (size_t)row * e.ldr + col, left, e.run, r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] += r[i];
   }
   const size_t at = (size_t)row * e.ldo + col;
-  if (e.dtype == 0) store8((float*)e.out + at, left, e.vec, y);
-  else if (e.dtype == 1) store8((b16*)e.out + at, left, e.vec, y);
-  else store8((h16*)e.out + at, left, e.vec, y);
+  if (e.dtype == 0) store8((float*)e.out + at, left, e.run, y);
+  else if (e.dtype == 1) store8((b16*)e.out + at, left, e.run, y);
+  else store8((h16*)e.out + at, left, e.run, y);
+}
+// the same where nothing follows the product
+template <typename T>
+__device__ __forceinline__ void plain8(const Epilogue& e, const float* const acc, const int row, const int col, const int left) {
+  store8((T*)e.out + (size_t)row * e.ldo + col, left, e.run, acc);
 }
 __device__ __forceinline__ void epilogue_columns(const Epilogue& e, const int col, const int left, float* const b, float* const ps) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) { b[i] = 0.f; ps[i] = 1.f; }
-  if (e.bias) load8_as(e.dtype, e.bias, col, left, false, b);
-  if (e.ps) load8(e.ps + col, left, false, ps);
+  if (e.bias) load8_as(e.dtype, e.bias, col, left, 1, b);
+  if (e.ps) load8(e.ps + col, left, 1, ps);
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------------
@@ -111,8 +137,9 @@ struct GemmArgs {
   int M, N, R;                    // rows and columns of the output, length of the sum (R: a multiple of 16 bytes where an operand is straight)
   int qx, px;                     // crossed operands: readable columns (a multiple of 8)
   int splits, per;                // parts of the sum, and stages of each
-  float* ws;                      // [splits][M][ldw] partial sums when splits > 1
+  float* ws;                      // [splits][M][ldw] partial sums when splits > 1, and behind them [splits][M] of the rows' own sums
   size_t ldw;
+  void* sums;                     // dW: NULL, or [M]: the sum of each row of Q (db), of the output's type
   Epilogue e;
 };
 
@@ -269,6 +296,20 @@ __global__ __launch_bounds__(NQ * NP * 64) void gemm_kernel(const GemmArgs a) {
 #pragma unroll
     for (int j = 0; j < TQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+  // db: the rows' own sums are one more column of the product, against a fragment of ones
+  const bool own = QX && PX && a.sums && p0 == 0 && wp == 0;
+  f32x4 osum[QX && PX ? TQ : 1];
+  i32x4 ones;
+  if constexpr (QX && PX) {
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    T8 o;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (T)1.f;
+    ones = __builtin_bit_cast(i32x4, o);
+#pragma unroll
+    for (int j = 0; j < TQ; ++j) osum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
   if (s0 < s1) {
     sq.load(lds0, a.R - s0 * BK);
     sp.load(lds0 + SQ, a.R - s0 * BK);
@@ -304,17 +345,35 @@ __global__ __launch_bounds__(NQ * NP * 64) void gemm_kernel(const GemmArgs a) {
         for (int i = 0; i < TP; ++i)
 #pragma unroll
           for (int j = 0; j < TQ; ++j) acc[i][j] = Mma<T>::run(p[i], q[j], acc[i][j]);
+        if constexpr (QX && PX) {
+          if (own)
+#pragma unroll
+            for (int j = 0; j < TQ; ++j) osum[j] = Mma<T>::run(ones, q[j], osum[j]);
+        }
       }
     }
   }
   wait_barrier<0>();                      // the buffers are free: each wave turns its tiles into rows of its own piece of them
+  if constexpr (QX && PX) {
+    if (own && (threadIdx.x & 63) < 16) {
+#pragma unroll
+      for (int j = 0; j < TQ; ++j) {
+        const int row = q0 + wq * WQ + j * 16 + (threadIdx.x & 15);
+        if (row < a.M) {
+          if (a.splits == 1) ((T*)a.sums)[row] = (T)osum[j][0];
+          else a.ws[(size_t)a.splits * a.M * a.ldw + (size_t)part * a.M + row] = osum[j][0];
+        }
+      }
+    }
+  }
 
   constexpr int PITCH = WP + 4, LPR = WP / 8, RPP = 64 / LPR;         // floats per row, lanes per row, rows per pass
   const int lane = threadIdx.x & 63;
   float* const turn = reinterpret_cast<float*>(lds) + wave * 16 * PITCH;
   const int col = p0 + wp * WP + (lane % LPR) * 8, left = a.N - col;
+  constexpr bool FULL = !QX && !PX;       // the products of the backward pass are stored as they are
   float b[8], ps[8];
-  if (a.splits == 1) epilogue_columns(a.e, col, left, b, ps);
+  if (FULL && a.splits == 1) epilogue_columns(a.e, col, left, b, ps);
 #pragma unroll
   for (int j = 0; j < TQ; ++j) {
 #pragma unroll
@@ -329,7 +388,8 @@ __global__ __launch_bounds__(NQ * NP * 64) void gemm_kernel(const GemmArgs a) {
       if (row < a.M && left > 0) {
         const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
         if (a.splits == 1) {
-          epilogue8(a.e, v, row, col, left, b, ps);
+          if constexpr (FULL) epilogue8(a.e, v, row, col, left, b, ps);
+          else plain8<T>(a.e, v, row, col, left);
         } else {
           float* const w = a.ws + ((size_t)part * a.M + row) * a.ldw + col;      // ldw is a multiple of 8
           *reinterpret_cast<f32x4*>(w) = v0;
@@ -341,19 +401,44 @@ __global__ __launch_bounds__(NQ * NP * 64) void gemm_kernel(const GemmArgs a) {
   }
 }
 
-// the parts of a divided sum, added in order, and what follows the product
+// the parts of a divided sum, added in a fixed order, and what follows the product.  Eight neighbouring columns are one item; SL threads
+// share an item's parts (few items and many parts: one thread each would be a handful of workgroups on long chains of loads)
+template <int SL>
 __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a) {
-  const int per_row = (a.N + 7) / 8;
-  const size_t id = (size_t)blockIdx.x * 256 + threadIdx.x;
-  if (id >= (size_t)a.M * per_row) return;
-  const int row = (int)(id / per_row), col = (int)(id % per_row) * 8;
-  const float* w = a.ws + (size_t)row * a.ldw + col;
-  float v[8] = {};
+  constexpr int ITEMS = 256 / SL;
+  __shared__ float red[SL][ITEMS][9];
+  const int per_row = (a.N + 7) / 8, item = threadIdx.x % ITEMS, slice = threadIdx.x / ITEMS;
+  const size_t id = (size_t)blockIdx.x * ITEMS + item;
+  const bool in = id < (size_t)a.M * per_row;
+  const int row = in ? (int)(id / per_row) : 0, col = in ? (int)(id % per_row) * 8 : 0;
+  float v[9] = {};                   // [8]: the row's own sum
+  const bool own = in && a.sums && col == 0;
+  if (in) {
+    const size_t part = (size_t)a.M * a.ldw;
+    const float* const w = a.ws + (size_t)row * a.ldw + col;
 #pragma unroll 4
-  for (int s = 0; s < a.splits; ++s, w += (size_t)a.M * a.ldw) {
-    const f32x4 x = *reinterpret_cast<const f32x4*>(w), y = *reinterpret_cast<const f32x4*>(w + 4);
+    for (int s = slice; s < a.splits; s += SL) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(w + s * part), y = *reinterpret_cast<const f32x4*>(w + s * part + 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { v[i] += x[i]; v[4 + i] += y[i]; }
+      for (int i = 0; i < 4; ++i) { v[i] += x[i]; v[4 + i] += y[i]; }
+    }
+    if (own)
+      for (int s = slice; s < a.splits; s += SL) v[8] += a.ws[a.splits * part + (size_t)s * a.M + row];
+  }
+  if constexpr (SL > 1) {
+#pragma unroll
+    for (int i = 0; i < 9; ++i) red[slice][item][i] = v[i];
+    __syncthreads();
+    if (slice) return;
+#pragma unroll
+    for (int k = 1; k < SL; ++k)
+#pragma unroll
+      for (int i = 0; i < 9; ++i) v[i] += red[k][item][i];
+  }
+  if (!in) return;
+  if (own) {
+    if (a.e.dtype == 1) ((b16*)a.sums)[row] = (b16)v[8];
+    else ((h16*)a.sums)[row] = (h16)v[8];
   }
   float b[8], ps[8];
   epilogue_columns(a.e, col, a.N - col, b, ps);
@@ -418,6 +503,182 @@ __global__ __launch_bounds__(512) void gemv_kernel(const GemmArgs a) {
   }
 }
 
+// ---- narrow rows: up to 256 values in and out ----------------------------------------------------------------------------------
+// Pixels' channels: a product of few columns is bound by the rows' traffic, and tiles that meet in shared memory only delay it.  Here the
+// whole weight stays in shared memory, a wave takes 16 rows at a time straight from memory into the multiply's operand and back, and
+// what used to be launches of their own rides along:
+//   forward   x may have any pitch and offset; its rows as whole pieces (the operand of dW) are written on the way
+//   backward  dz = dy act'(z) is formed in the operand's registers and written for dW
+// Shared memory: the weight as [TP * 16 columns][KS * 32 places], 16 bytes between rows that keep 16 rows' pieces in different banks.
+struct RowsArgs {
+  const void *x, *w;
+  const unsigned short* d;        // backward: derivative [rows][ldd], or NULL
+  void* xp;                       // NULL, or the operand's rows with pitch roundup(K, 8) and zeros behind them
+  size_t ldx, ldw, ldd, rows;
+  int N, K, xrun, wrun, turn;     // turn: bytes of shared memory per wave for rows that cannot be stored in runs of 4 (0: they can)
+  Epilogue e;                     // out without gaps
+};
+// eight neighbouring 16-bit values as they are stored; zeros from `left` on.  `room`: how many values the matrix still has from p on -
+// where a row ends inside the eight, the next row's are read along (one load at any 2-byte address) and cleared
+template <typename T>
+__device__ __forceinline__ i32x4 raw8(const T* const p, const int left, const bool whole, const size_t room) {
+  i32x4 r = {0, 0, 0, 0};
+  if (left <= 0) return r;
+  if (whole) return *reinterpret_cast<const i32x4*>(p);
+  if (room >= 8) {
+    __builtin_memcpy(&r, p, 16);
+  } else {
+    const unsigned short* const u = reinterpret_cast<const unsigned short*>(p);
+    for (int i = 0; i < (int)room; ++i) {
+      const int v = (int)((unsigned)u[i] << (16 * (i & 1)));
+      if (i < 2) r[0] |= v;
+      else if (i < 4) r[1] |= v;
+      else if (i < 6) r[2] |= v;
+      else r[3] |= v;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r[i] = left >= 2 * i + 2 ? r[i] : left == 2 * i + 1 ? r[i] & 0xffff : 0;
+  return r;
+}
+template <typename T, int KS, bool BWD, int NW>
+__global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
+  constexpr int PITCH = KS * 64 + 16, NT = NW * 64;
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int N = a.N, K = a.K, kp = (K + 7) & ~7, tp = (N + 15) / 16;
+  float* const bias = reinterpret_cast<float*>(lds + tp * 16 * PITCH);
+  unsigned char* const scratch = lds + tp * 16 * PITCH + tp * 64;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, q = lane & 15;
+
+  const bool xwhole = a.xrun == 8, wwhole = a.wrun == 8;
+  const size_t xend = (a.rows - 1) * a.ldx + K, wend = (size_t)((BWD ? K : N) - 1) * a.ldw + (BWD ? N : K);
+  if constexpr (!BWD) {           // w [N][K]
+    for (int ch = threadIdx.x; ch < tp * 16 * KS * 4; ch += NT) {
+      const int p = ch / (KS * 4), c = ch % (KS * 4) * 8;
+      const size_t at = p * a.ldw + c;
+      *reinterpret_cast<i32x4*>(lds + p * PITCH + c * 2) = raw8((const T*)a.w + at, p < N ? K - c : 0, wwhole, wend - at);
+    }
+  } else {                        // w [K][N]: turned; neighbouring threads take neighbouring places of the sum, whose stores share no bank
+    for (int ch = threadIdx.x; ch < KS * 32 * tp * 2; ch += NT) {
+      const int r = ch % (KS * 32), c = ch / (KS * 32) * 8;
+      const size_t at = r * a.ldw + c;
+      const T8 v = __builtin_bit_cast(T8, raw8((const T*)a.w + at, r < K ? N - c : 0, wwhole, wend - at));
+#pragma unroll
+      for (int i = 0; i < 8; ++i) *reinterpret_cast<T*>(lds + (c + i) * PITCH + r * 2) = v[i];
+    }
+  }
+  for (int c = threadIdx.x; c < tp * 16; c += NT) bias[c] = !BWD && a.e.bias && c < N ? (float)((const T*)a.e.bias)[c] : 0.f;
+  __syncthreads();
+
+  const size_t tiles = (a.rows + 15) / 16;
+  for (size_t t = (size_t)blockIdx.x * NW + wave; t < tiles; t += (size_t)gridDim.x * NW) {
+    const size_t row0 = t * 16, row = row0 + q;
+    const bool in = row < a.rows;
+    i32x4 xf[KS];
+    u16x8 dv[BWD ? KS : 1];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int c = ks * 32 + g * 8;
+      xf[ks] = raw8((const T*)a.x + row * a.ldx + c, in ? K - c : 0, xwhole, xend - (row * a.ldx + c));
+      if constexpr (BWD) {
+        if (a.d && in && c < kp) dv[ks] = *reinterpret_cast<const u16x8*>(a.d + row * a.ldd + c);
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int c = ks * 32 + g * 8;
+      if (BWD && a.d) {
+        const T8 h = __builtin_bit_cast(T8, xf[ks]);
+        T8 r;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float v = (float)h[i];
+          v = in && c + i < K ? v * act_slope(dv[ks][i]) : 0.f;
+          r[i] = (T)v;
+        }
+        xf[ks] = __builtin_bit_cast(i32x4, r);
+      }
+      if (a.xp && in && c < kp) *reinterpret_cast<i32x4*>((T*)a.xp + row * kp + c) = xf[ks];
+    }
+    unsigned char* const turn = scratch + wave * a.turn;
+    // four tiles of 16 columns at a time: enough independent multiplies, few enough registers for 16 waves per compute unit
+#pragma unroll 1
+    for (int p4 = 0; p4 < tp; p4 += 4) {
+      f32x4 acc[4];
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        acc[p] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if (p4 + p < tp) {
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks)
+            acc[p] = Mma<T>::run(*reinterpret_cast<const i32x4*>(lds + ((p4 + p) * 16 + q) * PITCH + ks * 64 + g * 16), xf[ks], acc[p]);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        const int col = (p4 + p) * 16 + g * 4;
+        if (p4 + p >= tp) break;
+        float y[4];
+        if constexpr (BWD) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[i] = acc[p][i];
+        } else {
+          const f32x4 b = *reinterpret_cast<const f32x4*>(bias + col);
+          float z[4], d[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) z[i] = acc[p][i] + b[i];
+          if (a.e.d) {
+            act_apply<4, true>(a.e.act, z, y, d);
+            u32x2 c;
+            c[0] = act_code(d[0], z[0]) | act_code(d[1], z[1]) << 16;
+            c[1] = act_code(d[2], z[2]) | act_code(d[3], z[3]) << 16;
+            if (in && col < (int)a.e.ldd) *reinterpret_cast<u32x2*>(a.e.d + row * a.e.ldd + col) = c;
+          } else {
+            act_apply<4, false>(a.e.act, z, y, d);
+          }
+          if (a.e.res && in) {
+            const T* const r = (const T*)a.e.res + row * a.e.ldr + col;
+            if (a.e.run >= 4) {
+              if (col < N) {
+                const T4 v = *reinterpret_cast<const T4*>(r);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] += (float)v[i];
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (col + i < N) y[i] += (float)r[i];
+            }
+          }
+        }
+        T4 h;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h[i] = (T)y[i];
+        if (!a.turn) {
+          if (in && col < N) *reinterpret_cast<T4*>((T*)a.e.out + row * N + col) = h;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (col + i < N) *reinterpret_cast<T*>(turn + (q * N + col + i) * 2) = h[i];
+        }
+      }
+    }
+    if (a.turn) {                 // 16 whole rows are one stretch of memory
+      __builtin_amdgcn_wave_barrier();
+      const int bytes = (int)(a.rows - row0 < 16 ? a.rows - row0 : 16) * N * 2;
+      unsigned char* const out = (unsigned char*)a.e.out + row0 * N * 2;
+      for (int b = lane * 16; b < bytes; b += 1024) {
+        if (b + 16 <= bytes) *reinterpret_cast<i32x4*>(out + b) = *reinterpret_cast<const i32x4*>(turn + b);
+        else
+          for (int k = b; k < bytes; k += 2) *reinterpret_cast<unsigned short*>(out + k) = *reinterpret_cast<const unsigned short*>(turn + k);
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+}
+
 // ---- rows of any width, pitch and offset, laid out again with a pitch of whole 16-byte pieces and zeros behind each row --------
 template <typename T>
 __global__ __launch_bounds__(256) void pack_rows_kernel(const T* const src, const size_t ld, T* const dst, const int cols, const int ldd, const size_t rows) {
@@ -439,7 +700,7 @@ struct DzArgs {
   void* dz;                       // or NULL: only the sums
   float* partial;                 // [gridDim.y][N] or NULL
   size_t rows, lddy, ldd, lddz;
-  int N, vec;
+  int N, run;
 };
 template <typename T, int L>
 __global__ __launch_bounds__(256) void dz_kernel(const DzArgs a) {
@@ -448,17 +709,27 @@ __global__ __launch_bounds__(256) void dz_kernel(const DzArgs a) {
   const int col = (blockIdx.x * L + lane) * 8, left = a.N - col;
   float sum[8] = {};
   if (left > 0) {
-    for (size_t row = (size_t)blockIdx.y * G + grp; row < a.rows; row += (size_t)gridDim.y * G) {
-      float v[8];
-      load8((const T*)a.dy + row * a.lddy + col, left, a.vec, v);
-      if (a.d) {
-        const u16x8 c = *reinterpret_cast<const u16x8*>(a.d + row * a.ldd + col);
+    constexpr int U = 4;                     // rows whose loads are in flight together
+    const size_t step = (size_t)gridDim.y * G;
+    for (size_t row = (size_t)blockIdx.y * G + grp; row < a.rows; row += U * step) {
+      float v[U][8];
+      u16x8 c[U];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < left ? v[i] * act_slope(c[i]) : 0.f;
-      }
+      for (int k = 0; k < U; ++k)
+        if (row + k * step < a.rows) {
+          load8((const T*)a.dy + (row + k * step) * a.lddy + col, left, a.run, v[k]);
+          if (a.d) c[k] = *reinterpret_cast<const u16x8*>(a.d + (row + k * step) * a.ldd + col);
+        }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] += v[i];
-      if (a.dz) store8((T*)a.dz + row * a.lddz + col, 8, true, v);           // zeros behind the last column
+      for (int k = 0; k < U; ++k)
+        if (row + k * step < a.rows) {
+          if (a.d)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[k][i] = i < left ? v[k][i] * act_slope(c[k][i]) : 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) sum[i] += v[k][i];
+          if (a.dz) store8((T*)a.dz + (row + k * step) * a.lddz + col, 8, 8, v[k]);           // zeros behind the last column
+        }
     }
   }
   if (!a.partial) return;
@@ -478,7 +749,7 @@ inline int dz_lanes(const int N) { return N <= 64 ? 8 : N <= 128 ? 16 : N <= 256
 inline int dz_groups(const size_t rows, const int N) {
   const int L = dz_lanes(N), cols = (N + L * 8 - 1) / (L * 8);
   size_t g = (rows + 256 / L - 1) / (256 / L);
-  const size_t most = 2048 / cols < 64 ? 64 : 2048 / cols;
+  const size_t most = 1024 / cols < 64 ? 64 : 1024 / cols;
   return (int)(g < most ? g : most);
 }
 
@@ -508,9 +779,10 @@ inline size_t up8(const size_t n) { return (n + 7) & ~(size_t)7; }
 template <typename T, bool QX, bool PX, int BQ, int BP, int NQ, int NP>
 hipError_t gemm_go(const GemmArgs& a, hipStream_t s) {
   static std::atomic<unsigned long long> optin{0};
-  constexpr int stage = (BQ + BP) * 128 * 2, turn = NQ * NP * 16 * (BP / NP + 4) * 4, bytes = stage > turn ? stage : turn;
+  constexpr int stage = (BQ + BP) * 128, turn = NQ * NP * 16 * (BP / NP + 4) * 4, most = 2 * stage > turn ? 2 * stage : turn;
+  const int need = a.per > 1 ? 2 * stage : stage, bytes = need > turn ? need : turn;      // one stage: one buffer, more workgroups at a time
   const void* const fn = reinterpret_cast<const void*>(&gemm_kernel<T, QX, PX, BQ, BP, NQ, NP>);
-  if (const hipError_t e = lds_optin(fn, bytes, optin); e != hipSuccess) return e;
+  if (const hipError_t e = lds_optin(fn, most, optin); e != hipSuccess) return e;
   const long wgs = (long)((a.M + BQ - 1) / BQ) * ((a.N + BP - 1) / BP) * a.splits;
   hipLaunchKernelGGL((gemm_kernel<T, QX, PX, BQ, BP, NQ, NP>), dim3((unsigned)wgs), dim3(NQ * NP * 64), bytes, s, a);
   return hipGetLastError();
@@ -529,10 +801,54 @@ int gemm_run(GemmArgs a, hipStream_t s) {
   if (e != hipSuccess) return pw_rc(e);
   if (p.splits > 1) {
     const size_t n = (size_t)a.M * ((a.N + 7) / 8);
-    hipLaunchKernelGGL(gemm_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
+    if (p.splits >= 16) hipLaunchKernelGGL((gemm_join_kernel<16>), dim3((unsigned)((n + 15) / 16)), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((gemm_join_kernel<1>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a);
     return pw_rc(hipGetLastError());
   }
   return SELFC_OK;
+}
+
+// ---- narrow rows: which instance, and the shared memory it takes ----------------------------------------------------------------
+constexpr int ROWS_MAX = 256;
+struct RowsPlan { int ks, nw, turn, lds, per_cu; };
+inline RowsPlan rows_plan(const int N, const int K, const bool runs4) {
+  RowsPlan p{};
+  const int tp = (N + 15) / 16;
+  p.ks = K <= 64 ? 2 : K <= 128 ? 4 : 8;
+  const int weight = tp * 16 * (p.ks * 64 + 16) + tp * 64;
+  p.nw = weight > 32 * 1024 ? 8 : 4;               // a large weight is shared by more waves
+  p.turn = runs4 ? 0 : 32 * N;
+  p.lds = weight + p.nw * p.turn;
+  const int most = 16 / p.nw;                      // 16 waves per compute unit
+  p.per_cu = 160 * 1024 / p.lds < most ? 160 * 1024 / p.lds : most;
+  return p;
+}
+// both directions of a layer have to fit
+inline bool rows_ok(const int n, const int k) {
+  return n <= ROWS_MAX && k <= ROWS_MAX && rows_plan(n, k, false).lds <= 160 * 1024 && rows_plan(k, n, false).lds <= 160 * 1024;
+}
+template <typename T, bool BWD>
+int rows_run(RowsArgs a, hipStream_t s) {
+  const RowsPlan p = rows_plan(a.N, a.K, row_run(a.e.out, a.N, a.N, 2) >= 4);
+  a.turn = p.turn;
+  // workgroups that the chip holds at a time, each with its copy of the weight, or as many as there are tiles for
+  const size_t need = (a.rows + p.nw * 16 - 1) / (p.nw * 16), hold = 256 * (size_t)p.per_cu;
+  const dim3 grid((unsigned)(need < hold ? need : hold)), blk(p.nw * 64);
+#define ROWS(KS, NW)                                                                                                              \
+  {                                                                                                                               \
+    static std::atomic<unsigned long long> optin{0};                                                                              \
+    const void* const fn = reinterpret_cast<const void*>(&rows_kernel<T, KS, BWD, NW>);                                           \
+    if (const hipError_t e = lds_optin(fn, 160 * 1024, optin); e != hipSuccess) return pw_rc(e);                                  \
+    hipLaunchKernelGGL((rows_kernel<T, KS, BWD, NW>), grid, blk, p.lds, s, a);                                                    \
+  }
+  if (p.ks == 2 && p.nw == 4) ROWS(2, 4)
+  else if (p.ks == 2) ROWS(2, 8)
+  else if (p.ks == 4 && p.nw == 4) ROWS(4, 4)
+  else if (p.ks == 4) ROWS(4, 8)
+  else if (p.nw == 4) ROWS(8, 4)
+  else ROWS(8, 8)
+#undef ROWS
+  return pw_rc(hipGetLastError());
 }
 
 constexpr int GEMV_ROWS = 16;
@@ -548,7 +864,8 @@ Epilogue make_epilogue(void* out, size_t ldo, const void* bias, const void* res,
   Epilogue e{};
   const size_t es = dtype ? 2 : 4;
   e.out = out; e.bias = bias; e.res = res; e.ldo = ldo; e.ldr = ldr; e.dtype = dtype; e.act = act;
-  e.vec = N % 8 == 0 && aligned_to(out, 16) && (ldo * es) % 16 == 0 && (!res || (aligned_to(res, 16) && (ldr * es) % 16 == 0));
+  e.run = row_run(out, ldo, N, es);
+  if (res) { const int r = row_run(res, ldr, N, es); e.run = r < e.run ? r : e.run; }
   return e;
 }
 
@@ -610,7 +927,7 @@ int selfc_linear_dz(const void* dy, size_t lddy, const void* slope, void* dz, si
   if (slope && !aligned_to(slope, 16)) return SELFC_EINVAL;
   DzArgs a{};
   a.dy = dy; a.d = (const unsigned short*)slope; a.dz = dz; a.partial = db ? partial : nullptr; a.rows = rows; a.lddy = lddy; a.ldd = up8(n); a.lddz = lddz; a.N = n;
-  a.vec = n % 8 == 0 && aligned_to(dy, 16) && lddy % 8 == 0;
+  a.run = row_run(dy, rows > 1 ? lddy : n, n, 2);
   hipStream_t s = (hipStream_t)stream;
   const int L = dz_lanes(n), groups = dz_groups(rows, n);
   if (groups) {
@@ -638,13 +955,51 @@ int selfc_linear_dx(const void* dz, size_t lddz, const void* w, size_t ldw, void
   return dtype == 1 ? gemm_run<b16, false, true>(a, (hipStream_t)stream) : gemm_run<h16, false, true>(a, (hipStream_t)stream);
 }
 
-int selfc_linear_dw(const void* dz, size_t lddz, const void* x, size_t ldx, void* dw, float* ws, size_t rows, int n, int k, int dtype, void* stream) {
+size_t selfc_linear_dw_floats(size_t rows, int n, int k) {
+  if (rows < 1 || rows > 0x3fffffff || n < 1 || k < 1) return 0;
+  const Plan p = gemm_plan(n, k, (int)rows, 2);
+  return p.splits > 1 ? (size_t)p.splits * n * (up8(k) + 1) : 0;
+}
+
+int selfc_linear_dw(const void* dz, size_t lddz, const void* x, size_t ldx, void* dw, void* db, float* ws, size_t rows, int n, int k, int dtype, void* stream) {
   if (!dz || !x || !dw || !lin_shape(n, k, 1) || rows < 1 || rows > 0x3fffffff || (dtype != 1 && dtype != 2)) return SELFC_EINVAL;
   if (!rows_fit(dz, lddz, up8(n), 2) || lddz < up8(n) || !rows_fit(x, ldx, up8(k), 2) || ldx < up8(k)) return SELFC_EINVAL;
   GemmArgs a{};
-  a.q = dz; a.p = x; a.ldq = lddz; a.ldp = ldx; a.M = n; a.N = k; a.R = (int)rows; a.qx = (int)up8(n); a.px = (int)up8(k); a.ws = ws;
+  a.q = dz; a.p = x; a.ldq = lddz; a.ldp = ldx; a.M = n; a.N = k; a.R = (int)rows; a.qx = (int)up8(n); a.px = (int)up8(k); a.ws = ws; a.sums = db;
   a.e = make_epilogue(dw, k, nullptr, nullptr, 0, dtype, ACT_NONE, k);
   return dtype == 1 ? gemm_run<b16, true, true>(a, (hipStream_t)stream) : gemm_run<h16, true, true>(a, (hipStream_t)stream);
+}
+
+int selfc_linear_rows_ok(int n, int k) { return n >= 1 && k >= 1 && rows_ok(n, k); }
+
+int selfc_linear_rows(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, int act, const void* res, size_t ldr, void* y,
+                      void* slope, void* xp, size_t rows, int n, int k, int dtype, void* stream) {
+  if (rows == 0) return SELFC_OK;
+  if (!x || !w || !y || n < 1 || k < 1 || !rows_ok(n, k) || rows > 0x3fffffff || act < ACT_NONE || act > ACT_SILU || (dtype != 1 && dtype != 2)) return SELFC_EINVAL;
+  if ((rows > 1 && ldx < (size_t)k) || (n > 1 && ldw < (size_t)k) || (res && rows > 1 && ldr < (size_t)n)) return SELFC_EINVAL;
+  if (!aligned_to(y, 16) || (slope && !aligned_to(slope, 16)) || (xp && !aligned_to(xp, 16))) return SELFC_EINVAL;
+  RowsArgs a{};
+  a.x = x; a.w = w; a.xp = xp; a.ldx = ldx; a.ldw = ldw; a.rows = rows; a.N = n; a.K = k;
+  a.xrun = row_run(x, rows > 1 ? ldx : k, k, 2);
+  a.wrun = row_run(w, n > 1 ? ldw : k, k, 2);
+  a.e.out = y; a.e.bias = bias; a.e.res = res; a.e.ldr = ldr; a.e.act = act; a.e.d = (unsigned short*)slope; a.e.ldd = up8(n);
+  a.e.run = res ? row_run(res, rows > 1 ? ldr : n, n, 2) : 8;
+  return dtype == 1 ? rows_run<b16, false>(a, (hipStream_t)stream) : rows_run<h16, false>(a, (hipStream_t)stream);
+}
+
+int selfc_linear_rows_bwd(const void* dy, size_t lddy, const void* slope, const void* w, size_t ldw, void* dx, void* dz,
+                          size_t rows, int n, int k, int dtype, void* stream) {
+  if (rows < 1 || !dy || !w || !dx || n < 1 || k < 1 || !rows_ok(n, k) || rows > 0x3fffffff || (dtype != 1 && dtype != 2)) return SELFC_EINVAL;
+  if ((rows > 1 && lddy < (size_t)n) || (n > 1 && ldw < (size_t)k)) return SELFC_EINVAL;
+  if (!aligned_to(dx, 16) || (slope && !aligned_to(slope, 16)) || (dz && !aligned_to(dz, 16))) return SELFC_EINVAL;
+  RowsArgs a{};
+  a.x = dy; a.w = w; a.d = (const unsigned short*)slope; a.xp = dz;
+  a.ldx = lddy; a.ldw = ldw; a.ldd = up8(n); a.rows = rows; a.N = k; a.K = n;
+  a.xrun = row_run(dy, rows > 1 ? lddy : n, n, 2);
+  a.wrun = row_run(w, n > 1 ? ldw : k, k, 2);
+  a.e.out = dx;
+  hipStream_t s = (hipStream_t)stream;
+  return dtype == 1 ? rows_run<b16, true>(a, s) : rows_run<h16, true>(a, s);
 }
 
 }  // extern "C"

@@ -37,12 +37,12 @@ struct RnArgs {
   void *h, *y;
   float* scale;
   size_t rows, ldx, ldr;
-  int C, w_f32, vec;          // vec: every base and pitch is a multiple of 16 bytes (8 for the 8-bit output) and C of 8
+  int C, w_f32, run;          // run: values per load and store (8, 4, 2 or 1)
   float eps;
 };
 
 // L lanes per row, NV vectors of 8 values per lane
-template <typename T, int L, int NV, bool Q8>
+template <typename T, int L, int NV, bool Q8, bool RUN8>
 __global__ __launch_bounds__(256) void rmsnorm_kernel(const RnArgs a) {
   __shared__ float red[8];
   const int lane = threadIdx.x & (L - 1);
@@ -51,26 +51,26 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const RnArgs a) {
   const T* const x = (const T*)a.x + row * a.ldx;
   const T* const r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
   const int C = a.C;
-  const bool vec = a.vec;
+  const int run = RUN8 ? 8 : a.run;           // whole 16-byte pieces: no other loads are compiled in
   float h[NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (j * L + lane) * 8;
-    load8(x + c, C - c, vec, h[j]);
+    load8(x + c, C - c, run, h[j]);
   }
   if (r) {
     float t[NV][8];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * L + lane) * 8;
-      load8(r + c, C - c, vec, t[j]);
+      load8(r + c, C - c, run, t[j]);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * L + lane) * 8;
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[j][i] = (float)(T)(h[j][i] + t[j][i]);
-      if (c < C) store8((T*)a.h + row * C + c, C - c, vec, h[j]);
+      if (c < C) store8((T*)a.h + row * C + c, C - c, run, h[j]);
     }
   }
   float ss = 0.f;
@@ -85,15 +85,15 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const RnArgs a) {
   for (int j = 0; j < NV; ++j) {
     const int c = (j * L + lane) * 8;
     float w[8];
-    if (a.w_f32) load8((const float*)a.w + c, C - c, vec, w);
-    else load8((const T*)a.w + c, C - c, vec, w);
+    if (a.w_f32) load8((const float*)a.w + c, C - c, run, w);
+    else load8((const T*)a.w + c, C - c, run, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       h[j][i] = h[j][i] * rstd * w[i];
       if constexpr (Q8) most = fmaxf(most, fabsf(h[j][i]));
     }
     if constexpr (!Q8) {
-      if (c < C) store8((T*)a.y + row * C + c, C - c, vec, h[j]);
+      if (c < C) store8((T*)a.y + row * C + c, C - c, run, h[j]);
     }
   }
   if constexpr (Q8) {
@@ -111,7 +111,7 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const RnArgs a) {
         int hi = __builtin_amdgcn_cvt_pk_fp8_f32(h[j][4] * inv, h[j][5] * inv, 0, false);
         hi = __builtin_amdgcn_cvt_pk_fp8_f32(h[j][6] * inv, h[j][7] * inv, hi, true);
         unsigned char* const q = (unsigned char*)a.y + row * C + c;
-        if (vec) {
+        if (run == 8) {
           *reinterpret_cast<u32x2*>(q) = u32x2{(unsigned)lo, (unsigned)hi};
         } else {
 #pragma unroll
@@ -128,17 +128,17 @@ struct RnBwdArgs {
   void* dx;
   float* partial;             // [gridDim.x][C]
   size_t rows, ldh;
-  int C, w_f32, vec, want_dx;
+  int C, w_f32, run, want_dx;
   float eps;
 };
 
-template <typename T, int L, int NV>
+template <typename T, int L, int NV, bool RUN8>
 __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(const RnBwdArgs a) {
   __shared__ float red[2][8];
   constexpr int G = 256 / L;                 // rows at a time
   const int lane = threadIdx.x & (L - 1), grp = threadIdx.x / L;
   const int C = a.C;
-  const bool vec = a.vec;
+  const int run = RUN8 ? 8 : a.run;           // whole 16-byte pieces: no other loads are compiled in
   float dw[NV][8] = {};
   int turn = 0;
   for (size_t row = (size_t)blockIdx.x * G + grp; row < a.rows; row += (size_t)gridDim.x * G, turn ^= 1) {
@@ -146,16 +146,16 @@ __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(const RnBwdArgs a) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * L + lane) * 8;
-      load8((const T*)a.h + row * a.ldh + c, C - c, vec, h[j]);
-      load8((const T*)a.dy + row * C + c, C - c, vec, dy[j]);
+      load8((const T*)a.h + row * a.ldh + c, C - c, run, h[j]);
+      load8((const T*)a.dy + row * C + c, C - c, run, dy[j]);
     }
     float ss = 0.f, dot = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * L + lane) * 8;
       float w[8];
-      if (a.w_f32) load8((const float*)a.w + c, C - c, vec, w);
-      else load8((const T*)a.w + c, C - c, vec, w);
+      if (a.w_f32) load8((const float*)a.w + c, C - c, run, w);
+      else load8((const T*)a.w + c, C - c, run, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         ss += h[j][i] * h[j][i];
@@ -170,9 +170,9 @@ __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(const RnBwdArgs a) {
     for (int j = 0; j < NV; ++j) {
       const int c = (j * L + lane) * 8;
       float w[8], add[8], out[8];
-      if (a.w_f32) load8((const float*)a.w + c, C - c, vec, w);
-      else load8((const T*)a.w + c, C - c, vec, w);
-      if (a.dh) load8((const T*)a.dh + row * C + c, C - c, vec, add);
+      if (a.w_f32) load8((const float*)a.w + c, C - c, run, w);
+      else load8((const T*)a.w + c, C - c, run, w);
+      if (a.dh) load8((const T*)a.dh + row * C + c, C - c, run, add);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float n = h[j][i] * rstd;
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(const RnBwdArgs a) {
         out[i] = rstd * (dy[j][i] * w[i] - n * c2);
         if (a.dh) out[i] += add[i];
       }
-      if (a.want_dx && c < C) store8((T*)a.dx + row * C + c, C - c, vec, out);
+      if (a.want_dx && c < C) store8((T*)a.dx + row * C + c, C - c, run, out);
     }
   }
   if (!a.partial) return;
@@ -257,7 +257,12 @@ namespace {
 // the kernel for a row of C values: lanes per row and vectors per lane
 template <typename T, bool Q8>
 void rn_launch(const RnArgs& a, hipStream_t s) {
-#define RN(L, NV) hipLaunchKernelGGL((rmsnorm_kernel<T, L, NV, Q8>), dim3((unsigned)((a.rows + 256 / L - 1) / (256 / L))), dim3(256), 0, s, a)
+#define RN(L, NV)                                                                                                            \
+  do {                                                                                                                        \
+    const dim3 grid((unsigned)((a.rows + 256 / L - 1) / (256 / L)));                                                          \
+    if (a.run == 8) hipLaunchKernelGGL((rmsnorm_kernel<T, L, NV, Q8, true>), grid, dim3(256), 0, s, a);                       \
+    else hipLaunchKernelGGL((rmsnorm_kernel<T, L, NV, Q8, false>), grid, dim3(256), 0, s, a);                                 \
+  } while (0)
   const int C = a.C;
   if (C <= 64) RN(8, 1);
   else if (C <= 128) RN(16, 1);
@@ -272,7 +277,11 @@ void rn_launch(const RnArgs& a, hipStream_t s) {
 }
 template <typename T>
 void rn_bwd_launch(const RnBwdArgs& a, const int groups, hipStream_t s) {
-#define RN(L, NV) hipLaunchKernelGGL((rmsnorm_bwd_kernel<T, L, NV>), dim3((unsigned)groups), dim3(256), 0, s, a)
+#define RN(L, NV)                                                                                                            \
+  do {                                                                                                                        \
+    if (a.run == 8) hipLaunchKernelGGL((rmsnorm_bwd_kernel<T, L, NV, true>), dim3((unsigned)groups), dim3(256), 0, s, a);     \
+    else hipLaunchKernelGGL((rmsnorm_bwd_kernel<T, L, NV, false>), dim3((unsigned)groups), dim3(256), 0, s, a);               \
+  } while (0)
   const int C = a.C;
   if (C <= 64) RN(8, 1);
   else if (C <= 128) RN(16, 1);
@@ -302,8 +311,9 @@ int selfc_rmsnorm(const void* x, size_t ldx, const void* r, size_t ldr, const vo
   const size_t es = dtype ? 2 : 4;
   RnArgs a{};
   a.x = x; a.r = r; a.w = w; a.h = h; a.y = y; a.scale = q8_scale; a.rows = rows; a.ldx = ldx; a.ldr = ldr; a.C = C; a.w_f32 = w_f32; a.eps = eps;
-  a.vec = C % 8 == 0 && aligned_to(x, 16) && (rows == 1 || (ldx * es) % 16 == 0) && aligned_to(w, 16) && aligned_to(y, q8_scale ? 8 : 16) &&
-          (!r || (aligned_to(r, 16) && (rows == 1 || (ldr * es) % 16 == 0) && aligned_to(h, 16)));
+  const auto least = [](const int p, const int q) { return p < q ? p : q; };
+  a.run = least(row_run(x, rows > 1 ? ldx : C, C, es), least(row_run(w, C, C, w_f32 ? 4 : es), row_run(y, C, C, q8_scale ? 1 : es)));
+  if (r) a.run = least(a.run, least(row_run(r, rows > 1 ? ldr : C, C, es), row_run(h, C, C, es)));
   hipStream_t s = (hipStream_t)stream;
   if (q8_scale) {
     if (dtype == 0) rn_launch<float, true>(a, s);
@@ -327,8 +337,10 @@ int selfc_rmsnorm_bwd(const void* h, size_t ldh, const void* w, int w_f32, const
   RnBwdArgs a{};
   a.h = h; a.w = w; a.dy = dy; a.dh = dh; a.dx = dx; a.partial = dw ? partial : nullptr; a.rows = rows; a.ldh = ldh; a.C = C; a.w_f32 = w_f32;
   a.want_dx = dx != nullptr; a.eps = eps;
-  a.vec = C % 8 == 0 && aligned_to(h, 16) && (rows <= 1 || (ldh * es) % 16 == 0) && aligned_to(w, 16) && aligned_to(dy, 16) &&
-          (!dh || aligned_to(dh, 16)) && (!dx || aligned_to(dx, 16));
+  const auto least = [](const int p, const int q) { return p < q ? p : q; };
+  a.run = least(row_run(h, rows > 1 ? ldh : C, C, es), least(row_run(w, C, C, w_f32 ? 4 : es), row_run(dy, C, C, es)));
+  if (dh) a.run = least(a.run, row_run(dh, C, C, es));
+  if (dx) a.run = least(a.run, row_run(dx, C, C, es));
   hipStream_t s = (hipStream_t)stream;
   const int groups = rn_bwd_groups(rows, C);
   if (groups) {

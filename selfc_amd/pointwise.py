@@ -6,7 +6,8 @@
     y = linear_q8(q, s, wq, ws, ...)                  the same on e4m3 rows and an e4m3 weight (quantize_rows)
 
 The last axis is the row; leading axes may be any.  Rows may have any length, pitch and offset: rows that the kernels cannot read
-in 16-byte pieces are laid out again first (one more launch; widths that are multiples of 8 - of 16 in 8 bits - avoid it).
+in 16-byte pieces are laid out again first (one more launch; widths that are multiples of 8 - of 16 in 8 bits - avoid it; 16-bit layers
+of up to about 200 values each way read any layout in place).
 Everything runs on the current stream of the tensors' device, allocates from torch's allocator only, and may be captured into a
 graph.  As for every torch module, a backward pass is captured only when no eager graph over the same leaves is alive any more
 (drop the losses of the eager steps first); such a capture is refused here (autograd would end the process).
@@ -267,18 +268,45 @@ def _run_linear(xp, ldx, k, wp, ldw, n, xs, ws_, bias, act, r2, out_dtype, want_
     return y, slope
 
 
+def _narrow(n: int, k: int) -> bool:
+    return n <= 256 and k <= 256 and bool(_lib.lib().selfc_linear_rows_ok(n, k))
+
+
+def _run_rows(x2, w2, bias, act, r2, want_slope, want_pieces):
+    """(y, slope, x as whole pieces) of a narrow layer: one launch, any layout of x and the weight."""
+    (rows, k), n = x2.shape, w2.shape[0]
+    dev, dt = x2.device, x2.dtype
+    y = torch.empty((rows, n), dtype=dt, device=dev)
+    slope = torch.empty((rows, -(-n // 8) * 8), dtype=torch.int16, device=dev) if want_slope else None
+    xp = None
+    if want_pieces:
+        whole = k % 8 == 0 and x2.data_ptr() % 16 == 0 and _pitch(x2) % 8 == 0 and _pitch(x2) < (1 << 21)
+        xp = x2 if whole else torch.empty((rows, -(-k // 8) * 8), dtype=dt, device=dev)
+    if rows:
+        rt.call("selfc_linear_rows", x2.data_ptr(), _pitch(x2), w2.data_ptr(), _pitch(w2), _ptr(bias), act, _ptr(r2), 0 if r2 is None else _pitch(r2),
+                y.data_ptr(), _ptr(slope), None if xp is None or xp is x2 else xp.data_ptr(), rows, n, k, _DTYPE[dt], _stream(x2))
+    return y, slope, xp
+
+
 class LinearFn(torch.autograd.Function):
-    """linear on matrices.  Kept for the backward pass: x and the weight as the kernels read them, and the activation's derivative
-    as 16-bit fixed point."""
+    """linear on matrices.  Kept for the backward pass: x as the kernels read it, the weight, and the activation's derivative as 16-bit
+    fixed point."""
 
     @staticmethod
     def forward(ctx, x2, weight, bias, r2, act):
+        n, k = weight.shape
+        need = ctx.needs_input_grad
+        slope = act != 0 and any(need[:3])
+        ctx.narrow = _narrow(n, k)
         with on_device(x2):
-            xp, ldx = _pieces(x2)
-            wp, ldw = _pieces(weight)
-            need = ctx.needs_input_grad
-            y, slope = _run_linear(xp, ldx, x2.shape[1], wp, ldw, weight.shape[0], None, None, bias, act, r2, x2.dtype, act != 0 and any(need[:3]))
-        ctx.dims = (x2.shape[0], weight.shape[0], x2.shape[1], ldx, ldw)
+            if ctx.narrow:
+                y, slope, xp = _run_rows(x2, weight, bias, act, r2, slope, need[1])
+                wp, ldw = weight, _pitch(weight)
+            else:
+                xp, ldx = _pieces(x2)
+                wp, ldw = _pieces(weight)
+                y, slope = _run_linear(xp, ldx, k, wp, ldw, n, None, None, bias, act, r2, x2.dtype, slope)
+        ctx.dims = (x2.shape[0], n, k, ldw)
         ctx.save_for_backward(xp if need[1] else None, wp if need[0] else None, slope)
         ctx.dtype = x2.dtype
         return y
@@ -287,36 +315,41 @@ class LinearFn(torch.autograd.Function):
     def backward(ctx, dy):
         _no_second(ctx)
         xp, wp, slope = ctx.saved_tensors
-        rows, n, k, ldx, ldw = ctx.dims
+        rows, n, k, ldw = ctx.dims
         want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
         dev, dt, code, stream = dy.device, ctx.dtype, _DTYPE[ctx.dtype], _stream(dy)
         dx = dw = db = None
+        if rows == 0:
+            return (torch.empty((0, k), dtype=dt, device=dev) if want_x else None, torch.zeros((n, k), dtype=dt, device=dev) if want_w else None,
+                    torch.zeros(n, dtype=dt, device=dev) if want_b else None, (dy if want_r else None), None)
         L = _lib.lib()
         with on_device(dy):
             g = _rows(dy)
-            if rows == 0:
-                dx = torch.empty((0, k), dtype=dt, device=dev) if want_x else None
-                dw = torch.zeros((n, k), dtype=dt, device=dev) if want_w else None
-                db = torch.zeros(n, dtype=dt, device=dev) if want_b else None
-                return dx, dw, db, (dy if want_r else None), None
-            up = -(-n // 8) * 8
-            products = want_x or want_w
-            as_is = slope is None and n % 8 == 0 and g.data_ptr() % 16 == 0 and (rows == 1 or _pitch(g) % 8 == 0) and _pitch(g) < (1 << 21)
-            dz, lddz = (g, _pitch(g)) if as_is else (torch.empty((rows, up), dtype=dt, device=dev) if products else None, up)
-            if want_b:
+            ldg, up = _pitch(g), -(-n // 8) * 8
+            as_is = slope is None and n % 8 == 0 and g.data_ptr() % 16 == 0 and ldg % 8 == 0 and ldg < (1 << 21)
+            rows_kernel = want_x and ctx.narrow
+            make_dz = not as_is and (want_w or (want_x and not rows_kernel))
+            dz, lddz = (torch.empty((rows, up), dtype=dt, device=dev), up) if make_dz else (g, ldg)
+            if want_b:                              # with dW it comes out of that product
                 db = torch.empty(n, dtype=dt, device=dev)
-            if want_b or (products and not as_is):
-                part = torch.empty(L.selfc_linear_dz_floats(rows, n), dtype=torch.float32, device=dev) if want_b else None
-                rt.call("selfc_linear_dz", g.data_ptr(), _pitch(g), _ptr(slope), None if as_is or not products else dz.data_ptr(), up, _ptr(db), _ptr(part),
-                        rows, n, code, stream)
             if want_x:
                 dx = torch.empty((rows, k), dtype=dt, device=dev)
+            if rows_kernel:
+                rt.call("selfc_linear_rows_bwd", g.data_ptr(), ldg, _ptr(slope), wp.data_ptr(), ldw, dx.data_ptr(), dz.data_ptr() if make_dz else None,
+                        rows, n, k, code, stream)
+            alone = want_b and not want_w
+            if alone or (make_dz and not rows_kernel):
+                part = torch.empty(L.selfc_linear_dz_floats(rows, n), dtype=torch.float32, device=dev) if alone else None
+                rt.call("selfc_linear_dz", g.data_ptr(), ldg, _ptr(slope), dz.data_ptr() if make_dz and not rows_kernel else None, up,
+                        db.data_ptr() if alone else None, _ptr(part), rows, n, code, stream)
+            if want_x and not rows_kernel:
                 work = _ws(rows, k, n, 2, dev)
                 rt.call("selfc_linear_dx", dz.data_ptr(), lddz, wp.data_ptr(), ldw, dx.data_ptr(), _ptr(work), rows, n, k, code, stream)
             if want_w:
                 dw = torch.empty((n, k), dtype=dt, device=dev)
-                work = _ws(n, k, rows, 2, dev)
-                rt.call("selfc_linear_dw", dz.data_ptr(), lddz, xp.data_ptr(), ldx, dw.data_ptr(), _ptr(work), rows, n, k, code, stream)
+                floats = L.selfc_linear_dw_floats(rows, n, k)
+                work = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
+                rt.call("selfc_linear_dw", dz.data_ptr(), lddz, xp.data_ptr(), _pitch(xp), dw.data_ptr(), _ptr(db), _ptr(work), rows, n, k, code, stream)
         return dx, dw, db, (dy if want_r else None), None
 
 
@@ -324,8 +357,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(x weight^T + bias) + residual; x (..., in), weight (out, in), both bf16 or both f16, bias (out,) and residual (..., out) of the
     same type.  act: "none", "relu", "lrelu" (0.2), "gelu" (erf), "silu".  Sums, bias, activation and residual in fp32, one rounding at the end;
-    in the backward pass dy act'(z) is rounded to x's type once, as the operand of both products.  Up to 16 rows the weight streams
-    through a kernel of its own.  Sums are added in a fixed order."""
+    in the backward pass dy act'(z) is rounded to x's type once, as the operand of both products.  Wide weights
+    stream through a kernel of its own for up to 16 rows; layers of up to about 200 values each way keep theirs in shared memory.  Sums are added in a fixed order."""
     dt = x.dtype
     if dt is not torch.bfloat16 and dt is not torch.float16:
         _lib.require_gpu(x)
@@ -340,9 +373,13 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
         _watch(y)
     else:
         with on_device(x):
-            xp, ldx = _pieces(x2)
-            wp, ldw = _pieces(w2)
-            y, _ = _run_linear(xp, ldx, x2.shape[1], wp, ldw, weight.shape[0], None, None, b, ACTS[act], r2, dt, False)
+            n, k = w2.shape
+            if _narrow(n, k):
+                y = _run_rows(x2, w2, b, ACTS[act], r2, False, False)[0]
+            else:
+                xp, ldx = _pieces(x2)
+                wp, ldw = _pieces(w2)
+                y, _ = _run_linear(xp, ldx, k, wp, ldw, n, None, None, b, ACTS[act], r2, dt, False)
     return y if x.dim() == 2 else y.view(x.shape[:-1] + weight.shape[:1])
 
 

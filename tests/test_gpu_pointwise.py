@@ -195,7 +195,7 @@ def product_bound(dt, k, z, size, y):
 
 
 SHAPES = [(1, 1, 1), (1, 64, 16), (3, 8, 5), (16, 4096, 40), (16, 51, 204), (17, 64, 64), (33, 51, 3), (65, 200, 130), (128, 128, 128), (130, 520, 72),
-          (300, 64, 129), (257, 130, 257), (700, 96, 8), (70, 2056, 66), (64, 8192, 64)]
+          (300, 64, 129), (257, 130, 257), (700, 96, 8), (70, 2056, 66), (64, 8192, 64), (300, 515, 723), (40, 1000, 301), (19, 333, 258)]
 
 
 @pytest.mark.parametrize("dt", T16)
@@ -231,6 +231,31 @@ def test_product_gradients(dt, m, k, n, act):
     for got, want, mag, err, terms in ((gx, dz @ W, dz.abs() @ W.abs(), off @ W.abs(), n), (gw, dz.t() @ X, dz.abs().t() @ X.abs(), off.t() @ X.abs(), m),
                                        (gb, dz.sum(0), dz.abs().sum(0), off.sum(0), m)):
         within(got, want, (want.abs() + err) * u(dt) * 1.01 + err + (terms + 10) * U32 * mag * 1.01 + TINY[dt])
+
+
+@pytest.mark.parametrize("dt", T16)
+@pytest.mark.parametrize("m,k,n", [(1500, 328, 2000), (3600, 336, 3590), (2100, 520, 300), (20000, 200, 100), (4200, 130, 66)])
+def test_product_of_many_tiles(dt, m, k, n):
+    """Sizes that fill the chip with large tiles (and long narrow ones); the reference in 64 bits on the GPU."""
+    gen = torch.Generator().manual_seed(m + k + n)
+    x, w, b, dy, r = (t.cuda() for t in (rnd(gen, m, k, dtype=dt), rnd(gen, n, k, scale=k ** -0.5, dtype=dt), rnd(gen, n, dtype=dt), rnd(gen, m, n, dtype=dt),
+                                         rnd(gen, m, n, dtype=dt)))
+    z, size, y, d = product_ref(x, w, b, r, "silu")
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    out = pw().linear(leaves[0], leaves[1], bias=leaves[2], act="silu", residual=r)
+    within(out, y.cpu(), product_bound(dt, k, z, size, y).cpu())
+    grads = torch.autograd.grad(out, leaves, dy)
+    X, W, D = x.double(), w.double(), dy.double()
+    dz = D * d
+    off = dz.abs() * u(dt) + D.abs() * (2.0 ** -16 + 2.0 ** -20 + (k + 10) * U32 * size) + TINY[dt]
+    for got, want, mag, err, terms in ((grads[0], dz @ W, dz.abs() @ W.abs(), off @ W.abs(), n), (grads[1], dz.t() @ X, dz.abs().t() @ X.abs(), off.t() @ X.abs(), m),
+                                       (grads[2], dz.sum(0), dz.abs().sum(0), off.sum(0), m)):
+        within(got, want.cpu(), ((want.abs() + err) * u(dt) * 1.01 + err + (terms + 10) * U32 * mag * 1.01 + TINY[dt]).cpu())
+    if k % 16 == 0:
+        q, s = pw().quantize_rows(x)
+        wq, ws = pw().quantize_rows(w)
+        z, size, y, _ = product_ref(q.float(), wq.float(), b, r, "none", (s, ws))
+        within(pw().linear_q8(q, s, wq, ws, bias=b, residual=r, out_dtype=dt), y.cpu(), product_bound(dt, k, z, size, y).cpu())
 
 
 @pytest.mark.parametrize("out", T16 + [torch.float32])
