@@ -467,7 +467,7 @@ int selfc_linear_dw(const void* dz, size_t lddz, const void* x, size_t ldx, void
 /* Narrow layers (selfc_linear_rows_ok(n, k): up to 256 each way, their weight in shared memory): bf16 / f16 rows and weights of any pitch and
  * offset.  y without gaps, slope as above, xp (or NULL): receives x's rows with pitch roundup(k, 8) and zeros behind them (selfc_linear_dw's
  * operand).  The backward call makes dx [rows][k] and dz (or NULL; as selfc_linear_dz) from dy and slope (or NULL: no activation).
- * y, dx, slope, xp, dz 16-byte aligned. */
+ * slope, xp, dz 16-byte aligned. */
 int selfc_linear_rows_ok(int n, int k);
 int selfc_linear_rows(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, int act, const void* res, size_t ldr, void* y,
                       void* slope, void* xp, size_t rows, int n, int k, int dtype, void* stream);

@@ -64,20 +64,11 @@ __device__ __forceinline__ int aw_find(const AwTable& t, const unsigned wg) {
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(a)) + __popcll(__ballot(b)) - 1);
 }
 
-__device__ __forceinline__ unsigned wave_umax(unsigned v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned w = __shfl_xor(v, o);
-    v = w > v ? w : v;
-  }
-  return v;
-}
-
 // the block's scale 2^(floor(log2 most) - top), not below 2^-126; 1 for an empty block.  `inv` = 1 / scale, exact.
-__device__ __forceinline__ float aw_scale(const unsigned most, const int top, float& inv) {
-  int e = (int)(most >> 23) - top;           // biased exponent of the scale
+__device__ __forceinline__ float aw_scale(const float most, const int top, float& inv) {
+  int e = (int)(__builtin_bit_cast(unsigned, most) >> 23) - top;           // biased exponent of the scale
   e = e < 1 ? 1 : e;
-  if (most == 0) e = 127;
+  if (most == 0.f) e = 127;
   inv = __builtin_bit_cast(float, (unsigned)(254 - e) << 23);
   return __builtin_bit_cast(float, (unsigned)e << 23);
 }
@@ -170,7 +161,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwTable tab, const AwH
   for (int u = 0; u < AW_U; ++u) {
     if (base + u * AW_BLOCK >= n) break;
     const unsigned long long at = base + u * AW_BLOCK + lane * 4;
-    unsigned mmost = 0, vmost = 0;
+    float mmost = 0.f, vmost = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float gi = gv[u][i];
@@ -183,10 +174,9 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwTable tab, const AwH
       const float den = __builtin_amdgcn_sqrtf(vi) * ibc2 + hy.eps;
       pv[u][i] = pv[u][i] * keep - rate * (mi * __builtin_amdgcn_rcpf(den));
       if constexpr (BITS == 8) {
-        const unsigned am = __builtin_bit_cast(unsigned, mi) & 0x7fffffffu, av = __builtin_bit_cast(unsigned, vi) & 0x7fffffffu;
-        const bool in = at + i < n;
-        mmost = in && am < 0x7f800000u && am > mmost ? am : mmost;
-        vmost = in && av < 0x7f800000u && av > vmost ? av : vmost;
+        const float am = fabsf(mi);            // v is not negative; values behind the tensor's end are 0
+        mmost = fmaxf(mmost, am < INFINITY ? am : 0.f);
+        vmost = fmaxf(vmost, vi < INFINITY ? vi : 0.f);
       }
     }
     if (vec && at + 4 <= n) {
@@ -213,7 +203,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwTable tab, const AwH
       }
     } else {
       float im, iv;
-      const float sm = aw_scale(wave_umax(mmost), 7, im), sv = aw_scale(wave_umax(vmost), 14, iv);
+      const float sm = aw_scale(lanes_max<64>(mmost), 7, im), sv = aw_scale(lanes_max<64>(vmost), 14, iv);
       float mq[4], vq[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -244,14 +234,13 @@ __global__ __launch_bounds__(256) void grad_norm_kernel(const AwTable tab, const
     const unsigned long long base = (unsigned long long)(c - en.wg0) * AW_CHUNK;
     const unsigned long long left = en.n - base;
     const T* const q = g + base;
-    const bool vec = aligned16((const void*)q);
 #pragma unroll
     for (int j = 0; j < AW_CHUNK / 2048; ++j) {
       const long at = j * 2048 + threadIdx.x * 8;
       if ((unsigned long long)at < left) {
         float v[8];
         const unsigned long long l = left - at;
-        load8(q + at, l > 8 ? 8 : (long)l, vec && l >= 8 ? 8 : 1, v);
+        load8(q + at, l > 8 ? 8 : (long)l, at + base ? 8 : 0, v);
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc += (double)v[i] * (double)v[i];
       }

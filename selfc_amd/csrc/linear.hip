@@ -36,7 +36,7 @@ struct Epilogue {
   const float *qs, *ps;           // scales of the rows and of the columns
   unsigned short* d;              // [M][ldd] derivative
   size_t ldo, ldr, ldd;
-  int dtype, act, run;            // run: values per load and store of a row (row_run)
+  int dtype, act;
 };
 
 // N values z -> activation y and, with D, its derivative d.  GELU: z phi(z) with phi = 1 - erfc(|z| / sqrt 2) / 2 mirrored at 0, erfc by
@@ -86,10 +86,10 @@ __device__ __forceinline__ float act_slope(const unsigned c) {
   return c == 65535u ? __builtin_nanf("") : (float)((int)c - 16384) * 0x1p-15f;
 }
 
-__device__ __forceinline__ void load8_as(const int dtype, const void* const p, const size_t at, const long left, const int run, float* const v) {
-  if (dtype == 0) load8((const float*)p + at, left, run, v);
-  else if (dtype == 1) load8((const b16*)p + at, left, run, v);
-  else load8((const h16*)p + at, left, run, v);
+__device__ __forceinline__ void load8_as(const int dtype, const void* const p, const size_t at, const int left, const int before, float* const v) {
+  if (dtype == 0) load8((const float*)p + at, left, before, v);
+  else if (dtype == 1) load8((const b16*)p + at, left, before, v);
+  else load8((const h16*)p + at, left, before, v);
 }
 
 // eight neighbouring columns of one row: acc is the product's sum, b and ps the columns' bias and scale
@@ -109,25 +109,25 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, const float* const 
     act_apply<8, false>(e.act, z, y, d);
   }
   if (e.res) {
-    load8_as(e.dtype, e.res, (size_t)row * e.ldr + col, left, e.run, r);
+    load8_as(e.dtype, e.res, (size_t)row * e.ldr + col, left, col, r);
 #pragma unroll
     for (int i = 0; i < 8; ++i) y[i] += r[i];
   }
   const size_t at = (size_t)row * e.ldo + col;
-  if (e.dtype == 0) store8((float*)e.out + at, left, e.run, y);
-  else if (e.dtype == 1) store8((b16*)e.out + at, left, e.run, y);
-  else store8((h16*)e.out + at, left, e.run, y);
+  if (e.dtype == 0) store8((float*)e.out + at, left, y);
+  else if (e.dtype == 1) store8((b16*)e.out + at, left, y);
+  else store8((h16*)e.out + at, left, y);
 }
 // the same where nothing follows the product
 template <typename T>
 __device__ __forceinline__ void plain8(const Epilogue& e, const float* const acc, const int row, const int col, const int left) {
-  store8((T*)e.out + (size_t)row * e.ldo + col, left, e.run, acc);
+  store8((T*)e.out + (size_t)row * e.ldo + col, left, acc);
 }
 __device__ __forceinline__ void epilogue_columns(const Epilogue& e, const int col, const int left, float* const b, float* const ps) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) { b[i] = 0.f; ps[i] = 1.f; }
-  if (e.bias) load8_as(e.dtype, e.bias, col, left, 1, b);
-  if (e.ps) load8(e.ps + col, left, 1, ps);
+  if (e.bias) load8_as(e.dtype, e.bias, col, left, col, b);
+  if (e.ps) load8(e.ps + col, left, col, ps);
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------------
@@ -515,31 +515,30 @@ struct RowsArgs {
   const unsigned short* d;        // backward: derivative [rows][ldd], or NULL
   void* xp;                       // NULL, or the operand's rows with pitch roundup(K, 8) and zeros behind them
   size_t ldx, ldw, ldd, rows;
-  int N, K, xrun, wrun, turn;     // turn: bytes of shared memory per wave for rows that cannot be stored in runs of 4 (0: they can)
+  int N, K;
   Epilogue e;                     // out without gaps
 };
-// eight neighbouring 16-bit values as they are stored; zeros from `left` on.  `room`: how many values the matrix still has from p on -
-// where a row ends inside the eight, the next row's are read along (one load at any 2-byte address) and cleared
-template <typename T>
-__device__ __forceinline__ i32x4 raw8(const T* const p, const int left, const bool whole, const size_t room) {
-  i32x4 r = {0, 0, 0, 0};
-  if (left <= 0) return r;
-  if (whole) return *reinterpret_cast<const i32x4*>(p);
-  if (room >= 8) {
-    __builtin_memcpy(&r, p, 16);
-  } else {
-    const unsigned short* const u = reinterpret_cast<const unsigned short*>(p);
-    for (int i = 0; i < (int)room; ++i) {
-      const int v = (int)((unsigned)u[i] << (16 * (i & 1)));
-      if (i < 2) r[0] |= v;
-      else if (i < 4) r[1] |= v;
-      else if (i < 6) r[2] |= v;
-      else r[3] |= v;
-    }
-  }
+// Two neighbouring tiles' results: four consecutive columns of each per lane (columns 4 g of its tile) -> eight consecutive ones of one
+// tile (g = 0, 1: the first's columns 0, 8; g = 2, 3: the second's), and back: two exchanges of 16- and 32-lane halves per register pair.
+__device__ __forceinline__ u32x4 joined(const u32x2* const t) {
+  u32x4 r;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r[i] = left >= 2 * i + 2 ? r[i] : left == 2 * i + 1 ? r[i] & 0xffff : 0;
+  for (int k = 0; k < 2; ++k) {
+    const u32x2 a = __builtin_amdgcn_permlane32_swap(t[0][k], t[1][k], false, false);
+    const u32x2 b = __builtin_amdgcn_permlane16_swap(a[0], a[1], false, false);
+    r[k] = b[0];
+    r[2 + k] = b[1];
+  }
   return r;
+}
+__device__ __forceinline__ void apart(const u32x4 r, u32x2* const t) {
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const u32x2 a = __builtin_amdgcn_permlane16_swap(r[k], r[2 + k], false, false);
+    const u32x2 b = __builtin_amdgcn_permlane32_swap(a[0], a[1], false, false);
+    t[0][k] = b[0];
+    t[1][k] = b[1];
+  }
 }
 template <typename T, int KS, bool BWD, int NW>
 __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
@@ -549,22 +548,17 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
   extern __shared__ __align__(16) unsigned char lds[];
   const int N = a.N, K = a.K, kp = (K + 7) & ~7, tp = (N + 15) / 16;
   float* const bias = reinterpret_cast<float*>(lds + tp * 16 * PITCH);
-  unsigned char* const scratch = lds + tp * 16 * PITCH + tp * 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, q = lane & 15;
 
-  const bool xwhole = a.xrun == 8, wwhole = a.wrun == 8;
-  const size_t xend = (a.rows - 1) * a.ldx + K, wend = (size_t)((BWD ? K : N) - 1) * a.ldw + (BWD ? N : K);
   if constexpr (!BWD) {           // w [N][K]
     for (int ch = threadIdx.x; ch < tp * 16 * KS * 4; ch += NT) {
       const int p = ch / (KS * 4), c = ch % (KS * 4) * 8;
-      const size_t at = p * a.ldw + c;
-      *reinterpret_cast<i32x4*>(lds + p * PITCH + c * 2) = raw8((const T*)a.w + at, p < N ? K - c : 0, wwhole, wend - at);
+      *reinterpret_cast<u32x4*>(lds + p * PITCH + c * 2) = raw8((const T*)a.w + p * a.ldw + c, p < N ? K - c : 0, c);
     }
   } else {                        // w [K][N]: turned; neighbouring threads take neighbouring places of the sum, whose stores share no bank
     for (int ch = threadIdx.x; ch < KS * 32 * tp * 2; ch += NT) {
       const int r = ch % (KS * 32), c = ch / (KS * 32) * 8;
-      const size_t at = r * a.ldw + c;
-      const T8 v = __builtin_bit_cast(T8, raw8((const T*)a.w + at, r < K ? N - c : 0, wwhole, wend - at));
+      const T8 v = __builtin_bit_cast(T8, raw8((const T*)a.w + r * a.ldw + c, r < K ? N - c : 0, c));
 #pragma unroll
       for (int i = 0; i < 8; ++i) *reinterpret_cast<T*>(lds + (c + i) * PITCH + r * 2) = v[i];
     }
@@ -581,7 +575,7 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int c = ks * 32 + g * 8;
-      xf[ks] = raw8((const T*)a.x + row * a.ldx + c, in ? K - c : 0, xwhole, xend - (row * a.ldx + c));
+      xf[ks] = __builtin_bit_cast(i32x4, raw8((const T*)a.x + row * a.ldx + c, in ? K - c : 0, c));
       if constexpr (BWD) {
         if (a.d && in && c < kp) dv[ks] = *reinterpret_cast<const u16x8*>(a.d + row * a.ldd + c);
       }
@@ -602,7 +596,6 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
       }
       if (a.xp && in && c < kp) *reinterpret_cast<i32x4*>((T*)a.xp + row * kp + c) = xf[ks];
     }
-    unsigned char* const turn = scratch + wave * a.turn;
     // four tiles of 16 columns at a time: enough independent multiplies, few enough registers for 16 waves per compute unit
 #pragma unroll 1
     for (int p4 = 0; p4 < tp; p4 += 4) {
@@ -617,64 +610,52 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
         }
       }
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        const int col = (p4 + p) * 16 + g * 4;
-        if (p4 + p >= tp) break;
-        float y[4];
-        if constexpr (BWD) {
+      for (int pp = 0; pp < 4; pp += 2) {
+        if (p4 + pp >= tp) break;
+        const int col8 = (p4 + pp + (g >> 1)) * 16 + (g & 1) * 8, left = in ? N - col8 : 0;      // this lane's eight columns of the pair
+        u32x2 yp[2], cp[2], rp[2];
+        if (!BWD && a.e.res) apart(raw8((const T*)a.e.res + row * a.e.ldr + col8, left, col8), rp);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) y[i] = acc[p][i];
-        } else {
-          const f32x4 b = *reinterpret_cast<const f32x4*>(bias + col);
-          float z[4], d[4];
+        for (int h = 0; h < 2; ++h) {
+          float y[4];
+          if constexpr (BWD) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) z[i] = acc[p][i] + b[i];
-          if (a.e.d) {
-            act_apply<4, true>(a.e.act, z, y, d);
-            u32x2 c;
-            c[0] = act_code(d[0], z[0]) | act_code(d[1], z[1]) << 16;
-            c[1] = act_code(d[2], z[2]) | act_code(d[3], z[3]) << 16;
-            if (in && col < (int)a.e.ldd) *reinterpret_cast<u32x2*>(a.e.d + row * a.e.ldd + col) = c;
+            for (int i = 0; i < 4; ++i) y[i] = acc[pp + h][i];
           } else {
-            act_apply<4, false>(a.e.act, z, y, d);
-          }
-          if (a.e.res && in) {
-            const T* const r = (const T*)a.e.res + row * a.e.ldr + col;
-            if (a.e.run >= 4) {
-              if (col < N) {
-                const T4 v = *reinterpret_cast<const T4*>(r);
+            const int col = (p4 + pp + h) * 16 + g * 4;
+            f32x4 b = {0.f, 0.f, 0.f, 0.f};
+            if (p4 + pp + h < tp) b = *reinterpret_cast<const f32x4*>(bias + col);
+            float z[4], d[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] += (float)v[i];
-              }
+            for (int i = 0; i < 4; ++i) z[i] = acc[pp + h][i] + b[i];
+            if (a.e.d) {
+              act_apply<4, true>(a.e.act, z, y, d);
+              cp[h] = u32x2{act_code(d[0], z[0]) | act_code(d[1], z[1]) << 16, act_code(d[2], z[2]) | act_code(d[3], z[3]) << 16};
             } else {
+              act_apply<4, false>(a.e.act, z, y, d);
+            }
+            if (a.e.res) {
+              const T4 v = __builtin_bit_cast(T4, rp[h]);
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (col + i < N) y[i] += (float)r[i];
+              for (int i = 0; i < 4; ++i) y[i] += (float)v[i];
             }
           }
+          yp[h] = __builtin_bit_cast(u32x2, T4{(T)y[0], (T)y[1], (T)y[2], (T)y[3]});
         }
-        T4 h;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) h[i] = (T)y[i];
-        if (!a.turn) {
-          if (in && col < N) *reinterpret_cast<T4*>((T*)a.e.out + row * N + col) = h;
+        if (!BWD && a.e.d) {
+          const u32x4 c = joined(cp);
+          if (in && col8 < (int)a.e.ldd) *reinterpret_cast<u32x4*>(a.e.d + row * a.e.ldd + col8) = c;
+        }
+        const u32x4 o = joined(yp);
+        unsigned short* const out = (unsigned short*)a.e.out + row * N + col8;
+        if (left >= 8) {
+          __builtin_memcpy(out, &o, 16);
         } else {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (col + i < N) *reinterpret_cast<T*>(turn + (q * N + col + i) * 2) = h[i];
+          for (int i = 0; i < 8; ++i)
+            if (i < left) out[i] = (unsigned short)(o[i / 2] >> (16 * (i & 1)));
         }
       }
-    }
-    if (a.turn) {                 // 16 whole rows are one stretch of memory
-      __builtin_amdgcn_wave_barrier();
-      const int bytes = (int)(a.rows - row0 < 16 ? a.rows - row0 : 16) * N * 2;
-      unsigned char* const out = (unsigned char*)a.e.out + row0 * N * 2;
-      for (int b = lane * 16; b < bytes; b += 1024) {
-        if (b + 16 <= bytes) *reinterpret_cast<i32x4*>(out + b) = *reinterpret_cast<const i32x4*>(turn + b);
-        else
-          for (int k = b; k < bytes; k += 2) *reinterpret_cast<unsigned short*>(out + k) = *reinterpret_cast<const unsigned short*>(turn + k);
-      }
-      __builtin_amdgcn_wave_barrier();
     }
   }
 }
@@ -700,13 +681,13 @@ struct DzArgs {
   void* dz;                       // or NULL: only the sums
   float* partial;                 // [gridDim.y][N] or NULL
   size_t rows, lddy, ldd, lddz;
-  int N, run;
+  int N;
 };
-template <typename T, int L>
+template <typename T, int L, bool WHOLE>
 __global__ __launch_bounds__(256) void dz_kernel(const DzArgs a) {
   constexpr int G = 256 / L;
   const int lane = threadIdx.x & (L - 1), grp = threadIdx.x / L;
-  const int col = (blockIdx.x * L + lane) * 8, left = a.N - col;
+  const int col = (blockIdx.x * L + lane) * 8, left = WHOLE ? (col < a.N ? 8 : 0) : a.N - col;       // WHOLE: N is a multiple of 8
   float sum[8] = {};
   if (left > 0) {
     constexpr int U = 4;                     // rows whose loads are in flight together
@@ -717,7 +698,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const DzArgs a) {
 #pragma unroll
       for (int k = 0; k < U; ++k)
         if (row + k * step < a.rows) {
-          load8((const T*)a.dy + (row + k * step) * a.lddy + col, left, a.run, v[k]);
+          load8((const T*)a.dy + (row + k * step) * a.lddy + col, left, col, v[k]);
           if (a.d) c[k] = *reinterpret_cast<const u16x8*>(a.d + (row + k * step) * a.ldd + col);
         }
 #pragma unroll
@@ -728,7 +709,7 @@ __global__ __launch_bounds__(256) void dz_kernel(const DzArgs a) {
             for (int i = 0; i < 8; ++i) v[k][i] = i < left ? v[k][i] * act_slope(c[k][i]) : 0.f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) sum[i] += v[k][i];
-          if (a.dz) store8((T*)a.dz + (row + k * step) * a.lddz + col, 8, 8, v[k]);           // zeros behind the last column
+          if (a.dz) store8((T*)a.dz + (row + k * step) * a.lddz + col, 8, v[k]);           // zeros behind the last column
         }
     }
   }
@@ -810,27 +791,21 @@ int gemm_run(GemmArgs a, hipStream_t s) {
 
 // ---- narrow rows: which instance, and the shared memory it takes ----------------------------------------------------------------
 constexpr int ROWS_MAX = 256;
-struct RowsPlan { int ks, nw, turn, lds, per_cu; };
-inline RowsPlan rows_plan(const int N, const int K, const bool runs4) {
+struct RowsPlan { int ks, nw, lds, per_cu; };
+inline RowsPlan rows_plan(const int N, const int K) {
   RowsPlan p{};
   const int tp = (N + 15) / 16;
   p.ks = K <= 64 ? 2 : K <= 128 ? 4 : 8;
-  const int weight = tp * 16 * (p.ks * 64 + 16) + tp * 64;
-  p.nw = weight > 32 * 1024 ? 8 : 4;               // a large weight is shared by more waves
-  p.turn = runs4 ? 0 : 32 * N;
-  p.lds = weight + p.nw * p.turn;
+  p.lds = tp * 16 * (p.ks * 64 + 16) + tp * 64;
+  p.nw = p.lds > 32 * 1024 ? 8 : 4;                // a large weight is shared by more waves
   const int most = 16 / p.nw;                      // 16 waves per compute unit
   p.per_cu = 160 * 1024 / p.lds < most ? 160 * 1024 / p.lds : most;
   return p;
 }
-// both directions of a layer have to fit
-inline bool rows_ok(const int n, const int k) {
-  return n <= ROWS_MAX && k <= ROWS_MAX && rows_plan(n, k, false).lds <= 160 * 1024 && rows_plan(k, n, false).lds <= 160 * 1024;
-}
+inline bool rows_ok(const int n, const int k) { return n <= ROWS_MAX && k <= ROWS_MAX; }        // 133 KiB at most: it fits
 template <typename T, bool BWD>
 int rows_run(RowsArgs a, hipStream_t s) {
-  const RowsPlan p = rows_plan(a.N, a.K, row_run(a.e.out, a.N, a.N, 2) >= 4);
-  a.turn = p.turn;
+  const RowsPlan p = rows_plan(a.N, a.K);
   // workgroups that the chip holds at a time, each with its copy of the weight, or as many as there are tiles for
   const size_t need = (a.rows + p.nw * 16 - 1) / (p.nw * 16), hold = 256 * (size_t)p.per_cu;
   const dim3 grid((unsigned)(need < hold ? need : hold)), blk(p.nw * 64);
@@ -860,12 +835,9 @@ inline bool rows_fit(const void* p, const size_t ld, const size_t cols, const si
   return aligned_to(p, 16) && (ld * es) % 16 == 0 && (cols * es) % 16 == 0 && ld < (1u << 21);
 }
 
-Epilogue make_epilogue(void* out, size_t ldo, const void* bias, const void* res, size_t ldr, int dtype, int act, int N) {
+Epilogue make_epilogue(void* out, size_t ldo, const void* bias, const void* res, size_t ldr, int dtype, int act) {
   Epilogue e{};
-  const size_t es = dtype ? 2 : 4;
   e.out = out; e.bias = bias; e.res = res; e.ldo = ldo; e.ldr = ldr; e.dtype = dtype; e.act = act;
-  e.run = row_run(out, ldo, N, es);
-  if (res) { const int r = row_run(res, ldr, N, es); e.run = r < e.run ? r : e.run; }
   return e;
 }
 
@@ -904,7 +876,7 @@ int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const flo
   if ((rows > 1 && ldx < (size_t)k) || (n > 1 && ldw < (size_t)k) || (res && rows > 1 && ldr < (size_t)n)) return SELFC_EINVAL;
   GemmArgs a{};
   a.q = x; a.p = w; a.ldq = ldx; a.ldp = ldw; a.M = (int)rows; a.N = n; a.R = k; a.ws = ws;
-  a.e = make_epilogue(y, n, bias, res, ldr, out_dtype, act, n);
+  a.e = make_epilogue(y, n, bias, res, ldr, out_dtype, act);
   a.e.qs = x_scale; a.e.ps = w_scale; a.e.d = (unsigned short*)slope; a.e.ldd = up8(n);
   hipStream_t s = (hipStream_t)stream;
   if (rows <= GEMV_ROWS) {
@@ -927,14 +899,15 @@ int selfc_linear_dz(const void* dy, size_t lddy, const void* slope, void* dz, si
   if (slope && !aligned_to(slope, 16)) return SELFC_EINVAL;
   DzArgs a{};
   a.dy = dy; a.d = (const unsigned short*)slope; a.dz = dz; a.partial = db ? partial : nullptr; a.rows = rows; a.lddy = lddy; a.ldd = up8(n); a.lddz = lddz; a.N = n;
-  a.run = row_run(dy, rows > 1 ? lddy : n, n, 2);
   hipStream_t s = (hipStream_t)stream;
   const int L = dz_lanes(n), groups = dz_groups(rows, n);
   if (groups) {
     const dim3 grid((n + L * 8 - 1) / (L * 8), groups), blk(256);
-#define DZ(L_)                                                                       \
-  if (dtype == 1) hipLaunchKernelGGL((dz_kernel<b16, L_>), grid, blk, 0, s, a);      \
-  else hipLaunchKernelGGL((dz_kernel<h16, L_>), grid, blk, 0, s, a)
+#define DZ(L_)                                                                                         \
+  if (dtype == 1 && n % 8 == 0) hipLaunchKernelGGL((dz_kernel<b16, L_, true>), grid, blk, 0, s, a);    \
+  else if (dtype == 1) hipLaunchKernelGGL((dz_kernel<b16, L_, false>), grid, blk, 0, s, a);            \
+  else if (n % 8 == 0) hipLaunchKernelGGL((dz_kernel<h16, L_, true>), grid, blk, 0, s, a);             \
+  else hipLaunchKernelGGL((dz_kernel<h16, L_, false>), grid, blk, 0, s, a)
     if (L == 8) { DZ(8); }
     else if (L == 16) { DZ(16); }
     else if (L == 32) { DZ(32); }
@@ -951,7 +924,7 @@ int selfc_linear_dx(const void* dz, size_t lddz, const void* w, size_t ldw, void
   if (!rows_fit(dz, lddz, up8(n), 2) || lddz < up8(n) || !rows_fit(w, ldw, up8(k), 2) || ldw < up8(k)) return SELFC_EINVAL;
   GemmArgs a{};
   a.q = dz; a.p = w; a.ldq = lddz; a.ldp = ldw; a.M = (int)rows; a.N = k; a.R = n; a.px = (int)up8(k); a.ws = ws;
-  a.e = make_epilogue(dx, k, nullptr, nullptr, 0, dtype, ACT_NONE, k);
+  a.e = make_epilogue(dx, k, nullptr, nullptr, 0, dtype, ACT_NONE);
   return dtype == 1 ? gemm_run<b16, false, true>(a, (hipStream_t)stream) : gemm_run<h16, false, true>(a, (hipStream_t)stream);
 }
 
@@ -966,7 +939,7 @@ int selfc_linear_dw(const void* dz, size_t lddz, const void* x, size_t ldx, void
   if (!rows_fit(dz, lddz, up8(n), 2) || lddz < up8(n) || !rows_fit(x, ldx, up8(k), 2) || ldx < up8(k)) return SELFC_EINVAL;
   GemmArgs a{};
   a.q = dz; a.p = x; a.ldq = lddz; a.ldp = ldx; a.M = n; a.N = k; a.R = (int)rows; a.qx = (int)up8(n); a.px = (int)up8(k); a.ws = ws; a.sums = db;
-  a.e = make_epilogue(dw, k, nullptr, nullptr, 0, dtype, ACT_NONE, k);
+  a.e = make_epilogue(dw, k, nullptr, nullptr, 0, dtype, ACT_NONE);
   return dtype == 1 ? gemm_run<b16, true, true>(a, (hipStream_t)stream) : gemm_run<h16, true, true>(a, (hipStream_t)stream);
 }
 
@@ -980,10 +953,7 @@ int selfc_linear_rows(const void* x, size_t ldx, const void* w, size_t ldw, cons
   if (!aligned_to(y, 16) || (slope && !aligned_to(slope, 16)) || (xp && !aligned_to(xp, 16))) return SELFC_EINVAL;
   RowsArgs a{};
   a.x = x; a.w = w; a.xp = xp; a.ldx = ldx; a.ldw = ldw; a.rows = rows; a.N = n; a.K = k;
-  a.xrun = row_run(x, rows > 1 ? ldx : k, k, 2);
-  a.wrun = row_run(w, n > 1 ? ldw : k, k, 2);
   a.e.out = y; a.e.bias = bias; a.e.res = res; a.e.ldr = ldr; a.e.act = act; a.e.d = (unsigned short*)slope; a.e.ldd = up8(n);
-  a.e.run = res ? row_run(res, rows > 1 ? ldr : n, n, 2) : 8;
   return dtype == 1 ? rows_run<b16, false>(a, (hipStream_t)stream) : rows_run<h16, false>(a, (hipStream_t)stream);
 }
 
@@ -995,8 +965,6 @@ int selfc_linear_rows_bwd(const void* dy, size_t lddy, const void* slope, const 
   RowsArgs a{};
   a.x = dy; a.w = w; a.d = (const unsigned short*)slope; a.xp = dz;
   a.ldx = lddy; a.ldw = ldw; a.ldd = up8(n); a.rows = rows; a.N = k; a.K = n;
-  a.xrun = row_run(dy, rows > 1 ? lddy : n, n, 2);
-  a.wrun = row_run(w, n > 1 ? ldw : k, k, 2);
   a.e.out = dx;
   hipStream_t s = (hipStream_t)stream;
   return dtype == 1 ? rows_run<b16, true>(a, s) : rows_run<h16, true>(a, s);

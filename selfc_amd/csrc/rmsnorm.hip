@@ -18,16 +18,19 @@ namespace {
 
 constexpr int RN_MAX = 16384;
 constexpr float E4M3_MAX = 448.f;
+#define LEFT(c) (WHOLE ? ((c) < C ? 8 : 0) : C - (c))
 
-// sum / max over a row's lanes.  L <= 64: a butterfly; L = 256: the workgroup, through four LDS words (two sets, used in turn, so
-// that one barrier per reduction is enough)
+// sum / max over a row's lanes.  L <= 64: a butterfly; more: the workgroup, through one LDS word per wave (callers use two sets in
+// turn, so that one barrier per reduction is enough)
 template <int L, bool MAX>
 __device__ __forceinline__ float row_reduce(float v, float* const red) {
   v = MAX ? lanes_max<(L < 64 ? L : 64)>(v) : lanes_sum<(L < 64 ? L : 64)>(v);
-  if constexpr (L == 256) {
+  if constexpr (L > 64) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = MAX ? fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])) : (red[0] + red[1]) + (red[2] + red[3]);
+    v = red[0];
+#pragma unroll
+    for (int i = 1; i < L / 64; ++i) v = MAX ? fmaxf(v, red[i]) : v + red[i];
   }
   return v;
 }
@@ -37,12 +40,12 @@ struct RnArgs {
   void *h, *y;
   float* scale;
   size_t rows, ldx, ldr;
-  int C, w_f32, run;          // run: values per load and store (8, 4, 2 or 1)
+  int C, w_f32;
   float eps;
 };
 
-// L lanes per row, NV vectors of 8 values per lane
-template <typename T, int L, int NV, bool Q8, bool RUN8>
+// L lanes per row, NV vectors of 8 values per lane.  WHOLE: C is a multiple of 8, so that no vector is cut by the row's end
+template <typename T, int L, int NV, bool Q8, bool WHOLE>
 __global__ __launch_bounds__(256) void rmsnorm_kernel(const RnArgs a) {
   __shared__ float red[8];
   const int lane = threadIdx.x & (L - 1);
@@ -51,26 +54,25 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const RnArgs a) {
   const T* const x = (const T*)a.x + row * a.ldx;
   const T* const r = a.r ? (const T*)a.r + row * a.ldr : nullptr;
   const int C = a.C;
-  const int run = RUN8 ? 8 : a.run;           // whole 16-byte pieces: no other loads are compiled in
   float h[NV][8];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
     const int c = (j * L + lane) * 8;
-    load8(x + c, C - c, run, h[j]);
+    load8(x + c, LEFT(c), c, h[j]);
   }
   if (r) {
     float t[NV][8];
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * L + lane) * 8;
-      load8(r + c, C - c, run, t[j]);
+      load8(r + c, LEFT(c), c, t[j]);
     }
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * L + lane) * 8;
 #pragma unroll
       for (int i = 0; i < 8; ++i) h[j][i] = (float)(T)(h[j][i] + t[j][i]);
-      if (c < C) store8((T*)a.h + row * C + c, C - c, run, h[j]);
+      if (c < C) store8((T*)a.h + row * C + c, LEFT(c), h[j]);
     }
   }
   float ss = 0.f;
@@ -85,15 +87,15 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const RnArgs a) {
   for (int j = 0; j < NV; ++j) {
     const int c = (j * L + lane) * 8;
     float w[8];
-    if (a.w_f32) load8((const float*)a.w + c, C - c, run, w);
-    else load8((const T*)a.w + c, C - c, run, w);
+    if (a.w_f32) load8((const float*)a.w + c, LEFT(c), c, w);
+    else load8((const T*)a.w + c, LEFT(c), c, w);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       h[j][i] = h[j][i] * rstd * w[i];
       if constexpr (Q8) most = fmaxf(most, fabsf(h[j][i]));
     }
     if constexpr (!Q8) {
-      if (c < C) store8((T*)a.y + row * C + c, C - c, run, h[j]);
+      if (c < C) store8((T*)a.y + row * C + c, LEFT(c), h[j]);
     }
   }
   if constexpr (Q8) {
@@ -111,8 +113,9 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const RnArgs a) {
         int hi = __builtin_amdgcn_cvt_pk_fp8_f32(h[j][4] * inv, h[j][5] * inv, 0, false);
         hi = __builtin_amdgcn_cvt_pk_fp8_f32(h[j][6] * inv, h[j][7] * inv, hi, true);
         unsigned char* const q = (unsigned char*)a.y + row * C + c;
-        if (run == 8) {
-          *reinterpret_cast<u32x2*>(q) = u32x2{(unsigned)lo, (unsigned)hi};
+        const int two[2] = {lo, hi};
+        if (c + 8 <= C) {
+          __builtin_memcpy(q, two, 8);
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
@@ -128,59 +131,75 @@ struct RnBwdArgs {
   void* dx;
   float* partial;             // [gridDim.x][C]
   size_t rows, ldh;
-  int C, w_f32, run, want_dx;
+  int C, w_f32, want_dx;
   float eps;
 };
 
-template <typename T, int L, int NV, bool RUN8>
-__global__ __launch_bounds__(256) void rmsnorm_bwd_kernel(const RnBwdArgs a) {
-  __shared__ float red[2][8];
-  constexpr int G = 256 / L;                 // rows at a time
+// The next row's values are on their way while a row is worked on: they stay as they are stored until their turn (the widest rows'
+// workgroups have no registers left for that).
+template <typename T, int L, int NV, bool WHOLE>
+__global__ __launch_bounds__(L > 256 ? L : 256) void rmsnorm_bwd_kernel(const RnBwdArgs a) {
+  constexpr int NT = L > 256 ? L : 256, G = NT / L;                // rows at a time
+  constexpr bool AHEAD = L < 1024;
+  __shared__ float red[2][2][L > 64 ? L / 64 : 1];
   const int lane = threadIdx.x & (L - 1), grp = threadIdx.x / L;
   const int C = a.C;
-  const int run = RUN8 ? 8 : a.run;           // whole 16-byte pieces: no other loads are compiled in
+  const size_t step = (size_t)gridDim.x * G;
   float dw[NV][8] = {};
-  int turn = 0;
-  for (size_t row = (size_t)blockIdx.x * G + grp; row < a.rows; row += (size_t)gridDim.x * G, turn ^= 1) {
-    float h[NV][8], dy[NV][8];
+  Raw8<T> nh[NV], ny[NV], nd[NV];
+  const auto fetch = [&](const size_t row) {
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * L + lane) * 8;
-      load8((const T*)a.h + row * a.ldh + c, C - c, run, h[j]);
-      load8((const T*)a.dy + row * C + c, C - c, run, dy[j]);
+      nh[j].load((const T*)a.h + row * a.ldh + c, LEFT(c), c);
+      ny[j].load((const T*)a.dy + row * C + c, LEFT(c), c);
+      if (a.dh) nd[j].load((const T*)a.dh + row * C + c, LEFT(c), c);
     }
+  };
+  size_t row = (size_t)blockIdx.x * G + grp;
+  if (AHEAD && row < a.rows) fetch(row);
+  for (int turn = 0; row < a.rows; row += step, turn ^= 1) {
+    if (!AHEAD) fetch(row);
+    Raw8<T> rh[NV], ry[NV], rd[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) { rh[j] = nh[j]; ry[j] = ny[j]; rd[j] = nd[j]; }
+    if (AHEAD && row + step < a.rows) fetch(row + step);
     float ss = 0.f, dot = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * L + lane) * 8;
-      float w[8];
-      if (a.w_f32) load8((const float*)a.w + c, C - c, run, w);
-      else load8((const T*)a.w + c, C - c, run, w);
+      float h[8], dy[8], w[8];
+      rh[j].expand(h);
+      ry[j].expand(dy);
+      if (a.w_f32) load8((const float*)a.w + c, LEFT(c), c, w);
+      else load8((const T*)a.w + c, LEFT(c), c, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        ss += h[j][i] * h[j][i];
-        dot += dy[j][i] * w[i] * h[j][i];
+        ss += h[i] * h[i];
+        dot += dy[i] * w[i] * h[i];
       }
     }
-    ss = row_reduce<L, false>(ss, red[turn]);
-    dot = row_reduce<L, false>(dot, red[turn] + 4);
+    ss = row_reduce<L, false>(ss, red[turn][0]);
+    dot = row_reduce<L, false>(dot, red[turn][1]);
     const float rstd = 1.f / sqrtf(ss / (float)C + a.eps);
     const float c2 = dot * rstd / (float)C;                      // mean(dy w n)
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       const int c = (j * L + lane) * 8;
-      float w[8], add[8], out[8];
-      if (a.w_f32) load8((const float*)a.w + c, C - c, run, w);
-      else load8((const T*)a.w + c, C - c, run, w);
-      if (a.dh) load8((const T*)a.dh + row * C + c, C - c, run, add);
+      float h[8], dy[8], w[8], add[8], out[8];
+      rh[j].expand(h);
+      ry[j].expand(dy);
+      if (a.dh) rd[j].expand(add);
+      if (a.w_f32) load8((const float*)a.w + c, LEFT(c), c, w);
+      else load8((const T*)a.w + c, LEFT(c), c, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float n = h[j][i] * rstd;
-        dw[j][i] += dy[j][i] * n;
-        out[i] = rstd * (dy[j][i] * w[i] - n * c2);
+        const float n = h[i] * rstd;
+        dw[j][i] += dy[i] * n;
+        out[i] = rstd * (dy[i] * w[i] - n * c2);
         if (a.dh) out[i] += add[i];
       }
-      if (a.want_dx && c < C) store8((T*)a.dx + row * C + c, C - c, run, out);
+      if (a.want_dx && c < C) store8((T*)a.dx + row * C + c, LEFT(c), out);
     }
   }
   if (!a.partial) return;
@@ -220,7 +239,13 @@ __global__ __launch_bounds__(1024) void colsum_kernel(const float* const partial
   const int col = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
   float acc = 0.f;
   if (col < C)
-    for (int g = slice; g < rows; g += 64) acc += partial[(size_t)g * C + col];
+    for (int g = slice; g < rows; g += 512) {          // eight loads in flight
+      float v[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] = g + k * 64 < rows ? partial[(size_t)(g + k * 64) * C + col] : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) acc += v[k];
+    }
   __shared__ float red[64][17];
   red[slice][threadIdx.x & 15] = acc;
   __syncthreads();
@@ -231,11 +256,11 @@ __global__ __launch_bounds__(1024) void colsum_kernel(const float* const partial
   if (slice == 0 && col < C) out[col] = (T)red[0][threadIdx.x & 15];
 }
 
-// workgroups of the backward pass: enough to fill the chip several times, few enough that the partial sums stay small beside the rows
+// workgroups of the backward pass: two to four per compute unit; a workgroup's partial sums are C values to write and read again
 inline int rn_bwd_groups(const size_t rows, const int C) {
-  const int L = C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 2048 ? 64 : 256;
-  const size_t need = (rows + 256 / L - 1) / (256 / L);
-  return (int)(need < 1024 ? need : 1024);
+  const int at_a_time = C <= 64 ? 32 : C <= 128 ? 16 : C <= 256 ? 8 : C <= 1024 ? 4 : 1;
+  const size_t need = (rows + at_a_time - 1) / at_a_time, most = C <= 2048 ? 1024 : 512;
+  return (int)(need < most ? need : most);
 }
 
 }  // namespace
@@ -260,7 +285,7 @@ void rn_launch(const RnArgs& a, hipStream_t s) {
 #define RN(L, NV)                                                                                                            \
   do {                                                                                                                        \
     const dim3 grid((unsigned)((a.rows + 256 / L - 1) / (256 / L)));                                                          \
-    if (a.run == 8) hipLaunchKernelGGL((rmsnorm_kernel<T, L, NV, Q8, true>), grid, dim3(256), 0, s, a);                       \
+    if (C % 8 == 0) hipLaunchKernelGGL((rmsnorm_kernel<T, L, NV, Q8, true>), grid, dim3(256), 0, s, a);                       \
     else hipLaunchKernelGGL((rmsnorm_kernel<T, L, NV, Q8, false>), grid, dim3(256), 0, s, a);                                 \
   } while (0)
   const int C = a.C;
@@ -279,8 +304,9 @@ template <typename T>
 void rn_bwd_launch(const RnBwdArgs& a, const int groups, hipStream_t s) {
 #define RN(L, NV)                                                                                                            \
   do {                                                                                                                        \
-    if (a.run == 8) hipLaunchKernelGGL((rmsnorm_bwd_kernel<T, L, NV, true>), dim3((unsigned)groups), dim3(256), 0, s, a);     \
-    else hipLaunchKernelGGL((rmsnorm_bwd_kernel<T, L, NV, false>), dim3((unsigned)groups), dim3(256), 0, s, a);               \
+    const dim3 grid((unsigned)groups), blk(L > 256 ? L : 256);                                                                \
+    if (C % 8 == 0) hipLaunchKernelGGL((rmsnorm_bwd_kernel<T, L, NV, true>), grid, blk, 0, s, a);                             \
+    else hipLaunchKernelGGL((rmsnorm_bwd_kernel<T, L, NV, false>), grid, blk, 0, s, a);                                       \
   } while (0)
   const int C = a.C;
   if (C <= 64) RN(8, 1);
@@ -288,10 +314,10 @@ void rn_bwd_launch(const RnBwdArgs& a, const int groups, hipStream_t s) {
   else if (C <= 256) RN(32, 1);
   else if (C <= 512) RN(64, 1);
   else if (C <= 1024) RN(64, 2);
-  else if (C <= 2048) RN(64, 4);
+  else if (C <= 2048) RN(256, 1);
   else if (C <= 4096) RN(256, 2);
-  else if (C <= 8192) RN(256, 4);
-  else RN(256, 8);
+  else if (C <= 8192) RN(512, 2);
+  else RN(1024, 2);
 #undef RN
 }
 
@@ -308,12 +334,8 @@ int selfc_rmsnorm(const void* x, size_t ldx, const void* r, size_t ldr, const vo
   if (!rn_shape(rows, C, dtype) || !x || !w || !y || (r != nullptr) != (h != nullptr) || !(eps >= 0.f)) return SELFC_EINVAL;
   if (rows > 1 && (ldx < (size_t)C || (r && ldr < (size_t)C))) return SELFC_EINVAL;
   if (rows == 0) return SELFC_OK;
-  const size_t es = dtype ? 2 : 4;
   RnArgs a{};
   a.x = x; a.r = r; a.w = w; a.h = h; a.y = y; a.scale = q8_scale; a.rows = rows; a.ldx = ldx; a.ldr = ldr; a.C = C; a.w_f32 = w_f32; a.eps = eps;
-  const auto least = [](const int p, const int q) { return p < q ? p : q; };
-  a.run = least(row_run(x, rows > 1 ? ldx : C, C, es), least(row_run(w, C, C, w_f32 ? 4 : es), row_run(y, C, C, q8_scale ? 1 : es)));
-  if (r) a.run = least(a.run, least(row_run(r, rows > 1 ? ldr : C, C, es), row_run(h, C, C, es)));
   hipStream_t s = (hipStream_t)stream;
   if (q8_scale) {
     if (dtype == 0) rn_launch<float, true>(a, s);
@@ -333,14 +355,9 @@ int selfc_rmsnorm_bwd(const void* h, size_t ldh, const void* w, int w_f32, const
                       float* partial, size_t rows, int C, int dtype, float eps, void* stream) {
   if (!rn_shape(rows, C, dtype) || !h || !w || !dy || (!dx && !dw) || (dw && !partial) || !(eps >= 0.f)) return SELFC_EINVAL;
   if (rows > 1 && ldh < (size_t)C) return SELFC_EINVAL;
-  const size_t es = dtype ? 2 : 4;
   RnBwdArgs a{};
   a.h = h; a.w = w; a.dy = dy; a.dh = dh; a.dx = dx; a.partial = dw ? partial : nullptr; a.rows = rows; a.ldh = ldh; a.C = C; a.w_f32 = w_f32;
   a.want_dx = dx != nullptr; a.eps = eps;
-  const auto least = [](const int p, const int q) { return p < q ? p : q; };
-  a.run = least(row_run(h, rows > 1 ? ldh : C, C, es), least(row_run(w, C, C, w_f32 ? 4 : es), row_run(dy, C, C, es)));
-  if (dh) a.run = least(a.run, row_run(dh, C, C, es));
-  if (dx) a.run = least(a.run, row_run(dx, C, C, es));
   hipStream_t s = (hipStream_t)stream;
   const int groups = rn_bwd_groups(rows, C);
   if (groups) {
