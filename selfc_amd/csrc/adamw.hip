@@ -18,8 +18,9 @@
 // 30 % standard deviation of v, 15 % of the step's size, against 160 % if every step re-rounded every value).  A nonzero v never
 // rounds to zero: m / sqrt(v) stays bounded.  Values that are not finite are held as NaN and do not enter their block's scale.
 //
-// Bound: memory (28 bytes a value in 32 bits; 16 in 8 bits with fp32 tensors, 10 with 16-bit ones) - about 60 vector
-// instructions a value for the 8-bit form, which is near the rate at which the memory delivers.
+// Bound: memory (28 bytes a value in 32 bits; 16 in 8 bits with fp32 tensors, 10 with 16-bit ones), as long as the 8-bit form stays below
+// about 100 vector instructions a value: its first form, with every value's end-of-tensor check and general rounding, took 106 and
+// was bound by them.
 #include "pointwise.hpp"
 #include <math.h>
 
@@ -64,13 +65,10 @@ __device__ __forceinline__ int aw_find(const AwTable& t, const unsigned wg) {
   return __builtin_amdgcn_readfirstlane(__popcll(__ballot(a)) + __popcll(__ballot(b)) - 1);
 }
 
-// the block's scale 2^(floor(log2 most) - top), not below 2^-126; 1 for an empty block.  `inv` = 1 / scale, exact.
-__device__ __forceinline__ float aw_scale(const float most, const int top, float& inv) {
-  int e = (int)(__builtin_bit_cast(unsigned, most) >> 23) - top;           // biased exponent of the scale
-  e = e < 1 ? 1 : e;
-  if (most == 0.f) e = 127;
-  inv = __builtin_bit_cast(float, (unsigned)(254 - e) << 23);
-  return __builtin_bit_cast(float, (unsigned)e << 23);
+// biased exponent of a block's scale 2^(floor(log2 most) - top), not below 2^-126; of 1 for an empty block
+__device__ __forceinline__ int aw_exponent(const unsigned most, const int top) {
+  const int e = (int)(most >> 23) - top;
+  return most == 0 ? 127 : e < 1 ? 1 : e;
 }
 
 // |y| rounded down after adding u steps of the 8-bit format's grid (least: exponent of its smallest normal number, digits: of its
@@ -88,136 +86,188 @@ __device__ __forceinline__ float aw_round(const float y, const float u) {
   return ay < 0x7f800000u ? r : __builtin_nanf("");
 }
 
-template <typename T, int BITS>
-__global__ __launch_bounds__(256) void adamw_kernel(const AwTable tab, const AwHyper hy, void* const m_, void* const v_,
-                                                    float* const ms, float* const vs) {
-#pragma clang fp contract(off)
-  const unsigned wg = blockIdx.x;
-  const int ti = aw_find(tab, wg);
-  const AwEntry& en = tab.e[ti];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  T* const p = (T*)en.p;
-  const T* const g = (const T*)en.g;
-  const unsigned long long n = en.n;
-  const unsigned long long base = (unsigned long long)(wg - en.wg0) * AW_CHUNK + (unsigned)wave * (AW_U * AW_BLOCK);
-  if (base >= n) return;
-  const size_t blk0 = (size_t)en.block0 + (size_t)(base / AW_BLOCK);       // first of this wave's blocks in the state
-  const size_t s0 = blk0 * AW_BLOCK;
-
-  constexpr bool NARROW = sizeof(T) == 2;
-  const bool vec = (((size_t)p | (size_t)g) & (NARROW ? 7 : 15)) == 0;
-  typedef T T4 __attribute__((ext_vector_type(4)));
-  float pv[AW_U][4], gv[AW_U][4], mv[AW_U][4], vv[AW_U][4];
-  unsigned m8[AW_U], v8[AW_U];
+// Four moments -> 8 bits with the block's scale.  x[i]: the dither's 16 bits.  For normal numbers of the 8-bit format, adding u steps and
+// rounding down is an integer addition below the kept digits and a mask; a block that holds smaller ones (or some that are not finite)
+// takes the general form.
+template <int TOP, int LEAST, int DIGITS, bool FLOOR>
+__device__ __forceinline__ float aw_hold(const float* const m, const unsigned* const x, float* const q) {
+  unsigned a[4], most = 0, least = 0xffffffffu;
 #pragma unroll
-  for (int u = 0; u < AW_U; ++u) {
-    const unsigned long long at = base + u * AW_BLOCK + lane * 4;
-    if (base + u * AW_BLOCK < n) {
-      if (vec && at + 4 <= n) {
-        const T4 a = *reinterpret_cast<const T4*>(p + at), b = *reinterpret_cast<const T4*>(g + at);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { pv[u][i] = (float)a[i]; gv[u][i] = (float)b[i]; }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          pv[u][i] = at + i < n ? (float)p[at + i] : 0.f;
-          gv[u][i] = at + i < n ? (float)g[at + i] : 0.f;
-        }
-      }
-      const size_t st = s0 + u * AW_BLOCK + lane * 4;
-      if constexpr (BITS == 32) {
-        const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)m_ + st), b = *reinterpret_cast<const f32x4*>((const float*)v_ + st);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { mv[u][i] = a[i]; vv[u][i] = b[i]; }
-      } else {
-        m8[u] = *reinterpret_cast<const unsigned*>((const unsigned char*)m_ + st);
-        v8[u] = *reinterpret_cast<const unsigned*>((const unsigned char*)v_ + st);
-        const float sm = ms[blk0 + u], sv = vs[blk0 + u];
-        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(m8[u], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(m8[u], true);
-        const f32x2 c = __builtin_amdgcn_cvt_pk_f32_bf8(v8[u], false), d = __builtin_amdgcn_cvt_pk_f32_bf8(v8[u], true);
-        mv[u][0] = a[0] * sm; mv[u][1] = a[1] * sm; mv[u][2] = b[0] * sm; mv[u][3] = b[1] * sm;
-        vv[u][0] = c[0] * sv; vv[u][1] = c[1] * sv; vv[u][2] = d[0] * sv; vv[u][3] = d[1] * sv;
-      }
-    }
+  for (int i = 0; i < 4; ++i) {
+    a[i] = __builtin_bit_cast(unsigned, m[i]) & 0x7fffffffu;
+    most = a[i] > most ? a[i] : most;
+    least = a[i] - 1 < least ? a[i] - 1 : least;             // the smallest that is not 0, less one
   }
-
-  // what the step's number and the rate make of the formulas: from the host, or (captured steps) from device memory
-  float bc1 = hy.bc1, bc2s = hy.bc2s;
-  unsigned key = hy.key;
-  if (en.step) {
-    const unsigned long long t = (unsigned long long)*en.step;
-    bc1 = (float)(1.0 - aw_pow(hy.beta1_d, t));
-    bc2s = (float)sqrt(1.0 - aw_pow(hy.beta2_d, t));
-    key = aw_mix(hy.seed ^ aw_mix((unsigned)t));
-  }
-  const float lr = hy.lr_dev ? *hy.lr_dev : hy.lr;
-  const float keep = 1.f - lr * hy.wd, rate = lr / bc1, ibc2 = 1.f / bc2s;
-  float coef = 1.f;
-  if (hy.norm) coef = fminf(hy.max_norm / (*hy.norm + 1e-6f), 1.f);
-  const bool clip = hy.norm != nullptr;
-  const unsigned tkey = aw_mix(key ^ aw_mix((unsigned)(tab.place0 + ti)));
-
-#pragma unroll
-  for (int u = 0; u < AW_U; ++u) {
-    if (base + u * AW_BLOCK >= n) break;
-    const unsigned long long at = base + u * AW_BLOCK + lane * 4;
-    float mmost = 0.f, vmost = 0.f;
+  most = lanes_max<64>(most);
+  int e = aw_exponent(most, TOP);
+  const int floor_e = e + LEAST;                             // exponent of the smallest moment that is a normal number of the format
+  bool plain = most < 0x7f800000u && floor_e >= 1;
+  if (plain) plain = __all(least >= ((unsigned)floor_e << 23) - 1);
+  if (plain) {
+    const float inv = __builtin_bit_cast(float, (unsigned)(254 - e) << 23);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float gi = gv[u][i];
-      if (clip) gi = gi * coef;
-      const float mi = hy.b1 * mv[u][i] + hy.omb1 * gi;
-      const float vi = hy.b2 * vv[u][i] + hy.omb2 * (gi * gi);
-      mv[u][i] = mi;
-      vv[u][i] = vi;
-      // one-ulp square root and reciprocal: the step is a small part of p, its last bits are below p's
-      const float den = __builtin_amdgcn_sqrtf(vi) * ibc2 + hy.eps;
-      pv[u][i] = pv[u][i] * keep - rate * (mi * __builtin_amdgcn_rcpf(den));
-      if constexpr (BITS == 8) {
-        const float am = fabsf(mi);            // v is not negative; values behind the tensor's end are 0
-        mmost = fmaxf(mmost, am < INFINITY ? am : 0.f);
-        vmost = fmaxf(vmost, vi < INFINITY ? vi : 0.f);
+      const float y = m[i] * inv;
+      q[i] = __builtin_bit_cast(float, (__builtin_bit_cast(unsigned, y) + (x[i] << (23 - DIGITS - 16))) & (0xffffffffu << (23 - DIGITS)));
+    }
+  } else {
+    most = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = a[i] < 0x7f800000u && a[i] > most ? a[i] : most;
+    e = aw_exponent(lanes_max<64>(most), TOP);
+    const float inv = __builtin_bit_cast(float, (unsigned)(254 - e) << 23);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = aw_round<LEAST, DIGITS, FLOOR>(m[i] * inv, (float)x[i] * 0x1p-16f);
+  }
+  return __builtin_bit_cast(float, (unsigned)e << 23);
+}
+
+// what a step's number, rate and norm make of the formulas
+struct AwStep { float keep, rate, ibc2, coef; unsigned key; };
+
+// 256 values of a tensor, four consecutive ones per lane.  FULL: all of them exist and p and g are aligned.
+template <typename T, int BITS, bool FULL>
+struct AwPart {
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  float p[4], g[4], m[4], v[4];
+  // pt, gt: the tensor's first value of this part; left: how many it has; st: the part's first value in the state, bk: its block
+  __device__ __forceinline__ void load(const T* const pt, const T* const gt, const unsigned long long left, const void* const ms, const void* const vs,
+                                       const float* const sm, const float* const sv, const int lane) {
+    const int at = lane * 4;
+    if (FULL) {
+      const T4 a = *reinterpret_cast<const T4*>(pt + at), b = *reinterpret_cast<const T4*>(gt + at);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { p[i] = (float)a[i]; g[i] = (float)b[i]; }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[i] = (unsigned)(at + i) < left ? (float)pt[at + i] : 0.f;
+        g[i] = (unsigned)(at + i) < left ? (float)gt[at + i] : 0.f;
       }
     }
-    if (vec && at + 4 <= n) {
-      T4 a;
+    if constexpr (BITS == 32) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>((const float*)ms + at), b = *reinterpret_cast<const f32x4*>((const float*)vs + at);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = (T)pv[u][i];
-      *reinterpret_cast<T4*>(p + at) = a;
+      for (int i = 0; i < 4; ++i) { m[i] = a[i]; v[i] = b[i]; }
+    } else {
+      const unsigned m8 = *reinterpret_cast<const unsigned*>((const unsigned char*)ms + at), v8 = *reinterpret_cast<const unsigned*>((const unsigned char*)vs + at);
+      const float ss = *sm, qs = *sv;
+      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(m8, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(m8, true);
+      const f32x2 c = __builtin_amdgcn_cvt_pk_f32_bf8(v8, false), d = __builtin_amdgcn_cvt_pk_f32_bf8(v8, true);
+      m[0] = a[0] * ss; m[1] = a[1] * ss; m[2] = b[0] * ss; m[3] = b[1] * ss;
+      v[0] = c[0] * qs; v[1] = c[1] * qs; v[2] = d[0] * qs; v[3] = d[1] * qs;
+    }
+  }
+  __device__ __forceinline__ void step(T* const pt, const unsigned long long left, const unsigned place, void* const ms, void* const vs,
+                                       float* const sm, float* const sv, const int lane, const AwStep& s, const AwHyper& hy) {
+#pragma clang fp contract(off)
+    const int at = lane * 4;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float gi = g[i];
+      if (hy.norm) gi = gi * s.coef;
+      m[i] = hy.b1 * m[i] + hy.omb1 * gi;
+      v[i] = hy.b2 * v[i] + hy.omb2 * (gi * gi);
+      // one-ulp square root and reciprocal: the step is a small part of p, its last bits are below p's
+      const float den = fmaf(__builtin_amdgcn_sqrtf(v[i]), s.ibc2, hy.eps);
+      p[i] = fmaf(-s.rate, m[i] * __builtin_amdgcn_rcpf(den), p[i] * s.keep);
+    }
+    if (FULL) {
+      *reinterpret_cast<T4*>(pt + at) = T4{(T)p[0], (T)p[1], (T)p[2], (T)p[3]};
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (at + i < n) p[at + i] = (T)pv[u][i];
+        if ((unsigned)(at + i) < left) pt[at + i] = (T)p[i];
     }
-    const size_t st = s0 + u * AW_BLOCK + lane * 4;
     if constexpr (BITS == 32) {
-      float* const mp = (float*)m_ + st;
-      float* const vp = (float*)v_ + st;
-      if (at + 4 <= n) {
-        *reinterpret_cast<f32x4*>(mp) = f32x4{mv[u][0], mv[u][1], mv[u][2], mv[u][3]};
-        *reinterpret_cast<f32x4*>(vp) = f32x4{vv[u][0], vv[u][1], vv[u][2], vv[u][3]};
+      if (FULL) {
+        *reinterpret_cast<f32x4*>((float*)ms + at) = f32x4{m[0], m[1], m[2], m[3]};
+        *reinterpret_cast<f32x4*>((float*)vs + at) = f32x4{v[0], v[1], v[2], v[3]};
       } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (at + i < n) { mp[i] = mv[u][i]; vp[i] = vv[u][i]; }
+          if ((unsigned)(at + i) < left) { ((float*)ms)[at + i] = m[i]; ((float*)vs)[at + i] = v[i]; }
       }
     } else {
-      float im, iv;
-      const float sm = aw_scale(lanes_max<64>(mmost), 7, im), sv = aw_scale(lanes_max<64>(vmost), 14, iv);
-      float mq[4], vq[4];
+      if (!FULL)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if ((unsigned)(at + i) >= left) m[i] = v[i] = 0.f;               // behind the tensor's end: as they were
+      unsigned um[4], uv[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const unsigned x = aw_mix((unsigned)(at + i) ^ tkey);
-        mq[i] = at + i < n ? aw_round<-6, 3, false>(mv[u][i] * im, (float)(x & 0xffffu) * 0x1p-16f) : 0.f;
-        vq[i] = at + i < n ? aw_round<-14, 2, true>(vv[u][i] * iv, (float)(x >> 16) * 0x1p-16f) : 0.f;
+        const unsigned x = aw_mix((place + at + i) ^ s.key);
+        um[i] = x & 0xffffu;
+        uv[i] = x >> 16;
       }
+      float mq[4], vq[4];
+      const float ss = aw_hold<7, -6, 3, false>(m, um, mq), qs = aw_hold<14, -14, 2, true>(v, uv, vq);
       int a = __builtin_amdgcn_cvt_pk_fp8_f32(mq[0], mq[1], 0, false);
       a = __builtin_amdgcn_cvt_pk_fp8_f32(mq[2], mq[3], a, true);
       int b = __builtin_amdgcn_cvt_pk_bf8_f32(vq[0], vq[1], 0, false);
       b = __builtin_amdgcn_cvt_pk_bf8_f32(vq[2], vq[3], b, true);
-      *reinterpret_cast<int*>((unsigned char*)m_ + st) = a;
-      *reinterpret_cast<int*>((unsigned char*)v_ + st) = b;
-      if (lane == 0) { ms[blk0 + u] = sm; vs[blk0 + u] = sv; }
+      *reinterpret_cast<int*>((unsigned char*)ms + at) = a;
+      *reinterpret_cast<int*>((unsigned char*)vs + at) = b;
+      if (lane == 0) { *sm = ss; *sv = qs; }
+    }
+  }
+};
+
+template <typename T, int BITS>
+__global__ __launch_bounds__(256) void adamw_kernel(const AwTable tab, const AwHyper hy, void* const m_, void* const v_,
+                                                    float* const ms, float* const vs) {
+  const unsigned wg = blockIdx.x;
+  const int ti = aw_find(tab, wg);
+  const AwEntry& en = tab.e[ti];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned long long n = en.n;
+  const unsigned long long base = (unsigned long long)(wg - en.wg0) * AW_CHUNK + (unsigned)wave * (AW_U * AW_BLOCK);
+  if (base >= n) return;
+  T* const p = (T*)en.p + base;
+  const T* const g = (const T*)en.g + base;
+  const size_t blk0 = (size_t)en.block0 + (size_t)(base / AW_BLOCK);       // first of this wave's blocks in the state
+  constexpr int SB = BITS / 8;
+  unsigned char* const m = (unsigned char*)m_ + blk0 * AW_BLOCK * SB;
+  unsigned char* const v = (unsigned char*)v_ + blk0 * AW_BLOCK * SB;
+  float* const sm = ms + blk0;
+  float* const sv = vs + blk0;
+  const unsigned long long left = n - base;
+  const bool full = left >= AW_U * AW_BLOCK && (((size_t)p | (size_t)g) & (4 * sizeof(T) - 1)) == 0;
+
+  AwPart<T, BITS, true> part[AW_U];
+  if (full) {
+#pragma unroll
+    for (int u = 0; u < AW_U; ++u)
+      part[u].load(p + u * AW_BLOCK, g + u * AW_BLOCK, AW_BLOCK, m + u * AW_BLOCK * SB, v + u * AW_BLOCK * SB, sm + u, sv + u, lane);
+  }
+  // from the host, or (captured steps) from device memory
+  float bc1 = hy.bc1, bc2s = hy.bc2s;
+  AwStep s;
+  s.key = hy.key;
+  if (en.step) {
+    const unsigned long long t = (unsigned long long)*en.step;
+    bc1 = (float)(1.0 - aw_pow(hy.beta1_d, t));
+    bc2s = (float)sqrt(1.0 - aw_pow(hy.beta2_d, t));
+    s.key = aw_mix(hy.seed ^ aw_mix((unsigned)t));
+  }
+  const float lr = hy.lr_dev ? *hy.lr_dev : hy.lr;
+  s.keep = 1.f - lr * hy.wd;
+  s.rate = lr / bc1;
+  s.ibc2 = 1.f / bc2s;
+  s.coef = hy.norm ? fminf(hy.max_norm / (*hy.norm + 1e-6f), 1.f) : 1.f;
+  s.key = aw_mix(s.key ^ aw_mix((unsigned)(tab.place0 + ti)));
+
+  if (full) {
+#pragma unroll
+    for (int u = 0; u < AW_U; ++u)
+      part[u].step(p + u * AW_BLOCK, AW_BLOCK, (unsigned)base + u * AW_BLOCK, m + u * AW_BLOCK * SB, v + u * AW_BLOCK * SB, sm + u, sv + u, lane, s, hy);
+  } else {
+    AwPart<T, BITS, false> one;
+#pragma unroll 1
+    for (int u = 0; u < AW_U && (unsigned long long)u * AW_BLOCK < left; ++u) {
+      const unsigned long long l = left - u * AW_BLOCK;
+      one.load(p + u * AW_BLOCK, g + u * AW_BLOCK, l, m + u * AW_BLOCK * SB, v + u * AW_BLOCK * SB, sm + u, sv + u, lane);
+      one.step(p + u * AW_BLOCK, l, (unsigned)base + u * AW_BLOCK, m + u * AW_BLOCK * SB, v + u * AW_BLOCK * SB, sm + u, sv + u, lane, s, hy);
     }
   }
 }

@@ -101,13 +101,16 @@ __device__ __forceinline__ void store8(T* const p, const long left, const float*
 // Sums and maxima over groups of L consecutive lanes (L a power of two up to 64); every lane gets the same result.  Partner lanes come
 // through the data-parallel paths of the vector unit (a lane's neighbours, mirrored halves, exchanged rows), not through shared memory.
 struct OpSum { static __device__ __forceinline__ float run(const float a, const float b) { return a + b; } };
-struct OpMax { static __device__ __forceinline__ float run(const float a, const float b) { return fmaxf(a, b); } };
-template <int CTRL>
-__device__ __forceinline__ float dpp(const float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+struct OpMax {
+  static __device__ __forceinline__ float run(const float a, const float b) { return fmaxf(a, b); }
+  static __device__ __forceinline__ unsigned run(const unsigned a, const unsigned b) { return a > b ? a : b; }
+};
+template <int CTRL, typename V>
+__device__ __forceinline__ V dpp(const V v) {
+  return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
 }
-template <int L, typename OP>
-__device__ __forceinline__ float lanes_op(float v) {
+template <int L, typename OP, typename V>
+__device__ __forceinline__ V lanes_op(V v) {
   if constexpr (L > 1) v = OP::run(v, dpp<0xB1>(v));           // quad_perm [1, 0, 3, 2]
   if constexpr (L > 2) v = OP::run(v, dpp<0x4E>(v));           // quad_perm [2, 3, 0, 1]
   if constexpr (L > 4) v = OP::run(v, dpp<0x141>(v));          // row_half_mirror: the other four of eight
@@ -116,19 +119,19 @@ __device__ __forceinline__ float lanes_op(float v) {
     const unsigned u = __builtin_bit_cast(unsigned, v);
     const u32x2 r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
     const unsigned a = r[0], b = r[1];           // (a bit cast of a vector's element takes element 0)
-    v = OP::run(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    v = OP::run(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b));
   }
   if constexpr (L > 32) {
     const unsigned u = __builtin_bit_cast(unsigned, v);
     const u32x2 r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    const unsigned a = r[0], b = r[1];           // (a bit cast of a vector's element takes element 0)
-    v = OP::run(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+    const unsigned a = r[0], b = r[1];
+    v = OP::run(__builtin_bit_cast(V, a), __builtin_bit_cast(V, b));
   }
   return v;
 }
 template <int L>
 __device__ __forceinline__ float lanes_sum(const float v) { return lanes_op<L, OpSum>(v); }
-template <int L>
-__device__ __forceinline__ float lanes_max(const float v) { return lanes_op<L, OpMax>(v); }
+template <int L, typename V>
+__device__ __forceinline__ V lanes_max(const V v) { return lanes_op<L, OpMax>(v); }
 
 }  // namespace selfc
