@@ -323,34 +323,46 @@ __global__ __launch_bounds__(NQ * NP * 64) void gemm_kernel(const GemmArgs a) {
     }
     const unsigned char* const lq = lds + cur * STAGE;
     const unsigned char* const lp = lq + SQ;
-    if constexpr (ES == 1) {
-      i32x4 q[TQ][2];
+    // TQ multiplies per step and piece of P; the pieces are requested AHEAD steps before their multiplies, and the schedule is held to
+    // that (left alone, the compiler moves every read to right in front of its use and the matrix units wait for shared memory)
+    constexpr int HALF = ES == 1 ? 1 : 2, STEPS = HALF * TP, AHEAD = STEPS < 3 ? STEPS : 3, W = ES == 1 ? 2 : 1;
+    constexpr int RP = (PX ? 2 : 1) * W, RQ = (QX ? 2 : 1) * W;           // reads per piece
+    i32x4 q[HALF][TQ][W], p[AHEAD + 1][W];
+    const auto read_q = [&](const int h) {
 #pragma unroll
-      for (int j = 0; j < TQ; ++j) { q[j][0] = fq.read(lq, j, 0); q[j][1] = fq.read(lq, j, 1); }
+      for (int j = 0; j < TQ; ++j)
 #pragma unroll
-      for (int i = 0; i < TP; ++i) {
-        const i32x4 p0_ = fp.read(lp, i, 0), p1_ = fp.read(lp, i, 1);
+        for (int w = 0; w < W; ++w) q[h][j][w] = fq.read(lq, j, ES == 1 ? w : h);
+    };
+    const auto read_p = [&](const int n) {
 #pragma unroll
-        for (int j = 0; j < TQ; ++j) acc[i][j] = mma8(p0_, p1_, q[j][0], q[j][1], acc[i][j]);
+      for (int w = 0; w < W; ++w) p[n % (AHEAD + 1)][w] = fp.read(lp, n % TP, ES == 1 ? w : n / TP);
+    };
+    read_q(0);
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) read_p(n);
+    __builtin_amdgcn_sched_group_barrier(0x100, TQ * RQ + AHEAD * RP, 0);
+#pragma unroll
+    for (int n = 0; n < STEPS; ++n) {
+      const int h = n / TP, i = n % TP, slot = n % (AHEAD + 1);
+      const bool more = n + AHEAD < STEPS, next_q = HALF == 2 && n == (TP > 2 ? TP - 2 : 0);
+      if (more) read_p(n + AHEAD);
+      if (next_q) read_q(1);
+#pragma unroll
+      for (int j = 0; j < TQ; ++j) {
+        if constexpr (ES == 1) acc[i][j] = mma8(p[slot][0], p[slot][W - 1], q[h][j][0], q[h][j][W - 1], acc[i][j]);
+        else acc[i][j] = Mma<T>::run(p[slot][0], q[h][j][0], acc[i][j]);
       }
-    } else {
+      if (more) __builtin_amdgcn_sched_group_barrier(0x100, RP, 0);
+      if (next_q) __builtin_amdgcn_sched_group_barrier(0x100, TQ * RQ, 0);
+      __builtin_amdgcn_sched_group_barrier(0x8, TQ, 0);
+    }
+    if constexpr (QX && PX) {
+      if (own)
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        i32x4 q[TQ], p[TP];
+        for (int h = 0; h < HALF; ++h)
 #pragma unroll
-        for (int j = 0; j < TQ; ++j) q[j] = fq.read(lq, j, ks);
-#pragma unroll
-        for (int i = 0; i < TP; ++i) p[i] = fp.read(lp, i, ks);
-#pragma unroll
-        for (int i = 0; i < TP; ++i)
-#pragma unroll
-          for (int j = 0; j < TQ; ++j) acc[i][j] = Mma<T>::run(p[i], q[j], acc[i][j]);
-        if constexpr (QX && PX) {
-          if (own)
-#pragma unroll
-            for (int j = 0; j < TQ; ++j) osum[j] = Mma<T>::run(ones, q[j], osum[j]);
-        }
-      }
+          for (int j = 0; j < TQ; ++j) osum[j] = Mma<T>::run(ones, q[h][j][0], osum[j]);
     }
   }
   wait_barrier<0>();                      // the buffers are free: each wave turns its tiles into rows of its own piece of them
