@@ -4,7 +4,6 @@
 ``train.RescaleTrainer`` uses for ``train_opt["optimizer"] == "AdamW"``."""
 from __future__ import annotations
 
-from operator import attrgetter
 from typing import List, Optional, Sequence
 
 import numpy as np
@@ -38,73 +37,86 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-_T = torch.Tensor
-_dtype_of = attrgetter("dtype")
+def _host():
+    """csrc/host.cpp; like the kernels' library it is built, not optional"""
+    global _HOST
+    if _HOST is None:
+        try:
+            from . import _host as _HOST
+        except ImportError as e:
+            raise RuntimeError("selfc_amd/_host.so is missing: build it with `make -C selfc_amd/csrc`") from e
+    return _HOST
 
 
-def _one_kind(ts, first, what):
-    """All tensors of the first one's type on its GPU (checked for hundreds of tensors per step: in whole-list passes)."""
-    dt, dev = first.dtype, first.get_device()
-    if set(map(_dtype_of, ts)) != {dt} or set(map(_T.get_device, ts)) != {dev}:
-        i, t = next((i, t) for i, t in enumerate(ts) if t.dtype is not dt or t.get_device() != dev)
-        raise RuntimeError(f"selfc_amd: {what} {i} is {t.dtype} on {t.device}, expected {dt} on {first.device}: one call takes one type on one GPU")
+_HOST = None
 
 
 def _table(params, grads, steps):
-    """The C table of (parameter, gradient, step, size) per tensor, the tensors it points to beyond the caller's own, the first tensor."""
+    """(the C table of (parameter, gradient, step, size) per tensor, tensors it points to beyond the caller's own, the first tensor, blocks
+    of the moments)."""
+    tab = np.empty((len(grads), 4), dtype=np.uint64)
+    got = _host().table(params, grads, steps, tab.__array_interface__["data"][0])
+    if got is not None:
+        live, blocks = got
+        first = params[0] if params else next((g for g in grads if g is not None), None) if live else None
+        if first is not None:
+            _lib.require_gpu(first)
+            _need(first.dtype in _DTYPE, lambda: f"{first.dtype} tensors; expected float32, bfloat16 or float16")
+        return tab, (), first, blocks
+    keep = _look_closer(params, grads, steps)
+    got = _host().table([_as_flat(p) for p in params] if params is not None else None, [None if g is None else _as_flat(g) for g in grads], steps,
+                        tab.__array_interface__["data"][0])
+    _need(got is not None, "the tensors cannot be read")
+    return tab, keep, params[0] if params else next(g for g in grads if g is not None), got[1]
+
+
+def _as_flat(t):
+    """the memory of a dense tensor, in its own order"""
+    return t.detach().as_strided((t.numel(),), (1,))
+
+
+def _look_closer(params, grads, steps):
+    """Not everything is of one kind and contiguous: say what is refused; bring gradients into their tensors' order."""
     keep = []
-    n = len(grads)
-    tab = np.zeros((n, 4), dtype=np.uint64)
-    _need(params is None or len(params) == n, lambda: f"{len(params)} tensors and {n} gradients")
-    some = [i for i, g in enumerate(grads) if g is not None]
-    live = grads if len(some) == n else [grads[i] for i in some]
-    first = params[0] if params else live[0] if live else None
-    if first is None:
-        return tab, keep, None
+    _need(params is None or len(params) == len(grads), lambda: f"{len(params)} tensors and {len(grads)} gradients")
+    every = [(f"tensor {i}", t) for i, t in enumerate(params or [])] + [(f"gradient {i}", t) for i, t in enumerate(grads) if t is not None]
+    _need(all(torch.is_tensor(t) for _, t in every), "expected tensors")
+    first = every[0][1]
     _lib.require_gpu(first)
     _need(first.dtype in _DTYPE, lambda: f"{first.dtype} tensors; expected float32, bfloat16 or float16")
-    if params is not None:
-        _one_kind(params, first, "tensor")
-    if live:
-        _one_kind(live, first, "gradient")
-    if params is not None:
-        mine = params if len(some) == n else [params[i] for i in some]
-        if list(map(_T.size, mine)) != list(map(_T.size, live)):
-            i = next(k for k, p, g in zip(some, mine, live) if p.shape != g.shape)
-            raise RuntimeError(f"selfc_amd: gradient {i} has shape {tuple(grads[i].shape)}, its tensor {tuple(params[i].shape)}")
-        if not (all(map(_T.is_contiguous, mine)) and all(map(_T.is_contiguous, live))):
-            for i, p, g in zip(some, mine, live):
-                if not (p.is_contiguous() and g.is_contiguous()):
-                    _need(g.layout is torch.strided and _dense(p), lambda: f"tensor {i} does not fill one stretch of memory (strides {p.stride()})")
-                    if g.stride() != p.stride():
-                        grads[i] = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
-                        keep.append(grads[i])
-        tab[:, 0] = list(map(_T.data_ptr, params))
-        tab[:, 3] = list(map(_T.numel, params))
-    else:
-        for i in some:
-            if not grads[i].is_contiguous() and not _dense(grads[i]):
-                grads[i] = grads[i].contiguous()
+    for name, t in every:
+        if t.dtype is not first.dtype or t.device != first.device or t.layout is not torch.strided:
+            raise RuntimeError(f"selfc_amd: {name} is {t.dtype} on {t.device} ({t.layout}), expected {first.dtype} on {first.device}: one call takes one type on one GPU")
+    for i, g in enumerate(grads):
+        if g is None:
+            continue
+        if params is None:
+            if not _dense(g):
+                grads[i] = g.contiguous()
                 keep.append(grads[i])
-        tab[some, 3] = [grads[i].numel() for i in some]
-    if len(some) == n:
-        tab[:, 1] = list(map(_T.data_ptr, grads))
-    else:
-        tab[some, 1] = [grads[i].data_ptr() for i in some]
-    if steps is not None:
-        tab[:, 2] = list(map(_T.data_ptr, steps))
-    return tab, keep, first
+            continue
+        p = params[i]
+        _need(p.shape == g.shape, lambda: f"gradient {i} has shape {tuple(g.shape)}, its tensor {tuple(p.shape)}")
+        _need(_dense(p), lambda: f"tensor {i} does not fill one stretch of memory (strides {p.stride()})")
+        if g.stride() != p.stride():
+            grads[i] = torch.empty_strided(p.shape, p.stride(), dtype=p.dtype, device=p.device).copy_(g)
+            keep.append(grads[i])
+    for i, p in enumerate(params or []):
+        _need(_dense(p), lambda: f"tensor {i} does not fill one stretch of memory (strides {p.stride()})")
+    _need(steps is None or (len(steps) == len(grads) and all(torch.is_tensor(s) and s.dtype is torch.float32 and s.device == first.device and s.numel() == 1 for s in steps)),
+          "step: expected a float32 scalar on the tensors' GPU for each tensor")
+    return keep
 
 
 def grad_norm(grads: Sequence[Optional[torch.Tensor]]) -> torch.Tensor:
     """2-norm of all gradients (None entries are skipped) of one type on one GPU, as a device scalar; squares are summed in 64 bits."""
     grads = list(grads)
-    tab, keep, first = _table(None, grads, None)
+    tab, keep, first, _ = _table(None, grads, None)
     _need(first is not None, "grad_norm needs a gradient")
     with on_device(first):
         out = torch.empty((), dtype=torch.float32, device=first.device)
         part = torch.empty(_lib.lib().selfc_grad_norm_partials(len(grads)), dtype=torch.float64, device=first.device)
-        rt.call("selfc_grad_norm", tab.ctypes.data, len(grads), _DTYPE[first.dtype], part.data_ptr(), out.data_ptr(), _stream(first))
+        rt.call("selfc_grad_norm", tab.__array_interface__["data"][0], len(grads), _DTYPE[first.dtype], part.data_ptr(), out.data_ptr(), _stream(first))
     return out
 
 
@@ -126,7 +138,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     _need(0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0, lambda: f"betas are ({beta1}, {beta2})")
     grads = list(grads)
     steps = step if isinstance(step, (list, tuple)) else None
-    tab, keep, first = _table(params, grads, steps)
+    tab, keep, first, blocks = _table(params, grads, steps)
     if first is None:
         return
     bits8 = exp_avg.dtype is torch.float8_e4m3fn
@@ -135,13 +147,12 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
         _need(exp_avg_scale is not None and exp_avg_sq_scale is not None, "8-bit moments need their scales")
     else:
         _need(exp_avg.dtype is torch.float32 and exp_avg_sq.dtype is torch.float32, lambda: f"moments are {exp_avg.dtype} and {exp_avg_sq.dtype}: expected float32, or float8_e4m3fn and float8_e5m2")
-    size = int((-(-tab[:, 3].astype(np.int64) // BLOCK)).sum()) * BLOCK
-    for name, t, n in (("exp_avg", exp_avg, size), ("exp_avg_sq", exp_avg_sq, size)) + ((("exp_avg_scale", exp_avg_scale, size // BLOCK), ("exp_avg_sq_scale", exp_avg_sq_scale, size // BLOCK)) if bits8 else ()):
-        _need(t.device == first.device and t.is_contiguous() and t.numel() >= n, lambda: f"{name}: expected {n} contiguous values on {first.device}, got {tuple(t.shape)} on {t.device}")
-        _need(n == size or t.dtype is torch.float32, lambda: f"{name} is {t.dtype}, expected float32")
+    size, dev = blocks * BLOCK, first.device
+    for name, t, n in (("exp_avg", exp_avg, size), ("exp_avg_sq", exp_avg_sq, size)) + ((("exp_avg_scale", exp_avg_scale, blocks), ("exp_avg_sq_scale", exp_avg_sq_scale, blocks)) if bits8 else ()):
+        if t.device != dev or not t.is_contiguous() or t.numel() < n:
+            raise RuntimeError(f"selfc_amd: {name}: expected {n} contiguous values on {dev}, got {tuple(t.shape)} on {t.device}")
+    _need(not bits8 or (exp_avg_scale.dtype is torch.float32 and exp_avg_sq_scale.dtype is torch.float32), "the scales are float32")
     if steps is not None:
-        _need(len(steps) == len(grads) and all(s.dtype is torch.float32 and s.get_device() == first.get_device() and s.numel() == 1 for s in steps),
-              "step: expected a float32 scalar on the tensors' GPU for each tensor")
         host_step = 1.0
     else:
         host_step = float(step)
@@ -157,13 +168,13 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     if norm is not None:
         _need(norm.dtype is torch.float32 and norm.numel() == 1 and norm.device == first.device, "norm: expected a float32 scalar on the tensors' GPU")
     with on_device(first):
-        rt.call("selfc_adamw_step", tab.ctypes.data, len(grads), _DTYPE[first.dtype], 8 if bits8 else 32, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
+        rt.call("selfc_adamw_step", tab.__array_interface__["data"][0], len(grads), _DTYPE[first.dtype], 8 if bits8 else 32, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
                 rt._ptr(exp_avg_scale) if bits8 else None, rt._ptr(exp_avg_sq_scale) if bits8 else None, 0.0 if lr_dev is not None else float(lr),
                 rt._ptr(lr_dev), float(beta1), float(beta2), float(eps), float(weight_decay), host_step, int(seed) & 0xFFFFFFFF, rt._ptr(norm),
                 float(max_norm or 0.0), _stream(first))
     del keep
     # the kernel wrote through raw pointers: autograd's saved-tensor checks and the packed-weight caches go by version
-    torch.autograd.graph.increment_version([p for p, g in zip(params, grads) if g is not None])
+    _host().written(params, grads)
 
 
 class _Bucket:
