@@ -217,6 +217,23 @@ def lib():
     return _lib
 
 
+_host = None
+
+
+def host():
+    """selfc_amd/_host.so (csrc/host.cpp) with the loaded library's entry points bound; raises RuntimeError when it has not been built."""
+    global _host
+    if _host is None:
+        L = lib()
+        try:
+            from . import _host as h
+        except ImportError as e:
+            raise RuntimeError("selfc_amd/_host.so is missing or does not fit this torch: build it with `make -C selfc_amd/csrc`") from e
+        h.bind({name: C.cast(getattr(L, name), C.c_void_p).value for name in SYMBOLS if name.startswith(("selfc_rmsnorm", "selfc_linear", "selfc_pack"))})
+        _host = h
+    return _host
+
+
 def check(rc, what):
     if rc == 0:
         return

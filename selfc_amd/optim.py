@@ -37,25 +37,11 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
-def _host():
-    """csrc/host.cpp; like the kernels' library it is built, not optional"""
-    global _HOST
-    if _HOST is None:
-        try:
-            from . import _host as _HOST
-        except ImportError as e:
-            raise RuntimeError("selfc_amd/_host.so is missing: build it with `make -C selfc_amd/csrc`") from e
-    return _HOST
-
-
-_HOST = None
-
-
 def _table(params, grads, steps):
     """(the C table of (parameter, gradient, step, size) per tensor, tensors it points to beyond the caller's own, the first tensor, blocks
     of the moments)."""
     tab = np.empty((len(grads), 4), dtype=np.uint64)
-    got = _host().table(params, grads, steps, tab.__array_interface__["data"][0])
+    got = _lib.host().table(params, grads, steps, tab.__array_interface__["data"][0])
     if got is not None:
         live, blocks = got
         first = params[0] if params else next((g for g in grads if g is not None), None) if live else None
@@ -64,7 +50,7 @@ def _table(params, grads, steps):
             _need(first.dtype in _DTYPE, lambda: f"{first.dtype} tensors; expected float32, bfloat16 or float16")
         return tab, (), first, blocks
     keep = _look_closer(params, grads, steps)
-    got = _host().table([_as_flat(p) for p in params] if params is not None else None, [None if g is None else _as_flat(g) for g in grads], steps,
+    got = _lib.host().table([_as_flat(p) for p in params] if params is not None else None, [None if g is None else _as_flat(g) for g in grads], steps,
                         tab.__array_interface__["data"][0])
     _need(got is not None, "the tensors cannot be read")
     return tab, keep, params[0] if params else next(g for g in grads if g is not None), got[1]
@@ -174,7 +160,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
                 float(max_norm or 0.0), _stream(first))
     del keep
     # the kernel wrote through raw pointers: autograd's saved-tensor checks and the packed-weight caches go by version
-    _host().written(params, grads)
+    _lib.host().written(params, grads)
 
 
 class _Bucket:

@@ -72,40 +72,17 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _pitch(t: torch.Tensor) -> int:
-    rows, cols = t.shape
-    return t.stride(0) if rows > 1 else max(cols, 1)
-
-
-def _pieces(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """(matrix, pitch) that the product's kernels can read: 16-byte aligned rows of whole 16-byte pieces."""
-    es, (rows, cols) = t.element_size(), t.shape
-    per = 16 // es
-    ld = t.stride(0) if rows > 1 else cols
-    if not t.data_ptr() % 16 and not cols % per and not ld % per and ld < (1 << 21):
-        return t, ld
-    ldd = -(-cols // per) * per
-    out = torch.empty((rows, ldd), dtype=t.dtype, device=t.device)
-    rt.call("selfc_pack_rows", t.data_ptr(), ld, out.data_ptr(), rows, cols, ldd, es, _stream(t))
-    return out, ldd
-
-
-def _ws(rows: int, cols: int, total: int, es: int, device) -> Optional[torch.Tensor]:
-    n = _lib.lib().selfc_linear_ws_floats(rows, cols, total, es)
-    return torch.empty(n, dtype=torch.float32, device=device) if n else None
-
-
-_ptr = rt._ptr
 
 # -- captured backward passes ----------------------------------------------------------------------------------------------------
-_EAGER = "selfc_amd_eager_graph"
+_MARK = "selfc_amd_graph_of"
 
 
 def _watch(out: torch.Tensor):
     """A leaf's gradient accumulator lives as long as a graph that reaches it and remembers the stream it was made on.  If an eager
     graph is still alive when a captured backward pass reaches the same leaf, autograd waits for that stream inside the capture and
-    the process ends.  So: the accumulators that an eager call reaches are marked with its stream, and a call under capture that meets
-    another stream's mark refuses."""
+    the process ends; if a captured graph's outputs are still alive when an eager pass does, and the capture's stream is gone
+    (runtime.graph_capture destroys its own), it ends as well.  So: the accumulators that a call reaches are marked with the stream
+    and with whether it was being captured, and a call that meets such a mark refuses."""
     here = _raw_stream(out.get_device())
     capturing = torch.cuda.is_current_stream_capturing()
     for node, _ in out.grad_fn.next_functions:
@@ -116,16 +93,13 @@ def _watch(out: torch.Tensor):
             if node is None:
                 continue
         meta = node.metadata
-        if not capturing:
-            meta[_EAGER] = here
-        elif meta.get(_EAGER, here) != here:
+        made, captured = meta.setdefault(_MARK, (here, capturing))
+        if capturing and not captured and made != here:
             _bad("a graph of an earlier eager call over the same parameters is still alive; its gradients cannot be accumulated inside a "
                  "capture - drop that call's outputs and losses first")
-
-
-def _no_second(ctx):
-    if torch.is_grad_enabled():
-        _bad("no second derivatives (create_graph=True)")
+        if captured and not capturing and made in rt.CLOSED_STREAMS:
+            _bad("a captured call's outputs over the same parameters still hold their graph, whose stream is gone - keep detached outputs of a "
+                 "capture")
 
 
 # -- norm ------------------------------------------------------------------------------------------------------------------------
@@ -150,53 +124,6 @@ def _norm_args(x, weight, residual, eps):
             _bad(f"residual has shape {tuple(residual.shape)}, x {tuple(shape)}")
 
 
-def _run_norm(x2, r2, weight, eps, q8: bool):
-    rows, cols = x2.shape
-    dev, dt = x2.device, x2.dtype
-    y = torch.empty((rows, cols), dtype=torch.float8_e4m3fn if q8 else dt, device=dev)
-    scale = torch.empty(rows, dtype=torch.float32, device=dev) if q8 else None
-    h = torch.empty((rows, cols), dtype=dt, device=dev) if r2 is not None else None
-    if rows:
-        rt.call("selfc_rmsnorm", x2.data_ptr(), _pitch(x2), _ptr(r2), 0 if r2 is None else _pitch(r2), weight.data_ptr(),
-                weight.dtype is torch.float32, _ptr(h), y.data_ptr(), _ptr(scale), rows, cols, _DTYPE[dt], eps, _stream(x2))
-    return y, scale, h
-
-
-class RMSNormFn(torch.autograd.Function):
-    """rms_norm on matrices; the gradient needs h and the weight only (the row's statistic is recomputed)."""
-
-    @staticmethod
-    def forward(ctx, x2, r2, weight, eps):
-        with on_device(x2):
-            y, _, h = _run_norm(x2, r2, weight, eps, False)
-        ctx.eps = eps
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x2 if h is None else h, weight)
-        return (y,) if h is None else (y, h)
-
-    @staticmethod
-    def backward(ctx, dy, dh=None):
-        _no_second(ctx)
-        h, weight = ctx.saved_tensors
-        to_x, to_r, want_w, _ = ctx.needs_input_grad
-        want_x = to_x or to_r
-        if dy is None:                     # only h was used
-            return (dh if to_x else None), (dh if to_r else None), None, None
-        rows, cols = h.shape
-        dy = dy.contiguous()
-        dh = dh.contiguous() if dh is not None else None
-        with on_device(h):
-            dx = torch.empty((rows, cols), dtype=h.dtype, device=h.device) if want_x else None
-            dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if want_w else None
-            part = torch.empty(_lib.lib().selfc_rmsnorm_bwd_floats(rows, cols), dtype=torch.float32, device=h.device) if want_w else None
-            if rows:
-                rt.call("selfc_rmsnorm_bwd", h.data_ptr(), _pitch(h), weight.data_ptr(), weight.dtype is torch.float32, dy.data_ptr(), _ptr(dh),
-                        _ptr(dx), _ptr(dw), _ptr(part), rows, cols, _DTYPE[h.dtype], ctx.eps, _stream(h))
-            elif dw is not None:
-                dw.zero_()
-        return (dx if to_x else None), (dx if to_r else None), dw, None
-
-
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
     """(y, h): h = x + residual rounded to x's type (x itself without a residual), y = h / sqrt(mean(h^2) + eps) * weight.
 
@@ -204,13 +131,11 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     fp32 in a fixed order.  Gradients flow to x, residual and weight, from y and h."""
     _norm_args(x, weight, residual, eps)
     x2, r2, weight = _rows(x), None if residual is None else _rows(residual), weight.contiguous()
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
-        out = RMSNormFn.apply(x2, r2, weight, float(eps))
-        _watch(out[0])
-        y, h = out if r2 is not None else (out[0], None)
-    else:
-        with on_device(x):
-            y, _, h = _run_norm(x2, r2, weight, float(eps), False)
+    grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad))
+    with on_device(x):
+        y, _, h = _lib.host().norm(x2, r2, weight, eps, False, grad, _stream(x))
+    if grad:
+        _watch(y)
     if x.dim() == 2:
         return y, (x if h is None else h)
     return y.view(x.shape), (x if h is None else h.view(x.shape))
@@ -227,7 +152,9 @@ def rms_norm_q8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.
     _norm_args(x, weight, residual, eps)
     _no_grad_only("rms_norm_q8", x, weight, residual)
     with on_device(x):
-        q, scale, h = _run_norm(_rows(x), None if residual is None else _rows(residual), weight.contiguous(), float(eps), True)
+        q, scale, h = _lib.host().norm(_rows(x), None if residual is None else _rows(residual), weight.contiguous(), eps, True, False, _stream(x))
+    if x.dim() == 2:
+        return q, scale, (x if h is None else h)
     return q.view(x.shape), scale.view(x.shape[:-1]), (x if h is None else h.view(x.shape))
 
 
@@ -255,104 +182,6 @@ def _linear_args(x, weight, bias, act, residual, out_dtype):
             _bad(f"residual has shape {tuple(residual.shape)}, expected {tuple(shape[:-1] + weight.shape[:1])}")
 
 
-def _run_linear(xp, ldx, k, wp, ldw, n, xs, ws_, bias, act, r2, out_dtype, want_slope):
-    rows, dev = xp.shape[0], xp.device
-    y = torch.empty((rows, n), dtype=out_dtype, device=dev)
-    slope = torch.empty((rows, -(-n // 8) * 8), dtype=torch.int16, device=dev) if want_slope else None
-    if rows:
-        es = xp.element_size()
-        k = -(-k * es // 16) * 16 // es
-        work = _ws(rows, n, k, es, dev) if rows > 16 else None
-        rt.call("selfc_linear", xp.data_ptr(), ldx, wp.data_ptr(), ldw, _ptr(xs), _ptr(ws_), _ptr(bias), act, _ptr(r2),
-                0 if r2 is None else _pitch(r2), y.data_ptr(), _ptr(slope), _ptr(work), rows, n, k, _DTYPE[xp.dtype], _DTYPE[out_dtype], _stream(xp))
-    return y, slope
-
-
-def _narrow(n: int, k: int) -> bool:
-    return n <= 256 and k <= 256 and bool(_lib.lib().selfc_linear_rows_ok(n, k))
-
-
-def _run_rows(x2, w2, bias, act, r2, want_slope, want_pieces):
-    """(y, slope, x as whole pieces) of a narrow layer: one launch, any layout of x and the weight."""
-    (rows, k), n = x2.shape, w2.shape[0]
-    dev, dt = x2.device, x2.dtype
-    y = torch.empty((rows, n), dtype=dt, device=dev)
-    slope = torch.empty((rows, -(-n // 8) * 8), dtype=torch.int16, device=dev) if want_slope else None
-    xp = None
-    if want_pieces:
-        whole = k % 8 == 0 and x2.data_ptr() % 16 == 0 and _pitch(x2) % 8 == 0 and _pitch(x2) < (1 << 21)
-        xp = x2 if whole else torch.empty((rows, -(-k // 8) * 8), dtype=dt, device=dev)
-    if rows:
-        rt.call("selfc_linear_rows", x2.data_ptr(), _pitch(x2), w2.data_ptr(), _pitch(w2), _ptr(bias), act, _ptr(r2), 0 if r2 is None else _pitch(r2),
-                y.data_ptr(), _ptr(slope), None if xp is None or xp is x2 else xp.data_ptr(), rows, n, k, _DTYPE[dt], _stream(x2))
-    return y, slope, xp
-
-
-class LinearFn(torch.autograd.Function):
-    """linear on matrices.  Kept for the backward pass: x as the kernels read it, the weight, and the activation's derivative as 16-bit
-    fixed point."""
-
-    @staticmethod
-    def forward(ctx, x2, weight, bias, r2, act):
-        n, k = weight.shape
-        need = ctx.needs_input_grad
-        slope = act != 0 and any(need[:3])
-        ctx.narrow = _narrow(n, k)
-        with on_device(x2):
-            if ctx.narrow:
-                y, slope, xp = _run_rows(x2, weight, bias, act, r2, slope, need[1])
-                wp, ldw = weight, _pitch(weight)
-            else:
-                xp, ldx = _pieces(x2)
-                wp, ldw = _pieces(weight)
-                y, slope = _run_linear(xp, ldx, k, wp, ldw, n, None, None, bias, act, r2, x2.dtype, slope)
-        ctx.dims = (x2.shape[0], n, k, ldw)
-        ctx.save_for_backward(xp if need[1] else None, wp if need[0] else None, slope)
-        ctx.dtype = x2.dtype
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        _no_second(ctx)
-        xp, wp, slope = ctx.saved_tensors
-        rows, n, k, ldw = ctx.dims
-        want_x, want_w, want_b, want_r, _ = ctx.needs_input_grad
-        dev, dt, code, stream = dy.device, ctx.dtype, _DTYPE[ctx.dtype], _stream(dy)
-        dx = dw = db = None
-        if rows == 0:
-            return (torch.empty((0, k), dtype=dt, device=dev) if want_x else None, torch.zeros((n, k), dtype=dt, device=dev) if want_w else None,
-                    torch.zeros(n, dtype=dt, device=dev) if want_b else None, (dy if want_r else None), None)
-        L = _lib.lib()
-        with on_device(dy):
-            g = _rows(dy)
-            ldg, up = _pitch(g), -(-n // 8) * 8
-            as_is = slope is None and n % 8 == 0 and g.data_ptr() % 16 == 0 and ldg % 8 == 0 and ldg < (1 << 21)
-            rows_kernel = want_x and ctx.narrow
-            make_dz = not as_is and (want_w or (want_x and not rows_kernel))
-            dz, lddz = (torch.empty((rows, up), dtype=dt, device=dev), up) if make_dz else (g, ldg)
-            if want_b:                              # with dW it comes out of that product
-                db = torch.empty(n, dtype=dt, device=dev)
-            if want_x:
-                dx = torch.empty((rows, k), dtype=dt, device=dev)
-            if rows_kernel:
-                rt.call("selfc_linear_rows_bwd", g.data_ptr(), ldg, _ptr(slope), wp.data_ptr(), ldw, dx.data_ptr(), dz.data_ptr() if make_dz else None,
-                        rows, n, k, code, stream)
-            alone = want_b and not want_w
-            if alone or (make_dz and not rows_kernel):
-                part = torch.empty(L.selfc_linear_dz_floats(rows, n), dtype=torch.float32, device=dev) if alone else None
-                rt.call("selfc_linear_dz", g.data_ptr(), ldg, _ptr(slope), dz.data_ptr() if make_dz and not rows_kernel else None, up,
-                        db.data_ptr() if alone else None, _ptr(part), rows, n, code, stream)
-            if want_x and not rows_kernel:
-                work = _ws(rows, k, n, 2, dev)
-                rt.call("selfc_linear_dx", dz.data_ptr(), lddz, wp.data_ptr(), ldw, dx.data_ptr(), _ptr(work), rows, n, k, code, stream)
-            if want_w:
-                dw = torch.empty((n, k), dtype=dt, device=dev)
-                floats = L.selfc_linear_dw_floats(rows, n, k)
-                work = torch.empty(floats, dtype=torch.float32, device=dev) if floats else None
-                rt.call("selfc_linear_dw", dz.data_ptr(), lddz, xp.data_ptr(), _pitch(xp), dw.data_ptr(), _ptr(db), _ptr(work), rows, n, k, code, stream)
-        return dx, dw, db, (dy if want_r else None), None
-
-
 def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: str = "none",
            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(x weight^T + bias) + residual; x (..., in), weight (out, in), both bf16 or both f16, bias (out,) and residual (..., out) of the
@@ -367,19 +196,12 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
     x2, w2 = _rows(x), _rows(weight)
     b = None if bias is None else bias.contiguous()
     r2 = None if residual is None else _rows(residual)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        y = LinearFn.apply(x2, w2, b, r2, ACTS[act])
+    grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
+                                        or (residual is not None and residual.requires_grad))
+    with on_device(x):
+        y = _lib.host().linear(x2, w2, b, r2, ACTS[act], grad, _stream(x))
+    if grad:
         _watch(y)
-    else:
-        with on_device(x):
-            n, k = w2.shape
-            if _narrow(n, k):
-                y = _run_rows(x2, w2, b, ACTS[act], r2, False, False)[0]
-            else:
-                xp, ldx = _pieces(x2)
-                wp, ldw = _pieces(w2)
-                y, _ = _run_linear(xp, ldx, k, wp, ldw, n, None, None, b, ACTS[act], r2, dt, False)
     return y if x.dim() == 2 else y.view(x.shape[:-1] + weight.shape[:1])
 
 
@@ -411,9 +233,6 @@ def linear_q8(x: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w_sc
         if t.shape != shape:
             _bad(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     with on_device(x):
-        x2 = _rows(x)
-        xp, ldx = _pieces(x2)
-        wp, ldw = _pieces(_rows(weight))
-        y, _ = _run_linear(xp, ldx, x2.shape[1], wp, ldw, weight.shape[0], x_scale.reshape(-1).contiguous(), w_scale.contiguous(),
-                           None if bias is None else bias.contiguous(), ACTS[act], None if residual is None else _rows(residual), out_dtype, False)
+        y = _lib.host().linear_q8(_rows(x), x_scale.reshape(-1).contiguous(), _rows(weight), w_scale.contiguous(), None if bias is None else bias.contiguous(),
+                                  None if residual is None else _rows(residual), ACTS[act], _DTYPE[out_dtype], _stream(x))
     return y if x.dim() == 2 else y.view(x.shape[:-1] + weight.shape[:1])

@@ -267,6 +267,9 @@ SHUT_DOWN = False
 #: every live OwnStream (weak): closed by _shutdown() at interpreter exit, while the HIP runtime is still there
 _LIVE_STREAMS: "weakref.WeakSet" = weakref.WeakSet()
 
+#: handles of OwnStreams that were destroyed (and not handed out again): a gradient accumulator that remembers one must not be used
+CLOSED_STREAMS: set = set()
+
 
 def _shutdown():
     """atexit: destroy what must not be left to interpreter finalisation.  A hipGraph that died inside a reference cycle (a trainer:
@@ -304,6 +307,7 @@ class OwnStream:
         p = C.c_void_p()
         _lib.check(_lib.lib().selfc_stream_create(C.byref(p)), "selfc_stream_create")
         self.handle = p.value
+        CLOSED_STREAMS.discard(self.handle)
         _LIVE_STREAMS.add(self)
         dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
         self.stream = torch.cuda.ExternalStream(self.handle, device=dev)
@@ -312,6 +316,7 @@ class OwnStream:
         if self.handle:
             try:
                 self.stream.synchronize()
+                CLOSED_STREAMS.add(self.handle)
                 _lib.lib().selfc_stream_destroy(C.c_void_p(self.handle))
             except Exception:      # noqa: BLE001  (interpreter shutdown)
                 pass

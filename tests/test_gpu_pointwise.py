@@ -384,3 +384,54 @@ def test_captured_forward_and_backward_replay():
         torch.cuda.synchronize()
         for a, b in zip(got, run(fresh)):
             assert torch.equal(a, b), k
+
+
+def test_capture_over_an_eager_graph_that_is_alive_is_refused():
+    from selfc_amd import runtime as rt
+    w = torch.randn(40, 32).cuda().bfloat16().requires_grad_(True)
+    n = torch.ones(32).cuda().requires_grad_(True)
+    x = torch.randn(8, 32).cuda().bfloat16()
+    for call, leaf in ((lambda: pw().linear(x, w), w), (lambda: pw().rms_norm(x, n)[0], n)):
+        alive = call()
+        g = rt.new_graph()
+        with pytest.raises(RuntimeError, match="still alive"):
+            with rt.graph_capture(g, x.device):
+                call()
+        del alive
+        s = rt.warmup_stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            call()
+        torch.cuda.current_stream().wait_stream(s)
+        g = rt.new_graph()
+        with rt.graph_capture(g, x.device):
+            y = call()
+            got, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+        with pytest.raises(RuntimeError, match="captured call's outputs"):
+            call()
+        del y
+        for _ in range(2):
+            g.replay()
+            torch.cuda.synchronize()
+            ref = call()
+            want, = torch.autograd.grad(ref, leaf, torch.ones_like(ref))
+            assert torch.equal(got, want)
+            del ref
+
+
+def test_second_derivatives_are_refused():
+    w = torch.randn(40, 32).cuda().bfloat16().requires_grad_(True)
+    x = torch.randn(8, 32).cuda().bfloat16().requires_grad_(True)
+    for y in (pw().linear(x, w, act="silu"), pw().rms_norm(x, torch.ones(32).cuda())[0]):
+        with pytest.raises(RuntimeError, match="second"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
+def test_saved_tensors_that_were_written_over_are_noticed():
+    w = torch.randn(300, 512).cuda().half().requires_grad_(True)
+    x = torch.randn(20, 512).cuda().half().requires_grad_(True)
+    y = pw().linear(x, w)
+    with torch.no_grad():
+        w.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
