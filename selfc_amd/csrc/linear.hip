@@ -312,75 +312,98 @@ __global__ __launch_bounds__(NQ * NP * 64) void gemm_kernel(const GemmArgs a) {
     for (int j = 0; j < TQ; ++j) osum[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  if (s0 < s1) {
-    sq.begin(lds0, a.R - s0 * BK);
-    sp.begin(lds0 + SQ, a.R - s0 * BK);
+  // TQ multiplies per step and piece of P; the pieces are requested AHEAD steps before their multiplies, and the schedule is held to
+  // that (left alone, the compiler moves every read to right in front of its use and the matrix units wait for shared memory).
+  // A large tile has a compute unit to itself, so nothing hides what it waits for between two stages.  Its barrier stands AHEAD steps
+  // before a stage's end, where its last read is out: behind it the next stage's first pieces are read, and the loads of the stage after
+  // that set out over the last steps (8192 x 8192 x 8192 bf16: 828 us with the barrier between the stages, 788 this way).  Small tiles
+  // share a compute unit and fill each other's gaps: barrier between the stages, the next one's loads at once behind it, so that they have
+  // all of a stage to arrive (4096 x 2048 x 8192: 118 us, 142 to 155 with the early barrier).
+  constexpr bool EARLY = BQ * BP >= 256 * 256;
+  constexpr int HALF = ES == 1 ? 1 : 2, STEPS = HALF * TP, AHEAD = STEPS < 4 ? STEPS - 1 : 3, W = ES == 1 ? 2 : 1;
+  constexpr int TURN = EARLY ? STEPS - AHEAD : STEPS, RING = AHEAD + 1;
+  constexpr int RP = (PX ? 2 : 1) * W, RQ = (QX ? 2 : 1) * W;           // reads per piece
+  static_assert(STEPS % RING == 0, "a piece keeps its place in the ring from stage to stage");
+  constexpr int ALL = decltype(sq)::LOADS + decltype(sp)::LOADS;
+  i32x4 q[HALF][TQ][W], p[RING][W];
+  const auto read_q = [&](const int buf, const int h) {
 #pragma unroll
-    for (int it = 0; it < sq.LOADS; ++it) sq.issue(it);
+    for (int j = 0; j < TQ; ++j)
 #pragma unroll
-    for (int it = 0; it < sp.LOADS; ++it) sp.issue(it);
+      for (int w = 0; w < W; ++w) q[h][j][w] = fq.read(lds + buf * STAGE, j, ES == 1 ? w : h);
+  };
+  const auto read_p = [&](const int buf, const int n) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) p[n % RING][w] = fp.read(lds + buf * STAGE + SQ, n % TP, ES == 1 ? w : n / TP);
+  };
+  const auto read_first = [&](const int buf) {
+    read_q(buf, 0);
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) read_p(buf, n);
+    __builtin_amdgcn_sched_group_barrier(0x100, TQ * RQ + AHEAD * RP, 0);
+  };
+  const auto begin = [&](const int buf, const int s) {                  // behind the last stage: nothing is read, zeros are written
+    const int left = s < s1 ? a.R - s * BK : 0;
+    sq.begin(lds0 + buf * STAGE, left);
+    sp.begin(lds0 + buf * STAGE + SQ, left);
+  };
+  const auto issue = [&](const int k) {
+    if (k < sq.LOADS) sq.issue(k);
+    else sp.issue(k - sq.LOADS);
+  };
+  const auto load = [&](const int buf, const int s) {
+    begin(buf, s);
+#pragma unroll
+    for (int k = 0; k < ALL; ++k) issue(k);
+  };
+  if (s0 < s1) load(0, s0);
+  if constexpr (EARLY) {                  // both buffers are there whatever the number of stages
+    wait_barrier<0>();
+    load(1, s0 + 1);
+    read_first(0);
   }
+
   for (int s = s0; s < s1; ++s) {
     const int cur = (s - s0) & 1;
-    wait_barrier<0>();
-    // the next stage's loads: at once where a stage is short, so that they have all of it to arrive; spread over the first steps where it
-    // is long (256 x 256: 3 % faster than at once, 128 x 128: 25 % slower)
-    constexpr int ALL = decltype(sq)::LOADS + decltype(sp)::LOADS;
-    constexpr bool SPREAD = BQ * BP >= 256 * 256;
-    const auto issue = [&](const int k) {
-      if (k < sq.LOADS) sq.issue(k);
-      else sp.issue(k - sq.LOADS);
-    };
-    if (SPREAD || s + 1 < s1) {
-      const int left = s + 1 < s1 ? a.R - (s + 1) * BK : 0;
-      sq.begin(lds0 + (cur ^ 1) * STAGE, left);
-      sp.begin(lds0 + (cur ^ 1) * STAGE + SQ, left);
-      if constexpr (!SPREAD)
-#pragma unroll
-        for (int k = 0; k < ALL; ++k) issue(k);
+    if constexpr (!EARLY) {
+      wait_barrier<0>();
+      if (s + 1 < s1) load(cur ^ 1, s + 1);
+      read_first(cur);
     }
-    const unsigned char* const lq = lds + cur * STAGE;
-    const unsigned char* const lp = lq + SQ;
-    // TQ multiplies per step and piece of P; the pieces are requested AHEAD steps before their multiplies, and the schedule is held to
-    // that (left alone, the compiler moves every read to right in front of its use and the matrix units wait for shared memory)
-    constexpr int HALF = ES == 1 ? 1 : 2, STEPS = HALF * TP, AHEAD = STEPS < 3 ? STEPS : 3, W = ES == 1 ? 2 : 1;
-    constexpr int RP = (PX ? 2 : 1) * W, RQ = (QX ? 2 : 1) * W;           // reads per piece
-    i32x4 q[HALF][TQ][W], p[AHEAD + 1][W];
-    const auto read_q = [&](const int h) {
-#pragma unroll
-      for (int j = 0; j < TQ; ++j)
-#pragma unroll
-        for (int w = 0; w < W; ++w) q[h][j][w] = fq.read(lq, j, ES == 1 ? w : h);
-    };
-    const auto read_p = [&](const int n) {
-#pragma unroll
-      for (int w = 0; w < W; ++w) p[n % (AHEAD + 1)][w] = fp.read(lp, n % TP, ES == 1 ? w : n / TP);
-    };
-    read_q(0);
-#pragma unroll
-    for (int n = 0; n < AHEAD; ++n) read_p(n);
-    __builtin_amdgcn_sched_group_barrier(0x100, TQ * RQ + AHEAD * RP, 0);
 #pragma unroll
     for (int n = 0; n < STEPS; ++n) {
-      const int h = n / TP, i = n % TP, slot = n % (AHEAD + 1);
-      const bool more = n + AHEAD < STEPS, next_q = HALF == 2 && n == (TP > 2 ? TP - 2 : 0);
-      if (more) read_p(n + AHEAD);
-      if (next_q) read_q(1);
+      const int h = n / TP, i = n % TP, slot = n % RING;
+      const bool half = HALF == 2 && n == (TP > 2 ? TP - 2 : 0), next = EARLY && n == (HALF == 2 ? STEPS - 2 : STEPS - 1);
+      if (n == TURN) {
+        wait_barrier<0>();
+        begin(cur, s + 2);
+      }
+      if (n + AHEAD < STEPS) read_p(cur, n + AHEAD);
+      else if (EARLY) read_p(cur ^ 1, n + AHEAD - STEPS);
+      if (half) read_q(cur, 1);
+      if (next && HALF == 2) read_q(cur ^ 1, 0);
 #pragma unroll
       for (int j = 0; j < TQ; ++j) {
         if constexpr (ES == 1) acc[i][j] = mma8(p[slot][0], p[slot][W - 1], q[h][j][0], q[h][j][W - 1], acc[i][j]);
         else acc[i][j] = Mma<T>::run(p[slot][0], q[h][j][0], acc[i][j]);
       }
-      if (more) __builtin_amdgcn_sched_group_barrier(0x100, RP, 0);
-      if (next_q) __builtin_amdgcn_sched_group_barrier(0x100, TQ * RQ, 0);
+      if (next && HALF == 1) read_q(cur ^ 1, 0);
+      if (EARLY || n + AHEAD < STEPS) __builtin_amdgcn_sched_group_barrier(0x100, RP, 0);
+      if (half || (next && HALF == 2)) __builtin_amdgcn_sched_group_barrier(0x100, TQ * RQ, 0);
       __builtin_amdgcn_sched_group_barrier(0x8, TQ, 0);
-      if constexpr (SPREAD) {
-        constexpr int EACH = (ALL + STEPS / 2 - 1) / (STEPS / 2);
+      if (next && HALF == 1) __builtin_amdgcn_sched_group_barrier(0x100, TQ * RQ, 0);
+      if (n >= TURN) {
+        constexpr int EACH = (ALL + AHEAD - 1) / AHEAD;
 #pragma unroll
-        for (int k = n * EACH; k < (n + 1) * EACH && k < ALL; ++k) issue(k);
+        for (int k = (n - TURN) * EACH; k < (n - TURN + 1) * EACH && k < ALL; ++k) issue(k);
+      }
+      if constexpr (QX && PX) {
+        if (own && EARLY && i == (h == 0 ? 0 : TP - 1))
+#pragma unroll
+          for (int j = 0; j < TQ; ++j) osum[j] = Mma<T>::run(ones, q[h][j][0], osum[j]);
       }
     }
-    if constexpr (QX && PX) {
+    if constexpr (QX && PX && !EARLY) {
       if (own)
 #pragma unroll
         for (int h = 0; h < HALF; ++h)
@@ -796,7 +819,7 @@ template <typename T, bool QX, bool PX, int BQ, int BP, int NQ, int NP>
 hipError_t gemm_go(const GemmArgs& a, hipStream_t s) {
   static std::atomic<unsigned long long> optin{0};
   constexpr int stage = (BQ + BP) * 128, turn = NQ * NP * 16 * (BP / NP + 4) * 4, most = 2 * stage > turn ? 2 * stage : turn;
-  const int need = a.per > 1 ? 2 * stage : stage, bytes = need > turn ? need : turn;      // one stage: one buffer, more workgroups at a time
+  const int need = a.per > 1 || BQ * BP >= 256 * 256 ? 2 * stage : stage, bytes = need > turn ? need : turn;      // one stage: one buffer, more workgroups at a time
   const void* const fn = reinterpret_cast<const void*>(&gemm_kernel<T, QX, PX, BQ, BP, NQ, NP>);
   if (const hipError_t e = lds_optin(fn, most, optin); e != hipSuccess) return e;
   const long wgs = (long)((a.M + BQ - 1) / BQ) * ((a.N + BP - 1) / BP) * a.splits;
