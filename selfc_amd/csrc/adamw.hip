@@ -254,7 +254,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwTable tab, const AwH
   s.keep = 1.f - lr * hy.wd;
   s.rate = lr / bc1;
   s.ibc2 = 1.f / bc2s;
-  s.coef = hy.norm ? fminf(hy.max_norm / (*hy.norm + 1e-6f), 1.f) : 1.f;
+  s.coef = 1.f;
+  if (hy.norm) {                             // a norm that is not a number leaves none behind: min(1, NaN) is NaN here
+    const float c = hy.max_norm / (*hy.norm + 1e-6f);
+    s.coef = c >= 1.f ? 1.f : c;
+  }
   s.key = aw_mix(s.key ^ aw_mix((unsigned)(tab.place0 + ti)));
 
   if (full) {

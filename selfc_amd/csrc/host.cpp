@@ -6,7 +6,10 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/ATen.h>
+#include <algorithm>
 #include <cstdint>
+#include <utility>
+#include <vector>
 #include "../../include/selfc_hip.h"
 
 namespace {
@@ -67,6 +70,15 @@ PyObject* table(PyObject*, PyObject* args) {
         if (s.scalar_type() != at::kFloat || s.device() != first.device() || s.numel() != 1) Py_RETURN_NONE;
         row[2] = reinterpret_cast<std::uint64_t>(s.data_ptr());
       }
+    }
+    if (ps.fast && live > 1) {                 // each tensor is written by a workgroup of its own
+      std::vector<std::pair<std::uint64_t, std::uint64_t>> at;
+      at.reserve(live);
+      for (Py_ssize_t i = 0; i < n; ++i)
+        if (rows[4 * i + 1] && rows[4 * i + 3]) at.emplace_back(rows[4 * i], rows[4 * i] + rows[4 * i + 3] * first.element_size());
+      std::sort(at.begin(), at.end());
+      for (std::size_t i = 1; i < at.size(); ++i)
+        if (at[i].first < at[i - 1].second) throw std::runtime_error("selfc_amd: two of the tensors share memory (one is in the list twice, or they overlap)");
     }
     return Py_BuildValue("LL", live, blocks);
   } catch (const std::exception& e) {

@@ -112,7 +112,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
                max_norm: Optional[float] = None, norm: Optional[torch.Tensor] = None) -> None:
     """One AdamW step of `params` in place (decoupled weight decay; a tensor whose gradient is None is left as it is, with its moments).
 
-    All tensors have one type (fp32, bf16 or f16; gradients the same) and lie on one GPU; arithmetic is in fp32.  The moments of all
+    All tensors have one type (fp32, bf16 or f16; gradients the same), lie on one GPU and share no memory; arithmetic is in fp32.  The moments of all
     of them are held in two buffers of ``state_size`` values, tensor i behind the others at multiples of BLOCK values: fp32, or
     float8_e4m3fn (exp_avg) and float8_e5m2 (exp_avg_sq) with fp32 scales, one per BLOCK values.  In 8 bits the moments are rounded
     with a dither that is a function of (seed, step, the tensor's place in the list, the value's place in it): the same inputs give
@@ -120,7 +120,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
 
     step: the number of this step (from 1 on), or a list of device scalars, one per tensor, that hold it (captured steps).
     lr: a float or a device scalar.  norm, max_norm: gradients count as scaled by min(1, max_norm / (norm + 1e-6)); norm is a device
-    scalar (grad_norm); without it, it is computed here.  The gradients themselves are not changed."""
+    scalar (grad_norm); without it, it is computed here.  The gradients themselves are not changed.  A norm that is not finite acts as in
+    the formula: infinite, the finite gradients count as 0; not a number, no parameter that has a gradient stays one."""
     _need(0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0, lambda: f"betas are ({beta1}, {beta2})")
     grads = list(grads)
     steps = step if isinstance(step, (list, tuple)) else None
@@ -137,6 +138,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     for name, t, n in (("exp_avg", exp_avg, size), ("exp_avg_sq", exp_avg_sq, size)) + ((("exp_avg_scale", exp_avg_scale, blocks), ("exp_avg_sq_scale", exp_avg_sq_scale, blocks)) if bits8 else ()):
         if t.device != dev or not t.is_contiguous() or t.numel() < n:
             raise RuntimeError(f"selfc_amd: {name}: expected {n} contiguous values on {dev}, got {tuple(t.shape)} on {t.device}")
+    _need(exp_avg.data_ptr() != exp_avg_sq.data_ptr() or not size, "exp_avg and exp_avg_sq are the same memory")
     _need(not bits8 or (exp_avg_scale.dtype is torch.float32 and exp_avg_sq_scale.dtype is torch.float32), "the scales are float32")
     if steps is not None:
         host_step = 1.0
@@ -168,6 +170,7 @@ class _Bucket:
 
     def __init__(self, params: List[torch.Tensor], bits: int, capturable: bool, opt: torch.optim.Optimizer):
         self.params = params
+        self.strides = None if all(map(torch.Tensor.is_contiguous, params)) else [p.stride() for p in params]
         dev, size = params[0].device, state_size([p.numel() for p in params])
         kinds = (torch.float8_e4m3fn, torch.float8_e5m2) if bits == 8 else (torch.float32, torch.float32)
         self.m, self.v = (torch.zeros(size, dtype=torch.uint8 if bits == 8 else torch.float32, device=dev).view(k) for k in kinds)
@@ -184,6 +187,15 @@ class _Bucket:
                 for name, buf in zip(("exp_avg_scale", "exp_avg_sq_scale"), self.scales):
                     st[name] = buf[at // BLOCK:at // BLOCK + blocks]
             at += blocks * BLOCK
+
+
+    def check_layout(self):
+        """Moments lie in the order of their tensors' memory: that must not change under them."""
+        if self.strides is None:
+            same = all(map(torch.Tensor.is_contiguous, self.params))
+        else:
+            same = all(p.stride() == s for p, s in zip(self.params, self.strides))
+        _need(same, "a parameter's memory format changed after its moments were allocated - convert the model before the first step")
 
 
 class AdamW(torch.optim.Optimizer):
@@ -247,6 +259,8 @@ class AdamW(torch.optim.Optimizer):
             home = norms[0].device
             norm = norms[0] if len(norms) == 1 else torch.stack([n.to(home) for n in norms]).double().square().sum().sqrt().float()
             self.grad_norm = norm
+        for _, _, b, _ in work:
+            b.check_layout()
         for gi, bi, b, grads in work:
             group = self.param_groups[gi]
             kw = dict(lr=group["lr"], beta1=group["betas"][0], beta2=group["betas"][1], eps=group["eps"], weight_decay=group["weight_decay"],

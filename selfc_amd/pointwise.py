@@ -7,7 +7,7 @@
 
 The last axis is the row; leading axes may be any.  Rows may have any length, pitch and offset: rows that the kernels cannot read
 in 16-byte pieces are laid out again first (one more launch; widths that are multiples of 8 - of 16 in 8 bits - avoid it; 16-bit layers
-of up to about 200 values each way read any layout in place).
+of up to 256 values each way read any layout in place).
 Everything runs on the current stream of the tensors' device, allocates from torch's allocator only, and may be captured into a
 graph.  As for every torch module, a backward pass is captured only when no eager graph over the same leaves is alive any more
 (drop the losses of the eager steps first); such a capture is refused here (autograd would end the process).
@@ -29,7 +29,6 @@ _NAMES = {torch.float32: "float32", torch.bfloat16: "bfloat16", torch.float16: "
 MAX_NORM_COLS = 16384
 MAX_LINEAR = 1 << 20
 E4M3_MAX = 448.0
-
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
@@ -72,7 +71,6 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-
 # -- captured backward passes ----------------------------------------------------------------------------------------------------
 _MARK = "selfc_amd_graph_of"
 
@@ -88,10 +86,15 @@ def _watch(out: torch.Tensor):
     for node, _ in out.grad_fn.next_functions:
         if node is None:
             continue
-        if not hasattr(node, "variable"):                # rows of a leaf with more axes: a view in between
-            node = next((n for n, _ in node.next_functions if n is not None and hasattr(n, "variable")), None)
-            if node is None:
-                continue
+        for _ in range(4):                               # views and copies of a leaf in between: its rows, its transpose
+            if hasattr(node, "variable"):
+                break
+            before = [n for n, _ in node.next_functions if n is not None]
+            if len(before) != 1:
+                break
+            node = before[0]
+        if not hasattr(node, "variable"):
+            continue
         meta = node.metadata
         made, captured = meta.setdefault(_MARK, (here, capturing))
         if capturing and not captured and made != here:
@@ -134,8 +137,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Ten
     grad = torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad))
     with on_device(x):
         y, _, h = _lib.host().norm(x2, r2, weight, eps, False, grad, _stream(x))
-    if grad:
-        _watch(y)
+        if grad:
+            _watch(y)
     if x.dim() == 2:
         return y, (x if h is None else h)
     return y.view(x.shape), (x if h is None else h.view(x.shape))
@@ -186,8 +189,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(x weight^T + bias) + residual; x (..., in), weight (out, in), both bf16 or both f16, bias (out,) and residual (..., out) of the
     same type.  act: "none", "relu", "lrelu" (0.2), "gelu" (erf), "silu".  Sums, bias, activation and residual in fp32, one rounding at the end;
-    in the backward pass dy act'(z) is rounded to x's type once, as the operand of both products.  Wide weights
-    stream through a kernel of its own for up to 16 rows; layers of up to about 200 values each way keep theirs in shared memory.  Sums are added in a fixed order."""
+    in the backward pass dy act'(z) is rounded to x's type once, as the operand of both products.  Wide weights stream through a kernel of
+    their own for up to 16 rows; layers of up to 256 values each way keep theirs in shared memory.  Sums are added in a fixed order."""
     dt = x.dtype
     if dt is not torch.bfloat16 and dt is not torch.float16:
         _lib.require_gpu(x)
@@ -200,8 +203,8 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
                                         or (residual is not None and residual.requires_grad))
     with on_device(x):
         y = _lib.host().linear(x2, w2, b, r2, ACTS[act], grad, _stream(x))
-    if grad:
-        _watch(y)
+        if grad:
+            _watch(y)
     return y if x.dim() == 2 else y.view(x.shape[:-1] + weight.shape[:1])
 
 

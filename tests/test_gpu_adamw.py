@@ -342,3 +342,56 @@ def test_trainer_steps_with_adamw():
             assert all(torch.isfinite(p).all() for p in net.parameters())
         for a, b in zip(*logs):
             assert abs(a["loss"] / b["loss"] - 1) < 1e-2 and abs(a["grad_norm"] / b["grad_norm"] - 1) < 5e-2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_norm_that_is_not_finite(bits):
+    """min(1, max_norm / (norm + 1e-6)) as torch takes it: NaN stays, an infinite norm leaves finite gradients at 0."""
+    kinds = (torch.float8_e4m3fn, torch.float8_e5m2) if bits == 8 else (torch.float32, torch.float32)
+    for bad in (math.nan, math.inf):
+        ps = [torch.full((n,), 0.5).cuda() for n in (3, 4096 + 5)]
+        gs = [torch.full((n,), 0.25).cuda() for n in (3, 4096 + 5)]
+        gs[0][1] = bad
+        size = optim().state_size([3, 4101])
+        m, v = (torch.zeros(size, dtype=torch.float32).to(k).cuda() for k in kinds)
+        scales = [torch.ones(size // BLOCK).cuda() for _ in range(2)] if bits == 8 else [None, None]
+        optim().adamw_step(ps, gs, m, v, *scales, step=1, lr=0.1, weight_decay=0.0, max_norm=1.0)
+        if bad is math.nan:
+            assert torch.isnan(torch.cat(ps)).all()
+        else:
+            assert torch.isnan(ps[0][1]) and (ps[1] == 0.5).all() and (ps[0][[0, 2]] == 0.5).all()
+
+
+def test_offsets_past_32_bits():
+    """One tensor of more than 2^32 bytes and 2^31 values: its end moves as a tensor of its own does (the first step's update is made of
+    the moments before they are rounded)."""
+    tail, n = 300, 2 ** 31 + 300
+    gen = torch.Generator().manual_seed(5)
+    p, g = (torch.randn(tail, generator=gen) * s for s in (0.1, 0.01))
+    p, g = p.bfloat16().cuda(), g.bfloat16().cuda()
+    big, grad = (torch.zeros(n, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    big[-tail:], grad[-tail:] = p, g
+    size = optim().state_size([n])
+    m = torch.zeros(size, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    v = torch.zeros(size, dtype=torch.uint8, device="cuda").view(torch.float8_e5m2)
+    scales = [torch.ones(size // BLOCK, device="cuda") for _ in range(2)]
+    norm = optim().grad_norm([grad])
+    assert abs(norm.item() - g.double().norm().item()) <= norm.item() * 2 * U32
+    optim().adamw_step([big], [grad], m, v, *scales, step=1, lr=1e-2, max_norm=0.05, norm=norm)
+    size = optim().state_size([tail])
+    optim().adamw_step([p], [g], *(torch.zeros(size, device="cuda") for _ in range(2)), step=1, lr=1e-2, max_norm=0.05, norm=norm)
+    assert torch.equal(big[-tail:], p)
+    assert not big[:-tail].any() and m.view(torch.uint8)[n - tail:n].any()
+
+
+def test_memory_format_may_not_change_under_the_moments():
+    p = torch.randn(4, 3, 5, 5).cuda().requires_grad_(True)
+    opt = optim().AdamW([p])
+    p.grad = torch.randn_like(p)
+    opt.step()
+    before = p.detach().clone()
+    p.data = p.data.to(memory_format=torch.channels_last)
+    p.grad = p.grad.to(memory_format=torch.channels_last)
+    with pytest.raises(RuntimeError, match="memory format"):
+        opt.step()
+    assert torch.equal(p.detach(), before)

@@ -435,3 +435,106 @@ def test_saved_tensors_that_were_written_over_are_noticed():
         w.mul_(2)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("n,k", [(24, 40), (300, 264)])          # the weight in shared memory; tiles
+@pytest.mark.parametrize("bias", [None, False, True])
+@pytest.mark.parametrize("which", ["x", "w", "b", "r", "xr", "wr", "xb"])
+def test_product_gradients_one_at_a_time(n, k, bias, which):
+    """Every subset gets the gradients that all of them together get, whatever is missing or needs none."""
+    gen = torch.Generator().manual_seed(n)
+    x, w, b, r, dy = (t.half().cuda() for t in (rnd(gen, 37, k), rnd(gen, n, k, scale=k ** -0.5), rnd(gen, n), rnd(gen, 37, n), rnd(gen, 37, n)))
+    if bias is None:
+        which, b = which.replace("b", "") or "x", None
+    elif bias and "b" not in which:
+        which += "b"
+    full = {c: t.clone().requires_grad_(True) for c, t in zip("xwbr", (x, w, b, r)) if t is not None}
+    some = {c: t.clone().requires_grad_(c in which) for c, t in zip("xwbr", (x, w, b, r)) if t is not None}
+    ys = [pw().linear(d["x"], d["w"], d.get("b"), act="silu", residual=d["r"]) for d in (full, some)]
+    assert torch.equal(*ys)
+    all_of = dict(zip(full, torch.autograd.grad(ys[0], list(full.values()), dy)))
+    for c, g in zip(which, torch.autograd.grad(ys[1], [some[c] for c in which], dy)):
+        if c == "b" and "w" not in which:       # summed with dz instead of with dW: another order
+            d = dy.abs().double().sum(0) * 1.13
+            within(g, all_of[c].double().cpu(), (d * (2 * 50 * U32 + 2 ** -11) + all_of[c].double().abs() * 2 ** -10 + 2.0 ** -24).cpu())
+        else:
+            assert torch.equal(g, all_of[c]), c
+
+
+def test_product_gradient_against_differences():
+    """d/dx of sum(dy silu(x w^T + b)): a step of 2^-4 in one value, outputs in f16."""
+    gen = torch.Generator().manual_seed(12)
+    x, w, b, dy = (t.half().cuda() for t in (rnd(gen, 2, 24), rnd(gen, 16, 24, scale=0.2), rnd(gen, 16), rnd(gen, 2, 16)))
+    x = (x * 16).round() / 16                                      # so that x +- step are f16 values
+    leaf = x.clone().requires_grad_(True)
+    g, = torch.autograd.grad(pw().linear(leaf, w, b, act="silu"), leaf, dy)
+    step = 2.0 ** -4
+    for at in ((0, 0), (0, 23), (1, 9)):
+        up, down = x.clone(), x.clone()
+        up[at] += step
+        down[at] -= step
+        a, c = (pw().linear(t, w, b, act="silu").double() for t in (up, down))
+        D, W = dy[at[0]].double().abs(), w[:, at[1]].double().abs()
+        diff = ((a - c) * dy.double()).sum().item() / (2 * step)
+        # outputs' rounding; the difference's third-order term (silu's third derivative is below 0.4); dz's and the gradient's rounding
+        bound = ((D * (a.abs() + c.abs())[at[0]]).sum() * 2.0 ** -11 / (2 * step) + step ** 2 / 6 * 0.4 * (D * W ** 3).sum()
+                 + 1.13 * (D * W).sum() * (2.0 ** -11 + 2.0 ** -15) + abs(g[at].item()) * 2.0 ** -11 + 2.0 ** -20).item()
+        assert abs(diff - g[at].item()) <= bound
+
+
+def test_capture_over_a_transposed_weight_of_a_graph_that_is_alive_is_refused():
+    from selfc_amd import runtime as rt
+    w = torch.randn(32, 40).cuda().half().requires_grad_(True)
+    x = torch.randn(8, 32).cuda().half()
+    alive = pw().linear(x, w.t())
+    g = rt.new_graph()
+    with pytest.raises(RuntimeError, match="still alive"):
+        with rt.graph_capture(g, x.device):
+            pw().linear(x, w.t())
+    del alive
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# more than 2^31 values: only the last rows are not zeros
+# ---------------------------------------------------------------------------------------------------------------------
+def last_rows(gen, rows, cols):
+    part = rnd(gen, 3, cols, dtype=torch.bfloat16)
+    t = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    t[-3:] = part.cuda()
+    return t, part.cuda()
+
+
+def test_norm_offsets_past_32_bits():
+    gen = torch.Generator().manual_seed(21)
+    rows = 2 ** 25 + 5
+    (x, xs), (dy, dys) = last_rows(gen, rows, 64), last_rows(gen, rows, 64)
+    w = (rnd(gen, 64) + 1).cuda()
+    got, want = [], []
+    for a, d, out in ((x, dy, got), (xs, dys, want)):
+        a, b = a.requires_grad_(True), w.clone().requires_grad_(True)
+        y, _ = pw().rms_norm(a, b)
+        dx, dw = torch.autograd.grad(y, (a, b), d)
+        out += [y.detach()[-3:], dx[-3:], dw]
+        assert not y.detach()[:-3].any() and not dx[:-3].any()
+    for a, b in zip(got[:2], want[:2]):
+        assert torch.equal(a, b)
+    assert (got[2] - want[2]).abs().max() <= 4 * U32 * want[2].abs().max() * 3          # three rows, added in another order
+
+
+@pytest.mark.parametrize("rows,k,n", [(2 ** 25 + 5, 64, 64), (2 ** 21 + 3, 264, 1032), (2 ** 21 + 3, 1032, 264)])
+def test_product_offsets_past_32_bits(rows, k, n):
+    gen = torch.Generator().manual_seed(22)
+    (x, xs), (dy, dys) = last_rows(gen, rows, k), last_rows(gen, rows, n)
+    w = rnd(gen, n, k, scale=k ** -0.5, dtype=torch.bfloat16).cuda()
+    z, size, ref, d = product_ref(xs.cpu(), w.cpu(), None, None, "gelu")
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    y = pw().linear(x, w, act="gelu")
+    within(y[-3:], ref, product_bound(torch.bfloat16, k, z, size, ref))
+    assert not y.detach()[:-3].any()
+    gx, gw = torch.autograd.grad(y, (x, w), dy)
+    D, W, X, u16 = dys.double().cpu(), w.detach().double().cpu(), xs.detach().double().cpu(), u(torch.bfloat16)
+    dz = D * d
+    off = dz.abs() * u16 + D.abs() * (2.0 ** -16 + 2.0 ** -20 + (k + 10) * U32 * size)
+    for got, want, mag, err, terms in ((gx[-3:], dz @ W, dz.abs() @ W.abs(), off @ W.abs(), n), (gw, dz.t() @ X, dz.abs().t() @ X.abs(), off.t() @ X.abs(), 3)):
+        within(got, want, (want.abs() + err) * u16 * 1.01 + err + (terms + 10) * U32 * mag * 1.01 + TINY[torch.bfloat16])
+    assert not gx[:-3].any()

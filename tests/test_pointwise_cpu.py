@@ -92,6 +92,12 @@ def test_adamw_step_checks(monkeypatch):
     with pytest.raises(RuntimeError, match="betas"):
         optim.adamw_step([m(3)], [m(3)], m(256), m(256), beta1=1.0, **ok)
     optim.adamw_step([], [], m(0), m(0), **ok)
+    t, big = m(3), m(600)
+    for twice in ([t, t], [big[:300], big[299:]], [big, m(2), big[5:6]]):
+        with pytest.raises(RuntimeError, match="share memory"):
+            optim.adamw_step(twice, [x.clone() for x in twice], m(2048), m(2048), **ok)
+    with pytest.raises(RuntimeError, match="same memory"):
+        optim.adamw_step([t], [m(3)], big, big, **ok)
 
 
 def test_c_entries_refuse_without_launching():
