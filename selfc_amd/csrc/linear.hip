@@ -798,10 +798,14 @@ inline Plan gemm_plan(const int M, const int N, const int R, const int es) {
   const int stages = (int)(((long)R * es + 127) / 128);
   const auto tiles = [&](const int b) { return (long)((M + b - 1) / b) * ((N + b - 1) / b); };
   Plan p{256, 1, stages};
-  if (tiles(256) < 192 || stages < 4) p.tile = 128;
+  // Large tiles, one per compute unit at a time, where they fill the last round of the 256 units well (4096 x 4096 x 4096 in 256 of them: 106 us,
+  // 113 in tiles of 128; 8192 x 4096 x 4096 in 512: 211 and 235); not where a second round would be mostly empty (5120 x 4096 x 4096 in 320: 187 us, 164
+  // in tiles of 128).  From 1.5 rounds on the two differ by at most a few percent either way but for full rounds, which large tiles win.
+  const long large = tiles(256);
+  if (large < 192 || (large > 256 && large <= 384) || stages < 4) p.tile = 128;
   if (p.tile == 128 && tiles(128) < 192) p.tile = 64;
   const long t = tiles(p.tile);
-  if (t < 256 && stages > 8) {                     // too few tiles for 256 compute units: divide the sum, at least 4 stages a part
+  if (t < 256 && p.tile < 256 && stages > 8) {                     // too few tiles for 256 compute units: divide the sum, at least 4 stages a part
     long s = (512 + t - 1) / t;
     if (s > stages / 4) s = stages / 4;
     if (s > 256) s = 256;

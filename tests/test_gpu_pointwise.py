@@ -538,3 +538,33 @@ def test_product_offsets_past_32_bits(rows, k, n):
     for got, want, mag, err, terms in ((gx[-3:], dz @ W, dz.abs() @ W.abs(), off @ W.abs(), n), (gw, dz.t() @ X, dz.abs().t() @ X.abs(), off.t() @ X.abs(), 3)):
         within(got, want, (want.abs() + err) * u16 * 1.01 + err + (terms + 10) * U32 * mag * 1.01 + TINY[torch.bfloat16])
     assert not gx[:-3].any()
+
+
+@pytest.mark.parametrize("dt", T16)
+def test_all_three_products_in_large_tiles(dt):
+    """Every product of the layer fills the chip with large tiles, with odd sizes at every edge; the reference in 64 bits on the GPU."""
+    m, k, n = 3600, 3501, 3590
+    gen = torch.Generator().manual_seed(31)
+    x, w, b, dy = (t.cuda() for t in (rnd(gen, m, k, dtype=dt), rnd(gen, n, k, scale=k ** -0.5, dtype=dt), rnd(gen, n, dtype=dt), rnd(gen, m, n, dtype=dt)))
+    z, size, y, d = product_ref(x, w, b, None, "gelu")
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    out = pw().linear(leaves[0], leaves[1], bias=leaves[2], act="gelu")
+    within(out, y.cpu(), product_bound(dt, k, z, size, y).cpu())
+    grads = torch.autograd.grad(out, leaves, dy)
+    X, W, D = x.double(), w.double(), dy.double()
+    dz = D * d
+    off = dz.abs() * u(dt) + D.abs() * (2.0 ** -16 + 2.0 ** -20 + (k + 10) * U32 * size) + TINY[dt]
+    for got, want, mag, err, terms in ((grads[0], dz @ W, dz.abs() @ W.abs(), off @ W.abs(), n), (grads[1], dz.t() @ X, dz.abs().t() @ X.abs(), off.t() @ X.abs(), m),
+                                       (grads[2], dz.sum(0), dz.abs().sum(0), off.sum(0), m)):
+        within(got, want.cpu(), ((want.abs() + err) * u(dt) * 1.01 + err + (terms + 10) * U32 * mag * 1.01 + TINY[dt]).cpu())
+
+
+@pytest.mark.parametrize("m,k,n", [(3600, 1041, 3590), (3600, 512, 3590), (5000, 700, 4500)])
+def test_product_q8_of_many_tiles(m, k, n):
+    gen = torch.Generator().manual_seed(k)
+    q = rnd(gen, m, k, scale=30.0).clamp(-448, 448).to(torch.float8_e4m3fn).cuda()
+    xs = (torch.rand(m, generator=gen) * 0.01 + 0.001).cuda()
+    wq, ws = pw().quantize_rows(rnd(gen, n, k, scale=k ** -0.5).cuda())
+    r = rnd(gen, m, n, dtype=torch.bfloat16).cuda()
+    z, size, y, _ = product_ref(q.float(), wq.float(), None, r, "silu", (xs, ws))
+    within(pw().linear_q8(q, xs, wq, ws, act="silu", residual=r), y.cpu(), product_bound(torch.bfloat16, k, z, size, y).cpu())
