@@ -227,10 +227,18 @@ struct NormFn : torch::autograd::Function<NormFn> {
 };
 
 // ---- product -------------------------------------------------------------------------------------------------------------------
-bool narrow(const int64_t n, const int64_t k) { return n <= 256 && k <= 256 && api.selfc_linear_rows_ok((int)n, (int)k); }
+// Layers whose weight the rows' kernel holds in shared memory.  It reads any layout, so it takes all rows that would have to be laid out
+// first; of the others those whose number pays for every workgroup's copy of the weight: in f16, here and in tiles, 64 x 64 with 2,000 rows
+// 4.8 us, 5.1; 128 x 128 with 20,000 8.1, 7.2 and with 50,000 10.4, 11.9; 256 x 256 with 100,000 47.5, 40.2 and with 200,000 71.9, 76.4 (and their
+// gradients likewise)
+bool narrow(const Tensor& x, const Tensor& w) {
+  const int64_t n = w.size(0), k = w.size(1);
+  if (n > 256 || k > 256 || !api.selfc_linear_rows_ok((int)n, (int)k)) return false;
+  return !whole(x) || !whole(w) || n * k <= 4096 || x.size(0) >= 2 * n * k;
+}
 
 struct LinearOut { Tensor y, slope, xp; };          // xp: x as dW's product reads it
-// layers whose weight fits into shared memory: one launch, any layout of x and the weight
+// one launch, any layout of x and the weight
 LinearOut run_rows(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, const int act, const bool want_slope, const bool want_xp, void* const stream) {
   const int64_t rows = x.size(0), k = x.size(1), n = w.size(0);
   LinearOut o;
@@ -264,7 +272,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, const int64_t act, const int64_t stream) {
     const bool to_x = x.requires_grad(), to_w = w.requires_grad(), to_b = b && b->requires_grad();
     void* const s = reinterpret_cast<void*>(stream);
-    const bool slope = act != 0 && (to_x || to_w || to_b), small = narrow(w.size(0), w.size(1));
+    const bool slope = act != 0 && (to_x || to_w || to_b), small = narrow(x, w);
     Tensor wp = w;
     const LinearOut o = small ? run_rows(x, w, b.value_or(Tensor()), r.value_or(Tensor()), (int)act, slope, to_w, s)
                               : run_tiles(x, w, Tensor(), Tensor(), b.value_or(Tensor()), r.value_or(Tensor()), (int)act, x.scalar_type(), slope, s, wp);
@@ -367,7 +375,7 @@ PyObject* linear(PyObject*, PyObject* args) {
     const Tensor &x = THPVariable_Unpack(x_), &w = THPVariable_Unpack(w_);
     if (grad) return wrap(LinearFn::apply(x, w, maybe(b), maybe(r), (int64_t)act, (int64_t)stream));
     void* const s = reinterpret_cast<void*>(stream);
-    if (narrow(w.size(0), w.size(1))) return wrap(run_rows(x, w, tensor(b), tensor(r), act, false, false, s).y);
+    if (narrow(x, w)) return wrap(run_rows(x, w, tensor(b), tensor(r), act, false, false, s).y);
     Tensor wp;
     return wrap(run_tiles(x, w, Tensor(), Tensor(), tensor(b), tensor(r), act, x.scalar_type(), false, s, wp).y);
   });
