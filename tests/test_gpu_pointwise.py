@@ -592,3 +592,15 @@ def test_product_of_few_rows_and_long_sums(dt, m, k, n):
 def test_product_of_narrow_rows_in_whole_pieces(dt, m, k, n):
     """On both sides of where such layers go from tiles to the kernel that keeps their weight in shared memory."""
     test_product_of_many_tiles(dt, m, k, n)
+
+
+@pytest.mark.parametrize("shape,n", [((0, 301), 700), ((2, 0, 301), 24), ((0, 1000), 1001)])
+def test_wide_product_without_rows(shape, n):
+    k = shape[-1]
+    x, w, b = (torch.zeros(*s, dtype=torch.bfloat16).cuda().requires_grad_(True) for s in (shape, (n, k), (n,)))
+    y = pw().linear(x, w, bias=b, act="silu", residual=torch.zeros(*shape[:-1], n, dtype=torch.bfloat16).cuda())
+    y.sum().backward()
+    assert y.shape == shape[:-1] + (n,) and not w.grad.any() and not b.grad.any() and x.grad.shape == shape
+    q, s, _ = pw().rms_norm_q8(x.detach(), torch.ones(k).cuda())
+    wq, ws = pw().quantize_rows(w.detach())
+    assert s.shape == shape[:-1] and pw().linear_q8(q, s, wq, ws).shape == y.shape

@@ -115,6 +115,7 @@ def test_c_entries_refuse_without_launching():
     assert L.selfc_linear_ws_floats(64, 64, 8192, 2) > 0 and L.selfc_linear_ws_floats(0, 64, 64, 2) == 0
     assert L.selfc_linear_dw(one, 8, one, 8, one, None, None, 0, 8, 8, 2, None) == -1
     assert L.selfc_pack_rows(one, 5, one, 2, 5, 7, 2, None) == -1
+    assert L.selfc_pack_rows(None, 5, None, 0, 5, 8, 2, None) == 0                                       # no rows: no memory either
     assert L.selfc_adamw_block() == optim.BLOCK
 
 
