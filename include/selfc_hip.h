@@ -449,7 +449,7 @@ int selfc_rmsnorm_bwd(const void* h, size_t ldh, const void* w, int w_f32, const
  * x_scale[rows] and w_scale[n] multiply the sums; out_dtype 0..2).  act: 0 none, 1 ReLU, 2 LeakyReLU(0.2), 3 GELU (erf), 4 SiLU.
  * bias, res: out_dtype or NULL.  x and w: 16-byte aligned, pitch and k whole 16-byte pieces (selfc_pack_rows makes such rows of any
  * others).  slope (or NULL): u16 [rows][roundup(n, 8)], receives act' for selfc_linear_dz.  ws: selfc_linear_ws_floats(rows, n, k,
- * bytes of in_dtype) floats. */
+ * bytes of in_dtype) floats.  e4m3: the matrix unit cuts products below 2^-13 of the largest of eight neighbours; the rest is fp32. */
 size_t selfc_linear_ws_floats(size_t rows, int cols, int sum, int elem_bytes);
 int selfc_pack_rows(const void* src, size_t ld, void* dst, size_t rows, int cols, int ldd, int elem_bytes, void* stream);
 int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const float* x_scale, const float* w_scale, const void* bias, int act,
@@ -475,7 +475,7 @@ int selfc_linear_rows_bwd(const void* dy, size_t lddy, const void* slope, const 
                           size_t rows, int n, int k, int dtype, void* stream);
 
 /* csrc/adamw.hip.  One AdamW step of `count` tensors (a HOST array; it is read before the call returns) of one `dtype`.  A tensor
- * without a gradient is left as it is.  State: m and v hold all tensors, tensor i from the sum of roundup(n_j, selfc_adamw_block())
+ * without a gradient is left as it is; no two tensors may share memory.  State: m and v hold all tensors, tensor i from the sum of roundup(n_j, selfc_adamw_block())
  * over j < i on; state_bits 32: fp32; 8: e4m3 (m) and e5m2 (v) with one power-of-two step per block in m_scale / v_scale.
  * step: this step's number, from 1 on, or a device fp32 scalar per tensor; lr likewise.  norm (device, selfc_grad_norm) with max_norm:
  * gradients are scaled by min(1, max_norm / (norm + 1e-6)); the gradients themselves are not written.  seed: of the 8-bit dither. */

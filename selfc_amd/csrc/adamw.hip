@@ -20,7 +20,8 @@
 //
 // Bound: memory (28 bytes a value in 32 bits; 16 in 8 bits with fp32 tensors, 10 with 16-bit ones), as long as the 8-bit form stays below
 // about 100 vector instructions a value: its first form, with every value's end-of-tensor check and general rounding, took 106 and
-// was bound by them.
+// was bound by them (134 M bf16 values: 382 us).  Measured for 134 M values in 20 tensors: 32 bits with fp32 tensors 707 us (3.76 GB, 5.3 TB/s, a
+// large copy's rate), 8 bits with bf16 ones 250 us (1.35 GB, 5.4 TB/s); a single layer's five tensors 3.7 us.
 #include "pointwise.hpp"
 #include <math.h>
 

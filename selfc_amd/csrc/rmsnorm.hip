@@ -7,11 +7,13 @@
 //
 // Bound: memory.  A row is read once into registers, eight values per lane and load, and everything that is summed over it is a
 // butterfly over the lanes that share it: the smallest power of two of lanes (8..64) that covers the row, so narrow rows (64
-// channels: 8 lanes) leave no lane idle, up to 2,048 values; a workgroup of 256 up to 16,384.  dw: a workgroup keeps its columns'
-// sums in registers over all of its rows and writes one row of partial sums; a second launch adds them in a fixed order (no
-// atomics: the same bits every time).
+// channels: 8 lanes) leave no lane idle, up to 2,048 values; a workgroup of 256 up to 16,384.  The backward pass holds two rows
+// (h and dy), the next ones' and dw's sums as well, so its rows go to a workgroup from 1,024 values on (256, 512, 1,024 lanes: more lanes, not
+// more values per lane, which would spill).  dw: a workgroup keeps its columns' sums in registers over all of its rows and writes
+// one row of partial sums; a second launch adds them in a fixed order (no atomics: the same bits every time).
+// Measured (a large copy: 5.15 TB/s): 8,192 rows of 4,096 in bf16 with residual, forward 44 us (268 MB, 6.1 TB/s: part of the input is still in the
+// last cache), backward 63 us (268 MB and 17 MB of partial sums) + 5 for their sum; 200,704 rows of 64 in f16, 21, 23.5 and 4 us (103 MB each way).
 #include "pointwise.hpp"
-#include "prof.hpp"
 
 namespace selfc {
 namespace {
