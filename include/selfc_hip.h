@@ -448,16 +448,17 @@ int selfc_rmsnorm_bwd(const void* h, size_t ldh, const void* w, int w_f32, const
 /* csrc/linear.hip.  y[rows][n] = act(x w^T + bias) + res; x [rows][k], w [n][k] of in_dtype bf16 / f16 (out_dtype the same) or e4m3 (then
  * x_scale[rows] and w_scale[n] multiply the sums; out_dtype 0..2).  act: 0 none, 1 ReLU, 2 LeakyReLU(0.2), 3 GELU (erf), 4 SiLU.
  * bias, res: out_dtype or NULL.  x and w: 16-byte aligned, pitch and k whole 16-byte pieces (selfc_pack_rows makes such rows of any
- * others).  slope (or NULL): u16 [rows][roundup(n, 8)], receives act' for selfc_linear_dz.  ws: selfc_linear_ws_floats(rows, n, k,
+ * others).  slope (or NULL): receives act' for selfc_linear_dz: ReLU, LeakyReLU bits [rows][roundup(n, 8) / 8 bytes], others u16
+ * [rows][roundup(n, 8)], 16-byte aligned.  ws: selfc_linear_ws_floats(rows, n, k,
  * bytes of in_dtype) floats.  e4m3: the matrix unit cuts products below 2^-13 of the largest of eight neighbours; the rest is fp32. */
 size_t selfc_linear_ws_floats(size_t rows, int cols, int sum, int elem_bytes);
 int selfc_pack_rows(const void* src, size_t ld, void* dst, size_t rows, int cols, int ldd, int elem_bytes, void* stream);
 int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const float* x_scale, const float* w_scale, const void* bias, int act,
                  const void* res, size_t ldr, void* y, void* slope, float* ws, size_t rows, int n, int k, int in_dtype, int out_dtype, void* stream);
-/* dz = dy * slope (slope NULL: dy) into rows of pitch lddz = roundup(n, 8) with zeros behind them, and / or db = its column sums;
+/* dz = dy * slope (slope NULL: dy; act: whose slope it is) into rows of pitch lddz = roundup(n, 8) with zeros behind them, and / or db = its column sums;
  * partial: selfc_linear_dz_floats floats (only with db). */
 size_t selfc_linear_dz_floats(size_t rows, int n);
-int selfc_linear_dz(const void* dy, size_t lddy, const void* slope, void* dz, size_t lddz, void* db, float* partial, size_t rows, int n, int dtype, void* stream);
+int selfc_linear_dz(const void* dy, size_t lddy, const void* slope, int act, void* dz, size_t lddz, void* db, float* partial, size_t rows, int n, int dtype, void* stream);
 /* dx[rows][k] = dz w; dw[n][k] = dz^T x and db[n] (or NULL) = dz's column sums.  dz, w, x 16-byte aligned with pitches of whole 16-byte
  * pieces, zeros in dz behind column n.  ws: selfc_linear_ws_floats(rows, k, n, 2) and selfc_linear_dw_floats floats.  rows >= 1 for dw. */
 int selfc_linear_dx(const void* dz, size_t lddz, const void* w, size_t ldw, void* dx, float* ws, size_t rows, int n, int k, int dtype, void* stream);
@@ -466,12 +467,12 @@ int selfc_linear_dw(const void* dz, size_t lddz, const void* x, size_t ldx, void
 
 /* Narrow layers (selfc_linear_rows_ok(n, k): up to 256 each way, their weight in shared memory): bf16 / f16 rows and weights of any pitch and
  * offset.  y without gaps, slope as above, xp (or NULL): receives x's rows with pitch roundup(k, 8) and zeros behind them (selfc_linear_dw's
- * operand).  The backward call makes dx [rows][k] and dz (or NULL; as selfc_linear_dz) from dy and slope (or NULL: no activation).
- * slope, xp, dz 16-byte aligned. */
+ * operand).  The backward call makes dx [rows][k] and dz (or NULL; as selfc_linear_dz) from dy and slope (or NULL: no activation)
+ * of act.  xp, dz 16-byte aligned. */
 int selfc_linear_rows_ok(int n, int k);
 int selfc_linear_rows(const void* x, size_t ldx, const void* w, size_t ldw, const void* bias, int act, const void* res, size_t ldr, void* y,
                       void* slope, void* xp, size_t rows, int n, int k, int dtype, void* stream);
-int selfc_linear_rows_bwd(const void* dy, size_t lddy, const void* slope, const void* w, size_t ldw, void* dx, void* dz,
+int selfc_linear_rows_bwd(const void* dy, size_t lddy, const void* slope, int act, const void* w, size_t ldw, void* dx, void* dz,
                           size_t rows, int n, int k, int dtype, void* stream);
 
 /* csrc/adamw.hip.  One AdamW step of `count` tensors (a HOST array; it is read before the call returns) of one `dtype`.  A tensor

@@ -176,10 +176,10 @@ def lib():
             "selfc_rmsnorm_bwd": [vp, sz, vp, i, vp, vp, vp, vp, vp, sz, i, i, f, vp],
             "selfc_pack_rows": [vp, sz, vp, sz, i, i, i, vp],
             "selfc_linear": [vp, sz, vp, sz, vp, vp, vp, i, vp, sz, vp, vp, vp, sz, i, i, i, i, vp],
-            "selfc_linear_dz": [vp, sz, vp, vp, sz, vp, vp, sz, i, i, vp],
+            "selfc_linear_dz": [vp, sz, vp, i, vp, sz, vp, vp, sz, i, i, vp],
             "selfc_linear_rows_ok": [i, i],
             "selfc_linear_rows": [vp, sz, vp, sz, vp, i, vp, sz, vp, vp, vp, sz, i, i, i, vp],
-            "selfc_linear_rows_bwd": [vp, sz, vp, vp, sz, vp, vp, sz, i, i, i, vp],
+            "selfc_linear_rows_bwd": [vp, sz, vp, i, vp, sz, vp, vp, sz, i, i, i, vp],
             "selfc_linear_dx": [vp, sz, vp, sz, vp, vp, sz, i, i, i, vp],
             "selfc_linear_dw": [vp, sz, vp, sz, vp, vp, vp, sz, i, i, i, vp],
             "selfc_adamw_block": [],

@@ -237,13 +237,17 @@ bool narrow(const Tensor& x, const Tensor& w) {
   return !whole(x) || !whole(w) || n * k <= 4096 || x.size(0) >= 2 * n * k;
 }
 
+// room for the activation's derivative: a bit per value of ReLU and LeakyReLU, 16 bits of the others
+Tensor kept(const Tensor& like, const int64_t rows, const int64_t n, const int act) {
+  return act == 1 || act == 2 ? empty(like, {rows, up8(n) / 8}, at::kByte) : empty(like, {rows, up8(n)}, at::kShort);
+}
 struct LinearOut { Tensor y, slope, xp; };          // xp: x as dW's product reads it
 // one launch, any layout of x and the weight
 LinearOut run_rows(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& r, const int act, const bool want_slope, const bool want_xp, void* const stream) {
   const int64_t rows = x.size(0), k = x.size(1), n = w.size(0);
   LinearOut o;
   o.y = empty(x, {rows, n}, x.scalar_type());
-  if (want_slope) o.slope = empty(x, {rows, up8(n)}, at::kShort);
+  if (want_slope) o.slope = kept(x, rows, n, act);
   const bool as_is = !want_xp || whole(x);
   if (want_xp) o.xp = as_is ? x : empty(x, {rows, up8(k)}, x.scalar_type());
   if (rows)
@@ -256,7 +260,7 @@ LinearOut run_tiles(const Tensor& x, const Tensor& w, const Tensor& xs, const Te
   const int64_t rows = x.size(0), n = w.size(0), es = x.element_size(), k = (x.size(1) * es + 15) / 16 * 16 / es;
   LinearOut o;
   o.y = empty(x, {rows, n}, out);
-  if (want_slope) o.slope = empty(x, {rows, up8(n)}, at::kShort);
+  if (want_slope) o.slope = kept(x, rows, n, act);
   o.xp = pieces(x, stream);
   wp = pieces(w, stream);
   if (rows) {
@@ -267,7 +271,7 @@ LinearOut run_tiles(const Tensor& x, const Tensor& w, const Tensor& xs, const Te
   return o;
 }
 
-// kept for the backward pass: x as the kernels read it, the weight, and the activation's derivative as 16-bit fixed point
+// kept for the backward pass: x as the kernels read it, the weight, and the activation's derivative
 struct LinearFn : torch::autograd::Function<LinearFn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& b, const OptTensor& r, const int64_t act, const int64_t stream) {
     const bool to_x = x.requires_grad(), to_w = w.requires_grad(), to_b = b && b->requires_grad();
@@ -276,7 +280,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     Tensor wp = w;
     const LinearOut o = small ? run_rows(x, w, b.value_or(Tensor()), r.value_or(Tensor()), (int)act, slope, to_w, s)
                               : run_tiles(x, w, Tensor(), Tensor(), b.value_or(Tensor()), r.value_or(Tensor()), (int)act, x.scalar_type(), slope, s, wp);
-    ctx->saved_data["dims"] = std::vector<int64_t>{x.size(0), w.size(0), x.size(1), (int64_t)small, stream, b ? 1 : 0, r ? 1 : 0};
+    ctx->saved_data["dims"] = std::vector<int64_t>{x.size(0), w.size(0), x.size(1), (int64_t)small, stream, b ? 1 : 0, r ? 1 : 0, act};
     ctx->save_for_backward({to_w ? o.xp : Tensor(), to_x ? wp : Tensor(), o.slope});
     return o.y;
   }
@@ -306,12 +310,12 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     const bool as_is = !slope.defined() && whole(g), rows_kernel = to_x && small, make = !as_is && (to_w || (to_x && !rows_kernel));
     const Tensor dz = make ? empty(dy, {rows, up}, t) : g;
     if (rows_kernel)
-      check(api.selfc_linear_rows_bwd(g.data_ptr(), pitch(g), ptr(slope), wp.data_ptr(), pitch(wp), dx.data_ptr(), make ? dz.data_ptr() : nullptr, rows, (int)n,
+      check(api.selfc_linear_rows_bwd(g.data_ptr(), pitch(g), ptr(slope), (int)d[7], wp.data_ptr(), pitch(wp), dx.data_ptr(), make ? dz.data_ptr() : nullptr, rows, (int)n,
                                       (int)k, c, s), "selfc_linear_rows_bwd");
     const bool alone = to_b && !to_w;       // with dW, db comes out of that product
     if (alone || (make && !rows_kernel)) {
       const Tensor part = alone ? work(dy, api.selfc_linear_dz_floats(rows, (int)n)) : Tensor();
-      check(api.selfc_linear_dz(g.data_ptr(), pitch(g), ptr(slope), make && !rows_kernel ? dz.data_ptr() : nullptr, up, alone ? db.data_ptr() : nullptr, floats(part),
+      check(api.selfc_linear_dz(g.data_ptr(), pitch(g), ptr(slope), (int)d[7], make && !rows_kernel ? dz.data_ptr() : nullptr, up, alone ? db.data_ptr() : nullptr, floats(part),
                                 rows, (int)n, c, s), "selfc_linear_dz");
     }
     if (to_x && !rows_kernel) {

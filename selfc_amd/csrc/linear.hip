@@ -8,9 +8,10 @@
 // of the forward product) or with r as its row index ("crossed": W in dx, both in dW), and the latter is transposed on the way
 // from shared memory to registers (ds_read_b64_tr_b16), never in memory.
 //
-// The derivative act'(z) is kept for the backward pass as a 16-bit fixed-point number (steps of 2^-15 from -0.5; 65535: not a
-// number): every activation here has its derivative in [-0.13, 1.13], 0 and 1 are exact, and the error 2^-16 is 1/128 of
-// what keeping z in bf16 would cost - after it the backward pass needs neither z nor the activation's formula.
+// The derivative act'(z) is kept for the backward pass: of ReLU and LeakyReLU one bit per value (z > 0), of the others a 16-bit
+// fixed-point number (steps of 2^-15 from -0.5; 65535: not a number): their derivatives lie in [-0.13, 1.13], 0 and 1 are exact, and the
+// error 2^-16 is 1/128 of what keeping z in bf16 would cost - after it the backward pass needs neither z nor the activation's formula.
+// (Bits against codes: a layer of 200,704 x 128 x 128 in f16 with its gradients 94 us, 119; of 72,576 x 204 x 51 58, 73.)
 //
 // Four forms, chosen by the rules beside gemm_plan, gemv_takes and rows_plan below (and, between the last two, by the caller): tiles that meet in
 // shared memory (bound by the matrix units), the weight straight into registers for few rows (bound by the weight's bytes), the whole weight
@@ -28,6 +29,8 @@ int pw_colsum(const float* partial, int rows, int C, int dtype, void* out, hipSt
 namespace {
 
 enum { ACT_NONE, ACT_RELU, ACT_LRELU, ACT_GELU, ACT_SILU };
+constexpr float LRELU = 0.2f;
+__host__ __device__ inline bool act_bits(const int act) { return act == ACT_RELU || act == ACT_LRELU; }
 
 typedef h16 h16x8 __attribute__((ext_vector_type(8)));
 typedef b16 b16x8 __attribute__((ext_vector_type(8)));
@@ -40,7 +43,7 @@ struct Epilogue {
   void* out;                      // [M][ldo] of `dtype`
   const void *bias, *res;         // [N]; [M][ldr]
   const float *qs, *ps;           // scales of the rows and of the columns
-  unsigned short* d;              // [M][ldd] derivative
+  unsigned char* d;               // [M][ldd bytes] derivative: bits, eight neighbouring columns to a byte, or 16-bit codes
   size_t ldo, ldr, ldd;
   int dtype, act;
 };
@@ -57,7 +60,7 @@ __device__ __forceinline__ void act_apply(const int act, const float* const z, f
     for (int i = 0; i < N; ++i) { y[i] = z[i] <= 0.f ? 0.f : z[i]; if (D) d[i] = z[i] > 0.f ? 1.f : 0.f; }        // a NaN stays one
   } else if (act == ACT_LRELU) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) { const float s = z[i] > 0.f ? 1.f : 0.2f; y[i] = z[i] * s; if (D) d[i] = s; }
+    for (int i = 0; i < N; ++i) { const float s = z[i] > 0.f ? 1.f : LRELU; y[i] = z[i] * s; if (D) d[i] = s; }
   } else if (act == ACT_GELU) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -92,6 +95,11 @@ __device__ __forceinline__ float act_slope(const unsigned c) {
   return c == 65535u ? __builtin_nanf("") : (float)((int)c - 16384) * 0x1p-15f;
 }
 
+// dy times the derivative that a bit stands for; under a 0 of ReLU nothing comes through, whatever dy is
+__device__ __forceinline__ float bit_slope(const float dy, const unsigned bits, const int i, const float low) {
+  return bits >> i & 1 ? dy : low == 0.f ? 0.f : dy * low;
+}
+
 __device__ __forceinline__ void load8_as(const int dtype, const void* const p, const size_t at, const int left, const int before, float* const v) {
   if (dtype == 0) load8((const float*)p + at, left, before, v);
   else if (dtype == 1) load8((const b16*)p + at, left, before, v);
@@ -105,14 +113,20 @@ __device__ __forceinline__ void epilogue8(const Epilogue& e, const float* const 
   const float qs = e.qs ? e.qs[row] : 1.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) z[i] = (e.qs ? acc[i] * (qs * ps[i]) : acc[i]) + b[i];
-  if (e.d) {
+  if (e.d && !act_bits(e.act)) {
     act_apply<8, true>(e.act, z, y, d);
     u16x8 c;
 #pragma unroll
     for (int i = 0; i < 8; ++i) c[i] = (unsigned short)act_code(d[i], z[i]);
-    *reinterpret_cast<u16x8*>(e.d + (size_t)row * e.ldd + col) = c;          // ldd is a multiple of 8: always 16 bytes at a time
+    *reinterpret_cast<u16x8*>(e.d + (size_t)row * e.ldd + col * 2) = c;      // a row holds a multiple of 8: always 16 bytes at a time
   } else {
     act_apply<8, false>(e.act, z, y, d);
+    if (e.d) {
+      unsigned c = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c |= (z[i] > 0.f ? 1u : 0u) << i;
+      e.d[(size_t)row * e.ldd + col / 8] = (unsigned char)c;
+    }
   }
   if (e.res) {
     load8_as(e.dtype, e.res, (size_t)row * e.ldr + col, left, col, r);
@@ -581,7 +595,8 @@ __global__ __launch_bounds__(512) void gemv_kernel(const GemmArgs a) {
 // Shared memory: the weight as [TP * 16 columns][KS * 32 places], 16 bytes between rows that keep 16 rows' pieces in different banks.
 struct RowsArgs {
   const void *x, *w;
-  const unsigned short* d;        // backward: derivative [rows][ldd], or NULL
+  const unsigned char* d;         // backward: derivative [rows][ldd bytes], or NULL
+  float low;                      // and the derivative that a 0 bit stands for
   void* xp;                       // NULL, or the operand's rows with pitch roundup(K, 8) and zeros behind them
   size_t ldx, ldw, ldd, rows;
   int N, K;
@@ -609,8 +624,10 @@ __device__ __forceinline__ void apart(const u32x4 r, u32x2* const t) {
     t[1][k] = b[1];
   }
 }
-template <typename T, int KS, bool BWD, int NW>
+enum { ROWS_FWD, ROWS_FWD_KEEP, ROWS_BWD, ROWS_BWD_BITS };       // forward; and the derivative; backward with it as codes (or none), as bits
+template <typename T, int KS, int MODE, int NW>
 __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
+  constexpr bool BWD = MODE >= ROWS_BWD, BITS = MODE == ROWS_BWD_BITS, KEEP = MODE == ROWS_FWD_KEEP;
   constexpr int PITCH = KS * 64 + 16, NT = NW * 64;
   typedef T T8 __attribute__((ext_vector_type(8)));
   typedef T T4 __attribute__((ext_vector_type(4)));
@@ -640,13 +657,16 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
     const size_t row0 = t * 16, row = row0 + q;
     const bool in = row < a.rows;
     i32x4 xf[KS];
-    u16x8 dv[BWD ? KS : 1];
+    u16x8 dv[BWD && !BITS ? KS : 1];
+    unsigned char db[BITS ? KS : 1];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int c = ks * 32 + g * 8;
       xf[ks] = __builtin_bit_cast(i32x4, raw8((const T*)a.x + row * a.ldx + c, in ? K - c : 0, c));
-      if constexpr (BWD) {
-        if (a.d && in && c < kp) dv[ks] = *reinterpret_cast<const u16x8*>(a.d + row * a.ldd + c);
+      if constexpr (BITS) {
+        db[ks] = in && c < kp ? a.d[row * a.ldd + c / 8] : (unsigned char)0;
+      } else if constexpr (BWD) {
+        if (a.d && in && c < kp) dv[ks] = *reinterpret_cast<const u16x8*>(a.d + row * a.ldd + c * 2);
       }
     }
 #pragma unroll
@@ -658,7 +678,8 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           float v = (float)h[i];
-          v = in && c + i < K ? v * act_slope(dv[ks][i]) : 0.f;
+          if constexpr (BITS) v = bit_slope(v, db[ks], i, a.low);             // behind row and column ends v is 0
+          else v = in && c + i < K ? v * act_slope(dv[ks][i]) : 0.f;
           r[i] = (T)v;
         }
         xf[ks] = __builtin_bit_cast(i32x4, r);
@@ -697,11 +718,12 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
             float z[4], d[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) z[i] = acc[pp + h][i] + b[i];
-            if (a.e.d) {
+            if (KEEP && !act_bits(a.e.act)) {
               act_apply<4, true>(a.e.act, z, y, d);
               cp[h] = u32x2{act_code(d[0], z[0]) | act_code(d[1], z[1]) << 16, act_code(d[2], z[2]) | act_code(d[3], z[3]) << 16};
             } else {
               act_apply<4, false>(a.e.act, z, y, d);
+              if (KEEP) cp[h] = u32x2{(z[0] > 0.f ? 1u : 0u) | (z[1] > 0.f ? 2u : 0u) | (z[2] > 0.f ? 4u : 0u) | (z[3] > 0.f ? 8u : 0u), 0u};
             }
             if (a.e.res) {
               const T4 v = __builtin_bit_cast(T4, rp[h]);
@@ -711,9 +733,13 @@ __global__ __launch_bounds__(NW * 64) void rows_kernel(const RowsArgs a) {
           }
           yp[h] = __builtin_bit_cast(u32x2, T4{(T)y[0], (T)y[1], (T)y[2], (T)y[3]});
         }
-        if (!BWD && a.e.d) {
+        if (KEEP) {
           const u32x4 c = joined(cp);
-          if (in && col8 < (int)a.e.ldd) *reinterpret_cast<u32x4*>(a.e.d + row * a.e.ldd + col8) = c;
+          unsigned char* const kept = a.e.d + row * a.e.ldd;
+          if (in && left > 0) {
+            if (act_bits(a.e.act)) kept[col8 / 8] = (unsigned char)(c[0] | c[2] << 4);
+            else *reinterpret_cast<u32x4*>(kept + col8 * 2) = c;
+          }
         }
         const u32x4 o = joined(yp);
         unsigned short* const out = (unsigned short*)a.e.out + row * N + col8;
@@ -747,13 +773,14 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(const T* const src, cons
 // Bound: memory (8192 x 8192 bf16: 403 MB in 75 us, 5.4 TB/s).
 struct DzArgs {
   const void* dy;
-  const unsigned short* d;        // or NULL: no activation
+  const unsigned char* d;         // [rows][ldd bytes], or NULL: no activation
+  float low;                      // what a 0 bit stands for
   void* dz;                       // or NULL: only the sums
   float* partial;                 // [gridDim.y][N] or NULL
   size_t rows, lddy, ldd, lddz;
   int N;
 };
-template <typename T, int L, bool WHOLE>
+template <typename T, int L, bool WHOLE, bool BITS>
 __global__ __launch_bounds__(256) void dz_kernel(const DzArgs a) {
   constexpr int G = 256 / L;
   const int lane = threadIdx.x & (L - 1), grp = threadIdx.x / L;
@@ -764,19 +791,25 @@ __global__ __launch_bounds__(256) void dz_kernel(const DzArgs a) {
     const size_t step = (size_t)gridDim.y * G;
     for (size_t row = (size_t)blockIdx.y * G + grp; row < a.rows; row += U * step) {
       float v[U][8];
-      u16x8 c[U];
+      u16x8 c[BITS ? 1 : U];
+      unsigned char bits[BITS ? U : 1];
 #pragma unroll
       for (int k = 0; k < U; ++k)
         if (row + k * step < a.rows) {
           load8((const T*)a.dy + (row + k * step) * a.lddy + col, left, col, v[k]);
-          if (a.d) c[k] = *reinterpret_cast<const u16x8*>(a.d + (row + k * step) * a.ldd + col);
+          if constexpr (BITS) bits[k] = a.d[(row + k * step) * a.ldd + col / 8];
+          else if (a.d) c[k] = *reinterpret_cast<const u16x8*>(a.d + (row + k * step) * a.ldd + col * 2);
         }
 #pragma unroll
       for (int k = 0; k < U; ++k)
         if (row + k * step < a.rows) {
-          if (a.d)
+          if constexpr (BITS) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[k][i] = bit_slope(v[k][i], bits[k], i, a.low);           // 0 behind the last column
+          } else if (a.d) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[k][i] = i < left ? v[k][i] * act_slope(c[k][i]) : 0.f;
+          }
 #pragma unroll
           for (int i = 0; i < 8; ++i) sum[i] += v[k][i];
           if (a.dz) store8((T*)a.dz + (row + k * step) * a.lddz + col, 8, v[k]);           // zeros behind the last column
@@ -831,6 +864,9 @@ inline Plan gemm_plan(const int M, const int N, const int R, const int es) {
   return p;
 }
 inline size_t up8(const size_t n) { return (n + 7) & ~(size_t)7; }
+inline size_t slope_bytes(const int n, const int act) { return act_bits(act) ? up8(n) / 8 : up8(n) * 2; }      // of a row's kept derivative
+inline bool slope_ok(const void* const slope, const int act) { return !slope || act_bits(act) || aligned_to(slope, 16); }
+inline float slope_low(const int act) { return act == ACT_LRELU ? LRELU : 0.f; }
 
 template <typename T, bool QX, bool PX, int BQ, int BP, int NQ, int NP>
 hipError_t gemm_go(const GemmArgs& a, hipStream_t s) {
@@ -880,7 +916,7 @@ inline RowsPlan rows_plan(const int N, const int K) {
   return p;
 }
 inline bool rows_ok(const int n, const int k) { return n <= ROWS_MAX && k <= ROWS_MAX; }        // 133 KiB at most: it fits
-template <typename T, bool BWD>
+template <typename T, int MODE>
 int rows_run(RowsArgs a, hipStream_t s) {
   const RowsPlan p = rows_plan(a.N, a.K);
   // workgroups that the chip holds at a time, each with its copy of the weight, or as many as there are tiles for
@@ -889,9 +925,9 @@ int rows_run(RowsArgs a, hipStream_t s) {
 #define ROWS(KS, NW)                                                                                                              \
   {                                                                                                                               \
     static std::atomic<unsigned long long> optin{0};                                                                              \
-    const void* const fn = reinterpret_cast<const void*>(&rows_kernel<T, KS, BWD, NW>);                                           \
+    const void* const fn = reinterpret_cast<const void*>(&rows_kernel<T, KS, MODE, NW>);                                           \
     if (const hipError_t e = lds_optin(fn, 160 * 1024, optin); e != hipSuccess) return pw_rc(e);                                  \
-    hipLaunchKernelGGL((rows_kernel<T, KS, BWD, NW>), grid, blk, p.lds, s, a);                                                    \
+    hipLaunchKernelGGL((rows_kernel<T, KS, MODE, NW>), grid, blk, p.lds, s, a);                                                    \
   }
   if (p.ks == 2 && p.nw == 4) ROWS(2, 4)
   else if (p.ks == 2) ROWS(2, 8)
@@ -954,14 +990,14 @@ int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const flo
   if (rows == 0) return SELFC_OK;
   if (!x || !w || !y || !lin_shape(rows, n, k) || act < ACT_NONE || act > ACT_SILU || in_dtype < 1 || in_dtype > 3 || out_dtype < 0 || out_dtype > 2) return SELFC_EINVAL;
   const bool q8 = in_dtype == 3;
-  if (q8 != (x_scale != nullptr) || q8 != (w_scale != nullptr) || (!q8 && in_dtype != out_dtype) || (slope && q8)) return SELFC_EINVAL;
+  if (q8 != (x_scale != nullptr) || q8 != (w_scale != nullptr) || (!q8 && in_dtype != out_dtype) || (slope && q8) || !slope_ok(slope, act)) return SELFC_EINVAL;
   const size_t es = q8 ? 1 : 2;
   if (!rows_fit(x, ldx, k, es) || !rows_fit(w, ldw, k, es)) return SELFC_EINVAL;                 // selfc_pack_rows first
   if ((rows > 1 && ldx < (size_t)k) || (n > 1 && ldw < (size_t)k) || (res && rows > 1 && ldr < (size_t)n)) return SELFC_EINVAL;
   GemmArgs a{};
   a.q = x; a.p = w; a.ldq = ldx; a.ldp = ldw; a.M = (int)rows; a.N = n; a.R = k; a.ws = ws;
   a.e = make_epilogue(y, n, bias, res, ldr, out_dtype, act);
-  a.e.qs = x_scale; a.e.ps = w_scale; a.e.d = (unsigned short*)slope; a.e.ldd = up8(n);
+  a.e.qs = x_scale; a.e.ps = w_scale; a.e.d = (unsigned char*)slope; a.e.ldd = slope_bytes(n, act);
   hipStream_t s = (hipStream_t)stream;
   if (gemv_takes(rows, n, k, es)) {
     a.splits = 1;
@@ -977,26 +1013,32 @@ int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const flo
 
 size_t selfc_linear_dz_floats(size_t rows, int n) { return n < 1 ? 1 : (size_t)(dz_groups(rows, n) + 1) * n; }
 
-int selfc_linear_dz(const void* dy, size_t lddy, const void* slope, void* dz, size_t lddz, void* db, float* partial, size_t rows, int n, int dtype, void* stream) {
+int selfc_linear_dz(const void* dy, size_t lddy, const void* slope, int act, void* dz, size_t lddz, void* db, float* partial, size_t rows, int n, int dtype, void* stream) {
   if (!dy || n < 1 || (dtype != 1 && dtype != 2) || (db && !partial) || (!dz && !db) || rows > 0x3fffffff) return SELFC_EINVAL;
   if (dz && (!aligned_to(dz, 16) || lddz % 8 || lddz < up8(n))) return SELFC_EINVAL;
-  if (slope && !aligned_to(slope, 16)) return SELFC_EINVAL;
+  if (act < ACT_NONE || act > ACT_SILU || !slope_ok(slope, act)) return SELFC_EINVAL;
+  const bool bits = slope && act_bits(act);
   DzArgs a{};
-  a.dy = dy; a.d = (const unsigned short*)slope; a.dz = dz; a.partial = db ? partial : nullptr; a.rows = rows; a.lddy = lddy; a.ldd = up8(n); a.lddz = lddz; a.N = n;
+  a.dy = dy; a.d = (const unsigned char*)slope; a.dz = dz; a.partial = db ? partial : nullptr; a.rows = rows; a.lddy = lddy; a.lddz = lddz; a.N = n;
+  a.ldd = slope_bytes(n, act); a.low = slope_low(act);
   hipStream_t s = (hipStream_t)stream;
   const int L = dz_lanes(n), groups = dz_groups(rows, n);
   if (groups) {
     const dim3 grid((n + L * 8 - 1) / (L * 8), groups), blk(256);
-#define DZ(L_)                                                                                         \
-  if (dtype == 1 && n % 8 == 0) hipLaunchKernelGGL((dz_kernel<b16, L_, true>), grid, blk, 0, s, a);    \
-  else if (dtype == 1) hipLaunchKernelGGL((dz_kernel<b16, L_, false>), grid, blk, 0, s, a);            \
-  else if (n % 8 == 0) hipLaunchKernelGGL((dz_kernel<h16, L_, true>), grid, blk, 0, s, a);             \
-  else hipLaunchKernelGGL((dz_kernel<h16, L_, false>), grid, blk, 0, s, a)
+#define DZ2(T_, L_)                                                                                             \
+  {                                                                                                            \
+    if (n % 8 == 0 && bits) hipLaunchKernelGGL((dz_kernel<T_, L_, true, true>), grid, blk, 0, s, a);           \
+    else if (n % 8 == 0) hipLaunchKernelGGL((dz_kernel<T_, L_, true, false>), grid, blk, 0, s, a);             \
+    else if (bits) hipLaunchKernelGGL((dz_kernel<T_, L_, false, true>), grid, blk, 0, s, a);                   \
+    else hipLaunchKernelGGL((dz_kernel<T_, L_, false, false>), grid, blk, 0, s, a);                            \
+  }
+#define DZ(L_) if (dtype == 1) DZ2(b16, L_) else DZ2(h16, L_)
     if (L == 8) { DZ(8); }
     else if (L == 16) { DZ(16); }
     else if (L == 32) { DZ(32); }
     else { DZ(64); }
 #undef DZ
+#undef DZ2
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return pw_rc(e);
   }
   return db ? pw_colsum(partial, groups, n, dtype, db, s) : SELFC_OK;
@@ -1034,24 +1076,27 @@ int selfc_linear_rows(const void* x, size_t ldx, const void* w, size_t ldw, cons
   if (rows == 0) return SELFC_OK;
   if (!x || !w || !y || n < 1 || k < 1 || !rows_ok(n, k) || rows > 0x3fffffff || act < ACT_NONE || act > ACT_SILU || (dtype != 1 && dtype != 2)) return SELFC_EINVAL;
   if ((rows > 1 && ldx < (size_t)k) || (n > 1 && ldw < (size_t)k) || (res && rows > 1 && ldr < (size_t)n)) return SELFC_EINVAL;
-  if (!aligned_to(y, 16) || (slope && !aligned_to(slope, 16)) || (xp && !aligned_to(xp, 16))) return SELFC_EINVAL;
+  if (!aligned_to(y, 16) || !slope_ok(slope, act) || (xp && !aligned_to(xp, 16))) return SELFC_EINVAL;
   RowsArgs a{};
   a.x = x; a.w = w; a.xp = xp; a.ldx = ldx; a.ldw = ldw; a.rows = rows; a.N = n; a.K = k;
-  a.e.out = y; a.e.bias = bias; a.e.res = res; a.e.ldr = ldr; a.e.act = act; a.e.d = (unsigned short*)slope; a.e.ldd = up8(n);
-  return dtype == 1 ? rows_run<b16, false>(a, (hipStream_t)stream) : rows_run<h16, false>(a, (hipStream_t)stream);
+  a.e.out = y; a.e.bias = bias; a.e.res = res; a.e.ldr = ldr; a.e.act = act; a.e.d = (unsigned char*)slope; a.e.ldd = slope_bytes(n, act);
+  hipStream_t s = (hipStream_t)stream;
+  if (slope) return dtype == 1 ? rows_run<b16, ROWS_FWD_KEEP>(a, s) : rows_run<h16, ROWS_FWD_KEEP>(a, s);
+  return dtype == 1 ? rows_run<b16, ROWS_FWD>(a, s) : rows_run<h16, ROWS_FWD>(a, s);
 }
 
-int selfc_linear_rows_bwd(const void* dy, size_t lddy, const void* slope, const void* w, size_t ldw, void* dx, void* dz,
+int selfc_linear_rows_bwd(const void* dy, size_t lddy, const void* slope, int act, const void* w, size_t ldw, void* dx, void* dz,
                           size_t rows, int n, int k, int dtype, void* stream) {
   if (rows < 1 || !dy || !w || !dx || n < 1 || k < 1 || !rows_ok(n, k) || rows > 0x3fffffff || (dtype != 1 && dtype != 2)) return SELFC_EINVAL;
   if ((rows > 1 && lddy < (size_t)n) || (n > 1 && ldw < (size_t)k)) return SELFC_EINVAL;
-  if (!aligned_to(dx, 16) || (slope && !aligned_to(slope, 16)) || (dz && !aligned_to(dz, 16))) return SELFC_EINVAL;
+  if (act < ACT_NONE || act > ACT_SILU || !aligned_to(dx, 16) || !slope_ok(slope, act) || (dz && !aligned_to(dz, 16))) return SELFC_EINVAL;
   RowsArgs a{};
-  a.x = dy; a.w = w; a.d = (const unsigned short*)slope; a.xp = dz;
-  a.ldx = lddy; a.ldw = ldw; a.ldd = up8(n); a.rows = rows; a.N = k; a.K = n;
+  a.x = dy; a.w = w; a.d = (const unsigned char*)slope; a.low = slope_low(act); a.xp = dz;
+  a.ldx = lddy; a.ldw = ldw; a.ldd = slope_bytes(n, act); a.rows = rows; a.N = k; a.K = n;
   a.e.out = dx;
   hipStream_t s = (hipStream_t)stream;
-  return dtype == 1 ? rows_run<b16, true>(a, s) : rows_run<h16, true>(a, s);
+  if (slope && act_bits(act)) return dtype == 1 ? rows_run<b16, ROWS_BWD_BITS>(a, s) : rows_run<h16, ROWS_BWD_BITS>(a, s);
+  return dtype == 1 ? rows_run<b16, ROWS_BWD>(a, s) : rows_run<h16, ROWS_BWD>(a, s);
 }
 
 }  // extern "C"

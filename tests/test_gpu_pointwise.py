@@ -604,3 +604,28 @@ def test_wide_product_without_rows(shape, n):
     q, s, _ = pw().rms_norm_q8(x.detach(), torch.ones(k).cuda())
     wq, ws = pw().quantize_rows(w.detach())
     assert s.shape == shape[:-1] and pw().linear_q8(q, s, wq, ws).shape == y.shape
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 8, 8), (37, 51, 204), (40, 64, 60), (33, 300, 130), (70, 264, 520), (5000, 100, 12)])
+@pytest.mark.parametrize("act", ["relu", "lrelu"])
+def test_kept_signs(m, k, n, act):
+    """ReLU and LeakyReLU keep one bit per value.  Integers, so that every sum is exact and the kink is met: f(0) has the derivative of the
+    negative side; what is not finite in dy does not come through a ReLU that is shut."""
+    gen = torch.Generator().manual_seed(m * k)
+    x, w = (torch.randint(-2, 3, s, generator=gen).half() for s in ((m, k), (n, k)))
+    dy = torch.randint(-4, 5, (m, n), generator=gen).half() * 5
+    z = x.double() @ w.double().t()
+    d = torch.where(z > 0, 1.0, 0.0 if act == "relu" else 0.2).double()
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w)]
+    b = torch.zeros(n, dtype=torch.float16).cuda().requires_grad_(True)
+    y = pw().linear(*leaves, b, act=act)
+    dz = (dy.double() * d).float().half().double()            # 0, 5 j and j: whole numbers
+    gx, gw, gb = torch.autograd.grad(y, leaves + [b], dy.cuda(), retain_graph=True)
+    only_b, = torch.autograd.grad(y, b, dy.cuda(), retain_graph=True)
+    for got, want in ((gx, dz @ w.double()), (gw, dz.t() @ x.double()), (gb, dz.sum(0)), (only_b, dz.sum(0))):
+        assert torch.equal(got.cpu(), want.half())
+    if act == "relu":
+        bad = torch.where(z > 0, dy.double(), math.inf).half().cuda()
+        again = torch.autograd.grad(y, leaves + [b], bad)
+        for got, want in zip(again, (gx, gw, gb)):
+            assert torch.equal(got, want)
