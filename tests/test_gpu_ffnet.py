@@ -140,3 +140,29 @@ def test_trainer_runs_a_net_of_these():
         log = tr.optimize_parameters(x, low)
     assert all(v == v and abs(v) < 1e9 for v in log.values())
     assert any(not torch.equal(a, b) for a, b in zip(before, [p for p in net.parameters() if p.requires_grad]))
+
+
+def test_trainer_captures_a_net_of_these():
+    """The captured step takes the steps that the eager one takes."""
+    from selfc_amd.modules.Inv_arch import InvRescaleNet
+    from selfc_amd.modules.Subnet_constructor import subnet
+    from selfc_amd.train import TRAIN_OPT_LARGE, RescaleTrainer
+    x, low = torch.rand(2, 3, 32, 32).cuda(), torch.rand(2, 3, 8, 8).cuda()
+    ends = []
+    for captured in (False, True):
+        torch.manual_seed(6)
+        net = InvRescaleNet(3, 3, subnet("FFNet", "xavier"), [1, 1], 2).cuda()
+        tr = RescaleTrainer(net, dict(TRAIN_OPT_LARGE, optimizer="AdamW", state_bits=8), capturable=captured)
+        torch.manual_seed(7)
+        if captured:
+            tr.capture(x, low, warmup=2)
+        else:
+            for _ in range(2):
+                tr.optimize_parameters(x, low)
+        for _ in range(2):
+            log = tr.optimize_parameters(x, low)
+        assert all(v == v and abs(v) < 1e9 for v in log.values())
+        ends.append((log["loss"], [p.detach().clone() for p in net.parameters() if p.requires_grad]))
+    assert abs(ends[0][0] / ends[1][0] - 1) < 5e-2
+    for a, b in zip(*(e[1] for e in ends)):                   # four steps of the rate 2e-4 at most move a value by about 1e-3
+        assert (a - b).abs().max() <= 1e-3
