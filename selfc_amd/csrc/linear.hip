@@ -848,10 +848,15 @@ inline Plan gemm_plan(const int M, const int N, const int R, const int es) {
   // in tiles of 128).  From 1.5 rounds on the two differ by at most a few percent either way but for full rounds, which large tiles win.
   const long large = tiles(256);
   if (large < 192 || (large > 256 && large <= 384) || stages < 4) p.tile = 128;
-  if (p.tile == 128 && tiles(128) < 192) p.tile = 64;
+  // Too few tiles of 128 for the chip: tiles of 64, unless the sums are so long that reading the operands half as often pays for dividing them (f16,
+  // dW of 200,704 x 512 x 512 314 us in tiles of 64, 143; of 8192 x 1024 x 1024 73, 32; below, bf16 1024 x 2048 x 2048 17 and 30) and edges waste little
+  const long mid = tiles(128), small = tiles(64);
+  if (p.tile == 128 && mid < 192 && (mid * stages < 8192 || 4 * mid > small + small / 4)) p.tile = 64;
   const long t = tiles(p.tile);
   // too few tiles for 256 compute units: divide the sum, at least 4 stages a part (64 x 4096 x 4096 14.4 us, undivided 35.9; 256 x 512 x 8192 16.5, 66.4)
-  if (t < 256 && p.tile < 256 && stages > 8) {
+  // and one small tile per unit leaves it half idle over a long sum (1024 x 1024 x 4096 25 us, undivided 36; over a short one dividing costs: 1024 x 1024 x
+  // 1024 14, 9)
+  if (p.tile < 256 && ((t < 256 && stages > 8) || (p.tile == 64 && t < 512 && stages >= 48))) {
     long s = (512 + t - 1) / t;
     if (s > stages / 4) s = stages / 4;
     if (s > 256) s = 256;
