@@ -854,9 +854,9 @@ inline Plan gemm_plan(const int M, const int N, const int R, const int es) {
   if (p.tile == 128 && mid < 192 && (mid * stages < 8192 || 4 * mid > small + small / 4)) p.tile = 64;
   const long t = tiles(p.tile);
   // too few tiles for 256 compute units: divide the sum, at least 4 stages a part (64 x 4096 x 4096 14.4 us, undivided 35.9; 256 x 512 x 8192 16.5, 66.4)
-  // and one small tile per unit leaves it half idle over a long sum (1024 x 1024 x 4096 25 us, undivided 36; over a short one dividing costs: 1024 x 1024 x
-  // 1024 14, 9)
-  if (p.tile < 256 && ((t < 256 && stages > 8) || (p.tile == 64 && t < 512 && stages >= 48))) {
+  // and one such tile per unit leaves it half idle over a long sum (tiles of 64: 1024 x 1024 x 4096 25 us, undivided 36, but over a short one 1024 x 1024 x
+  // 1024 14, 9; of 128: 2048 x 2048 x 8192 70, 88, and 2048 x 2048 x 2048 34, 30)
+  if (p.tile < 256 && ((t < 256 && stages > 8) || (p.tile == 64 && t < 512 && stages >= 48) || (t == 256 && stages >= 64))) {
     long s = (512 + t - 1) / t;
     if (s > stages / 4) s = stages / 4;
     if (s > 256) s = 256;
