@@ -589,7 +589,7 @@ __global__ __launch_bounds__(512) void gemv_kernel(const GemmArgs a) {
 // Pixels' channels: a product of few columns is bound by the rows' traffic, and tiles that meet in shared memory only delay it.  Here the
 // whole weight stays in shared memory, a wave takes 16 rows at a time straight from memory into the multiply's operand and back, and
 // what used to be launches of their own rides along (f16, 200,704 x 64 x 64: 13.1 us, 52 MB, 3.9 TB/s; in tiles 21.6; 72,576 x 204 x 51 with its
-// gradients: 29 + 27 us, and dW 10 + 7):
+// gradients: 24 + 21 us, and dW 10 + 7):
 //   forward   x may have any pitch and offset; its rows as whole pieces (the operand of dW) are written on the way
 //   backward  dz = dy act'(z) is formed in the operand's registers and written for dW
 // Shared memory: the weight as [TP * 16 columns][KS * 32 places], 16 bytes between rows that keep 16 rows' pieces in different banks.
