@@ -115,6 +115,10 @@ def test_c_entries_refuse_without_launching():
     assert L.selfc_linear_ws_floats(64, 64, 8192, 2) > 0 and L.selfc_linear_ws_floats(0, 64, 64, 2) == 0
     assert L.selfc_linear_dw(one, 8, one, 8, one, None, None, 0, 8, 8, 2, None) == -1
     assert L.selfc_pack_rows(one, 5, one, 2, 5, 7, 2, None) == -1
+    assert L.selfc_linear_dz(one, 8, one, 9, one, 8, None, None, 2, 8, 2, None) == -1                    # activation
+    assert L.selfc_linear_dz(one, 8, C.c_void_p(8), 3, one, 8, None, None, 2, 8, 2, None) == -1          # 16-bit codes, not aligned
+    assert L.selfc_linear_rows_bwd(one, 8, one, 9, one, 8, one, None, 2, 8, 8, 2, None) == -1            # activation
+    assert L.selfc_linear_rows(one, 8, one, 8, None, 4, None, 0, one, C.c_void_p(8), None, 2, 8, 8, 2, None) == -1
     assert L.selfc_pack_rows(None, 5, None, 0, 5, 8, 2, None) == 0                                       # no rows: no memory either
     assert L.selfc_adamw_block() == optim.BLOCK
 
