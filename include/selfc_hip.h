@@ -453,6 +453,7 @@ int selfc_rmsnorm_bwd(const void* h, size_t ldh, const void* w, int w_f32, const
  * bytes of in_dtype) floats.  e4m3: the matrix unit cuts products below 2^-13 of the largest of eight neighbours; the rest is fp32. */
 size_t selfc_linear_ws_floats(size_t rows, int cols, int sum, int elem_bytes);
 int selfc_pack_rows(const void* src, size_t ld, void* dst, size_t rows, int cols, int ldd, int elem_bytes, void* stream);
+int selfc_linear_any_layout(size_t rows, int k, int elem_bytes); /* does selfc_linear read rows of this width, and so few, at any pitch and offset? */
 int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const float* x_scale, const float* w_scale, const void* bias, int act,
                  const void* res, size_t ldr, void* y, void* slope, float* ws, size_t rows, int n, int k, int in_dtype, int out_dtype, void* stream);
 /* dz = dy * slope (slope NULL: dy; act: whose slope it is) into rows of pitch lddz = roundup(n, 8) with zeros behind them, and / or db = its column sums;

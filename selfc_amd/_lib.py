@@ -44,7 +44,7 @@ SYMBOLS = [
     "selfc_coupling_bwd_x", "selfc_add_absmax", "selfc_subnet_bwd_phase_x", "selfc_stream_create", "selfc_stream_destroy", "selfc_set_pointers", "selfc_freq_fwd_ind", "selfc_freq_inv_ind", "selfc_nchw_to_latent_ind", "selfc_latent_to_nchw_ind",
     "selfc_nchw_to_nhwc4_ind", "selfc_nhwc4_to_nchw_ind", "selfc_graph_stats",
     "selfc_fin_job_bytes", "selfc_wgrad_finish_jobs", "selfc_subnet_bwd_phase_d", "selfc_gh_bwd_pair_scratch_bytes", "selfc_gh_bwd_pair", "selfc_recon_loss_blocks", "selfc_recon_loss", "selfc_wg_job_bytes", "selfc_wgrad_run_jobs", "selfc_clip_adam_blocks", "selfc_clip_adam", "selfc_globalagg_bwd_x",
-    "selfc_rmsnorm", "selfc_rmsnorm_bwd_floats", "selfc_rmsnorm_bwd", "selfc_linear_ws_floats", "selfc_pack_rows", "selfc_linear", "selfc_linear_dz_floats",
+    "selfc_rmsnorm", "selfc_rmsnorm_bwd_floats", "selfc_rmsnorm_bwd", "selfc_linear_ws_floats", "selfc_pack_rows", "selfc_linear_any_layout", "selfc_linear", "selfc_linear_dz_floats",
     "selfc_linear_dz", "selfc_linear_rows_ok", "selfc_linear_rows", "selfc_linear_rows_bwd", "selfc_linear_dw_floats", "selfc_linear_dx", "selfc_linear_dw", "selfc_adamw_block", "selfc_adamw_step", "selfc_grad_norm_partials", "selfc_grad_norm",
 ]
 
@@ -174,6 +174,7 @@ def lib():
         sigs.update({
             "selfc_rmsnorm": [vp, sz, vp, sz, vp, i, vp, vp, vp, sz, i, i, f, vp],
             "selfc_rmsnorm_bwd": [vp, sz, vp, i, vp, vp, vp, vp, vp, sz, i, i, f, vp],
+            "selfc_linear_any_layout": [sz, i, i],
             "selfc_pack_rows": [vp, sz, vp, sz, i, i, i, vp],
             "selfc_linear": [vp, sz, vp, sz, vp, vp, vp, i, vp, sz, vp, vp, vp, sz, i, i, i, i, vp],
             "selfc_linear_dz": [vp, sz, vp, i, vp, sz, vp, vp, sz, i, i, vp],

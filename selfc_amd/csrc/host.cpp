@@ -108,7 +108,7 @@ PyObject* written(PyObject*, PyObject* args) {
 
 // ---- the kernels' library --------------------------------------------------------------------------------------------------
 #define ENTRIES(X)                                                                                                                    \
-  X(selfc_rmsnorm) X(selfc_rmsnorm_bwd) X(selfc_rmsnorm_bwd_floats) X(selfc_linear_ws_floats) X(selfc_pack_rows) X(selfc_linear)       \
+  X(selfc_rmsnorm) X(selfc_rmsnorm_bwd) X(selfc_rmsnorm_bwd_floats) X(selfc_linear_ws_floats) X(selfc_pack_rows) X(selfc_linear_any_layout) X(selfc_linear)       \
   X(selfc_linear_dz_floats) X(selfc_linear_dz) X(selfc_linear_dw_floats) X(selfc_linear_dx) X(selfc_linear_dw) X(selfc_linear_rows_ok) \
   X(selfc_linear_rows) X(selfc_linear_rows_bwd)
 struct Api {
@@ -256,13 +256,16 @@ LinearOut run_rows(const Tensor& x, const Tensor& w, const Tensor& b, const Tens
   return o;
 }
 LinearOut run_tiles(const Tensor& x, const Tensor& w, const Tensor& xs, const Tensor& ws, const Tensor& b, const Tensor& r, const int act, const at::ScalarType out,
-                    const bool want_slope, void* const stream, Tensor& wp) {
-  const int64_t rows = x.size(0), n = w.size(0), es = x.element_size(), k = (x.size(1) * es + 15) / 16 * 16 / es;
+                    const bool want_slope, const bool grad, void* const stream, Tensor& wp) {
+  const int64_t rows = x.size(0), n = w.size(0), es = x.element_size();
+  // (the backward pass reads whole pieces)
+  const bool lies = !grad && api.selfc_linear_any_layout(rows, (int)x.size(1), (int)es) && !(whole(x) && whole(w));
+  const int64_t k = lies ? x.size(1) : (x.size(1) * es + 15) / 16 * 16 / es;
   LinearOut o;
   o.y = empty(x, {rows, n}, out);
   if (want_slope) o.slope = kept(x, rows, n, act);
-  o.xp = pieces(x, stream);
-  wp = pieces(w, stream);
+  o.xp = lies ? x : pieces(x, stream);
+  wp = lies ? w : pieces(w, stream);
   if (rows) {
     const Tensor part = work(x, api.selfc_linear_ws_floats(rows, (int)n, (int)k, (int)es));
     check(api.selfc_linear(o.xp.data_ptr(), pitch(o.xp), wp.data_ptr(), pitch(wp), floats(xs), floats(ws), ptr(b), act, ptr(r), r.defined() ? pitch(r) : 0,
@@ -279,7 +282,7 @@ struct LinearFn : torch::autograd::Function<LinearFn> {
     const bool slope = act != 0 && (to_x || to_w || to_b), small = narrow(x, w);
     Tensor wp = w;
     const LinearOut o = small ? run_rows(x, w, b.value_or(Tensor()), r.value_or(Tensor()), (int)act, slope, to_w, s)
-                              : run_tiles(x, w, Tensor(), Tensor(), b.value_or(Tensor()), r.value_or(Tensor()), (int)act, x.scalar_type(), slope, s, wp);
+                              : run_tiles(x, w, Tensor(), Tensor(), b.value_or(Tensor()), r.value_or(Tensor()), (int)act, x.scalar_type(), slope, true, s, wp);
     ctx->saved_data["dims"] = std::vector<int64_t>{x.size(0), w.size(0), x.size(1), (int64_t)small, stream, b ? 1 : 0, r ? 1 : 0, act};
     ctx->save_for_backward({to_w ? o.xp : Tensor(), to_x ? wp : Tensor(), o.slope});
     return o.y;
@@ -381,7 +384,7 @@ PyObject* linear(PyObject*, PyObject* args) {
     void* const s = reinterpret_cast<void*>(stream);
     if (narrow(x, w)) return wrap(run_rows(x, w, tensor(b), tensor(r), act, false, false, s).y);
     Tensor wp;
-    return wrap(run_tiles(x, w, Tensor(), Tensor(), tensor(b), tensor(r), act, x.scalar_type(), false, s, wp).y);
+    return wrap(run_tiles(x, w, Tensor(), Tensor(), tensor(b), tensor(r), act, x.scalar_type(), false, false, s, wp).y);
   });
 }
 
@@ -394,7 +397,7 @@ PyObject* linear_q8(PyObject*, PyObject* args) {
   return guarded([&]() -> PyObject* {
     Tensor wp;
     const at::ScalarType t = out == 0 ? at::kFloat : out == 1 ? at::kBFloat16 : at::kHalf;
-    return wrap(run_tiles(THPVariable_Unpack(x), THPVariable_Unpack(w), THPVariable_Unpack(xs), THPVariable_Unpack(ws), tensor(b), tensor(r), act, t, false,
+    return wrap(run_tiles(THPVariable_Unpack(x), THPVariable_Unpack(w), THPVariable_Unpack(xs), THPVariable_Unpack(ws), tensor(b), tensor(r), act, t, false, false,
                           reinterpret_cast<void*>(stream), wp).y);
   });
 }

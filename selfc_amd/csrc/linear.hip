@@ -530,17 +530,32 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a) {
 // ---- up to 16 rows: the weight is read once, straight into registers ------------------------------------------------------
 // A workgroup owns 16 columns of the output (16 rows of W); its eight waves take turns along the sum, two 64-byte pieces of each
 // weight row at a time, and meet in shared memory.  1 x 4096 x 4096 bf16: 7.5 us with its launch (33.6 MB: 4.5 TB/s), 16 rows 10.1.
-template <typename T>
+// Rows that are not whole 16-byte pieces at aligned places are read as they lie (laying the weight out first would move its bytes three times): every piece is a 16-byte access at any address, the last one of a row moved back to the row's end and shifted down.
+// 16 bytes at `at` of a row of `bytes` >= 16; zeros behind its end
+__device__ __forceinline__ i32x4 row16(const char* const row, const unsigned at, const unsigned bytes) {
+  const unsigned from = at < bytes - 16 ? at : bytes - 16, down = (at - from) * 8;
+  unsigned long long v[2];
+  __builtin_memcpy(v, row + from, 16);
+  unsigned long long lo = v[0], hi = v[1];
+  if (down) {
+    lo = down < 64 ? v[0] >> down | v[1] << (64 - down) : down < 128 ? v[1] >> (down - 64) : 0;
+    hi = down < 64 ? v[1] >> down : 0;
+  }
+  return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+}
+template <typename T, bool WHOLE>
 __global__ __launch_bounds__(512) void gemv_kernel(const GemmArgs a) {
   constexpr int ES = sizeof(T), PIECE = 16 / ES, NW = 8, U = 8;       // U stages of a wave, 16 KiB, on their way at a time
   __shared__ float red[NW][16][17];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, i = lane & 15;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, i = lane & 15;
   const int p0 = blockIdx.x * 16;
   const size_t wbytes = ((size_t)((a.N - p0 < 16 ? a.N - p0 : 16) - 1) * a.ldp + a.R) * ES, xbytes = ((size_t)(a.M - 1) * a.ldq + a.R) * ES;
   const buf_rsrc rw = make_rsrc((const char*)a.p + (size_t)p0 * a.ldp * ES, (unsigned)wbytes);
   const buf_rsrc rx = make_rsrc(a.q, (unsigned)xbytes);
   const unsigned wrow = p0 + i < a.N ? (unsigned)(i * a.ldp * ES) : BUF_OOB, xrow = i < a.M ? (unsigned)(i * a.ldq * ES) : BUF_OOB;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  const char* const wr = (const char*)a.p + ((size_t)p0 + (p0 + i < a.N ? i : 0)) * a.ldp * ES;       // rows that are not there: any, nothing is made of them
+  const char* const xr = (const char*)a.q + (size_t)(i < a.M ? i : 0) * a.ldq * ES;
   const int stages = (a.R + 8 * PIECE - 1) / (8 * PIECE);          // 128 bytes of a row per stage
   for (int s = wave; s < stages; s += NW * U) {
     i32x4 w[U][2], x[U][2];
@@ -551,6 +566,15 @@ __global__ __launch_bounds__(512) void gemv_kernel(const GemmArgs a) {
         const int piece = (s + u * NW) * 8 + h * 4 + g;
         const bool in = piece * PIECE < a.R;
         const unsigned off = (unsigned)piece * 16;
+        if constexpr (!WHOLE) {
+          if (s + u * NW >= stages) {
+            w[u][h] = x[u][h] = i32x4{0, 0, 0, 0};
+            continue;
+          }
+          w[u][h] = row16(wr, off, (unsigned)a.R * ES);
+          x[u][h] = row16(xr, off, (unsigned)a.R * ES);
+          continue;
+        }
         w[u][h] = __builtin_bit_cast(i32x4, buffer_load_b128(rw, in && wrow != BUF_OOB ? wrow + off : BUF_OOB, 0));
         x[u][h] = __builtin_bit_cast(i32x4, buffer_load_b128(rx, in && xrow != BUF_OOB ? xrow + off : BUF_OOB, 0));
       }
@@ -948,6 +972,9 @@ int rows_run(RowsArgs a, hipStream_t s) {
 // several where there are workgroups enough and x is next to nothing.  bf16, rows x columns x sum, here and in divided tiles:
 //   1 x 2048 x 2048 6.5 us, 8.2;  16 x 4096 x 4096 10.1, 11.5;  16 x 16384 x 4096 32, 37;  1 x 4096 x 8192 15.0, 17.0
 // and where the tiles are taken: 1 x 1024 x 8192 12.3, 9.2;  16 x 2048 x 8192 18.3, 12.6;  8 x 8192 x 8192 29.5, 25.5.
+// Rows as they lie, against laying them out first (f16): 16 x 1000 x 301 5.4 us, 9.5; 10 x 6832 x 1721 17, 29; 1 x 4096 x 4097 17.7, 30.0; 16 x 4096 x 4097
+// 28.6, 35.4; not for longer sums (16 x 2048 x 8193 52.6, 37.1) and not below one piece.
+inline bool gemv_any(const size_t rows, const int k, const size_t es) { return rows <= 16 && (size_t)k * es >= 16 && (size_t)k * es <= 8192 + 128; }
 inline bool gemv_takes(const size_t rows, const int n, const int k, const size_t es) {
   return rows <= 16 && ((size_t)k * es <= 8192 || (rows <= 4 && n >= 4096));
 }
@@ -990,6 +1017,8 @@ int selfc_pack_rows(const void* src, size_t ld, void* dst, size_t rows, int cols
   return pw_rc(hipGetLastError());
 }
 
+int selfc_linear_any_layout(size_t rows, int k, int elem_bytes) { return k >= 1 && (elem_bytes == 1 || elem_bytes == 2) && gemv_any(rows, k, elem_bytes); }
+
 int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const float* x_scale, const float* w_scale, const void* bias, int act,
                  const void* res, size_t ldr, void* y, void* slope, float* ws, size_t rows, int n, int k, int in_dtype, int out_dtype, void* stream) {
   if (rows == 0) return SELFC_OK;
@@ -997,19 +1026,24 @@ int selfc_linear(const void* x, size_t ldx, const void* w, size_t ldw, const flo
   const bool q8 = in_dtype == 3;
   if (q8 != (x_scale != nullptr) || q8 != (w_scale != nullptr) || (!q8 && in_dtype != out_dtype) || (slope && q8) || !slope_ok(slope, act)) return SELFC_EINVAL;
   const size_t es = q8 ? 1 : 2;
-  if (!rows_fit(x, ldx, k, es) || !rows_fit(w, ldw, k, es)) return SELFC_EINVAL;                 // selfc_pack_rows first
+  const bool whole = rows_fit(x, ldx, k, es) && rows_fit(w, ldw, k, es);
+  if (!whole && !(gemv_any(rows, k, es) && aligned_to(x, es) && aligned_to(w, es))) return SELFC_EINVAL;      // selfc_pack_rows first
   if ((rows > 1 && ldx < (size_t)k) || (n > 1 && ldw < (size_t)k) || (res && rows > 1 && ldr < (size_t)n)) return SELFC_EINVAL;
   GemmArgs a{};
   a.q = x; a.p = w; a.ldq = ldx; a.ldp = ldw; a.M = (int)rows; a.N = n; a.R = k; a.ws = ws;
   a.e = make_epilogue(y, n, bias, res, ldr, out_dtype, act);
   a.e.qs = x_scale; a.e.ps = w_scale; a.e.d = (unsigned char*)slope; a.e.ldd = slope_bytes(n, act);
   hipStream_t s = (hipStream_t)stream;
-  if (gemv_takes(rows, n, k, es)) {
+  if (!whole || gemv_takes(rows, n, k, es)) {
     a.splits = 1;
     const dim3 grid((n + 15) / 16), blk(512);
-    if (q8) hipLaunchKernelGGL((gemv_kernel<unsigned char>), grid, blk, 0, s, a);
-    else if (in_dtype == 1) hipLaunchKernelGGL((gemv_kernel<b16>), grid, blk, 0, s, a);
-    else hipLaunchKernelGGL((gemv_kernel<h16>), grid, blk, 0, s, a);
+#define GEMV(T_)                                                                            \
+  if (whole) hipLaunchKernelGGL((gemv_kernel<T_, true>), grid, blk, 0, s, a);               \
+  else hipLaunchKernelGGL((gemv_kernel<T_, false>), grid, blk, 0, s, a)
+    if (q8) { GEMV(unsigned char); }
+    else if (in_dtype == 1) { GEMV(b16); }
+    else { GEMV(h16); }
+#undef GEMV
     return pw_rc(hipGetLastError());
   }
   if (q8) return gemm_run<unsigned char, false, false>(a, s);

@@ -7,7 +7,7 @@
 
 The last axis is the row; leading axes may be any.  Rows may have any length, pitch and offset: rows that the kernels cannot read
 in 16-byte pieces are laid out again first (one more launch; widths that are multiples of 8 - of 16 in 8 bits - avoid it; 16-bit layers
-of up to 256 values each way read any layout in place).
+of up to 256 values each way, and products of up to 16 rows of up to 8 KiB without gradients, read any layout in place).
 Everything runs on the current stream of the tensors' device, allocates from torch's allocator only, and may be captured into a
 graph.  As for every torch module, a backward pass is captured only when no eager graph over the same leaves is alive any more
 (drop the losses of the eager steps first); such a capture is refused here (autograd would end the process).

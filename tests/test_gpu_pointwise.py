@@ -629,3 +629,39 @@ def test_kept_signs(m, k, n, act):
         again = torch.autograd.grad(y, leaves + [b], bad)
         for got, want in zip(again, (gx, gw, gb)):
             assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dt", T16)
+@pytest.mark.parametrize("m,k,n", [(1, 1721, 300), (10, 257, 683), (16, 301, 77), (4, 4101, 515), (2, 9, 300), (7, 263, 258), (1, 8201, 5000)])
+def test_product_of_few_rows_as_they_lie(dt, m, k, n):
+    """Odd widths, pitches and offsets; nothing from behind a row's end or from rows behind the last gets in."""
+    gen = torch.Generator().manual_seed(m + k + n)
+    x, w, b, r = rnd(gen, m, k, dtype=dt), rnd(gen, n, k, scale=k ** -0.5, dtype=dt), rnd(gen, n, dtype=dt), rnd(gen, m, n, dtype=dt)
+    z, size, y, _ = product_ref(x, w, b, r, "silu")
+    wide = [torch.full((t.shape[0] + 2, k + 11), math.nan, dtype=dt) for t in (x, w)]
+    for off in (0, 3, 8):
+        for t, into in zip((x, w), wide):
+            into.fill_(math.nan)
+            into[1:-1, off:off + k] = t
+        xv, wv = (t.cuda()[1:-1, off:off + k] for t in wide)
+        for a, c in ((x.cuda(), w.cuda()), (xv, wv), (x.cuda(), wv)):
+            got = pw().linear(a, c, bias=b.cuda(), act="silu", residual=r.cuda())
+            within(got, y, product_bound(dt, k, z, size, y))
+
+
+@pytest.mark.parametrize("m,k,n", [(1, 31, 49), (4, 3241, 67), (16, 4097, 64), (3, 17, 300), (16, 129, 20)])
+def test_product_q8_of_few_rows_as_they_lie(m, k, n):
+    gen = torch.Generator().manual_seed(m + k + n)
+    e = torch.float8_e4m3fn
+    q = rnd(gen, m, k, scale=30.0).clamp(-448, 448).to(e)
+    xs = torch.rand(m, generator=gen) * 0.01 + 0.001
+    wq, ws = pw().quantize_rows(rnd(gen, n, k, scale=k ** -0.5))
+    z, size, y, _ = product_ref(q.float(), wq.float(), None, None, "none", (xs, ws))
+    for off in (0, 1, 16):
+        views = []
+        for t in (q, wq):
+            into = torch.full((t.shape[0] + 2, k + 21), 0x7f, dtype=torch.uint8)          # not numbers
+            into[1:-1, off:off + k] = t.view(torch.uint8)
+            views.append(into.cuda().view(e)[1:-1, off:off + k])
+        got = pw().linear_q8(views[0], xs.cuda(), views[1], ws.cuda(), out_dtype=torch.float32)
+        within(got, y, product_bound(torch.float32, k, z, size, y) + unit_bound(q, wq, xs, ws, k) * 1.01)

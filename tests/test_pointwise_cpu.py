@@ -107,14 +107,17 @@ def test_c_entries_refuse_without_launching():
     assert L.selfc_rmsnorm(one, 4, one, 4, one, 1, None, one, None, 2, 4, 2, 1e-6, None) == -1           # a residual without its sum
     assert L.selfc_rmsnorm(one, 4, None, 4, one, 1, None, one, None, 2, 16385, 2, 1e-6, None) == -1
     assert L.selfc_rmsnorm(one, 4, None, 4, one, 1, None, one, None, 0, 4, 2, 1e-6, None) == 0           # no rows
-    assert L.selfc_linear(C.c_void_p(8), 8, one, 8, None, None, None, 0, None, 0, one, None, None, 2, 8, 8, 2, 2, None) == -1   # not aligned
-    assert L.selfc_linear(one, 9, one, 8, None, None, None, 0, None, 0, one, None, None, 2, 8, 8, 2, 2, None) == -1             # pitch
+    assert L.selfc_linear(C.c_void_p(8), 8, one, 8, None, None, None, 0, None, 0, one, None, None, 32, 8, 8, 2, 2, None) == -1   # not aligned
+    assert L.selfc_linear(one, 9, one, 8, None, None, None, 0, None, 0, one, None, None, 32, 8, 8, 2, 2, None) == -1             # pitch
     assert L.selfc_linear(one, 8, one, 8, None, None, None, 7, None, 0, one, None, None, 2, 8, 8, 2, 2, None) == -1             # activation
     assert L.selfc_linear(one, 16, one, 16, None, None, None, 0, None, 0, one, None, None, 2, 8, 16, 3, 2, None) == -1          # scales missing
     assert L.selfc_linear(one, 8192, one, 8192, None, None, None, 0, None, 0, one, None, None, 64, 64, 8192, 2, 2, None) == -1  # workspace missing
     assert L.selfc_linear_ws_floats(64, 64, 8192, 2) > 0 and L.selfc_linear_ws_floats(0, 64, 64, 2) == 0
     assert L.selfc_linear_dw(one, 8, one, 8, one, None, None, 0, 8, 8, 2, None) == -1
     assert L.selfc_pack_rows(one, 5, one, 2, 5, 7, 2, None) == -1
+    assert L.selfc_linear(one, 7, one, 7, None, None, None, 0, None, 0, one, None, None, 2, 8, 7, 2, 2, None) == -1              # below one piece
+    assert L.selfc_linear(C.c_void_p(17), 9, one, 9, None, None, None, 0, None, 0, one, None, None, 2, 8, 9, 2, 2, None) == -1   # half a value off
+    assert [L.selfc_linear_any_layout(r, k, e) for r, k, e in ((16, 8, 2), (17, 8, 2), (1, 7, 2), (1, 16, 1), (1, 15, 1), (1, 9000, 2))] == [1, 0, 0, 1, 0, 0]
     assert L.selfc_linear_dz(one, 8, one, 9, one, 8, None, None, 2, 8, 2, None) == -1                    # activation
     assert L.selfc_linear_dz(one, 8, C.c_void_p(8), 3, one, 8, None, None, 2, 8, 2, None) == -1          # 16-bit codes, not aligned
     assert L.selfc_linear_rows_bwd(one, 8, one, 9, one, 8, one, None, 2, 8, 8, 2, None) == -1            # activation
