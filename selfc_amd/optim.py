@@ -37,6 +37,11 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _order(t: torch.Tensor):
+    """The order of the tensor's axes in memory: the strides of those that have one."""
+    return tuple(st for st, n in zip(t.stride(), t.shape) if n != 1)
+
+
 def _table(params, grads, steps):
     """(the C table of (parameter, gradient, step, size) per tensor, tensors it points to beyond the caller's own, the first tensor, blocks
     of the moments)."""
@@ -283,7 +288,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """Adopts the groups' hyper-parameters and copies the moments into the existing buffers (a captured step keeps its tensors).
-        The saved state has to be of the same state_bits; a plain Adam / AdamW state file loads with state_bits=32."""
+        The saved state has to be of the same state_bits; a plain Adam / AdamW state file loads with state_bits=32.  In 8 bits it also has to be
+        in the parameters' memory format: the values that share a scale are neighbours in memory, so another order has other blocks."""
         saved, groups = state_dict["state"], state_dict["param_groups"]
         if [len(g["params"]) for g in groups] != [len(g["params"]) for g in self.param_groups]:
             raise ValueError("selfc_amd: the saved state has other parameter groups than this optimizer")
@@ -296,6 +302,9 @@ class AdamW(torch.optim.Optimizer):
             for k in want - {"step"}:
                 if st and (st[k].shape != self.state[p][k].shape or st[k].dtype != self.state[p][k].dtype):
                     raise ValueError(f"selfc_amd: saved {k} is {st[k].dtype} {tuple(st[k].shape)}, expected {self.state[p][k].dtype} {tuple(self.state[p][k].shape)}")
+                if st and self.state_bits == 8 and _order(st[k]) != _order(self.state[p][k]):
+                    raise ValueError(f"selfc_amd: saved {k} has strides {st[k].stride()}, its parameter {self.state[p][k].stride()}: 8-bit moments load into the memory "
+                                     "format they were saved in only - convert the model before the optimizer's first step")
         with torch.no_grad():
             for st, p in pairs:
                 for k, own in self.state[p].items():

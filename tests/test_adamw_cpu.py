@@ -1,4 +1,5 @@
 """The 8-bit moments' format, from its definition: scales, dither, rounding (the oracle of test_gpu_adamw.py), and what it promises."""
+import pytest
 import torch
 
 BLOCK = 256
@@ -88,3 +89,48 @@ def test_second_moment_follows_its_average():
     want = 1 + 3 * 0.999 ** 4000
     # the values' spread is about 30 %; the mean of 256 of them within 0.3 / 16 = 0.019: six of them
     assert abs(v.mean().item() - want) < 0.12 and v.min() >= 0.25 and v.max() <= 4
+
+
+def moved_state(p, bits):
+    """An optimizer over p whose moments are not zeros, and what they stand for, in p's shape."""
+    from selfc_amd import optim
+    opt = optim.AdamW([p], state_bits=bits)
+    opt.ensure_state()
+    b, = opt._buckets[0]
+    x = torch.randn(b.m.numel(), generator=torch.Generator().manual_seed(2)) * (torch.arange(b.m.numel()) // BLOCK % 5 * -3.0).exp()
+    if bits == 8:
+        codes, s = hold(x, torch.full_like(x, 0.5), 7, -6, 3, False)
+        b.m.copy_(codes.to(torch.float8_e4m3fn))
+        b.scales[0].copy_(s)
+    else:
+        b.m.copy_(x)
+    return opt, held(opt, p)
+
+
+def held(opt, p):
+    """exp_avg as numbers, from the buffers in p's memory order"""
+    b, = opt._buckets[0]
+    m = b.m.float() if b.scales[0] is None else b.m.float() * b.scales[0].repeat_interleave(BLOCK)
+    return m[:p.numel()].as_strided(p.shape, p.stride())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("shape", [(32, 16, 3, 3), (24, 40, 1, 1), (7, 3, 5, 5)])
+def test_state_of_another_memory_format(bits, shape):
+    """The blocks of 8-bit moments follow memory: a state either means what it meant where it was saved, or is refused."""
+    kinds = (torch.contiguous_format, torch.channels_last)
+    for a in kinds:
+        for b in kinds:
+            p, q = (torch.nn.Parameter(torch.zeros(shape).to(memory_format=k)) for k in (a, b))
+            opt, want = moved_state(p, bits)
+            again, before = moved_state(q, bits)
+            again._buckets[0][0].m.view(torch.uint8).zero_()
+            saved = opt.state_dict()
+            same = p.stride() == q.stride() or shape[2:] == (1, 1)
+            if bits == 8 and not same:
+                with pytest.raises(ValueError, match="memory format"):
+                    again.load_state_dict(saved)
+                assert not held(again, q).any()                # refused before anything was changed
+            else:
+                again.load_state_dict(saved)
+                assert torch.equal(held(again, q), want)
