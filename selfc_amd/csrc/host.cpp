@@ -173,6 +173,12 @@ void first_only() {
   if (at::GradMode::is_enabled()) throw std::runtime_error("selfc_amd: no second derivatives (create_graph=True)");
 }
 
+// forward-mode derivatives: the kernels make none, so an input that carries a tangent must not pass as a plain one
+void no_tangents(const std::initializer_list<PyObject*> inputs) {
+  for (PyObject* const o : inputs)
+    if (o != Py_None && THPVariable_Unpack(o)._fw_grad(0).defined()) throw std::runtime_error("selfc_amd: no forward-mode derivatives (an input is a dual tensor)");
+}
+
 // ---- norm ----------------------------------------------------------------------------------------------------------------------
 struct NormOut { Tensor y, scale, h; };
 NormOut run_norm(const Tensor& x, const Tensor& r, const Tensor& w, const double eps, const bool q8, void* const stream) {
@@ -360,6 +366,7 @@ PyObject* norm(PyObject*, PyObject* args) {
   unsigned long long stream;
   if (!PyArg_ParseTuple(args, "OOOdppK", &x, &r, &w, &eps, &q8, &grad, &stream)) return nullptr;
   return guarded([&]() -> PyObject* {
+    no_tangents({x, r, w});
     NormOut o;
     if (grad) {
       const variable_list v = NormFn::apply(THPVariable_Unpack(x), maybe(r), THPVariable_Unpack(w), eps, (int64_t)stream);
@@ -379,6 +386,7 @@ PyObject* linear(PyObject*, PyObject* args) {
   unsigned long long stream;
   if (!PyArg_ParseTuple(args, "OOOOipK", &x_, &w_, &b, &r, &act, &grad, &stream)) return nullptr;
   return guarded([&]() -> PyObject* {
+    no_tangents({x_, w_, b, r});
     const Tensor &x = THPVariable_Unpack(x_), &w = THPVariable_Unpack(w_);
     if (grad) return wrap(LinearFn::apply(x, w, maybe(b), maybe(r), (int64_t)act, (int64_t)stream));
     void* const s = reinterpret_cast<void*>(stream);
@@ -395,6 +403,7 @@ PyObject* linear_q8(PyObject*, PyObject* args) {
   unsigned long long stream;
   if (!PyArg_ParseTuple(args, "OOOOOOiiK", &x, &xs, &w, &ws, &b, &r, &act, &out, &stream)) return nullptr;
   return guarded([&]() -> PyObject* {
+    no_tangents({x, xs, w, ws, b, r});
     Tensor wp;
     const at::ScalarType t = out == 0 ? at::kFloat : out == 1 ? at::kBFloat16 : at::kHalf;
     return wrap(run_tiles(THPVariable_Unpack(x), THPVariable_Unpack(w), THPVariable_Unpack(xs), THPVariable_Unpack(ws), tensor(b), tensor(r), act, t, false, false,

@@ -11,7 +11,8 @@ of up to 256 values each way, and products of up to 16 rows of up to 8 KiB witho
 Everything runs on the current stream of the tensors' device, allocates from torch's allocator only, and may be captured into a
 graph.  As for every torch module, a backward pass is captured only when no eager graph over the same leaves is alive any more
 (drop the losses of the eager steps first); such a capture is refused here (autograd would end the process).
-Refused with an exception: tensors that are not on one GPU, types other than the ones named, shapes that do not match.
+Refused with an exception: tensors that are not on one GPU, types other than the ones named, shapes that do not match, second and
+forward-mode derivatives.
 """
 from __future__ import annotations
 

@@ -665,3 +665,19 @@ def test_product_q8_of_few_rows_as_they_lie(m, k, n):
             views.append(into.cuda().view(e)[1:-1, off:off + k])
         got = pw().linear_q8(views[0], xs.cuda(), views[1], ws.cuda(), out_dtype=torch.float32)
         within(got, y, product_bound(torch.float32, k, z, size, y) + unit_bound(q, wq, xs, ws, k) * 1.01)
+
+
+def test_forward_mode_and_transforms_are_refused():
+    import torch.autograd.forward_ad as fw
+    x, w, n = torch.randn(8, 32).cuda().half(), torch.randn(40, 32).cuda().half(), torch.ones(32).cuda()
+    e = torch.float8_e4m3fn
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: pw().linear(dual(x), w), lambda: pw().linear(x, dual(w).t()[:, :8].t()), lambda: pw().rms_norm(x, dual(n)), lambda: pw().rms_norm_q8(dual(x), n),
+                     lambda: pw().linear_q8(x.to(e), dual(torch.ones(8).cuda()), w.to(e), torch.ones(40).cuda())):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+    for call in (lambda: torch.func.jvp(lambda a: pw().linear(a, w), (x,), (x,)), lambda: torch.vmap(lambda a: pw().linear(a, w))(x.view(4, 2, 32)),
+                 lambda: torch.func.grad(lambda a: pw().rms_norm(a, n)[0].sum())(x)):
+        with pytest.raises(RuntimeError):
+            call()

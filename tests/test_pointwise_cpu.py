@@ -135,3 +135,22 @@ def test_nets_in_the_dense_blocks_layout_refuse_ffnet():
     assert isinstance(net, FFNet) and net.width == 64 and not net.out.weight.any()
     with pytest.raises(NotImplementedError):
         FFNet(3, 3, width=20)
+
+
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_tangents_are_refused(monkeypatch, needs_grad):
+    """An input of forward-mode derivatives would lose them; the check comes before the first launch."""
+    import torch.autograd.forward_ad as fw
+    h = _lib.host()
+    x, w, b, r, n, one = f(2, 4), f(3, 4), f(3), f(2, 3), f(4), torch.ones(2)
+    e = torch.float8_e4m3fn
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t.requires_grad_(needs_grad), torch.ones_like(t))  # noqa: E731
+        calls = [lambda: h.linear(dual(x), w, b, r, 0, needs_grad, 0), lambda: h.linear(x, dual(w), None, None, 0, needs_grad, 0),
+                 lambda: h.linear(x, w, dual(b), None, 0, needs_grad, 0), lambda: h.linear(x, w, None, dual(r), 0, needs_grad, 0),
+                 lambda: h.norm(dual(x), None, n, 1e-6, False, needs_grad, 0), lambda: h.norm(x, dual(f(2, 4)), n, 1e-6, False, needs_grad, 0),
+                 lambda: h.norm(x, None, dual(n), 1e-6, not needs_grad, needs_grad, 0),
+                 lambda: h.linear_q8(x.detach().to(e), dual(one), w.detach().to(e), torch.ones(3), None, None, 0, 2, 0)]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
