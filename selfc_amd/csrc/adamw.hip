@@ -123,8 +123,18 @@ __device__ __forceinline__ float aw_hold(const float* const m, const unsigned* c
   return __builtin_bit_cast(float, (unsigned)e << 23);
 }
 
-// what a step's number, rate and norm make of the formulas
-struct AwStep { float keep, rate, ibc2, coef; unsigned key; };
+// what a step's number, rate and norm make of the formulas; small: subnormal moments count
+struct AwStep { float keep, rate, ibc2, coef; unsigned key; bool small; };
+
+// m / (sqrt(v) ibc2 + eps) where a root or a denominator may be too small for the root's and the reciprocal's instructions, which take
+// subnormal numbers for 0
+__device__ __forceinline__ float aw_ratio(const float m, const float v, const float ibc2, const float eps) {
+  const bool low = v < 0x1p-96f;
+  const float root = __builtin_amdgcn_sqrtf(low ? v * 0x1p64f : v) * (low ? 0x1p-32f : 1.f);
+  const float den = fmaf(root, ibc2, eps);
+  const float up = den < 0x1p-96f ? 0x1p64f : 1.f;
+  return m * up * __builtin_amdgcn_rcpf(den * up);
+}
 
 // 256 values of a tensor, four consecutive ones per lane.  FULL: all of them exist and p and g are aligned.
 template <typename T, int BITS, bool FULL>
@@ -169,9 +179,17 @@ struct AwPart {
       if (hy.norm) gi = gi * s.coef;
       m[i] = hy.b1 * m[i] + hy.omb1 * gi;
       v[i] = hy.b2 * v[i] + hy.omb2 * (gi * gi);
-      // one-ulp square root and reciprocal: the step is a small part of p, its last bits are below p's
-      const float den = fmaf(__builtin_amdgcn_sqrtf(v[i]), s.ibc2, hy.eps);
-      p[i] = fmaf(-s.rate, m[i] * __builtin_amdgcn_rcpf(den), p[i] * s.keep);
+    }
+    // one-ulp square root and reciprocal: the step is a small part of p, its last bits are below p's
+    if (!s.small) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float den = fmaf(__builtin_amdgcn_sqrtf(v[i]), s.ibc2, hy.eps);
+        p[i] = fmaf(-s.rate, m[i] * __builtin_amdgcn_rcpf(den), p[i] * s.keep);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[i] = fmaf(-s.rate, aw_ratio(m[i], v[i], s.ibc2, hy.eps), p[i] * s.keep);
     }
     if (FULL) {
       *reinterpret_cast<T4*>(pt + at) = T4{(T)p[0], (T)p[1], (T)p[2], (T)p[3]};
@@ -255,6 +273,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(const AwTable tab, const AwH
   s.keep = 1.f - lr * hy.wd;
   s.rate = lr / bc1;
   s.ibc2 = 1.f / bc2s;
+  s.small = hy.eps < s.ibc2 * 0x1p-39f;      // else the root of a subnormal v, below 2^-63, is less than 2^-24 of eps after its correction
   s.coef = 1.f;
   if (hy.norm) {                             // a norm that is not a number leaves none behind: min(1, NaN) is NaN here
     const float c = hy.max_norm / (*hy.norm + 1e-6f);

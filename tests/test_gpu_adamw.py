@@ -395,3 +395,20 @@ def test_memory_format_may_not_change_under_the_moments():
     with pytest.raises(RuntimeError, match="memory format"):
         opt.step()
     assert torch.equal(p.detach(), before)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [0.0, 1e-42, 1e-30, 1e-14, 1e-12, 1e-8])
+@pytest.mark.parametrize("scale", [2e-20, 1e-19, 1e-18, 1e-17, 1e-10])
+def test_subnormal_second_moments(scale, eps, bits):
+    """Gradients whose squares are subnormal numbers: the step is the formula's, also where eps does not hide them."""
+    g = (torch.rand(2 * BLOCK + 5, generator=torch.Generator().manual_seed(2)) + 0.5) * scale
+    kinds = (torch.float8_e4m3fn, torch.float8_e5m2) if bits == 8 else (torch.float32, torch.float32)
+    p = torch.zeros(g.numel()).cuda()
+    state = [torch.zeros(3 * BLOCK).to(k).cuda() for k in kinds] + ([torch.ones(3).cuda() for _ in range(2)] if bits == 8 else [])
+    optim().adamw_step([p], [g.cuda()], *state, step=1, lr=1e-3, eps=eps, weight_decay=0.0)
+    m, v = moments(torch.zeros_like(g), torch.zeros_like(g), g, 0.9, 0.999)
+    assert v.min() > 0
+    want = -1e-3 * (m.double() / (1 - 0.9)) / ((v.double() / (1 - 0.999)).sqrt() + float(torch.tensor(eps)))
+    # the step's factors, root, reciprocal and products: 16 roundings; one more of eps for a root that is not seen next to it
+    assert ((p.cpu().double() - want).abs() <= 17 * U32 * want.abs()).all()
