@@ -127,12 +127,18 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     lr: a float or a device scalar.  norm, max_norm: gradients count as scaled by min(1, max_norm / (norm + 1e-6)); norm is a device
     scalar (grad_norm); without it, it is computed here.  The gradients themselves are not changed.  A norm that is not finite acts as in
     the formula: infinite, the finite gradients count as 0; not a number, no parameter that has a gradient stays one."""
+    _launch(_ready(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, step=step, lr=lr, beta1=beta1, beta2=beta2, eps=eps,
+                   weight_decay=weight_decay, seed=seed, max_norm=max_norm, norm=norm))
+
+
+def _ready(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, *, step, lr, beta1, beta2, eps, weight_decay, seed, max_norm, norm):
+    """Everything that adamw_step refuses, and what _launch then takes: nothing is changed yet."""
     _need(0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0, lambda: f"betas are ({beta1}, {beta2})")
     grads = list(grads)
     steps = step if isinstance(step, (list, tuple)) else None
     tab, keep, first, blocks = _table(params, grads, steps)
     if first is None:
-        return
+        return None
     bits8 = exp_avg.dtype is torch.float8_e4m3fn
     if bits8:
         _need(exp_avg_sq.dtype is torch.float8_e5m2, lambda: f"exp_avg is float8_e4m3fn, exp_avg_sq {exp_avg_sq.dtype}: expected float8_e5m2")
@@ -160,11 +166,20 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
         norm = None
     if norm is not None:
         _need(norm.dtype is torch.float32 and norm.numel() == 1 and norm.device == first.device, "norm: expected a float32 scalar on the tensors' GPU")
+    values = (tab, len(grads), _DTYPE[first.dtype], 8 if bits8 else 32, exp_avg, exp_avg_sq, exp_avg_scale if bits8 else None, exp_avg_sq_scale if bits8 else None,
+              0.0 if lr_dev is not None else float(lr), lr_dev, float(beta1), float(beta2), float(eps), float(weight_decay), host_step, int(seed) & 0xFFFFFFFF, norm,
+              float(max_norm or 0.0))
+    return values, first, keep, params, grads
+
+
+def _launch(ready) -> None:
+    """The launches of a step that _ready has checked."""
+    if ready is None:
+        return
+    (tab, count, dtype, bits, m, v, ms, vs, lr, lr_dev, b1, b2, eps, wd, step, seed, norm, max_norm), first, keep, params, grads = ready
     with on_device(first):
-        rt.call("selfc_adamw_step", tab.__array_interface__["data"][0], len(grads), _DTYPE[first.dtype], 8 if bits8 else 32, exp_avg.data_ptr(), exp_avg_sq.data_ptr(),
-                rt._ptr(exp_avg_scale) if bits8 else None, rt._ptr(exp_avg_sq_scale) if bits8 else None, 0.0 if lr_dev is not None else float(lr),
-                rt._ptr(lr_dev), float(beta1), float(beta2), float(eps), float(weight_decay), host_step, int(seed) & 0xFFFFFFFF, rt._ptr(norm),
-                float(max_norm or 0.0), _stream(first))
+        rt.call("selfc_adamw_step", tab.__array_interface__["data"][0], count, dtype, bits, m.data_ptr(), v.data_ptr(), rt._ptr(ms), rt._ptr(vs), lr, rt._ptr(lr_dev),
+                b1, b2, eps, wd, step, seed, rt._ptr(norm), max_norm, _stream(first))
     del keep
     # the kernel wrote through raw pointers: autograd's saved-tensor checks and the packed-weight caches go by version
     _lib.host().written(params, grads)
@@ -258,32 +273,40 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("selfc_amd: construct AdamW(..., capturable=True) to capture its step")
         work = [(gi, bi, b, [p.grad for p in b.params]) for gi in range(len(self.param_groups)) for bi, b in enumerate(self._group_buckets(gi))]
         work = [w for w in work if any(g is not None for g in w[3])]
-        norm = None
+        for _, _, b, _ in work:
+            b.check_layout()
+        norm = self.grad_norm
         if self.max_norm is not None and work:
             norms = [grad_norm(w[3]) for w in work]
             home = norms[0].device
             norm = norms[0] if len(norms) == 1 else torch.stack([n.to(home) for n in norms]).double().square().sum().sqrt().float()
-            self.grad_norm = norm
-        for _, _, b, _ in work:
-            b.check_layout()
+        # every group's arguments are checked before anything is counted or launched: a refused step leaves all as it was
+        ready = []
         for gi, bi, b, grads in work:
             group = self.param_groups[gi]
             kw = dict(lr=group["lr"], beta1=group["betas"][0], beta2=group["betas"][1], eps=group["eps"], weight_decay=group["weight_decay"],
-                      seed=self.seed + 0x10001 * gi + bi, max_norm=self.max_norm, norm=None if norm is None else norm.to(b.params[0].device))
+                      seed=self.seed + 0x10001 * gi + bi, max_norm=self.max_norm, norm=None if self.max_norm is None else norm.to(b.params[0].device))
             args = (b.m, b.v, *b.scales)
-            active = [i for i, g in enumerate(grads) if g is not None]
             if self.capturable:
-                with on_device(b.params[0]):
-                    if len(active) == len(grads):
-                        b.steps.add_(1)
-                    else:
-                        torch._foreach_add_([b.step_list[i] for i in active], 1)
-                adamw_step(b.params, grads, *args, step=b.step_list, **kw)
+                ready.append(_ready(b.params, grads, *args, step=b.step_list, **kw))
                 continue
-            steps = b.steps.numpy()
-            steps[active] += 1
+            steps = b.steps.numpy() + 1
+            active = [i for i, g in enumerate(grads) if g is not None]
             for t in sorted(set(steps[active].tolist())):          # usually one: parameters that were skipped before are behind
-                adamw_step(b.params, [g if g is not None and steps[i] == t else None for i, g in enumerate(grads)], *args, step=t, **kw)
+                ready.append(_ready(b.params, [g if g is not None and steps[i] == t else None for i, g in enumerate(grads)], *args, step=t, **kw))
+        self.grad_norm = norm
+        for _, _, b, grads in work:
+            active = [i for i, g in enumerate(grads) if g is not None]
+            if not self.capturable:
+                b.steps.numpy()[active] += 1
+            elif len(active) == len(grads):
+                with on_device(b.params[0]):
+                    b.steps.add_(1)
+            else:
+                with on_device(b.params[0]):
+                    torch._foreach_add_([b.step_list[i] for i in active], 1)
+        for r in ready:
+            _launch(r)
         return loss
 
     def load_state_dict(self, state_dict):

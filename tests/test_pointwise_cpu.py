@@ -154,3 +154,30 @@ def test_tangents_are_refused(monkeypatch, needs_grad):
         for call in calls:
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call()
+
+
+@pytest.mark.parametrize("capturable", [False, True])
+def test_a_refused_step_leaves_everything_as_it_was(monkeypatch, capturable):
+    """A group whose gradients are refused: no group's step is counted and nothing is launched; afterwards the count goes on from there."""
+    launched = []
+    monkeypatch.setattr(_lib, "require_gpu", lambda t: None)
+    monkeypatch.setattr(optim, "on_device", lambda t: optim.torch.no_grad())
+    monkeypatch.setattr(optim, "_stream", lambda t: 0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(optim.rt, "call", lambda *a: launched.append(a))
+    ps = [torch.nn.Parameter(torch.zeros(n, 3)) for n in (4, 300, 2)]
+    opt = optim.AdamW([{"params": ps[:1]}, {"params": ps[1:]}], capturable=capturable)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+    opt.step()
+    assert len(launched) == 2
+    good, ps[2].grad = ps[2].grad, torch.ones(2, 3).to_sparse()
+    for _ in range(3):
+        with pytest.raises(RuntimeError, match="gradient 1"):
+            opt.step()
+    assert len(launched) == 2 and all(opt.state[p]["step"].item() == 1 for p in ps)
+    ps[2].grad = good
+    opt.step()
+    assert len(launched) == 4 and all(opt.state[p]["step"].item() == 2 for p in ps)
+    if not capturable:
+        assert [a[15] for a in launched] == [1, 1, 2, 2]               # the numbers that the launches got
