@@ -79,8 +79,8 @@ _MARK = "selfc_amd_graph_of"
 def _watch(out: torch.Tensor):
     """A leaf's gradient accumulator lives as long as a graph that reaches it and remembers the stream it was made on.  If an eager
     graph is still alive when a captured backward pass reaches the same leaf, autograd waits for that stream inside the capture and
-    the process ends; if a captured graph's outputs are still alive when an eager pass does, and the capture's stream is gone
-    (runtime.graph_capture destroys its own), it ends as well.  So: the accumulators that a call reaches are marked with the stream
+    the process ends; if a captured graph's outputs are still alive when another pass does, eager or captured, and the capture's stream is
+    gone (runtime.graph_capture destroys its own), it ends as well.  So: the accumulators that a call reaches are marked with the stream
     and with whether it was being captured, and a call that meets such a mark refuses."""
     here = _raw_stream(out.get_device())
     capturing = torch.cuda.is_current_stream_capturing()
@@ -101,7 +101,7 @@ def _watch(out: torch.Tensor):
         if capturing and not captured and made != here:
             _bad("a graph of an earlier eager call over the same parameters is still alive; its gradients cannot be accumulated inside a "
                  "capture - drop that call's outputs and losses first")
-        if captured and not capturing and made in rt.CLOSED_STREAMS:
+        if captured and made != here and made in rt.CLOSED_STREAMS:
             _bad("a captured call's outputs over the same parameters still hold their graph, whose stream is gone - keep detached outputs of a "
                  "capture")
 

@@ -681,3 +681,27 @@ def test_forward_mode_and_transforms_are_refused():
                  lambda: torch.func.grad(lambda a: pw().rms_norm(a, n)[0].sum())(x)):
         with pytest.raises(RuntimeError):
             call()
+
+
+def test_capture_over_a_captured_graph_that_is_alive_is_refused():
+    """A second capture may not reach gradient accumulators that remember the first one's stream, which is gone."""
+    from selfc_amd import runtime as rt
+    w = torch.randn(40, 32).cuda().bfloat16().requires_grad_(True)
+    x = torch.randn(8, 32).cuda().bfloat16()
+
+    pool = rt.distinct_streams(1)[0]          # (a stream of the package's own could get the destroyed one's handle, which is then a live one again)
+    first, second = rt.new_graph(), rt.new_graph()
+    with rt.graph_capture(first, x.device):
+        y = pw().linear(x, w)
+    with pytest.raises(RuntimeError, match="captured call's outputs"):
+        with torch.cuda.graph(second, stream=pool):
+            pw().linear(x, w)
+    want = y.detach()
+    del y
+    second = rt.new_graph()
+    with torch.cuda.graph(second, stream=pool):
+        z = pw().linear(x, w)
+    for g in (first, second):
+        g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(want, z.detach()) and torch.equal(z.detach(), pw().linear(x, w.detach()))
