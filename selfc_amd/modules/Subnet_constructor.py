@@ -237,7 +237,7 @@ class FFNet(nn.Module):
 
     The receptive field is one pixel: for splits whose channels hold the neighbourhood already (HaarDownsampling, FrequencyAnalyzer).
     It takes any channel counts.  `serve_bits = 8` (an attribute; without gradients only): the layers' norms write e4m3 rows and their
-    products run on e4m3 weights, which are made once per version of the parameters."""
+    products run on e4m3 weights, which are made once per version of the parameters and stream (inside a captured call: by every replay)."""
     kind = None                 # not one of the dense-block kernels: InvBlockExp composes it (_forward_composed)
 
     def __init__(self, channel_in, channel_out, init='xavier', width=64, depth=2, INN_init=True):
@@ -272,7 +272,7 @@ class FFNet(nn.Module):
         train = ag.module_needs_grad(rows, self)
         if train and self.serve_bits == 8:
             raise NotImplementedError("FFNet: serve_bits = 8 has no gradients - set it to 16 to train")
-        ps = self._cast(dt) if train else self._laid_out(dt)
+        ps = self._cast(dt) if train else self._laid_out(rows)
         h = pw.linear(rows, ps["inp.w"], bias=ps["inp.b"])
         d = None                 # what the last layer adds to the stream
         for i in range(len(self.up)):
@@ -293,17 +293,32 @@ class FFNet(nn.Module):
             ps[name + ".w"], ps[name + ".b"] = m.weight.to(dt), m.bias.to(dt)
         return ps
 
-    def _laid_out(self, dt):
-        key = (dt, self.serve_bits) + rt.params_key(self)
-        if getattr(self, "_ff_key", None) != key:
-            from .. import pointwise as pw
-            with torch.no_grad():
-                self._ff = self._cast(dt)
-                if self.serve_bits == 8:
-                    for i, m in enumerate(self.up):
-                        self._ff[f"up{i}.q"] = pw.quantize_rows(m.weight)
-            self._ff_key = key
-        return self._ff
+    def _served(self, dt):
+        """the parameters as the operators take them without gradients"""
+        with torch.no_grad():
+            ps = self._cast(dt)
+            if self.serve_bits == 8:
+                from .. import pointwise as pw
+                for i, m in enumerate(self.up):
+                    ps[f"up{i}.q"] = pw.quantize_rows(m.weight)
+        return ps
+
+    def _laid_out(self, rows):
+        """`_served`, kept while the parameters stay as they are: one copy per stream, made on it, so that its readers are ordered behind it and a
+        copy that is dropped goes back to the memory of the stream that reads it.  A capture makes its own, inside the graph: its replays
+        follow the parameters, and neither it nor the eager calls hold on to the other's memory."""
+        if torch.cuda.is_current_stream_capturing():
+            return self._served(rows.dtype)
+        key = (rows.dtype, self.serve_bits) + rt.params_key(self)
+        if self.__dict__.get("_ff_key") != key:
+            self._ff, self._ff_key = {}, key
+        kept, stream = self._ff, torch.cuda.current_stream(rows.device).cuda_stream
+        ps = kept.get(stream)
+        if ps is None:
+            if len(kept) >= 4:
+                kept.pop(next(iter(kept)))
+            ps = kept[stream] = self._served(rows.dtype)
+        return ps
 
 
 def refuse_ffnet(subnet_type):

@@ -166,3 +166,71 @@ def test_trainer_captures_a_net_of_these():
     assert abs(ends[0][0] / ends[1][0] - 1) < 5e-2
     for a, b in zip(*(e[1] for e in ends)):                   # four steps of the rate 2e-4 at most move a value by about 1e-3
         assert (a - b).abs().max() <= 1e-3
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_weights_on_streams_of_their_own(bits):
+    """Calls without gradients on two streams, the weights changing in between, each call behind the change only: what one stream laid out, the
+    other does not read before it is there, nor after it is gone."""
+    from selfc_amd import runtime as rt
+    net = build(6, 6, width=64, depth=2).cuda()
+    net.serve_bits = bits
+    x = torch.randn(1, 6, 40, 40).cuda()
+    streams = rt.distinct_streams(2)
+    wants, gots = [], []
+    with torch.no_grad():
+        for k in range(6):
+            for p in net.parameters():
+                p.mul_(1.0 + 0.125 * (k + 1))
+            fresh = build(6, 6, width=64, depth=2).cuda()
+            fresh.load_state_dict(net.state_dict())
+            fresh.serve_bits = bits
+            wants.append(fresh(x))
+            for s in streams:
+                s.wait_stream(torch.cuda.current_stream())
+            for s in (streams if k % 2 else streams[::-1]):
+                with torch.cuda.stream(s):
+                    gots.append([net(x) for _ in range(2)])
+            for s in streams:
+                torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    assert len({k for k in net._ff}) == 2
+    for k, got in enumerate(gots):
+        assert all(torch.equal(y, wants[k // 2]) for y in got), k
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("warm", [False, True])
+def test_captured_call_follows_the_weights(bits, warm):
+    """A captured call without gradients, first of all calls or after an eager one: eager calls do not read what only a replay fills, and replays do
+    not read what an eager call has dropped."""
+    from selfc_amd import runtime as rt
+    net = build(6, 6, width=64, depth=2).cuda()
+    net.serve_bits = bits
+    x = torch.randn(1, 6, 24, 24).cuda()
+    twin = build(6, 6, width=64, depth=2).cuda()
+    twin.serve_bits = bits
+
+    def want():
+        twin.load_state_dict(net.state_dict())
+        return twin(x)
+    with torch.no_grad():
+        want()                                               # the kernels are loaded; `net` itself has not run
+        if warm:
+            net(x)
+        g = rt.new_graph()
+        with rt.graph_capture(g, x.device):
+            y = net(x)
+        assert torch.equal(net(x), want())                   # before any replay
+        for k in range(3):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want()), k
+            for p in net.parameters():
+                p.add_(0.0625)
+            assert torch.equal(net(x), want()), k            # the eager call drops what it had laid out
+            junk = [torch.full((64 * 256 + 1024 * i,), float("nan"), dtype=torch.float16, device="cuda") for i in range(32)]       # and its memory is used again
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, net(x)), k
+            del junk
