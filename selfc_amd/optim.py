@@ -149,7 +149,11 @@ def _ready(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, 
     for name, t, n in (("exp_avg", exp_avg, size), ("exp_avg_sq", exp_avg_sq, size)) + ((("exp_avg_scale", exp_avg_scale, blocks), ("exp_avg_sq_scale", exp_avg_sq_scale, blocks)) if bits8 else ()):
         if t.device != dev or not t.is_contiguous() or t.numel() < n:
             raise RuntimeError(f"selfc_amd: {name}: expected {n} contiguous values on {dev}, got {tuple(t.shape)} on {t.device}")
-    _need(exp_avg.data_ptr() != exp_avg_sq.data_ptr() or not size, "exp_avg and exp_avg_sq are the same memory")
+    at, at_sq, n = exp_avg.data_ptr(), exp_avg_sq.data_ptr(), size * exp_avg.element_size()
+    _need(at + n <= at_sq or at_sq + n <= at, "exp_avg and exp_avg_sq are the same memory, or share some")
+    if bits8:
+        used = sorted(((at, at + n), (at_sq, at_sq + n), *((t.data_ptr(), t.data_ptr() + 4 * blocks) for t in (exp_avg_scale, exp_avg_sq_scale))))
+        _need(all(x[1] <= y[0] for x, y in zip(used, used[1:])), "the moments and their scales share memory")
     _need(not bits8 or (exp_avg_scale.dtype is torch.float32 and exp_avg_sq_scale.dtype is torch.float32), "the scales are float32")
     if steps is not None:
         host_step = 1.0

@@ -181,3 +181,25 @@ def test_a_refused_step_leaves_everything_as_it_was(monkeypatch, capturable):
     assert len(launched) == 4 and all(opt.state[p]["step"].item() == 2 for p in ps)
     if not capturable:
         assert [a[15] for a in launched] == [1, 1, 2, 2]               # the numbers that the launches got
+
+
+def test_moments_that_overlap_are_refused(monkeypatch):
+    monkeypatch.setattr(_lib, "require_gpu", lambda t: None)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    buf, launched = torch.zeros(2048), []
+    monkeypatch.setattr(optim, "on_device", lambda t: optim.torch.no_grad())
+    monkeypatch.setattr(optim, "_stream", lambda t: 0)
+    monkeypatch.setattr(optim.rt, "call", lambda *a: launched.append(a))
+    p, ok = [torch.zeros(300)], dict(step=1, lr=1e-3)
+    for m, v in ((buf, buf[511:]), (buf[256:], buf), (buf, buf[:512])):
+        with pytest.raises(RuntimeError, match="memory"):
+            optim.adamw_step(p, [torch.ones(300)], m, v, **ok)
+    codes, s = torch.zeros(2048, dtype=torch.uint8), torch.ones(8)
+    m8, v8 = codes.view(torch.float8_e4m3fn), codes.view(torch.float8_e5m2)
+    for args in ((m8, v8[511:], s[:2], s[2:]), (m8, v8[512:], s, s[1:]), (m8, v8[512:], s, s), (m8, v8[512:], codes[1020:1028].view(torch.float32), s)):
+        with pytest.raises(RuntimeError, match="memory"):
+            optim.adamw_step(p, [torch.ones(300)], *args, **ok)
+    assert not launched
+    optim.adamw_step(p, [torch.ones(300)], buf, buf[512:], **ok)                 # the step uses 512 values of each
+    optim.adamw_step(p, [torch.ones(300)], m8, v8[512:], s, s[2:], **ok)
+    assert len(launched) == 2
