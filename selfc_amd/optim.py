@@ -229,7 +229,8 @@ class AdamW(torch.optim.Optimizer):
     state_bits: 32 (8 bytes of moments a value), or 8 (2 bytes, and 8 per BLOCK values for their scales).  max_norm: the gradients of all
     groups count as clipped to this global norm; ``grad_norm`` then holds the norm before clipping (a device scalar).  The ``.grad``
     tensors themselves are left as they are.  capturable: step numbers (and ``lr``, if it is a tensor) live on the GPU, so that a
-    captured step keeps counting.  A parameter without a gradient is skipped, with its moments and its step.  Ranks that hold equal
+    captured step keeps counting.  seed: of the dither of 8-bit moments (one of the groups' values, so ``state_dict`` holds it and a resumed run repeats
+    the bits).  A parameter without a gradient is skipped, with its moments and its step.  Ranks that hold equal
     parameters and gradients stay equal bit for bit."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01, *, state_bits: int = 32,
@@ -242,10 +243,10 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"betas {betas}, eps {eps}, weight_decay {weight_decay}")
         if max_norm is not None and not max_norm > 0:
             raise ValueError(f"max_norm is {max_norm}")
-        self.state_bits, self.max_norm, self.capturable, self.seed = state_bits, max_norm, bool(capturable), int(seed)
+        self.state_bits, self.max_norm, self.capturable = state_bits, max_norm, bool(capturable)
         self.grad_norm: Optional[torch.Tensor] = None
         self._buckets: dict = {}
-        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, seed=int(seed)))
 
     def __getstate__(self):
         raise TypeError("selfc_amd.AdamW is saved through state_dict(): its moments are views of shared buffers")
@@ -289,7 +290,7 @@ class AdamW(torch.optim.Optimizer):
         for gi, bi, b, grads in work:
             group = self.param_groups[gi]
             kw = dict(lr=group["lr"], beta1=group["betas"][0], beta2=group["betas"][1], eps=group["eps"], weight_decay=group["weight_decay"],
-                      seed=self.seed + 0x10001 * gi + bi, max_norm=self.max_norm, norm=None if self.max_norm is None else norm.to(b.params[0].device))
+                      seed=group["seed"] + 0x10001 * gi + bi, max_norm=self.max_norm, norm=None if self.max_norm is None else norm.to(b.params[0].device))
             args = (b.m, b.v, *b.scales)
             if self.capturable:
                 ready.append(_ready(b.params, grads, *args, step=b.step_list, **kw))

@@ -398,7 +398,7 @@ class RescaleTrainer:
         if isinstance(opt, optim.AdamW):
             if self.graph is not None:
                 for own, saved in zip(opt.param_groups, sd["param_groups"]):
-                    for k_ in ("betas", "eps", "weight_decay"):
+                    for k_ in ("betas", "eps", "weight_decay", "seed"):
                         if k_ in saved and torch.as_tensor(saved[k_]).tolist() != torch.as_tensor(own[k_]).tolist():
                             raise RuntimeError(f"optimizer state changes {k_} ({own[k_]!r} -> {saved[k_]!r}), a constant of the captured step: capture again")
             opt.load_state_dict(sd)                              # in place: a captured step keeps its tensors

@@ -412,3 +412,33 @@ def test_subnormal_second_moments(scale, eps, bits):
     want = -1e-3 * (m.double() / (1 - 0.9)) / ((v.double() / (1 - 0.999)).sqrt() + float(torch.tensor(eps)))
     # the step's factors, root, reciprocal and products: 16 roundings; one more of eps for a root that is not seen next to it
     assert ((p.cpu().double() - want).abs() <= 17 * U32 * want.abs()).all()
+
+
+def test_a_resumed_run_takes_the_seed_along():
+    """The dither of 8-bit moments goes on as if the run had not been interrupted, whatever seed the new optimizer was made with."""
+    g = torch.Generator().manual_seed(3)
+    grads = [torch.randn(700, generator=g).cuda() for _ in range(6)]
+
+    def start(seed):
+        p = torch.nn.Parameter(torch.zeros(700, device="cuda"))
+        return p, optim().AdamW([p], lr=1e-2, state_bits=8, seed=seed)
+
+    def run(p, opt, some):
+        for t in some:
+            p.grad = t
+            opt.step()
+    p, opt = start(77)
+    run(p, opt, grads[:3])
+    saved = {"state": {i: {n: t.clone() for n, t in s.items()} for i, s in opt.state_dict()["state"].items()}, "param_groups": opt.state_dict()["param_groups"]}
+    q, again = start(0)
+    r, other = start(0)
+    with torch.no_grad():
+        q.copy_(p)
+        r.copy_(p)
+    again.load_state_dict(saved)
+    other.load_state_dict({"state": saved["state"], "param_groups": [{k: v for k, v in gr.items() if k != "seed"} for gr in saved["param_groups"]]})
+    run(p, opt, grads[3:])
+    run(q, again, grads[3:])
+    run(r, other, grads[3:])
+    assert torch.equal(p, q) and torch.equal(opt.state[p]["exp_avg"].float(), again.state[q]["exp_avg"].float())
+    assert other.param_groups[0]["seed"] == 0 and not torch.equal(p, r)          # a state without one: the optimizer's own
