@@ -347,4 +347,4 @@ class AdamW(torch.optim.Optimizer):
                 if k == "lr" and torch.is_tensor(own.get("lr")):
                     own["lr"].fill_(float(v))
                 elif k in own and k != "params" or k == "initial_lr":
-                    own[k] = tuple(v) if isinstance(v, list) else v
+                    own[k] = tuple(v) if isinstance(v, list) else v.clone() if torch.is_tensor(v) else v          # (the saved tensors stay the other's)

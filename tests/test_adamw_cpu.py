@@ -134,3 +134,19 @@ def test_state_of_another_memory_format(bits, shape):
             else:
                 again.load_state_dict(saved)
                 assert torch.equal(held(again, q), want)
+
+
+def test_a_loaded_rate_is_a_copy():
+    """A rate that is a tensor of the saving optimizer's: its later changes stay there."""
+    from selfc_amd import optim
+    p, q, r = (torch.nn.Parameter(torch.zeros(3)) for _ in range(3))
+    a, b, c = optim.AdamW([p], lr=torch.tensor(0.5)), optim.AdamW([q], lr=0.25), optim.AdamW([r], lr=torch.tensor(0.125))
+    a.param_groups[0]["initial_lr"] = torch.tensor(0.75)
+    own = c.param_groups[0]["lr"]
+    for other in (b, c):
+        other.load_state_dict(a.state_dict())
+    a.param_groups[0]["lr"].fill_(9.0)
+    a.param_groups[0]["initial_lr"].fill_(9.0)
+    for other in (b, c):
+        assert float(other.param_groups[0]["lr"]) == 0.5 and float(other.param_groups[0]["initial_lr"]) == 0.75
+    assert c.param_groups[0]["lr"] is own
