@@ -12,6 +12,7 @@ import os
 from typing import Dict, List, Optional, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, runtime as rt
 from .packing import dense_channels, pack_planes_generic, pack_pointwise_T, pool_weight_map_grad, pool_weight_map_grad_batch, roundup
@@ -1479,3 +1480,80 @@ class GmmSampleFn(torch.autograd.Function):
         rt.call("selfc_gmm_sample_generic_bwd", ctx.rows.data_ptr(), ctx.eps.data_ptr(), dv.data_ptr(), draw.data_ptr(), n * h * w,
                 hf, k, c, hf, ls, sp)
         return draw.reshape(n, h, w, c).permute(0, 3, 1, 2).contiguous(), None, None, None, None
+
+
+# ------------------------------------------------------------------------------------------------------------
+# FFNet: rows of 16 bits between fp32 NCHW tensors and fp32 parameters
+# ------------------------------------------------------------------------------------------------------------
+
+class GradRange:
+    """The power of two that one call's gradients are scaled by between its fp32 ends.  A loss's gradient may have any size (a mean over large
+    frames: 1e-7, below f16's steps; the trainer's loss: parameter gradients past 65,504), so, as in the dense blocks' backward kernels, the
+    incoming gradient's largest value is brought to a place in f16's range and every result is scaled back in fp32.  That place is
+    2^12 / rows, at most 1: sums over all rows (the parameters' gradients) have a factor of 16 left for what the layers in between add, and
+    values down to 2^-18 of the largest are not lost at 2^18 rows."""
+
+    def __init__(self, rows: int):
+        self.shift = max(-12, min(0, 12 - max(rows, 1).bit_length()))
+        self.scale: Optional[torch.Tensor] = None           # [1] fp32, set by the backward pass's first node
+        self.inverse: Optional[torch.Tensor] = None
+
+    def take(self, g: torch.Tensor):
+        """scale and its inverse from max|g| (contiguous fp32, 16-byte aligned), on the device.  A NaN or an infinity in g stays one."""
+        amax = torch.empty(1, dtype=torch.float32, device=g.device)
+        if g.numel():
+            rt.call("selfc_bwd_scale", g.data_ptr(), g.numel(), amax.data_ptr(), _lib.stream_ptr())
+        else:
+            amax.zero_()
+        exponent = amax.view(torch.int32).bitwise_and_(0x7F800000).clamp_(max=240 << 23)          # of max|g|, biased, in a float's place
+        self.scale = (((254 + self.shift) << 23) - exponent).view(torch.float32)
+        self.inverse = exponent.sub_(self.shift << 23).view(torch.float32)
+
+
+class RowsInFn(torch.autograd.Function):
+    """x fp32 NCHW -> rows [N*H*W][C] of 16 bits."""
+
+    @staticmethod
+    def forward(ctx, x, dt, rng):
+        ctx.rng, ctx.shape = rng, x.shape
+        n, c, h, w = x.shape
+        return x.permute(0, 2, 3, 1).to(dt, memory_format=torch.contiguous_format).view(n * h * w, c)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        n, c, h, w = ctx.shape
+        return torch.mul(g, ctx.rng.inverse).view(n, h, w, c).permute(0, 3, 1, 2), None, None
+
+
+class RowsOutFn(torch.autograd.Function):
+    """rows [N*H*W][C] of 16 bits -> fp32 NCHW; its gradient is where the call's GradRange is taken."""
+
+    @staticmethod
+    def forward(ctx, rows, n, h, w, rng):
+        ctx.rng, ctx.dt = rng, rows.dtype
+        return rows.view(n, h, w, rows.shape[1]).permute(0, 3, 1, 2).to(torch.float32, memory_format=torch.contiguous_format)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        g = g.contiguous()
+        ctx.rng.take(g if g.data_ptr() % 16 == 0 else g.clone())
+        n, c, h, w = g.shape
+        rows = torch.empty((n, h, w, c), dtype=ctx.dt, device=g.device)
+        torch.mul(g.permute(0, 2, 3, 1), ctx.rng.scale, out=rows)
+        return rows.view(n * h * w, c), None, None, None, None
+
+
+class ParamFn(torch.autograd.Function):
+    """a parameter in the type the operators take it in; its gradient leaves the call's GradRange"""
+
+    @staticmethod
+    def forward(ctx, p, dt, rng):
+        ctx.rng = rng
+        return p.view_as(p) if p.dtype == dt else p.to(dt)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        return torch.mul(g, ctx.rng.inverse), None, None          # (both have an axis: fp32)

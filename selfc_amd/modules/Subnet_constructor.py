@@ -233,7 +233,8 @@ class FFNet(nn.Module):
     __getstate__ = cache_free_state
     """Per-pixel residual feed-forward subnet (no counterpart in the reference): a product into `width` channels, `depth` layers of
     [norm, product into 4 x width with GELU, product back] around a residual stream, and a normed product out - on the operators of
-    selfc_amd/pointwise.py, in the library's operand type (f16 or bf16) with fp32 parameters; differentiable.
+    selfc_amd/pointwise.py, in the library's operand type (f16 or bf16) with fp32 parameters; differentiable, with gradients of any size
+    (autograd.GradRange).
 
     The receptive field is one pixel: for splits whose channels hold the neighbourhood already (HaarDownsampling, FrequencyAnalyzer).
     It takes any channel counts.  `serve_bits = 8` (an attribute; without gradients only): the layers' norms write e4m3 rows and their
@@ -262,21 +263,22 @@ class FFNet(nn.Module):
             raise RuntimeError(f"expected {self.channel_in} input channels, got {c}")
         if self.serve_bits not in (8, 16):
             raise RuntimeError(f"FFNet.serve_bits is {self.serve_bits}, expected 8 or 16")
-        rows = x.permute(0, 2, 3, 1).reshape(n * h * w, c).to(_lib.operand_dtype())
-        y = self._run_rows(rows)
-        return y.view(n, h, w, self.channel_out).permute(0, 3, 1, 2).to(torch.float32, memory_format=torch.contiguous_format)
-
-    def _run_rows(self, rows):
-        from .. import autograd as ag, pointwise as pw
-        dt = rows.dtype
-        train = ag.module_needs_grad(rows, self)
+        from .. import autograd as ag
+        dt, rng = _lib.operand_dtype(), ag.GradRange(n * h * w)
+        train = ag.module_needs_grad(x, self)
         if train and self.serve_bits == 8:
             raise NotImplementedError("FFNet: serve_bits = 8 has no gradients - set it to 16 to train")
-        ps = self._cast(dt) if train else self._laid_out(rows)
+        rows = ag.RowsInFn.apply(x, dt, rng)
+        y = self._run_rows(rows, self._cast(dt, lambda p, t: ag.ParamFn.apply(p, t, rng)) if train else self._laid_out(rows))
+        return ag.RowsOutFn.apply(y, n, h, w, rng)
+
+    def _run_rows(self, rows, ps):
+        from .. import pointwise as pw
+        dt = rows.dtype
         h = pw.linear(rows, ps["inp.w"], bias=ps["inp.b"])
         d = None                 # what the last layer adds to the stream
         for i in range(len(self.up)):
-            if self.serve_bits == 8 and not train:
+            if self.serve_bits == 8:
                 q, s, h = pw.rms_norm_q8(h if d is None else d, ps[f"norm{i}"], residual=None if d is None else h)
                 u = pw.linear_q8(q, s, *ps[f"up{i}.q"], bias=ps[f"up{i}.b"], act="gelu", out_dtype=dt)
             else:
@@ -286,17 +288,17 @@ class FFNet(nn.Module):
         y, _ = pw.rms_norm(d, ps[f"norm{len(self.up)}"], residual=h)
         return pw.linear(y, ps["out.w"], bias=ps["out.b"])
 
-    def _cast(self, dt):
-        """the parameters as the operators take them (differentiable)"""
-        ps = {f"norm{i}": p for i, p in enumerate(self.norms)}
+    def _cast(self, dt, to):
+        """the parameters as the operators take them"""
+        ps = {f"norm{i}": to(p, p.dtype) for i, p in enumerate(self.norms)}
         for name, m in [("inp", self.inp), ("out", self.out)] + [(f"{k}{i}", m) for k in ("up", "down") for i, m in enumerate(getattr(self, k))]:
-            ps[name + ".w"], ps[name + ".b"] = m.weight.to(dt), m.bias.to(dt)
+            ps[name + ".w"], ps[name + ".b"] = to(m.weight, dt), to(m.bias, dt)
         return ps
 
     def _served(self, dt):
         """the parameters as the operators take them without gradients"""
         with torch.no_grad():
-            ps = self._cast(dt)
+            ps = self._cast(dt, lambda p, t: p.to(t))
             if self.serve_bits == 8:
                 from .. import pointwise as pw
                 for i, m in enumerate(self.up):

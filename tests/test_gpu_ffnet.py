@@ -234,3 +234,90 @@ def test_captured_call_follows_the_weights(bits, warm):
             torch.cuda.synchronize()
             assert torch.equal(y, net(x)), k
             del junk
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_trainer_steps_are_the_eager_ones(bits):
+    """Where two eager and two captured steps lead, against four eager ones: every tensor has moved, with every step, and the two ways lie a
+    hundredth of it apart at most.  (Step numbers are formed on the device there and on the host here, the rest is the same arithmetic on the
+    same values: differences are last bits of the updates, and f16 roundings that they turn over now and then.)"""
+    from selfc_amd.modules.Inv_arch import InvRescaleNet
+    from selfc_amd.modules.Subnet_constructor import subnet
+    from selfc_amd.train import TRAIN_OPT_LARGE, RescaleTrainer
+    gen = torch.Generator().manual_seed(8)
+    batches = [(torch.rand(2, 3, 32, 32, generator=gen).cuda(), torch.rand(2, 3, 8, 8, generator=gen).cuda()) for _ in range(3)]
+    ways = []
+    for captured in (False, True):
+        torch.manual_seed(6)
+        net = InvRescaleNet(3, 3, subnet("FFNet", "xavier"), [1, 1], 2)
+        for m in net.modules():
+            if isinstance(m, torch.nn.Linear):
+                torch.nn.init.normal_(m.bias, std=0.1)
+                torch.nn.init.normal_(m.weight, std=0.05)          # (the outputs as well, which start at 0: then nothing in front of them gets a gradient)
+        net.cuda()
+        params = [p for p in net.parameters() if p.requires_grad]
+        tr = RescaleTrainer(net, dict(TRAIN_OPT_LARGE, optimizer="AdamW", state_bits=bits), capturable=captured)
+        at = [[p.detach().clone() for p in params]]
+        if captured:
+            tr.capture(*batches[0], warmup=2)
+        else:
+            for _ in range(2):
+                tr.optimize_parameters(*batches[0])
+        at.append([p.detach().clone() for p in params])
+        for b in batches[1:]:
+            tr.optimize_parameters(*b)
+            at.append([p.detach().clone() for p in params])
+        assert all(tr.optimizer_G.state[p]["step"].item() == 4 for p in params)
+        for a, b in zip(at, at[1:]):
+            assert all(not torch.equal(x, y) for x, y in zip(a, b))
+        ways.append(at)
+    for i, (start, eager, replayed) in enumerate(zip(ways[0][0], ways[0][-1], ways[1][-1])):
+        moved = (eager - start).norm()
+        assert moved > 0 and (replayed - eager).norm() <= 0.01 * moved, (i, moved.item(), (replayed - eager).norm().item())
+
+
+def gradients(net, x, dy):
+    leaf = x.clone().requires_grad_(True)
+    return torch.autograd.grad(net(leaf), [leaf, *net.parameters()], dy)
+
+
+@pytest.mark.parametrize("shape", [(1, 7, 9), (2, 24, 20), (3, 64, 70)])
+def test_gradients_of_any_size(shape):
+    """A loss's gradient may be far below f16's steps or above its range: gradients scale with it, bit for bit."""
+    net = build(12, 9, width=32, depth=2).cuda()
+    n, h, w = shape
+    x, dy = torch.randn(n, 12, h, w).cuda(), torch.randn(n, 9, h, w).cuda()
+    want = gradients(net, x, dy)
+    assert all(torch.isfinite(g).all() and g.any() for g in want)
+    for j in (-80, -24, -12, 12, 24, 60):
+        for a, b in zip(gradients(net, x, dy * 2.0 ** j), want):
+            assert torch.equal(a, b * 2.0 ** j), j
+    for a, b in zip(gradients(net, x, torch.zeros_like(dy)), want):
+        assert not a.any()
+    bad = dy.clone()
+    bad[0, 1, 2, 3] = float("nan")
+    assert all(torch.isnan(g).any() for g in gradients(net, x, bad))
+    off = torch.cat([torch.zeros(1).cuda(), dy.flatten()])[1:].view_as(dy)          # at a place that is not 16-byte aligned
+    assert all(torch.equal(a, b) for a, b in zip(gradients(net, x, off), want))
+
+
+def test_gradients_that_add_up_over_many_rows():
+    """69,632 rows whose gradients have one sign: the sums over them are past f16's range, and the mean's gradient is below its steps."""
+    net = build(6, 6, width=16, depth=1)
+    x, dy = torch.randn(1, 6, 256, 272), torch.rand(1, 6, 256, 272) + 1
+    p = {k: v.detach().double().requires_grad_(True) for k, v in net.named_parameters()}
+    want = torch.autograd.grad(ref_ffnet(p, x.double(), 1), list(p.values()), dy.double())
+    net.cuda()
+    paths = 5 * (2 + 2)                       # as above
+    for scale in (1.0, 1.0 / dy.numel()):
+        got = gradients(net, x.cuda(), dy.cuda() * scale)[1:]
+        for k, a, b in zip(p, got, want):
+            assert rel(a, b * scale) < 2 * paths * 2.0 ** -11, k
+
+
+def test_a_frame_without_pixels():
+    net = build(6, 6, width=16, depth=1).cuda()
+    x = torch.zeros(0, 6, 8, 8).cuda().requires_grad_(True)
+    y = net(x)
+    y.sum().backward()
+    assert y.shape == (0, 6, 8, 8) and x.grad.shape == x.shape and all(not p.grad.any() for p in net.parameters())
