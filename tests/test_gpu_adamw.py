@@ -442,3 +442,64 @@ def test_a_resumed_run_takes_the_seed_along():
     run(r, other, grads[3:])
     assert torch.equal(p, q) and torch.equal(opt.state[p]["exp_avg"].float(), again.state[q]["exp_avg"].float())
     assert other.param_groups[0]["seed"] == 0 and not torch.equal(p, r)          # a state without one: the optimizer's own
+
+
+@pytest.mark.parametrize("noise", [0.0, 1.0])
+def test_8_bit_moments_reach_what_32_bit_ones_reach(noise):
+    """800 steps on a quadratic from a distance of 1 (root mean square), with gradients as they are or under noise of their own size.  Without
+    noise both forms end within one step's length of the target, a hundredth of the way.  With it the distance stays where the steps' length
+    holds it, and the 8-bit form's steps are off by 15 % (standard deviation) without a bias: within that of the 32-bit form's distance."""
+    target = torch.randn(2000, generator=torch.Generator().manual_seed(13)).cuda()
+    lr, ends, moved, first = 1e-2, [], [], None
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.zeros(2000, device="cuda"))
+        opt = optim().AdamW([p], lr=lr, weight_decay=0.0, state_bits=bits, seed=3)
+        gen = torch.Generator(device="cuda").manual_seed(14)
+        for k in range(800):
+            p.grad = p.detach() - target
+            if noise:
+                p.grad += noise * torch.randn(2000, generator=gen, device="cuda")
+            if k == 0:
+                first = p.grad.clone()
+            opt.step()
+            if k == 0:
+                moved.append(p.detach().clone())
+        ends.append((p.detach() - target).double().square().mean().sqrt().item())
+    # the first step goes against the gradient, by lr |g| / (|g| + eps): eps takes eps / |g| of it
+    assert torch.equal(*moved) and torch.equal(moved[0].sign(), -first.sign()) and ((moved[0].abs() - lr).abs() <= (32 * U32 + 1e-8 / first.abs()) * lr).all()
+    if noise:
+        assert max(ends) < 0.2 and abs(ends[1] / ends[0] - 1) < 0.15, ends
+    else:
+        assert max(ends) <= lr, ends
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_on_two_streams_at_once(bits):
+    """Two optimizers' clipped steps side by side, each on its stream and with its workspaces, are the steps that they take one by one."""
+    from selfc_amd import runtime as rt
+
+    def start(seed):
+        ps = [torch.nn.Parameter(t.cuda()) for t in make(SIZES, torch.float32, seed)[0]]
+        return ps, optim().AdamW(ps, lr=1e-2, state_bits=bits, max_norm=0.5)
+    grads = {seed: [[g.cuda() for g in make(SIZES, torch.float32, 100 * seed + k)[1]] for k in range(4)] for seed in (1, 2)}
+    want = {}
+    for seed in (1, 2):
+        ps, opt = start(seed)
+        for gs in grads[seed]:
+            for p, g in zip(ps, gs):
+                p.grad = g
+            opt.step()
+        want[seed] = [p.detach().clone() for p in ps] + [opt.grad_norm]
+    runs = {seed: start(seed) for seed in (1, 2)}
+    streams = dict(zip((1, 2), rt.distinct_streams(2)))
+    for s in streams.values():
+        s.wait_stream(torch.cuda.current_stream())
+    for k in range(4):
+        for seed, (ps, opt) in runs.items():
+            with torch.cuda.stream(streams[seed]):
+                for p, g in zip(ps, grads[seed][k]):
+                    p.grad = g
+                opt.step()
+    torch.cuda.synchronize()
+    for seed, (ps, opt) in runs.items():
+        assert all(torch.equal(a, b) for a, b in zip([p.detach() for p in ps] + [opt.grad_norm], want[seed]))

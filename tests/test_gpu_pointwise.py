@@ -705,3 +705,30 @@ def test_capture_over_a_captured_graph_that_is_alive_is_refused():
         g.replay()
     torch.cuda.synchronize()
     assert torch.equal(want, z.detach()) and torch.equal(z.detach(), pw().linear(x, w.detach()))
+
+
+def test_norms_on_two_streams_at_once():
+    """Forward and backward passes side by side, workspaces and all, give what they give one by one; so do the 8-bit forms."""
+    from selfc_amd import runtime as rt
+    gen = torch.Generator().manual_seed(19)
+    cases = [[t.cuda() for t in (rnd(gen, m, c, dtype=torch.bfloat16), rnd(gen, m, c, dtype=torch.bfloat16), rnd(gen, c) + 1, rnd(gen, m, c, dtype=torch.bfloat16))]
+             for m, c in ((700, 1032), (3000, 64))]
+
+    def run(x, r, w, dy):
+        leaves = [t.clone().requires_grad_(True) for t in (x, r, w)]
+        y, h = pw().rms_norm(leaves[0], leaves[2], residual=leaves[1])
+        return [y.detach(), h.detach(), *torch.autograd.grad((y, h), leaves, (dy, dy)), *(t.float() for t in pw().rms_norm_q8(x, w, residual=r))]
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    got = [[], []]
+    streams = rt.distinct_streams(2)
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        for s, c, out in zip(streams, cases, got):
+            with torch.cuda.stream(s):
+                out.append(run(*c))
+    torch.cuda.synchronize()
+    for outs, ref in zip(got, want):
+        for out in outs:
+            assert all(torch.equal(a, b) for a, b in zip(out, ref))
