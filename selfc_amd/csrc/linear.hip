@@ -10,7 +10,10 @@
 //
 // The derivative act'(z) is kept for the backward pass: of ReLU and LeakyReLU one bit per value (z > 0), of the others a 16-bit
 // fixed-point number (steps of 2^-15 from -0.5; 65535: not a number): their derivatives lie in [-0.13, 1.13], 0 and 1 are exact, and the
-// error 2^-16 is 1/128 of what keeping z in bf16 would cost - after it the backward pass needs neither z nor the activation's formula.
+// error is 2^-16 everywhere - after it the backward pass needs neither z nor the activation's formula.  Keeping z in bf16 instead would cost up
+// to 85 times that (GELU, near |z| = 0.7; in f16 11 times), but less where the activation is all but flat: from |z| = 4.2 on (f16: 3.5; SiLU 9.9 and
+// 7.0).  There the fixed step shows as a relative error: GELU's slope -5.0e-4 at z = -4 is kept to 3 %, the -7e-6 at -5 as 0; SiLU's
+// -4.1e-4 at -10 to 4 %, the -1.1e-5 at -14 as 0.
 // (Bits against codes: a layer of 200,704 x 128 x 128 in f16 with its gradients 94 us, 119; of 72,576 x 204 x 51 58, 73.)
 //
 // Four forms, chosen by the rules beside gemm_plan, gemv_takes and rows_plan below (and, between the last two, by the caller): tiles that meet in
@@ -322,7 +325,8 @@ __global__ __launch_bounds__(NQ * NP * 64) void gemm_kernel(const GemmArgs a) {
 #pragma unroll
     for (int j = 0; j < TQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // db: the rows' own sums are one more column of the product, against a fragment of ones
+  // db: the rows' own sums are one more column of the product, against a fragment of ones.  They are sums of dz as it is multiplied, rounded to
+  // T once; without dW there is no such product, and dz_kernel adds dz before it is rounded (one rounding of 2^-9 or 2^-12 a term less)
   const bool own = QX && PX && a.sums && p0 == 0 && wp == 0;
   f32x4 osum[QX && PX ? TQ : 1];
   i32x4 ones;
@@ -870,6 +874,8 @@ inline Plan gemm_plan(const int M, const int N, const int R, const int es) {
   // Large tiles, one per compute unit at a time, where they fill the last round of the 256 units well (4096 x 4096 x 4096 in 256 of them: 106 us,
   // 113 in tiles of 128; 8192 x 4096 x 4096 in 512: 211 and 235); not where a second round would be mostly empty (5120 x 4096 x 4096 in 320: 187 us, 164
   // in tiles of 128).  From 1.5 rounds on the two differ by at most a few percent either way but for full rounds, which large tiles win.
+  // What this does not weigh is how much of a tile exists: with far fewer columns or rows than a tile has, smaller ones would be quicker
+  // (60,000 x 20 x 4096 in large tiles 144 us, in tiles of 64 112 and in four parts 104; 40,000 x 20 x 4096 in tiles of 128 91, of 64 69; 64 x 50,257 x 768 30, 19).
   const long large = tiles(256);
   if (large < 192 || (large > 256 && large <= 384) || stages < 4) p.tile = 128;
   // Too few tiles of 128 for the chip: tiles of 64, unless the sums are so long that reading the operands half as often pays for dividing them (f16,
@@ -879,7 +885,8 @@ inline Plan gemm_plan(const int M, const int N, const int R, const int es) {
   const long t = tiles(p.tile);
   // too few tiles for 256 compute units: divide the sum, at least 4 stages a part (64 x 4096 x 4096 14.4 us, undivided 35.9; 256 x 512 x 8192 16.5, 66.4)
   // and one such tile per unit leaves it half idle over a long sum (tiles of 64: 1024 x 1024 x 4096 25 us, undivided 36, but over a short one 1024 x 1024 x
-  // 1024 14, 9; of 128: 2048 x 2048 x 8192 70, 88, and 2048 x 2048 x 2048 34, 30)
+  // 1024 14, 9; of 128: 2048 x 2048 x 8192 70, 88, and 2048 x 2048 x 2048 34, 30).  Exactly one: a few more already share units by themselves, and two
+  // parts each are a second round (2048 x 2049 x 8192, 272 tiles: 101 us, in two parts 111; 288 tiles 105, 115; 320 105, 120; 368 112, 129)
   if (p.tile < 256 && ((t < 256 && stages > 8) || (p.tile == 64 && t < 512 && stages >= 48) || (t == 256 && stages >= 64))) {
     long s = (512 + t - 1) / t;
     if (s > stages / 4) s = stages / 4;

@@ -9,10 +9,13 @@
 // butterfly over the lanes that share it: the smallest power of two of lanes (8..64) that covers the row, so narrow rows (64
 // channels: 8 lanes) leave no lane idle, up to 2,048 values; a workgroup of 256 up to 16,384.  The backward pass holds two rows
 // (h and dy), the next ones' and dw's sums as well, so its rows go to a workgroup from 1,024 values on (256, 512, 1,024 lanes: more lanes, not
-// more values per lane, which would spill).  dw: a workgroup keeps its columns' sums in registers over all of its rows and writes
+// more values per lane, which would spill; from 8,193 values on 1,024 lanes have 128 registers each, and 16-bit rows spill after all: 4 registers for whole
+// rows, 50 to 56 for widths that are not a multiple of 8).  dw: a workgroup keeps its columns' sums in registers over all of its rows and writes
 // one row of partial sums; a second launch adds them in a fixed order (no atomics: the same bits every time).
 // Measured (a large copy: 5.15 TB/s): 8,192 rows of 4,096 in bf16 with residual, forward 44 us (268 MB, 6.1 TB/s: part of the input is still in the
 // last cache), backward 63 us (268 MB and 17 MB of partial sums) + 5 for their sum; 200,704 rows of 64 in f16, 21, 23.5 and 4 us (103 MB each way).
+// Forward and backward from a graph, with an fp32 weight (what memory takes at a large copy's rate): 8,192 x 4,096 fp32 214 us (209), 200,704 x 64 fp32 79
+// (80); bf16 4,096 x 8,192 131 (104), 2,048 x 16,384 144 (104), 2,048 x 16,380 215 (104): the last two pay for their spills.
 #include "pointwise.hpp"
 
 namespace selfc {
@@ -104,7 +107,7 @@ __global__ __launch_bounds__(256) void rmsnorm_kernel(const RnArgs a) {
     most = row_reduce<L, true>(most, red + 4);
     // a row of zeros: scale 1; a row whose largest value is below 448 steps of 2^-126: that step, so that its reciprocal is finite
     const float scale = most > 0.f ? fmaxf(most / E4M3_MAX, 0x1p-126f) : 1.f;
-    const float inv = 1.f / scale;
+    const float inv = 1.f / scale;            // (a product with it differs from a division by up to a last bit: a value at a tie may take the neighbouring code)
     if (lane == 0) a.scale[row] = scale;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {

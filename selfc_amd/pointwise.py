@@ -190,7 +190,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] =
            residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """act(x weight^T + bias) + residual; x (..., in), weight (out, in), both bf16 or both f16, bias (out,) and residual (..., out) of the
     same type.  act: "none", "relu", "lrelu" (0.2), "gelu" (erf), "silu".  Sums, bias, activation and residual in fp32, one rounding at the end;
-    in the backward pass dy act'(z) is rounded to x's type once, as the operand of both products.  Wide weights stream through a kernel of
+    in the backward pass dy act'(z) is rounded to x's type once, as the operand of both products; the bias's gradient is the sum of that operand
+    (without the weight's gradient: of the numbers before their rounding).  act' of GELU and SiLU is kept in steps of 2^-15.  Gradients are of
+    x's type: in f16 a loss has to be scaled so that they fit (FFNet does).  Wide weights stream through a kernel of
     their own for up to 16 rows; layers of up to 256 values each way keep theirs in shared memory.  Sums are added in a fixed order."""
     dt = x.dtype
     if dt is not torch.bfloat16 and dt is not torch.float16:
