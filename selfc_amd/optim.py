@@ -127,11 +127,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[Optional[torch.Te
     lr: a float or a device scalar.  norm, max_norm: gradients count as scaled by min(1, max_norm / (norm + 1e-6)); norm is a device
     scalar (grad_norm); without it, it is computed here.  The gradients themselves are not changed.  A norm that is not finite acts as in
     the formula: infinite, the finite gradients count as 0; not a number, no parameter that has a gradient stays one."""
-    _launch(_ready(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, step=step, lr=lr, beta1=beta1, beta2=beta2, eps=eps,
-                   weight_decay=weight_decay, seed=seed, max_norm=max_norm, norm=norm))
+    _launch(_ready(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, step, lr, beta1, beta2, eps, weight_decay, seed, max_norm, norm))
 
 
-def _ready(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, *, step, lr, beta1, beta2, eps, weight_decay, seed, max_norm, norm):
+def _ready(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, step, lr, beta1, beta2, eps, weight_decay, seed, max_norm, norm):
     """Everything that adamw_step refuses, and what _launch then takes: nothing is changed yet."""
     _need(0.0 <= beta1 < 1.0 and 0.0 <= beta2 < 1.0, lambda: f"betas are ({beta1}, {beta2})")
     grads = list(grads)
@@ -149,7 +148,7 @@ def _ready(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, 
     for name, t, n in (("exp_avg", exp_avg, size), ("exp_avg_sq", exp_avg_sq, size)) + ((("exp_avg_scale", exp_avg_scale, blocks), ("exp_avg_sq_scale", exp_avg_sq_scale, blocks)) if bits8 else ()):
         if t.device != dev or not t.is_contiguous() or t.numel() < n:
             raise RuntimeError(f"selfc_amd: {name}: expected {n} contiguous values on {dev}, got {tuple(t.shape)} on {t.device}")
-    at, at_sq, n = exp_avg.data_ptr(), exp_avg_sq.data_ptr(), size * exp_avg.element_size()
+    at, at_sq, n = exp_avg.data_ptr(), exp_avg_sq.data_ptr(), size if bits8 else 4 * size
     _need(at + n <= at_sq or at_sq + n <= at, "exp_avg and exp_avg_sq are the same memory, or share some")
     if bits8:
         used = sorted(((at, at + n), (at_sq, at_sq + n), *((t.data_ptr(), t.data_ptr() + 4 * blocks) for t in (exp_avg_scale, exp_avg_sq_scale))))
@@ -170,21 +169,19 @@ def _ready(params, grads, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, 
         norm = None
     if norm is not None:
         _need(norm.dtype is torch.float32 and norm.numel() == 1 and norm.device == first.device, "norm: expected a float32 scalar on the tensors' GPU")
-    values = (tab, len(grads), _DTYPE[first.dtype], 8 if bits8 else 32, exp_avg, exp_avg_sq, exp_avg_scale if bits8 else None, exp_avg_sq_scale if bits8 else None,
-              0.0 if lr_dev is not None else float(lr), lr_dev, float(beta1), float(beta2), float(eps), float(weight_decay), host_step, int(seed) & 0xFFFFFFFF, norm,
-              float(max_norm or 0.0))
-    return values, first, keep, params, grads
+    args = (tab.__array_interface__["data"][0], len(grads), _DTYPE[first.dtype], 8 if bits8 else 32, at, at_sq,
+            rt._ptr(exp_avg_scale) if bits8 else None, rt._ptr(exp_avg_sq_scale) if bits8 else None, 0.0 if lr_dev is not None else float(lr), rt._ptr(lr_dev),
+            float(beta1), float(beta2), float(eps), float(weight_decay), host_step, int(seed) & 0xFFFFFFFF, rt._ptr(norm), float(max_norm or 0.0))
+    return first, args, (tab, keep, norm), params, grads
 
 
 def _launch(ready) -> None:
     """The launches of a step that _ready has checked."""
     if ready is None:
         return
-    (tab, count, dtype, bits, m, v, ms, vs, lr, lr_dev, b1, b2, eps, wd, step, seed, norm, max_norm), first, keep, params, grads = ready
+    first, args, _, params, grads = ready          # (the third: what the arguments' addresses point to beyond the caller's own)
     with on_device(first):
-        rt.call("selfc_adamw_step", tab.__array_interface__["data"][0], count, dtype, bits, m.data_ptr(), v.data_ptr(), rt._ptr(ms), rt._ptr(vs), lr, rt._ptr(lr_dev),
-                b1, b2, eps, wd, step, seed, rt._ptr(norm), max_norm, _stream(first))
-    del keep
+        rt.call("selfc_adamw_step", *args, _stream(first))
     # the kernel wrote through raw pointers: autograd's saved-tensor checks and the packed-weight caches go by version
     _lib.host().written(params, grads)
 
