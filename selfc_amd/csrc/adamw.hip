@@ -23,7 +23,7 @@
 // was bound by them (134 M bf16 values: 382 us).  Measured for 134 M values in 20 tensors: 32 bits with fp32 tensors 707 us (3.76 GB, 5.3 TB/s, a
 // large copy's rate), with bf16 ones 557 (3.0 GB), 8 bits with bf16 ones 250 us (1.35 GB, 5.4 TB/s), with fp32 ones 397 (2.2 GB); the norm of the gradients in front
 // of a clipped step 91 (fp32), 49 (bf16).  A single layer's five tensors 3.7 us.  Step numbers on the device cost every lane two powers in fp64: nothing next
-// to 32-bit moments, 8 bits with bf16 tensors 254 -> 330 us.
+// to 32-bit moments, 8 bits with bf16 tensors 250 -> 264 us.
 #include "pointwise.hpp"
 #include <math.h>
 

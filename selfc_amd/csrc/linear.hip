@@ -14,12 +14,14 @@
 // to 85 times that (GELU, near |z| = 0.7; in f16 11 times), but less where the activation is all but flat: from |z| = 4.2 on (f16: 3.5; SiLU 9.9 and
 // 7.0).  There the fixed step shows as a relative error: GELU's slope -5.0e-4 at z = -4 is kept to 3 %, the -7e-6 at -5 as 0; SiLU's
 // -4.1e-4 at -10 to 4 %, the -1.1e-5 at -14 as 0.
-// (Bits against codes: a layer of 200,704 x 128 x 128 in f16 with its gradients 94 us, 119; of 72,576 x 204 x 51 58, 73.)
+// (Bits against codes - LeakyReLU against GELU, launches replayed from a graph: a layer of 200,704 x 128 x 128 in f16 with its gradients 108 us, 131; of
+// 72,576 x 204 x 51 60, 79.)
 //
 // Four forms, chosen by the rules beside gemm_plan, gemv_takes and rows_plan below (and, between the last two, by the caller): tiles that meet in
 // shared memory (bound by the matrix units), the weight straight into registers for few rows (bound by the weight's bytes), the whole weight
 // in shared memory for narrow layers (bound by the rows' bytes).  Measured, bf16: 8192 x 8192 x 8192 788 us (1,395 TFLOP/s; a library's plain product
-// 670), its two crossed forms 800 and 810 (library 785 and 905); e4m3 395 us (2,780 TFLOP/s).  In the large tiles the matrix units are busy for 60 % of
+// 666), its two crossed forms 800 and 810 (library 785 and 905); e4m3 395 us (2,780 TFLOP/s).  What follows the product shows where a unit has one tile
+// after the other: 8192 x 8192 x 2048 232 us plain, 256 with GELU, 284 with its derivative's 134 MB too.  In the large tiles the matrix units are busy for 60 % of
 // the cycles and the clock has fallen to 2.0 GHz; no shared-memory conflicts; the waves wait at the stages' barriers for 28 % of the time.  With four
 // waves of 128 x 128 instead of eight of 64 x 128 (a third less shared-memory traffic, one wave per SIMD) 1,062 us.
 #include "pointwise.hpp"
@@ -533,7 +535,8 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(const GemmArgs a) {
 
 // ---- up to 16 rows: the weight is read once, straight into registers ------------------------------------------------------
 // A workgroup owns 16 columns of the output (16 rows of W); its eight waves take turns along the sum, two 64-byte pieces of each
-// weight row at a time, and meet in shared memory.  1 x 4096 x 4096 bf16: 7.5 us with its launch (33.6 MB: 4.5 TB/s), 16 rows 10.1.
+// weight row at a time, and meet in shared memory.  1 x 4096 x 4096 bf16: 9.5 us with its launch from memory (33.6 MB: 3.5 TB/s), 7.3 where
+// the last cache holds the weight; 16 rows 12.2 and 10.0; e4m3 8.1 and 7.3.
 // Rows that are not whole 16-byte pieces at aligned places are read as they lie (laying the weight out first would move its bytes three times): every piece is a 16-byte access at any address, the last one of a row moved back to the row's end and shifted down.
 // 16 bytes at `at` of a row of `bytes` >= 16; zeros behind its end
 __device__ __forceinline__ i32x4 row16(const char* const row, const unsigned at, const unsigned bytes) {
@@ -976,9 +979,11 @@ int rows_run(RowsArgs a, hipStream_t s) {
 }
 
 // Few rows: a workgroup per 16 columns reads its part of the weight in one go (8192 bytes of the sum per row are on their way at once), or in
-// several where there are workgroups enough and x is next to nothing.  bf16, rows x columns x sum, here and in divided tiles:
-//   1 x 2048 x 2048 6.5 us, 8.2;  16 x 4096 x 4096 10.1, 11.5;  16 x 16384 x 4096 32, 37;  1 x 4096 x 8192 15.0, 17.0
-// and where the tiles are taken: 1 x 1024 x 8192 12.3, 9.2;  16 x 2048 x 8192 18.3, 12.6;  8 x 8192 x 8192 29.5, 25.5.
+// several where there are workgroups enough and x is next to nothing.  bf16, rows x columns x sum, here and in divided tiles, from memory (and with
+// the weight in the last cache):
+//   1 x 2048 x 2048 7.1 us, 10.2 (7.1, 10.2);  1 x 4096 x 4096 9.5, 13.9 (7.3, 10.5);  16 x 4096 x 4096 12.2, 14.6 (10.0, 11.5);
+//   1 x 4096 x 8192 17.2, 21.5 (14.3, 15.9);  16 x 16384 x 4096 40, 39 (31, 24)
+// and where the tiles are taken: 1 x 1024 x 8192 12.5, 10.3 (11.4, 9.9);  16 x 2048 x 8192 19.9, 14.3 (17.1, 11.2);  8 x 8192 x 8192 34, 38 (28, 24).
 // Rows as they lie, against laying them out first (f16): 16 x 1000 x 301 5.4 us, 9.5; 10 x 6832 x 1721 17, 29; 1 x 4096 x 4097 17.7, 30.0; 16 x 4096 x 4097
 // 28.6, 35.4; not for longer sums (16 x 2048 x 8193 52.6, 37.1) and not below one piece.
 inline bool gemv_any(const size_t rows, const int k, const size_t es) { return rows <= 16 && (size_t)k * es >= 16 && (size_t)k * es <= 8192 + 128; }
