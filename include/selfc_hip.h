@@ -436,7 +436,8 @@ int selfc_globalagg_bwd_x(const float* x, const float* dy, float* dx, const floa
 
 /* csrc/rmsnorm.hip.  h = x + r rounded to `dtype` (r and h together, or both NULL: h is x), y = h / sqrt(mean(h^2) + eps) * w over the
  * last axis of C <= 16384 values.  q8_scale NULL: y of `dtype`; else y is e4m3 and q8_scale[row] its step (largest |y| = 448 steps; 1 for
- * a row of zeros).  w: fp32 (w_f32) or `dtype`.  h and y are written without gaps. */
+ * a row of zeros).  w: fp32 (w_f32) or `dtype`.  h and y are written without gaps.  A launch has fewer than 2^32 lanes: at most 2^29 rows of up to
+ * 64 values, 2^28 of up to 128, 2^27 of 256, 2^26 of 2048, 2^24 of more (each less 32). */
 int selfc_rmsnorm(const void* x, size_t ldx, const void* r, size_t ldr, const void* w, int w_f32, void* h, void* y, float* q8_scale,
                   size_t rows, int C, int dtype, float eps, void* stream);
 /* Gradient with respect to x (= r's) and w: dx = the norm's part + dh (dh NULL: none), dw of w's type.  dy, dh, dx without gaps; dx or dw

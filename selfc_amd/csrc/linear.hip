@@ -1022,7 +1022,7 @@ int selfc_pack_rows(const void* src, size_t ld, void* dst, size_t rows, int cols
   if (rows == 0) return SELFC_OK;
   if (!src || !dst || !aligned_to(dst, 16)) return SELFC_EINVAL;
   const size_t n = rows * (size_t)(ldd * elem_bytes / 16);
-  if ((n + 255) / 256 > 0x7fffffffull) return SELFC_EINVAL;
+  if (n > 0xffffff00ull) return SELFC_EINVAL;                    // a launch has fewer than 2^32 lanes
   const dim3 grid((unsigned)((n + 255) / 256)), blk(256);
   if (elem_bytes == 2) hipLaunchKernelGGL((pack_rows_kernel<unsigned short>), grid, blk, 0, (hipStream_t)stream, (const unsigned short*)src, ld, (unsigned short*)dst, cols, ldd, rows);
   else hipLaunchKernelGGL((pack_rows_kernel<unsigned char>), grid, blk, 0, (hipStream_t)stream, (const unsigned char*)src, ld, (unsigned char*)dst, cols, ldd, rows);

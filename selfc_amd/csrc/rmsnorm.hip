@@ -326,8 +326,11 @@ void rn_bwd_launch(const RnBwdArgs& a, const int groups, hipStream_t s) {
 #undef RN
 }
 
+// rows: a launch has fewer than 2^32 lanes, and the forward pass takes 8 (C <= 64) to 256 of them for a row
 bool rn_shape(const size_t rows, const int C, const int dtype) {
-  return C >= 1 && C <= RN_MAX && rows <= 0x7fffffffull && dtype >= 0 && dtype <= 2;
+  if (C < 1 || C > RN_MAX || dtype < 0 || dtype > 2) return false;
+  const size_t lanes = C <= 64 ? 8 : C <= 128 ? 16 : C <= 256 ? 32 : C <= 2048 ? 64 : 256;
+  return rows <= 0x7fffffffull && rows <= 0xffffff00ull / lanes;
 }
 
 }  // namespace

@@ -203,3 +203,14 @@ def test_moments_that_overlap_are_refused(monkeypatch):
     optim.adamw_step(p, [torch.ones(300)], buf, buf[512:], **ok)                 # the step uses 512 values of each
     optim.adamw_step(p, [torch.ones(300)], m8, v8[512:], s, s[2:], **ok)
     assert len(launched) == 2
+
+
+@pytest.mark.parametrize("cols,lanes", [(1, 8), (64, 8), (65, 16), (256, 32), (257, 64), (2048, 64), (2049, 256), (16384, 256)])
+def test_more_lanes_than_a_launch_has_are_refused(cols, lanes):
+    """Counts of rows that need 2^32 lanes: refused before a launch (whose size would not fit)."""
+    L, one = _lib.lib(), C.c_void_p(16)          # never read: refused by their numbers
+    for rows in (2 ** 32 // lanes, 2 ** 31 - 1, 2 ** 40):
+        assert L.selfc_rmsnorm(one, cols, None, 0, one, 1, None, one, None, rows, cols, 2, 1e-6, None) == -1
+        assert L.selfc_rmsnorm_bwd(one, cols, one, 1, one, None, one, None, None, rows, cols, 2, 1e-6, None) == -1
+    assert L.selfc_pack_rows(one, 5, one, 2 ** 32, 5, 8, 2, None) == -1
+    assert L.selfc_pack_rows(one, 20, one, 2 ** 31, 20, 32, 1, None) == -1
