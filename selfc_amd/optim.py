@@ -266,6 +266,18 @@ class AdamW(torch.optim.Optimizer):
             self._group_buckets(gi)
 
     @torch.no_grad()
+    def reset_state(self):
+        """Moments and step numbers back to zero, in place: a captured step goes on from there."""
+        for buckets in self._buckets.values():
+            for b in buckets:
+                for t in (b.m, b.v):
+                    (t.view(torch.uint8) if t.element_size() == 1 else t).zero_()
+                for t in b.scales:
+                    if t is not None:
+                        t.fill_(1.0)
+                b.steps.zero_()
+
+    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:

@@ -141,7 +141,9 @@ class MultiStepLR_Restart(_LRScheduler):
     def get_lr(self):
         it, groups = self.last_epoch, self.optimizer.param_groups
         if it in self.restarts:
-            if self.clear_state:
+            if self.clear_state and isinstance(self.optimizer, optim.AdamW):
+                self.optimizer.reset_state()             # (its state is views of buffers that a captured step holds)
+            elif self.clear_state:
                 self.optimizer.state = defaultdict(dict)
             w = self.restart_weights[self.restarts.index(it)]
             return [g["initial_lr"] * w for g in groups]

@@ -150,3 +150,26 @@ def test_a_loaded_rate_is_a_copy():
     for other in (b, c):
         assert float(other.param_groups[0]["lr"]) == 0.5 and float(other.param_groups[0]["initial_lr"]) == 0.75
     assert c.param_groups[0]["lr"] is own
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_restart_clears_the_moments_where_they_are(bits):
+    """MultiStepLR_Restart(clear_state): the buffers that a captured step holds are cleared, and stay the optimizer's."""
+    from selfc_amd.train import MultiStepLR_Restart
+    p = torch.nn.Parameter(torch.zeros(300, 5))
+    opt, before = moved_state(p, bits)
+    b, = opt._buckets[0]
+    b.steps.fill_(7)
+    assert before.any()
+    sch = MultiStepLR_Restart(opt, [100], restarts=[3], weights=[0.5], clear_state=True)
+    opt._opt_called = True                                   # (what a step leaves for the scheduler's check of their order)
+    at = [t.data_ptr() for t in (b.m, b.v, b.steps)]
+    for k in range(3):
+        assert torch.equal(held(opt, p), before) and opt.state[p]["step"].item() == 7
+        sch.step()
+    assert opt.param_groups[0]["lr"] == 0.5e-3
+    again, = opt._group_buckets(0)
+    assert again is b and at == [t.data_ptr() for t in (b.m, b.v, b.steps)]
+    assert not held(opt, p).any() and opt.state[p]["step"].item() == 0 and set(opt.state_dict()["state"]) == {0}
+    if bits == 8:
+        assert (b.scales[0] == 1).all() and (b.scales[1] == 1).all()

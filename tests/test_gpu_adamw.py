@@ -503,3 +503,32 @@ def test_steps_on_two_streams_at_once(bits):
     torch.cuda.synchronize()
     for seed, (ps, opt) in runs.items():
         assert all(torch.equal(a, b) for a, b in zip([p.detach() for p in ps] + [opt.grad_norm], want[seed]))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_captured_step_starts_anew_after_a_reset(bits):
+    from selfc_amd import runtime as rt
+    ps, gs = make([700, 33, 4097], torch.float32, 24)
+    a, b = ([torch.nn.Parameter(t.cuda()) for t in ps] for _ in range(2))
+    opt, fresh = optim().AdamW(a, lr=1e-2, state_bits=bits, capturable=True), optim().AdamW(b, lr=1e-2, state_bits=bits)
+    for p, q, g in zip(a, b, gs):
+        p.grad = g.cuda()
+        q.grad = p.grad
+    opt.ensure_state()
+    graph = rt.new_graph()
+    with rt.graph_capture(graph, a[0].device):
+        opt.step()
+    for _ in range(3):
+        graph.replay()
+    opt.reset_state()
+    with torch.no_grad():
+        for p, t in zip(a, ps):
+            p.copy_(t)
+    for k in range(2):
+        graph.replay()
+        fresh.step()
+        torch.cuda.synchronize()
+        for p, q in zip(a, b):
+            # 1 - beta^t is formed on the device there and on the host here, both in 64 bits
+            assert ((p - q).abs() <= (k + 1) * 8 * U32 * (1e-2 + q.abs())).all()
+    assert all(opt.state[p]["step"].item() == 2 for p in a)
