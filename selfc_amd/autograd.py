@@ -1490,8 +1490,8 @@ class GradRange:
     """The power of two that one call's gradients are scaled by between its fp32 ends.  A loss's gradient may have any size (a mean over large
     frames: 1e-7, below f16's steps; the trainer's loss: parameter gradients past 65,504), so, as in the dense blocks' backward kernels, the
     incoming gradient's largest value is brought to a place in f16's range and every result is scaled back in fp32.  That place is
-    2^12 / rows, at most 1: sums over all rows (the parameters' gradients) have a factor of 16 left for what the layers in between add, and
-    values down to 2^-18 of the largest are not lost at 2^18 rows."""
+    2^12 / rows, at most 1 and at least 2^-12: a sum over all of up to 2^24 rows (the parameters' gradients) leaves a factor of 8 for what the layers
+    in between add, and at 2^18 rows f16's smallest step is 2^-17 of the largest value."""
 
     def __init__(self, rows: int):
         self.shift = max(-12, min(0, 12 - max(rows, 1).bit_length()))
